@@ -6,6 +6,7 @@ and linked into one shared library that sits in the source tree.  ``python -m fu
 from __future__ import annotations
 
 import os
+import re
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -30,6 +31,17 @@ def _nvcc() -> str:
 
 def _newer(target: Path, deps) -> bool:
     return target.exists() and all(target.stat().st_mtime >= d.stat().st_mtime for d in deps)
+
+
+def _includes(src: Path, seen=None) -> list:
+    """The files of this repository that ``src`` includes with quotes, directly or through others."""
+    seen = set() if seen is None else seen
+    for name in re.findall(r'^\s*#include "([^"]+)"', src.read_text(), re.M):
+        path = (OBJDIR / name) if (OBJDIR / name).exists() else (src.parent / name).resolve()
+        if path.exists() and path not in seen:
+            seen.add(path)
+            _includes(path, seen)
+    return sorted(seen)
 
 
 def _embed_kernel_source() -> Path:
@@ -59,15 +71,14 @@ def build(force: bool = False, verbose: bool = False, extra_flags=()) -> Path:
     extra_flags = tuple(extra_flags) + tuple(os.environ.get("FUSEDMM_B200_NVCC_FLAGS", "").split())
     OBJDIR.mkdir(parents=True, exist_ok=True)
     LIBDIR.mkdir(parents=True, exist_ok=True)
-    embedded = _embed_kernel_source()
+    _embed_kernel_source()
     extra_flags = extra_flags + ("-I", str(OBJDIR))
-    headers = sorted(CSRC.glob("*.cuh")) + sorted((PKG.parent / "include").glob("*.h")) + [embedded]
     sources = sorted(CSRC.glob("*.cu"))
     nvcc = _nvcc()
     jobs = []
     for src in sources:
         obj = OBJDIR / (src.stem + ".o")
-        if force or not _newer(obj, [src] + headers):
+        if force or not _newer(obj, [src] + _includes(src)):
             jobs.append((src, obj))
 
     def compile_one(job):

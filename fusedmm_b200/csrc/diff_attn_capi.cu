@@ -1,0 +1,263 @@
+// diff_attn_capi.cu -- the entry points of differential attention (include/fusedmm_b200.h): argument checks, the choice of
+// the walk's shape, scratch layout.  The kernels are in diff_attn.cuh.
+#include "attn_host.h"
+#include "diff_attn.cuh"
+
+#include <climits>
+#include <cstdlib>
+
+namespace fmm {
+namespace attn {
+
+constexpr int LAM_BLOCKS = 256;
+
+// dlam[h] = sum over the rows: each block a run of rows, then one block the blocks' sums
+__global__ void __launch_bounds__(256) lam_sum_kernel(const float *in, long long rows, int heads, float *out, long long each)
+{
+   __shared__ float part[8][33];
+   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+   const long long r0 = blockIdx.x * each, r1 = r0 + each < rows ? r0 + each : rows;
+   for (int h0 = 0; h0 < heads; h0 += 32) {
+      const int h = h0 + lane;
+      float s = 0.0f;
+      if (h < heads)
+         for (long long r = r0 + w; r < r1; r += 8) s += in[r * heads + h];
+      part[w][lane] = s;
+      __syncthreads();
+      if (w == 0 && h < heads) {
+         float t = 0.0f;
+         for (int i = 0; i < 8; i++) t += part[i][lane];
+         out[static_cast<long long>(blockIdx.x) * heads + h] = t;
+      }
+      __syncthreads();
+   }
+}
+
+namespace {
+
+enum Walk { FORWARD, ROWS, COLUMNS };
+
+struct Shape {
+   WalkShape walk;
+   int units = 0, unit_blocks = 0, slot_heads = 0;
+   long long piece = 0, row_limit = 0, pieces = 0, part_bytes = 0;
+   long long scratch_bytes() const { return (pieces * 2 * units * part_bytes + 255) / 256 * 256 + (pieces * 8 + 255) / 256 * 256; }
+};
+
+constexpr long long SCRATCH_LIMIT = 128LL << 20;
+
+Shape choose_shape(Walk w, int dtype, bool vector, long long rows, long long edges, int heads, int kv_heads, int d, int dv, int sms)
+{
+   Shape s;
+   const int width = dtype == DT_F32 ? 4 : 8;
+   const int nk = 2 * ((d + width - 1) / width), nvv = (dv + width - 1) / width, need = nk > nvv ? nk : nvv;
+   s.walk.g = need <= 4 ? 4 : need <= 8 ? 8 : need <= 16 ? 16 : 32;
+   s.walk.nv = need <= 32 ? 1 : 2;
+   s.walk.vector = vector;
+   const int group = heads / kv_heads;
+   s.walk.qb = w == COLUMNS || !vector ? 1 : group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+   s.units = w == COLUMNS ? kv_heads : heads / s.walk.qb;
+   s.slot_heads = 1;
+   while (2 * s.slot_heads <= 32 / s.walk.g && s.units % (2 * s.slot_heads) == 0) s.slot_heads *= 2;
+   s.unit_blocks = s.units / s.slot_heads;
+   const int lane_floats = w == COLUMNS ? 2 * s.walk.nv * width : s.walk.qb * (2 * s.walk.nv * width + 2);
+   s.part_bytes = static_cast<long long>(lane_floats) * s.walk.g * 4;
+   const long long items = edges + ROW_ITEMS * rows, mean = edges / rows;
+   const bool few = rows * s.unit_blocks < 8LL * sms;
+   s.walk.together = mean >= 256 || (few && mean >= 64);
+   const long long lo = s.walk.together ? 256 : 64, hi = s.walk.together ? 8192 : 1024;
+   const long long jobs = static_cast<long long>(sms) * (s.walk.together ? 6 : 128);
+   s.piece = (items * s.unit_blocks + jobs - 1) / jobs;
+   s.piece = s.piece < lo ? lo : s.piece > hi ? hi : s.piece;
+   for (;; s.piece *= 2) {
+      s.pieces = (items + s.piece - 1) / s.piece;
+      if (s.pieces * 2 * s.units * s.part_bytes <= SCRATCH_LIMIT && s.pieces * s.unit_blocks < INT_MAX / 2) break;
+   }
+   s.row_limit = s.walk.together ? s.piece : s.piece > 512 ? s.piece : 512;
+   return s;
+}
+
+void apply(AttnParams &p, const Shape &s, char *scratch)
+{
+   p.units = s.units; p.unit_blocks = s.unit_blocks; p.slot_heads = s.slot_heads;
+   p.piece = s.piece; p.row_limit = s.row_limit; p.pieces = s.pieces;
+   p.partial = reinterpret_cast<float *>(scratch);
+   p.long_row = reinterpret_cast<long long *>(scratch + (s.pieces * 2 * s.units * s.part_bytes + 255) / 256 * 256);
+}
+
+int launch(Walk w, int dtype, const Shape &s, const AttnParams &p, cudaStream_t st)
+{
+   int r = -1;
+   if (w == FORWARD) r = dtype == DT_F32 ? walk_forward_f32(s.walk, p, st) : dtype == DT_BF16 ? walk_forward_bf16(s.walk, p, st) : walk_forward_f16(s.walk, p, st);
+   if (w == ROWS) r = dtype == DT_F32 ? walk_rows_f32(s.walk, p, st) : dtype == DT_BF16 ? walk_rows_bf16(s.walk, p, st) : walk_rows_f16(s.walk, p, st);
+   if (w == COLUMNS) r = dtype == DT_F32 ? walk_columns_f32(s.walk, p, st) : dtype == DT_BF16 ? walk_columns_bf16(s.walk, p, st) : walk_columns_f16(s.walk, p, st);
+   if (r == 0) return 0;
+   const int status = cuda_status();
+   return status ? status : FUSEDMM_B200_ERR_CUDA;
+}
+
+int check_sizes(int32_t dtype, int64_t m, int64_t n, int64_t nnz, int32_t heads, int32_t kv_heads, int32_t d, int32_t dv)
+{
+   if (dtype != DT_F32 && dtype != DT_BF16 && dtype != DT_F16) return FUSEDMM_B200_ERR_ARG;
+   if (m < 0 || n < 0 || nnz < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || d < 1 || dv < 1) return FUSEDMM_B200_ERR_ARG;
+   if (d > FUSEDMM_B200_ATTN_MAX_WIDTH / 2 || dv > FUSEDMM_B200_ATTN_MAX_WIDTH || heads > FUSEDMM_B200_ATTN_MAX_HEADS)
+      return FUSEDMM_B200_ERR_LIMIT;
+   if (m > (1LL << 48) || nnz > (1LL << 48)) return FUSEDMM_B200_ERR_LIMIT;
+   return 0;
+}
+
+// elements that one load of these rows may take at once; 16 bytes' worth: whole vectors
+struct Step {
+   int step;
+   size_t elt;
+   Step(int32_t dtype) : step(dtype == DT_F32 ? 4 : 8), elt(dtype == DT_F32 ? 4 : 2) {}
+   void with(const void *p, long long a, long long b, long long c)
+   {
+      while (step > 1 && (reinterpret_cast<uintptr_t>(p) % (step * elt) || a % step || b % step || c % step)) step /= 2;
+   }
+   bool vector() const { return step * elt == 16; }
+};
+
+long long round256(long long b) { return (b + 255) / 256 * 256; }
+long long max_ll(long long a, long long b) { return a > b ? a : b; }
+
+long long walk_scratch(Walk w, int dtype, long long rows, long long edges, int heads, int kv_heads, int d, int dv, int sms)
+{
+   if (rows == 0) return 0;
+   return max_ll(choose_shape(w, dtype, true, rows, edges, heads, kv_heads, d, dv, sms).scratch_bytes(),
+                 choose_shape(w, dtype, false, rows, edges, heads, kv_heads, d, dv, sms).scratch_bytes());
+}
+
+// scratch of the backward pass in front of the walks': stats, dlam of every row, the sums of runs of rows
+long long backward_front(long long m, int heads) { return round256(m * heads * 16) + round256(m * heads * 4) + round256(LAM_BLOCKS * heads * 4LL); }
+
+}  // namespace
+}  // namespace attn
+}  // namespace fmm
+
+using namespace fmm::attn;
+
+extern "C" {
+
+int64_t fusedmm_b200_diff_attention_workspace(int32_t backward, int32_t dtype, int64_t m, int64_t n, int64_t nnz,
+                                              int32_t heads, int32_t kv_heads, int32_t d, int32_t dv)
+{
+   if (int s = check_sizes(dtype, m, n, nnz, heads, kv_heads, d, dv)) return s;
+   int sms = 0;
+   if (int s = sm_count(&sms)) return s;
+   if (!backward) return walk_scratch(FORWARD, dtype, m, nnz, heads, kv_heads, d, dv, sms);
+   return backward_front(m, heads) + max_ll(walk_scratch(ROWS, dtype, m, nnz, heads, kv_heads, d, dv, sms),
+                                            walk_scratch(COLUMNS, dtype, n, nnz, heads, kv_heads, d, dv, sms));
+}
+
+int fusedmm_b200_diff_attention(int32_t dtype, int32_t ptr_bits, int32_t idx_bits, int64_t m, int64_t n, int64_t nnz,
+                                const void *rowptr, const void *colidx, const float *bias, int32_t heads, int32_t kv_heads,
+                                int32_t d, int32_t dv, const void *q, int64_t ldq, int64_t hsq, const void *k, int64_t ldk,
+                                int64_t hsk, const void *v, int64_t ldv, int64_t hsv, const float *lam, int64_t ldlam,
+                                double scale, void *out, float *lse, void *workspace, int64_t workspace_bytes, void *stream)
+{
+   if ((ptr_bits != 32 && ptr_bits != 64) || (idx_bits != 32 && idx_bits != 64)) return FUSEDMM_B200_ERR_ARG;
+   if (int s = check_sizes(dtype, m, n, nnz, heads, kv_heads, d, dv)) return s;
+   if (m == 0) return 0;
+   const bool gathers = nnz > 0 && n > 0;
+   if (!rowptr || !q || !lam || !out || (nnz > 0 && !colidx) || (gathers && (!k || !v))) return FUSEDMM_B200_ERR_ARG;
+   int sms = 0;
+   if (int s = sm_count(&sms)) return s;
+   const long long need = walk_scratch(FORWARD, dtype, m, nnz, heads, kv_heads, d, dv, sms);
+   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256) return FUSEDMM_B200_ERR_ARG;
+   if (!on_device({rowptr, q, lam, out, lse, workspace, nnz > 0 ? colidx : nullptr, nnz > 0 ? bias : nullptr,
+                   gathers ? k : nullptr, gathers ? v : nullptr}))
+      return FUSEDMM_B200_ERR_ARG;
+   Step step(dtype);
+   step.with(q, ldq, hsq, d);
+   step.with(k, ldk, hsk, d);
+   step.with(v, ldv, hsv, dv);
+   step.with(out, 0, 0, dv);
+   AttnParams p = {};
+   p.rowptr = rowptr; p.colidx = colidx; p.ptr64 = ptr_bits == 64; p.idx64 = idx_bits == 64;
+   p.m = m; p.n = n; p.nnz = nnz; p.bias = bias;
+   p.q = q; p.k = k; p.v = v; p.lam = lam;
+   p.ldq = ldq; p.hsq = hsq; p.ldk = ldk; p.hsk = hsk; p.ldv = ldv; p.hsv = hsv; p.ldlam = ldlam;
+   p.out = out; p.lse = lse;
+   p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads; p.d = d; p.dv = dv; p.step = step.step;
+   p.scale = static_cast<float>(scale);
+   const Shape s = choose_shape(FORWARD, dtype, step.vector(), m, nnz, heads, kv_heads, d, dv, sms);
+   apply(p, s, static_cast<char *>(workspace));
+   if (int r = launch(FORWARD, dtype, s, p, static_cast<cudaStream_t>(stream))) return r;
+   return finish_call(stream);
+}
+
+int fusedmm_b200_diff_attention_backward(int32_t dtype, int32_t ptr_bits, int32_t idx_bits, int64_t m, int64_t n, int64_t nnz,
+                                         const void *rowptr, const void *colidx, const float *bias, int32_t heads,
+                                         int32_t kv_heads, int32_t d, int32_t dv, const void *q, int64_t ldq, int64_t hsq,
+                                         const void *k, int64_t ldk, int64_t hsk, const void *v, int64_t ldv, int64_t hsv,
+                                         const float *lam, int64_t ldlam, double scale, const float *lse, const void *dout,
+                                         int64_t lddo, int64_t hsdo, const void *t_rowptr, const int32_t *t_row,
+                                         const int32_t *t_edge, void *dq, void *dk, void *dv_out, float *dlam, void *workspace,
+                                         int64_t workspace_bytes, void *stream)
+{
+   if ((ptr_bits != 32 && ptr_bits != 64) || (idx_bits != 32 && idx_bits != 64)) return FUSEDMM_B200_ERR_ARG;
+   if (int s = check_sizes(dtype, m, n, nnz, heads, kv_heads, d, dv)) return s;
+   if (m >= INT_MAX || n >= INT_MAX || nnz >= INT_MAX) return FUSEDMM_B200_ERR_LIMIT;
+   if (!dlam || (m > 0 && (!rowptr || !q || !lam || !lse || !dout || !dq)) || (n > 0 && (!k || !v || !dk || !dv_out || !t_rowptr)) ||
+       (nnz > 0 && (!colidx || !t_row || (bias && !t_edge))))
+      return FUSEDMM_B200_ERR_ARG;
+   const int64_t need = fusedmm_b200_diff_attention_workspace(1, dtype, m, n, nnz, heads, kv_heads, d, dv);
+   if (need < 0) return static_cast<int>(need);
+   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256) return FUSEDMM_B200_ERR_ARG;
+   if (!on_device({m > 0 ? rowptr : nullptr, m > 0 ? q : nullptr, m > 0 ? lam : nullptr, m > 0 ? lse : nullptr, m > 0 ? dout : nullptr,
+                   m > 0 ? dq : nullptr, n > 0 ? k : nullptr, n > 0 ? v : nullptr, n > 0 ? dk : nullptr, n > 0 ? dv_out : nullptr,
+                   n > 0 ? t_rowptr : nullptr, nnz > 0 ? colidx : nullptr, nnz > 0 ? t_row : nullptr,
+                   nnz > 0 ? bias : nullptr, nnz > 0 && bias ? t_edge : nullptr, m > 0 || ldlam == 0 ? dlam : nullptr, workspace}))
+      return FUSEDMM_B200_ERR_ARG;
+   int sms = 0;
+   if (int s = sm_count(&sms)) return s;
+   cudaStream_t st = static_cast<cudaStream_t>(stream);
+   char *ws = static_cast<char *>(workspace);
+   float *row_dlam = reinterpret_cast<float *>(ws + round256(m * heads * 16));
+   float *lam_part = reinterpret_cast<float *>(ws + round256(m * heads * 16) + round256(m * heads * 4));
+   char *scratch = ws + backward_front(m, heads);
+   Step step(dtype);
+   step.with(q, ldq, hsq, d);
+   step.with(k, ldk, hsk, d);
+   step.with(v, ldv, hsv, dv);
+   step.with(dout, lddo, hsdo, dv);
+   step.with(dq, 0, 0, d);
+   step.with(dk, 0, 0, d);
+   step.with(dv_out, 0, 0, dv);
+   AttnParams p = {};
+   p.bias = bias;
+   p.q = q; p.k = k; p.v = v; p.lam = lam; p.dout = dout;
+   p.ldq = ldq; p.hsq = hsq; p.ldk = ldk; p.hsk = hsk; p.ldv = ldv; p.hsv = hsv; p.ldo = lddo; p.hso = hsdo; p.ldlam = ldlam;
+   p.lse = const_cast<float *>(lse);
+   p.stats = reinterpret_cast<float2 *>(ws);
+   p.dlam = ldlam ? dlam : row_dlam;
+   p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads; p.d = d; p.dv = dv; p.step = step.step;
+   p.scale = static_cast<float>(scale);
+   p.nnz = nnz;
+   p.ptr64 = ptr_bits == 64;
+   if (m > 0) {
+      p.rowptr = rowptr; p.colidx = colidx; p.idx64 = idx_bits == 64; p.m = m; p.n = n; p.out = dq;
+      const Shape s = choose_shape(ROWS, dtype, step.vector(), m, p.nnz, heads, kv_heads, d, dv, sms);
+      apply(p, s, scratch);
+      if (int r = launch(ROWS, dtype, s, p, st)) return r;
+   }
+   if (!ldlam) {
+      if (m > 0) {
+         const long long each = (m + LAM_BLOCKS - 1) / LAM_BLOCKS;
+         lam_sum_kernel<<<LAM_BLOCKS, 256, 0, st>>>(row_dlam, m, heads, lam_part, each);
+         lam_sum_kernel<<<1, 256, 0, st>>>(lam_part, LAM_BLOCKS, heads, dlam, LAM_BLOCKS);
+      } else if (cudaMemsetAsync(dlam, 0, heads * sizeof(float), st) != cudaSuccess) {
+         return cuda_status();
+      }
+   }
+   if (n > 0) {
+      p.rowptr = t_rowptr; p.colidx = t_row; p.idx64 = 0; p.m = n; p.n = m; p.nnz = nnz; p.out = dk; p.out2 = dv_out; p.edge_of = t_edge;
+      const Shape s = choose_shape(COLUMNS, dtype, step.vector(), n, p.nnz, heads, kv_heads, d, dv, sms);
+      apply(p, s, scratch);
+      if (int r = launch(COLUMNS, dtype, s, p, st)) return r;
+   }
+   return finish_call(stream);
+}
+
+}  // extern "C"

@@ -481,6 +481,111 @@ const char *fusedmm_b200_version(void);
 /* Frees every device buffer the library holds (staging copies, hub-row scratch). */
 int fusedmm_b200_release(void);
 
+/* ------------------------------------------------------------------------------------------------
+ * Attention over the edges of a CSR, its gradient, and the step that makes its queries and keys.
+ *
+ * These entry points take device arrays only (of the current device), use no state of the library and allocate
+ * nothing: what they need beside their arguments is `workspace`, device memory of the caller's, aligned to 256
+ * bytes, of at least the bytes that the matching `_workspace` function returns (negative: a status).  It may be
+ * shared by calls that run one after the other, and by no two that may run at once.  `stream` is the cudaStream_t
+ * to enqueue on (cudaStreamLegacy, the value 1, for the legacy default stream); with NULL the call runs on the legacy
+ * default stream and returns when it is done.  They may be captured into a CUDA graph.  Inputs must not overlap outputs.
+ *
+ * dtype: 0 float, 2 bfloat16, 3 half; sums, softmax statistics and norms are held in float.  Strides count elements;
+ * the last axis of every array is dense.  Rows of any length, stride and alignment work; where address, strides and
+ * widths are multiples of 16 bytes the loads are 16 bytes wide.  Results are the same bits on every run.
+ * ---------------------------------------------------------------------------------------------- */
+#define FUSEDMM_B200_ATTN_MAX_WIDTH 256    /* d of qk_norm_rotary, 2 d and dv of diff_attention */
+#define FUSEDMM_B200_ATTN_MAX_HEADS 65536
+#define FUSEDMM_B200_ROTARY_MAX_AXES 4
+
+#define FUSEDMM_B200_POS_I32 0
+#define FUSEDMM_B200_POS_I64 1
+#define FUSEDMM_B200_POS_F32 2
+#define FUSEDMM_B200_POS_F64 3
+
+/*
+ * Norm of each head of the queries and keys, and rotation by the positions of their rows, in one pass:
+ *
+ *     y = x * rsqrt(mean(x^2) + eps) * w        (norm != 0; w NULL: all ones)
+ *     theta_i = sum_a pos[row][a] * freq[a][i], i < pairs
+ *     (y_lo, y_hi) -> (y_lo cos theta_i - y_hi sin theta_i, y_hi cos theta_i + y_lo sin theta_i)
+ *
+ * The pairs are the elements (i, i + pairs), or (2i, 2i + 1) with `interleaved`; elements from 2 pairs on are not
+ * turned.  A pair that belongs to one axis has freq 0 on the others.  q is [rows][hq][d] with the strides ldq (rows) and
+ * hsq (heads), k likewise; either may have no heads.  wq, wk have d elements of w_dtype (0, or dtype).  pos is
+ * [rows][axes] of pos_type with the strides ldp, asp; freq is [axes][pairs], dense.  Angles are formed in double.  With
+ * pairs 0 nothing is turned and pos, freq are not read.  q_out and k_out are dense.
+ */
+int fusedmm_b200_qk_norm_rotary(int32_t dtype, int64_t rows, int32_t hq, int32_t hk, int32_t d, const void *q, int64_t ldq,
+                                int64_t hsq, const void *k, int64_t ldk, int64_t hsk, int32_t w_dtype, const void *wq,
+                                const void *wk, int32_t norm, double eps, int32_t pos_type, const void *pos, int64_t ldp,
+                                int64_t asp, int32_t axes, const double *freq, int32_t pairs, int32_t interleaved,
+                                void *q_out, void *k_out, void *stream);
+
+/*
+ * Its gradient: dq, dk (dense) from the gradients dq_out, dk_out of its results (strides lddq, hsdq, lddk, hsdk), and
+ * dwq, dwk [d] in float (either may be NULL; both NULL: no workspace is needed).
+ */
+int64_t fusedmm_b200_qk_norm_rotary_backward_workspace(int64_t rows, int32_t d);
+int fusedmm_b200_qk_norm_rotary_backward(int32_t dtype, int64_t rows, int32_t hq, int32_t hk, int32_t d, const void *q,
+                                         int64_t ldq, int64_t hsq, const void *k, int64_t ldk, int64_t hsk, int32_t w_dtype,
+                                         const void *wq, const void *wk, int32_t norm, double eps, int32_t pos_type,
+                                         const void *pos, int64_t ldp, int64_t asp, int32_t axes, const double *freq,
+                                         int32_t pairs, int32_t interleaved, const void *dq_out, int64_t lddq, int64_t hsdq,
+                                         const void *dk_out, int64_t lddk, int64_t hsdk, void *dq, void *dk, float *dwq,
+                                         float *dwk, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Differential attention over the edges of a CSR.  For every row u < m, every head h and its kv head
+ * g = h / (heads / kv_heads), with e over the edges (u, v) of the row:
+ *
+ *     s^c_e = scale * q[u][h][c] . k[v][g][c] + bias[e]     (c = 0, 1)
+ *     p^c = softmax of s^c over the row's edges
+ *     out[u][h] = sum_e (p^0_e - lam[h] p^1_e) v[v][g]
+ *
+ * rowptr has m + 1 entries of ptr_bits (non-decreasing, within [0, nnz]; the edges of row u are rowptr[u] ..
+ * rowptr[u + 1] - 1), colidx nnz entries of idx_bits: rows of k and v, in any order and as often as they like (nodes of a
+ * graph, or the slots of a cache that a token attends to).  An edge whose id is outside [0, n), or whose bias is -inf, is
+ * no edge: its k and v are not read.  A row without edges gives out = 0 and lse = -inf.  bias (nnz floats) may be NULL.
+ * q is [m][heads][2][d] with the strides ldq, hsq; k is [n][kv_heads][2][d]; v is [n][kv_heads][dv]; lam is
+ * [m][heads] with the row stride ldlam, or [heads] with ldlam 0.  out [m][heads][dv] and lse [m][heads][2] (natural
+ * logarithms of the two maps' sums; may be NULL) are dense.  Long rows are cut, so that one row of many edges (a single
+ * token's) fills the GPU.
+ */
+int64_t fusedmm_b200_diff_attention_workspace(int32_t backward, int32_t dtype, int64_t m, int64_t n, int64_t nnz,
+                                              int32_t heads, int32_t kv_heads, int32_t d, int32_t dv);
+int fusedmm_b200_diff_attention(int32_t dtype, int32_t ptr_bits, int32_t idx_bits, int64_t m, int64_t n, int64_t nnz,
+                                const void *rowptr, const void *colidx, const float *bias, int32_t heads, int32_t kv_heads,
+                                int32_t d, int32_t dv, const void *q, int64_t ldq, int64_t hsq, const void *k, int64_t ldk,
+                                int64_t hsk, const void *v, int64_t ldv, int64_t hsv, const float *lam, int64_t ldlam,
+                                double scale, void *out, float *lse, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Its gradient.  lse is the forward call's, dout [m][heads][dv] has the strides lddo, hsdo; t_rowptr (ptr_bits), t_row
+ * and t_edge (needed with a bias) are the transposed pattern, from fusedmm_b200_csr_transpose.  Results, dense:
+ * dq [m][heads][2][d], dk [n][kv_heads][2][d], dv_out [n][kv_heads][dv] in dtype, and dlam in float: [m][heads], or
+ * [heads] (summed over the rows) with ldlam 0.  bias has no gradient.  m, n and nnz below 2^31 - 1.
+ */
+int fusedmm_b200_diff_attention_backward(int32_t dtype, int32_t ptr_bits, int32_t idx_bits, int64_t m, int64_t n, int64_t nnz,
+                                         const void *rowptr, const void *colidx, const float *bias, int32_t heads,
+                                         int32_t kv_heads, int32_t d, int32_t dv, const void *q, int64_t ldq, int64_t hsq,
+                                         const void *k, int64_t ldk, int64_t hsk, const void *v, int64_t ldv, int64_t hsv,
+                                         const float *lam, int64_t ldlam, double scale, const float *lse, const void *dout,
+                                         int64_t lddo, int64_t hsdo, const void *t_rowptr, const int32_t *t_row,
+                                         const int32_t *t_edge, void *dq, void *dk, void *dv_out, float *dlam, void *workspace,
+                                         int64_t workspace_bytes, void *stream);
+
+/*
+ * The transposed pattern: the edges of column c are t_rowptr[c] .. t_rowptr[c + 1] - 1 (t_rowptr has n + 1 entries of
+ * ptr_bits), t_row holds their rows and t_edge (may be NULL) their positions in colidx, in the order of the positions.
+ * Edges whose column is outside [0, n) are left out.  m, n and nnz below 2^31 - 1.
+ */
+int64_t fusedmm_b200_csr_transpose_workspace(int64_t m, int64_t n, int64_t nnz);
+int fusedmm_b200_csr_transpose(int32_t ptr_bits, int32_t idx_bits, int64_t m, int64_t n, int64_t nnz, const void *rowptr,
+                               const void *colidx, void *t_rowptr, int32_t *t_row, int32_t *t_edge, void *workspace,
+                               int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,139 @@
+"""Refusals of the attention operators, checked before anything reaches a GPU, and the shapes they announce to a compiler."""
+import ctypes as C
+
+import pytest
+import torch
+
+from fusedmm_b200 import api, torch_op
+
+I, L, P, D = C.c_int32, C.c_int64, C.c_void_p, C.c_double
+
+
+def attention_args(m=4, n=5, nnz=7, heads=4, kvh=2, d=8, dv=16, dtype=torch.float32):
+    return dict(rowptr=torch.tensor([0, nnz] + [nnz] * (m - 1), dtype=torch.int32), colidx=torch.zeros(nnz, dtype=torch.int32),
+                bias=None, q=torch.zeros(m, heads, 2, d, dtype=dtype), k=torch.zeros(n, kvh, 2, d, dtype=dtype),
+                v=torch.zeros(n, kvh, dv, dtype=dtype), lam=torch.zeros(heads), scale=1.0)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(q=torch.zeros(4, 4, 2, 8, dtype=torch.float64)), "float32, bfloat16 or float16"),
+    (dict(k=torch.zeros(5, 2, 2, 8, dtype=torch.bfloat16)), "share one type"),
+    (dict(q=torch.zeros(4, 4, 3, 8)), "heads, 2, d"),
+    (dict(q=torch.zeros(3, 4, 2, 8)), "rowptr"),
+    (dict(k=torch.zeros(5, 2, 2, 9)), "d of q"),
+    (dict(k=torch.zeros(5, 3, 2, 8), v=torch.zeros(5, 3, 16)), "multiple"),
+    (dict(v=torch.zeros(6, 2, 16)), "v must be"),
+    (dict(v=torch.zeros(5, 2, 300)), "dv between"),
+    (dict(q=torch.zeros(4, 4, 2, 129), k=torch.zeros(5, 2, 2, 129)), "d must be between"),
+    (dict(lam=torch.zeros(3)), "lam must be"),
+    (dict(lam=torch.zeros(4, dtype=torch.float64)), "lam must be float32"),
+    (dict(lam=torch.zeros(1, 4).expand(4, 4)), "lam must be"),
+    (dict(lam=torch.zeros(5, 4)), "lam must be"),
+    (dict(bias=torch.zeros(6)), "bias"),
+    (dict(bias=torch.zeros(7, dtype=torch.float64)), "bias"),
+    (dict(rowptr=torch.zeros(5)), "rowptr must be int32"),
+    (dict(colidx=torch.zeros(14, dtype=torch.int32)[::2]), "dense vector"),
+    (dict(q=torch.zeros(4, 4, 8, 2).transpose(2, 3)), "must be dense"),
+    (dict(), "CUDA tensor"),
+])
+def test_attention_refuses(change, text):
+    with pytest.raises(ValueError, match=text):
+        api._attention_args(**{**attention_args(), **change})
+
+
+def rotary_args(**change):
+    return {**dict(q=torch.zeros(6, 3, 16), k=torch.zeros(6, 1, 16), q_weight=None, k_weight=None, pos=torch.zeros(6, 2),
+                   freq=torch.zeros(2, 8, dtype=torch.float64), eps=1e-6, interleaved=False), **change}
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(q=torch.zeros(6, 3, 16, dtype=torch.float64)), "float32, bfloat16 or float16"),
+    (dict(q=torch.zeros(6, 48)), "rows, heads, d"),
+    (dict(k=torch.zeros(5, 1, 16)), "k must be"),
+    (dict(k=torch.zeros(6, 1, 16, dtype=torch.float16)), "share one type"),
+    (dict(q=torch.zeros(6, 3, 300), k=None), "between 1 and 256"),
+    (dict(pos=None), "come together"),
+    (dict(freq=None), "come together"),
+    (dict(freq=torch.zeros(2, 8)), "float64"),
+    (dict(freq=torch.zeros(3, 8, dtype=torch.float64)), "axes, pairs"),
+    (dict(freq=torch.zeros(2, 9, dtype=torch.float64)), "half of d"),
+    (dict(pos=torch.zeros(5, 2)), "pos must be"),
+    (dict(pos=torch.zeros(6, 5), freq=torch.zeros(5, 8, dtype=torch.float64)), "one to four"),
+    (dict(pos=torch.zeros(6, 2, dtype=torch.int16)), "pos must be"),
+    (dict(q_weight=torch.zeros(15)), "d entries"),
+    (dict(q_weight=torch.zeros(16), eps=None), "without eps"),
+    (dict(q_weight=torch.zeros(16, dtype=torch.bfloat16)), "type of q"),
+    (dict(k_weight=torch.zeros(16), k=None), "without k"),
+    (dict(eps=-1.0), "negative"),
+    (dict(q=torch.zeros(6, 16, 3).transpose(1, 2)), "must be dense"),
+    (dict(), "CUDA tensor"),
+])
+def test_rotary_refuses(change, text):
+    with pytest.raises(ValueError, match=text):
+        api._rotary_args(**rotary_args(**change))
+
+
+def test_c_entries_check_their_arguments_first():
+    """Statuses of calls that are wrong whatever the machine: -3 invalid argument, -4 beyond a limit."""
+    lib = api.lib()
+    ws = lib.fusedmm_b200_diff_attention_workspace
+    ws.restype, ws.argtypes = L, [I, I, L, L, L, I, I, I, I]
+    assert ws(0, 1, 4, 4, 8, 2, 1, 8, 8) == -3           # double
+    assert ws(0, 0, -1, 4, 8, 2, 1, 8, 8) == -3
+    assert ws(0, 0, 4, 4, 8, 3, 2, 8, 8) == -3           # heads no multiple of kv heads
+    assert ws(0, 0, 4, 4, 8, 2, 1, 129, 8) == -4
+    assert ws(0, 0, 4, 4, 8, 2, 1, 8, 257) == -4
+    fwd = lib.fusedmm_b200_diff_attention
+    fwd.restype, fwd.argtypes = I, list(api._ATTN_IN) + [P, P, P, L, P]
+    good = dict(dtype=0, pb=32, ib=32, m=4, n=4, nnz=8, rp=256, ci=256, bias=None, h=2, kvh=1, d=8, dv=8, q=256, ldq=32, hsq=16, k=256,
+                ldk=16, hsk=16, v=256, ldv=8, hsv=8, lam=256, ldlam=0, scale=1.0, out=256, lse=None, ws=256, wb=1 << 40, stream=None)
+    for change, status in ((dict(pb=16), -3), (dict(ib=8), -3), (dict(m=-1), -3), (dict(dtype=7), -3), (dict(h=0), -3),
+                           (dict(q=None), -3), (dict(k=None), -3), (dict(ci=None), -3), (dict(lam=None), -3), (dict(out=None), -3),
+                           (dict(d=200), -4), (dict(m=1 << 60), -4), (dict(m=0), 0)):
+        assert fwd(*{**good, **change}.values()) == status, change
+    back = lib.fusedmm_b200_diff_attention_backward
+    back.restype, back.argtypes = I, list(api._ATTN_IN) + [P, P, L, L, P, P, P, P, P, P, P, P, L, P]
+    good = dict(list(good.items())[:25], lse=256, do=256, ldo=16, hso=8, tp=256, tr=256, te=None, dq=256, dk=256, dvo=256, dlam=256, ws=256,
+                wb=1 << 40, stream=None)
+    for change, status in ((dict(m=(1 << 31) - 1), -4), (dict(lse=None), -3), (dict(do=None), -3), (dict(tp=None), -3), (dict(tr=None), -3),
+                           (dict(bias=256), -3), (dict(dlam=None), -3), (dict(dk=None), -3)):
+        assert back(*{**good, **change}.values()) == status, change
+    tr = lib.fusedmm_b200_csr_transpose
+    tr.restype, tr.argtypes = I, [I, I, L, L, L, P, P, P, P, P, P, L, P]
+    assert tr(32, 32, 4, 4, 1 << 31, 256, 256, 256, 256, 256, 256, 1 << 40, None) == -4
+    assert tr(32, 16, 4, 4, 8, 256, 256, 256, 256, 256, 256, 1 << 40, None) == -3
+    assert tr(32, 32, 4, 4, 8, 256, None, 256, 256, 256, 256, 1 << 40, None) == -3
+    assert tr(32, 32, 4, 4, 8, 256, 256, 256, 256, 256, 256, 8, None) == -3      # too little scratch
+    assert tr(32, 32, 4, 4, 8, 256, 256, 256, 256, 256, 260, 1 << 40, None) == -3  # not aligned
+    rot = lib.fusedmm_b200_qk_norm_rotary
+    rot.restype, rot.argtypes = I, list(api._ROTARY_IN) + [P, P, P]
+    good = dict(dtype=0, rows=4, hq=2, hk=1, d=8, q=256, ldq=16, hsq=8, k=256, ldk=8, hsk=8, wt=0, wq=None, wk=None, norm=1, eps=1e-6, pt=0,
+                pos=256, ldp=1, asp=1, axes=1, freq=256, pairs=4, il=0, qo=256, ko=256, stream=None)
+    for change, status in ((dict(dtype=1), -3), (dict(pairs=5), -3), (dict(axes=5), -3), (dict(axes=0), -3), (dict(pt=4), -3), (dict(d=257), -4),
+                           (dict(eps=float("nan")), -3), (dict(norm=0, wq=256), -3), (dict(wt=2), -3), (dict(q=None), -3), (dict(freq=None), -3),
+                           (dict(rows=0, q=None, k=None, pos=None, freq=None), 0)):
+        assert rot(*{**good, **change}.values()) == status, change
+
+
+def test_host_tensors_have_no_kernel():
+    a = attention_args()
+    with pytest.raises(NotImplementedError):
+        torch_op.diff_attention(a["rowptr"], a["colidx"], a["q"], a["k"], a["v"], a["lam"])
+    with pytest.raises(NotImplementedError):
+        torch_op.qk_norm_rotary(torch.zeros(2, 2, 8), eps=1e-6)
+
+
+def test_shapes_for_a_compiler():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        dev = "cuda"
+        q = torch.empty(6, 4, 2, 8, dtype=torch.bfloat16, device=dev)
+        k, v = torch.empty(9, 2, 2, 8, dtype=torch.bfloat16, device=dev), torch.empty(9, 2, 12, dtype=torch.bfloat16, device=dev)
+        rowptr, colidx = torch.empty(7, dtype=torch.int64, device=dev), torch.empty(30, dtype=torch.int32, device=dev)
+        lam = torch.empty(4, device=dev)
+        t = torch_op.csr_transpose(rowptr, colidx, 9)
+        assert [x.shape[0] for x in t] == [10, 30, 30] and t[0].dtype == torch.int64
+        out, lse = torch_op.diff_attention(rowptr, colidx, q, k, v, lam, transposed=t, return_lse=True)
+        assert out.shape == (6, 4, 12) and out.dtype == torch.bfloat16 and lse.shape == (6, 4, 2)
+        a, b = torch_op.qk_norm_rotary(torch.empty(6, 4, 8, device=dev), torch.empty(6, 2, 8, device=dev), eps=1e-6)
+        assert a.shape == (6, 4, 8) and b.shape == (6, 2, 8)
