@@ -83,6 +83,61 @@ struct Elt<__half> {
    }
 };
 
+// Two floats in one register pair: one instruction issues both of their multiply-adds (the walks below are bound by issue
+// slots, not by the multipliers: 16 pairs a clock and quarter of an SM either way).
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 f2(float a, float b)
+{
+   F2 r;
+   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+   return r;
+}
+__device__ __forceinline__ float2 f2_parts(F2 x)
+{
+   float2 r;
+   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+   return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c)
+{
+   F2 r;
+   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+   return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b)
+{
+   F2 r;
+   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+   return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b)
+{
+   F2 r;
+   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+   return r;
+}
+__device__ __forceinline__ float sum2(F2 x)
+{
+   const float2 p = f2_parts(x);
+   return p.x + p.y;
+}
+template <typename T>
+__device__ __forceinline__ void unpack_pairs(const uint4 &r, F2 (&f)[Elt<T>::W / 2])
+{
+   float t[Elt<T>::W];
+   Elt<T>::unpack(r, t);
+#pragma unroll
+   for (int i = 0; i < Elt<T>::W / 2; i++) f[i] = f2(t[2 * i], t[2 * i + 1]);
+}
+
+// 2^x; results below the smallest normal number are 0
+__device__ __forceinline__ float exp2_fast(float x)
+{
+   float r;
+   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+   return r;
+}
+
 __device__ __forceinline__ uint4 ldg16(const void *p) { return __ldg(static_cast<const uint4 *>(p)); }
 
 // `left` elements (any number, also <= 0) of the vector at p; what lies behind them reads as zero.  `step`: the elements

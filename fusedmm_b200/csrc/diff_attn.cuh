@@ -9,11 +9,11 @@
 // Three walks of the same shape: the forward and the dq pass go over the rows and gather k and v; the dk, dv pass goes over
 // the columns of the transposed pattern and gathers q and do.  No atomics: every sum is taken in a fixed order.
 //
-// The gathered rows decide the layout.  A slot of G lanes takes one head of one edge; its two halves hold the two maps'
-// parts of k (or q), so the two dots are one butterfly of G/2 lanes and each half owns the running maximum and sum of its
-// map; v (or do) lies over all G lanes.  The slots of a warp take neighbouring heads of the same edge, as far as there are
-// heads (their rows are adjacent in memory and all slots run in step), and alternate edges beyond that, joined at the row's
-// end.  QB query heads that share a kv head are computed together from one load.
+// The gathered rows decide the layout.  A slot of G lanes takes one head of one edge, NV vectors of 16 bytes to a lane; its
+// two halves hold the two maps' parts of k (or q), so the two dots are one butterfly of G/2 lanes and each half owns the
+// running maximum and sum of its map; v (or do) lies over all G lanes.  The slots of a warp take neighbouring heads of the
+// same edge, as far as there are heads (their rows are adjacent in memory and all slots run in step), and alternate edges
+// beyond that, joined at the row's end.  QB query heads that share a kv head are computed together from one load.
 //
 // Work is cut at equal parts ("pieces") of the items nnz + ROW_ITEMS * m, so that hub rows, single long rows of a decoding
 // step and empty rows are spread alike, without a pass over the pattern: a warp finds its first row by a 32-ary search in
@@ -29,15 +29,15 @@ namespace fmm {
 namespace attn {
 
 constexpr int ROW_ITEMS = 8;        // what a row costs beside its edges, in edges
-constexpr int PIECE_WARPS = 8;      // warps of a block
+constexpr int PIECE_WARPS = 4;      // warps of a block whose warps have pieces of their own
+constexpr int JOINT_WARPS = 8;      // warps of a block that share a row
 constexpr int JOIN_PIECES = 8;      // pieces a joining block looks after
 
 struct AttnParams {
    const void *rowptr, *colidx;  // row walks: the pattern; column walk: the transposed one (colidx: 32-bit row ids)
    int ptr64, idx64;
    long long m, n, nnz;          // rows walked, rows that can be gathered, length of colidx
-   const float *bias;
-   const int *edge_of;           // column walk: position of an edge in `bias`
+   const float *bias;            // column walk: in the order of the transposed pattern
    const void *q, *k, *v, *dout;
    const float *lam;
    long long ldq, hsq, ldk, hsk, ldv, hsv, ldo, hso, ldlam;
@@ -125,54 +125,114 @@ __device__ __forceinline__ float add_over(float v)
    return v;
 }
 
-// a vector of W floats of scratch, 16 bytes at a time
+// a vector of 2N floats of scratch, 16 bytes at a time
 template <int N>
-__device__ __forceinline__ void put_floats(float *p, const float (&f)[N])
+__device__ __forceinline__ void put_pairs(float *p, const F2 (&f)[N])
 {
 #pragma unroll
-   for (int i = 0; i < N; i += 4) *reinterpret_cast<float4 *>(p + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+   for (int i = 0; i < N; i += 2) *reinterpret_cast<ulonglong2 *>(p + 2 * i) = make_ulonglong2(f[i], f[i + 1]);
 }
 template <int N>
-__device__ __forceinline__ void get_floats(const float *p, float (&f)[N])
+__device__ __forceinline__ void get_pairs(const float *p, F2 (&f)[N])
 {
 #pragma unroll
-   for (int i = 0; i < N; i += 4) {
-      const float4 a = *reinterpret_cast<const float4 *>(p + i);
-      f[i] = a.x; f[i + 1] = a.y; f[i + 2] = a.z; f[i + 3] = a.w;
+   for (int i = 0; i < N; i += 2) {
+      const ulonglong2 a = *reinterpret_cast<const ulonglong2 *>(p + 2 * i);
+      f[i] = a.x;
+      f[i + 1] = a.y;
    }
 }
+__device__ __forceinline__ F2 shfl_xor_pair(F2 v, int x) { return __shfl_xor_sync(FULL, v, x); }
 
-// 32 edges of a row, one to a lane: the id to gather (-1: no edge here, or one that is masked) and its bias
-struct EdgeBatch {
-   long long id;
-   float bias;
-   __device__ __forceinline__ void load(const AttnParams &p, long long e, long long end)
+// 32 edges, one to a lane, fetched ahead: the ids of a row's next 32 edges, or of the next row's first, are under way while
+// the present ones are worked on (edges of neighbouring rows are neighbours).
+struct EdgeStream {
+   long long at = -1;
+   int low = 0, high = 0;  // as loaded: a use would wait for the load
+   float bias = 0.0f;
+   __device__ __forceinline__ void fetch(const AttnParams &p, long long from, int lane)
    {
-      id = -1;
-      bias = 0.0f;
-      if (e < end) {
-         id = load_index(p.colidx, p.idx64, e);
-         if (id < 0 || id >= p.n) id = -1;
-         if (p.bias) {
-            bias = __ldg(p.bias + (p.edge_of ? static_cast<long long>(__ldg(p.edge_of + e)) : e));
-            if (bias == -INFINITY) id = -1;
+      at = from;
+      const long long e = from + lane;
+      if (e < p.nnz) {
+         if (p.idx64) {
+            const int2 v = __ldg(static_cast<const int2 *>(p.colidx) + e);
+            low = v.x;
+            high = v.y;
+         } else {
+            low = __ldg(static_cast<const int *>(p.colidx) + e);
          }
+         if (p.bias) bias = __ldg(p.bias + e);
       }
    }
+   // the id to gather, -1 for an edge that is none: behind the end, outside [0, n), or masked
+   __device__ __forceinline__ int take(const AttnParams &p, long long from, long long end, int lane)
+   {
+      if (at != from) fetch(p, from, lane);
+      const bool inside = static_cast<unsigned>(low) < static_cast<unsigned>(p.n) && (!p.idx64 || high == 0);
+      return from + lane < end && inside && bias != -INFINITY ? low : -1;
+   }
 };
+
+// Rows of one gathered array as a slot's lanes hold them: vector t of a lane is `skip` elements behind vector t - 1.
+// EXACT: the lanes' vectors cover the row and nothing else; RAGGED: vectors, some lanes past the row's end; PIECES: rows
+// that are no vectors.  Edges that are none read zeros from `zero_row`, so that nothing of theirs is touched and no lane
+// needs a branch.
+enum Form { PIECES = 0, RAGGED = 1, EXACT = 2 };
+static __device__ __align__(16) uint4 zero_row[64];
+
+template <typename T, int NV, int FORM>
+struct Gather {
+   const char *base;
+   unsigned stride;  // bytes
+   int left;         // elements from the lane's first vector to the row's end
+   __device__ __forceinline__ Gather(const void *array, long long ld, long long offset, int x, int width)
+      : base(static_cast<const char *>(array) + (offset + x) * static_cast<long long>(sizeof(T))),
+        stride(static_cast<unsigned>(ld * static_cast<long long>(sizeof(T)))), left(width - x) {}
+   template <int SKIP>
+   __device__ __forceinline__ void load(int id, uint4 (&r)[NV], int step) const
+   {
+      const T *row = reinterpret_cast<const T *>(base + static_cast<unsigned long long>(static_cast<unsigned>(id)) * stride);
+      if (FORM == EXACT && id < 0) row = reinterpret_cast<const T *>(zero_row);
+#pragma unroll
+      for (int t = 0; t < NV; t++) {
+         if constexpr (FORM == EXACT) r[t] = ldg16(row + t * SKIP);
+         else r[t] = ld_row<T, FORM != PIECES>(row + t * SKIP, id >= 0 ? left - t * SKIP : 0, step);
+      }
+   }
+   // a row of the walk itself: it is there
+   template <int SKIP>
+   __device__ __forceinline__ void load_pairs(long long row, F2 (&f)[NV][Elt<T>::W / 2], int step) const
+   {
+      const T *src = reinterpret_cast<const T *>(base + row * static_cast<long long>(stride));
+#pragma unroll
+      for (int t = 0; t < NV; t++) unpack_pairs<T>(ld_row<T, FORM != PIECES>(src + t * SKIP, left - t * SKIP, step), f[t]);
+   }
+};
+
+template <int N>
+__device__ __forceinline__ void unpair(const F2 (&f)[N], float (&o)[2 * N])
+{
+#pragma unroll
+   for (int i = 0; i < N; i++) {
+      const float2 a = f2_parts(f[i]);
+      o[2 * i] = a.x;
+      o[2 * i + 1] = a.y;
+   }
+}
 
 // ---------------------------------------------------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int G, int NV, int QB, bool VECTOR>
+template <typename T, int G, int NV, int QB, int FORM>
 struct Forward {
-   static constexpr int W = Elt<T>::W, U = NV * QB > 2 ? 1 : 2;
+   static constexpr int W = Elt<T>::W, P = W / 2, U = 2;
+   static constexpr int KSKIP = (G / 2) * W, VSKIP = G * W;
    static constexpr int LANE_FLOATS = QB * (2 * NV * W + 2);  // partial state of a lane
    struct State {
-      float acc[QB][2][NV][W];  // sums of p v for the two maps
-      float top[QB], sum[QB];   // of this half's map
+      F2 acc[QB][2][NV][P];    // sums of p v for the two maps
+      float top[QB], sum[QB];  // of this half's map
    };
-   float q[QB][NV][W];
    State s;
 
    static __device__ __forceinline__ void clear(State &s)
@@ -186,62 +246,59 @@ struct Forward {
 #pragma unroll
             for (int t = 0; t < NV; t++)
 #pragma unroll
-               for (int j = 0; j < W; j++) s.acc[b][c][t][j] = 0.0f;
+               for (int j = 0; j < P; j++) s.acc[b][c][t][j] = 0;
       }
    }
 
-   __device__ __forceinline__ void run(const AttnParams &p, const Place &at, long long row, long long e0, long long e1, int warp, int warps)
+   __device__ __forceinline__ void run(const AttnParams &p, const Place &at, EdgeStream &edges, long long row, long long e0, long long e1,
+                                       int warp, int warps)
    {
       clear(s);
+      if (e0 + 32 * warp >= e1) return;
       const int kv = at.unit / (p.group / QB), head0 = at.unit * QB;
+      const int x = at.in_half * W, y = at.in_slot * W;
+      const Gather<T, NV, FORM> kg(p.k, p.ldk, kv * p.hsk + at.half * p.d, x, p.d), vg(p.v, p.ldv, kv * p.hsv, y, p.dv);
+      F2 q[QB][NV][P];
 #pragma unroll
       for (int b = 0; b < QB; b++)
-#pragma unroll
-         for (int t = 0; t < NV; t++) {
-            const int x = (at.in_half + (G / 2) * t) * W;
-            const T *src = static_cast<const T *>(p.q) + row * p.ldq + (head0 + b) * p.hsq + at.half * p.d + x;
-            Elt<T>::unpack(ld_row<T, VECTOR>(src, p.d - x, p.step), q[b][t]);
-         }
-      const T *kbase = static_cast<const T *>(p.k) + kv * p.hsk + at.half * p.d;
-      const T *vbase = static_cast<const T *>(p.v) + kv * p.hsv;
+         Gather<T, NV, FORM>(p.q, p.ldq, (head0 + b) * p.hsq + at.half * p.d, x, p.d).template load_pairs<KSKIP>(row, q[b], p.step);
       for (long long base = e0 + 32 * warp; base < e1; base += 32 * warps) {
-         EdgeBatch batch;
-         batch.load(p, base + at.lane, e1);
+         const int my_id = edges.take(p, base, e1, at.lane);
+         const float my_bias = edges.bias;
+         edges.fetch(p, base + 32 * warps < e1 ? base + 32 * warps : e1 + 32 * warp, at.lane);
          const int count = static_cast<int>(e1 - base < 32 ? e1 - base : 32);
          for (int first = 0; first < count; first += U * at.edge_slots) {
-            long long id[U];
-            float bias[U];
+            int id[U];
             uint4 kr[U][NV], vr[U][NV];
 #pragma unroll
             for (int i = 0; i < U; i++) {
-               const int from = first + i * at.edge_slots + at.edge_slot;
-               id[i] = __shfl_sync(FULL, batch.id, from);
-               bias[i] = __shfl_sync(FULL, batch.bias, from);
-               const bool live = id[i] >= 0;
-#pragma unroll
-               for (int t = 0; t < NV; t++) {
-                  const int x = (at.in_half + (G / 2) * t) * W, y = (at.in_slot + G * t) * W;
-                  kr[i][t] = ld_row<T, VECTOR>(kbase + id[i] * p.ldk + x, live ? p.d - x : 0, p.step);
-                  vr[i][t] = ld_row<T, VECTOR>(vbase + id[i] * p.ldv + y, live ? p.dv - y : 0, p.step);
-               }
+               id[i] = __shfl_sync(FULL, my_id, first + i * at.edge_slots + at.edge_slot);
+               kg.template load<KSKIP>(id[i], kr[i], p.step);
+               vg.template load<VSKIP>(id[i], vr[i], p.step);
             }
             float score[QB][U];
 #pragma unroll
             for (int i = 0; i < U; i++) {
-               float k[NV][W];
+               F2 k[NV][P];
 #pragma unroll
-               for (int t = 0; t < NV; t++) Elt<T>::unpack(kr[i][t], k[t]);
+               for (int t = 0; t < NV; t++) unpack_pairs<T>(kr[i][t], k[t]);
+               const float bias = p.bias ? __shfl_sync(FULL, my_bias, first + i * at.edge_slots + at.edge_slot) : 0.0f;
 #pragma unroll
                for (int b = 0; b < QB; b++) {
-                  float dot = 0.0f;
+                  F2 dot = 0;
 #pragma unroll
                   for (int t = 0; t < NV; t++)
 #pragma unroll
-                     for (int j = 0; j < W; j++) dot = fmaf(q[b][t][j], k[t][j], dot);
-                  dot = add_over<G / 2>(dot);
-                  score[b][i] = id[i] >= 0 ? fmaf(dot, p.scale, bias[i]) : -INFINITY;
+                     for (int j = 0; j < P; j++) dot = fma2(q[b][t][j], k[t][j], dot);
+                  const float all = add_over<G / 2>(sum2(dot));
+                  score[b][i] = id[i] >= 0 ? fmaf(all, p.scale, bias) : -INFINITY;
                }
             }
+            F2 v[U][NV][P];
+#pragma unroll
+            for (int i = 0; i < U; i++)
+#pragma unroll
+               for (int t = 0; t < NV; t++) unpack_pairs<T>(vr[i][t], v[i][t]);
 #pragma unroll
             for (int b = 0; b < QB; b++) {
                float top = s.top[b];
@@ -250,52 +307,51 @@ struct Forward {
                // a row that has met no edge yet has the maximum -inf: its differences are taken from 0
                const float ref = top == -INFINITY ? 0.0f : top;
                if (__any_sync(FULL, top != s.top[b])) {
-                  const float mine = exp2f((s.top[b] - ref) * LOG2E), other = __shfl_xor_sync(FULL, mine, G / 2);
+                  const float mine = exp2_fast((s.top[b] - ref) * LOG2E), other = __shfl_xor_sync(FULL, mine, G / 2);
                   const float c0 = at.half ? other : mine, c1 = at.half ? mine : other;
+                  const F2 f0 = f2(c0, c0), f1 = f2(c1, c1);
                   s.sum[b] *= mine;
 #pragma unroll
                   for (int t = 0; t < NV; t++)
 #pragma unroll
-                     for (int j = 0; j < W; j++) {
-                        s.acc[b][0][t][j] *= c0;
-                        s.acc[b][1][t][j] *= c1;
+                     for (int j = 0; j < P; j++) {
+                        s.acc[b][0][t][j] = mul2(s.acc[b][0][t][j], f0);
+                        s.acc[b][1][t][j] = mul2(s.acc[b][1][t][j], f1);
                      }
                   s.top[b] = top;
                }
 #pragma unroll
                for (int i = 0; i < U; i++) {
                   // the difference is taken before the factor: scores near the type's largest numbers keep their order
-                  const float mine = exp2f((score[b][i] - ref) * LOG2E), other = __shfl_xor_sync(FULL, mine, G / 2);
-                  const float p0 = at.half ? other : mine, p1 = at.half ? mine : other;
+                  const float mine = exp2_fast((score[b][i] - ref) * LOG2E), other = __shfl_xor_sync(FULL, mine, G / 2);
+                  const float w0 = at.half ? other : mine, w1 = at.half ? mine : other;
+                  const F2 p0 = f2(w0, w0), p1 = f2(w1, w1);
                   s.sum[b] += mine;
 #pragma unroll
-                  for (int t = 0; t < NV; t++) {
-                     float v[W];
-                     Elt<T>::unpack(vr[i][t], v);
+                  for (int t = 0; t < NV; t++)
 #pragma unroll
-                     for (int j = 0; j < W; j++) {
-                        s.acc[b][0][t][j] = fmaf(p0, v[j], s.acc[b][0][t][j]);
-                        s.acc[b][1][t][j] = fmaf(p1, v[j], s.acc[b][1][t][j]);
+                     for (int j = 0; j < P; j++) {
+                        s.acc[b][0][t][j] = fma2(p0, v[i][t][j], s.acc[b][0][t][j]);
+                        s.acc[b][1][t][j] = fma2(p1, v[i][t][j], s.acc[b][1][t][j]);
                      }
-                  }
                }
             }
          }
       }
-      for (int x = G * p.slot_heads; x < 32; x <<= 1) {  // the slots that took alternate edges
+      for (int x2 = G * p.slot_heads; x2 < 32; x2 <<= 1) {  // the slots that took alternate edges
          State o;
 #pragma unroll
          for (int b = 0; b < QB; b++) {
-            o.top[b] = __shfl_xor_sync(FULL, s.top[b], x);
-            o.sum[b] = __shfl_xor_sync(FULL, s.sum[b], x);
+            o.top[b] = __shfl_xor_sync(FULL, s.top[b], x2);
+            o.sum[b] = __shfl_xor_sync(FULL, s.sum[b], x2);
 #pragma unroll
             for (int c = 0; c < 2; c++)
 #pragma unroll
                for (int t = 0; t < NV; t++)
 #pragma unroll
-                  for (int j = 0; j < W; j++) o.acc[b][c][t][j] = __shfl_xor_sync(FULL, s.acc[b][c][t][j], x);
+                  for (int j = 0; j < P; j++) o.acc[b][c][t][j] = shfl_xor_pair(s.acc[b][c][t][j], x2);
          }
-         join(s, o, at, (at.lane & x) != 0);
+         join(s, o, at, (at.lane & x2) != 0);
       }
    }
 
@@ -306,21 +362,22 @@ struct Forward {
 #pragma unroll
       for (int b = 0; b < QB; b++) {
          const float top = fmaxf(s.top[b], o.top[b]), ref = top == -INFINITY ? 0.0f : top;
-         const float fs = exp2f((s.top[b] - ref) * LOG2E), fo = exp2f((o.top[b] - ref) * LOG2E);
-         const float fs2 = __shfl_xor_sync(FULL, fs, G / 2), fo2 = __shfl_xor_sync(FULL, fo, G / 2);
+         float fs = exp2_fast((s.top[b] - ref) * LOG2E), fo = exp2_fast((o.top[b] - ref) * LOG2E);
          // a NaN score leaves its trace in the sum and the accumulators, the maximum skips it
          const float a = s.sum[b] * fs, c = o.sum[b] * fo;
          s.sum[b] = swap ? c + a : a + c;
          s.top[b] = top;
+         const float fs2 = __shfl_xor_sync(FULL, fs, G / 2), fo2 = __shfl_xor_sync(FULL, fo, G / 2);
 #pragma unroll
          for (int m = 0; m < 2; m++) {
-            const float f1 = m == at.half ? fs : fs2, f2 = m == at.half ? fo : fo2;
+            const float g1 = m == at.half ? fs : fs2, g2 = m == at.half ? fo : fo2;
+            const F2 f1 = f2(g1, g1), f2_ = f2(g2, g2);
 #pragma unroll
             for (int t = 0; t < NV; t++)
 #pragma unroll
-               for (int j = 0; j < W; j++) {
-                  const float x = s.acc[b][m][t][j], y = o.acc[b][m][t][j];
-                  s.acc[b][m][t][j] = swap ? fmaf(y, f2, x * f1) : fmaf(x, f1, y * f2);
+               for (int j = 0; j < P; j++) {
+                  const F2 x = mul2(s.acc[b][m][t][j], f1), y = mul2(o.acc[b][m][t][j], f2_);
+                  s.acc[b][m][t][j] = add2(x, y);
                }
          }
       }
@@ -334,7 +391,7 @@ struct Forward {
 #pragma unroll
          for (int c = 0; c < 2; c++)
 #pragma unroll
-            for (int t = 0; t < NV; t++) get_floats<W>(from + ((b * 2 + c) * NV + t) * W * G, o.acc[b][c][t]);
+            for (int t = 0; t < NV; t++) get_pairs<P>(from + ((b * 2 + c) * NV + t) * W * G, o.acc[b][c][t]);
          const float2 ts = *reinterpret_cast<const float2 *>(unit + QB * 2 * NV * W * G + (b * G + at.in_slot) * 2);
          o.top[b] = ts.x;
          o.sum[b] = ts.y;
@@ -349,7 +406,7 @@ struct Forward {
 #pragma unroll
          for (int c = 0; c < 2; c++)
 #pragma unroll
-            for (int t = 0; t < NV; t++) put_floats<W>(to + ((b * 2 + c) * NV + t) * W * G, s.acc[b][c][t]);
+            for (int t = 0; t < NV; t++) put_pairs<P>(to + ((b * 2 + c) * NV + t) * W * G, s.acc[b][c][t]);
          *reinterpret_cast<float2 *>(unit + QB * 2 * NV * W * G + (b * G + at.in_slot) * 2) = make_float2(s.top[b], s.sum[b]);
       }
    }
@@ -367,10 +424,12 @@ struct Forward {
 #pragma unroll
          for (int t = 0; t < NV; t++) {
             const int y = (at.in_slot + G * t) * W;
-            float o[W];
+            float a[W], c[W];
+            unpair(s.acc[b][0][t], a);
+            unpair(s.acc[b][1][t], c);
 #pragma unroll
-            for (int j = 0; j < W; j++) o[j] = s.acc[b][0][t][j] * f0 - s.acc[b][1][t][j] * f1;
-            st_row<T, VECTOR>(static_cast<T *>(p.out) + (row * p.heads + head) * p.dv + y, o, p.dv - y);
+            for (int j = 0; j < W; j++) a[j] = a[j] * f0 - c[j] * f1;
+            st_row<T, FORM != PIECES>(static_cast<T *>(p.out) + (row * p.heads + head) * p.dv + y, a, p.dv - y);
          }
          if (at.in_half == 0 && p.lse) p.lse[(row * p.heads + head) * 2 + at.half] = s.top[b] + LN2 * log2f(s.sum[b]);
       }
@@ -381,15 +440,15 @@ struct Forward {
 // backward over the rows: dq, dlam and the numbers the columns need.  With D^c unknown until the row's end, the sums
 // A = sum p dP k, B = sum p k and D = sum p dP are taken together; dq = scale (A - D B).
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int G, int NV, int QB, bool VECTOR>
+template <typename T, int G, int NV, int QB, int FORM>
 struct BackwardRows {
-   static constexpr int W = Elt<T>::W, U = NV * QB > 2 ? 1 : 2;
+   static constexpr int W = Elt<T>::W, P = W / 2, U = 2;
+   static constexpr int KSKIP = (G / 2) * W, VSKIP = G * W;
    static constexpr int LANE_FLOATS = QB * (2 * NV * W + 2);
    struct State {
-      float a[QB][NV][W], b[QB][NV][W];  // of this half's map
+      F2 a[QB][NV][P], b[QB][NV][P];  // of this half's map
       float delta[QB];
    };
-   float q[QB][NV][W], dout[QB][NV][W], lse[QB];
    State s;
 
    static __device__ __forceinline__ void clear(State &s)
@@ -400,94 +459,86 @@ struct BackwardRows {
 #pragma unroll
          for (int t = 0; t < NV; t++)
 #pragma unroll
-            for (int j = 0; j < W; j++) s.a[b][t][j] = s.b[b][t][j] = 0.0f;
+            for (int j = 0; j < P; j++) s.a[b][t][j] = s.b[b][t][j] = 0;
       }
    }
 
-   __device__ __forceinline__ void run(const AttnParams &p, const Place &at, long long row, long long e0, long long e1, int warp, int warps)
+   __device__ __forceinline__ void run(const AttnParams &p, const Place &at, EdgeStream &edges, long long row, long long e0, long long e1,
+                                       int warp, int warps)
    {
       clear(s);
+      if (e0 + 32 * warp >= e1) return;
       const int kv = at.unit / (p.group / QB), head0 = at.unit * QB;
+      const int x = at.in_half * W, y = at.in_slot * W;
+      const Gather<T, NV, FORM> kg(p.k, p.ldk, kv * p.hsk + at.half * p.d, x, p.d), vg(p.v, p.ldv, kv * p.hsv, y, p.dv);
+      F2 q[QB][NV][P], dout[QB][NV][P];
+      float lse[QB];
 #pragma unroll
       for (int b = 0; b < QB; b++) {
          lse[b] = __ldg(p.lse + (row * p.heads + head0 + b) * 2 + at.half);
-#pragma unroll
-         for (int t = 0; t < NV; t++) {
-            const int x = (at.in_half + (G / 2) * t) * W, y = (at.in_slot + G * t) * W;
-            const T *src = static_cast<const T *>(p.q) + row * p.ldq + (head0 + b) * p.hsq + at.half * p.d + x;
-            Elt<T>::unpack(ld_row<T, VECTOR>(src, p.d - x, p.step), q[b][t]);
-            const T *dsrc = static_cast<const T *>(p.dout) + row * p.ldo + (head0 + b) * p.hso + y;
-            Elt<T>::unpack(ld_row<T, VECTOR>(dsrc, p.dv - y, p.step), dout[b][t]);
-         }
+         Gather<T, NV, FORM>(p.q, p.ldq, (head0 + b) * p.hsq + at.half * p.d, x, p.d).template load_pairs<KSKIP>(row, q[b], p.step);
+         Gather<T, NV, FORM>(p.dout, p.ldo, (head0 + b) * p.hso, y, p.dv).template load_pairs<VSKIP>(row, dout[b], p.step);
       }
-      const T *kbase = static_cast<const T *>(p.k) + kv * p.hsk + at.half * p.d;
-      const T *vbase = static_cast<const T *>(p.v) + kv * p.hsv;
       for (long long base = e0 + 32 * warp; base < e1; base += 32 * warps) {
-         EdgeBatch batch;
-         batch.load(p, base + at.lane, e1);
+         const int my_id = edges.take(p, base, e1, at.lane);
+         const float my_bias = edges.bias;
+         edges.fetch(p, base + 32 * warps < e1 ? base + 32 * warps : e1 + 32 * warp, at.lane);
          const int count = static_cast<int>(e1 - base < 32 ? e1 - base : 32);
          for (int first = 0; first < count; first += U * at.edge_slots) {
-            long long id[U];
-            float bias[U];
+            int id[U];
             uint4 kr[U][NV], vr[U][NV];
 #pragma unroll
             for (int i = 0; i < U; i++) {
-               const int from = first + i * at.edge_slots + at.edge_slot;
-               id[i] = __shfl_sync(FULL, batch.id, from);
-               bias[i] = __shfl_sync(FULL, batch.bias, from);
-               const bool live = id[i] >= 0;
-#pragma unroll
-               for (int t = 0; t < NV; t++) {
-                  const int x = (at.in_half + (G / 2) * t) * W, y = (at.in_slot + G * t) * W;
-                  kr[i][t] = ld_row<T, VECTOR>(kbase + id[i] * p.ldk + x, live ? p.d - x : 0, p.step);
-                  vr[i][t] = ld_row<T, VECTOR>(vbase + id[i] * p.ldv + y, live ? p.dv - y : 0, p.step);
-               }
+               id[i] = __shfl_sync(FULL, my_id, first + i * at.edge_slots + at.edge_slot);
+               kg.template load<KSKIP>(id[i], kr[i], p.step);
+               vg.template load<VSKIP>(id[i], vr[i], p.step);
             }
 #pragma unroll
             for (int i = 0; i < U; i++) {
-               float k[NV][W], v[NV][W];
+               F2 k[NV][P], v[NV][P];
 #pragma unroll
                for (int t = 0; t < NV; t++) {
-                  Elt<T>::unpack(kr[i][t], k[t]);
-                  Elt<T>::unpack(vr[i][t], v[t]);
+                  unpack_pairs<T>(kr[i][t], k[t]);
+                  unpack_pairs<T>(vr[i][t], v[t]);
                }
+               const float bias = p.bias ? __shfl_sync(FULL, my_bias, first + i * at.edge_slots + at.edge_slot) : 0.0f;
 #pragma unroll
                for (int b = 0; b < QB; b++) {
-                  float dot = 0.0f, dp = 0.0f;
+                  F2 dots = 0, dps = 0;
 #pragma unroll
                   for (int t = 0; t < NV; t++)
 #pragma unroll
-                     for (int j = 0; j < W; j++) {
-                        dot = fmaf(q[b][t][j], k[t][j], dot);
-                        dp = fmaf(dout[b][t][j], v[t][j], dp);
+                     for (int j = 0; j < P; j++) {
+                        dots = fma2(q[b][t][j], k[t][j], dots);
+                        dps = fma2(dout[b][t][j], v[t][j], dps);
                      }
-                  dot = add_over<G / 2>(dot);
-                  dp = add_over<G>(dp);
+                  const float dot = add_over<G / 2>(sum2(dots)), dp = add_over<G>(sum2(dps));
                   // an edge that is masked has p = 0, and so has a row without edges (its lse is -inf)
-                  const float pr = id[i] >= 0 && lse[b] != -INFINITY ? exp2f((fmaf(dot, p.scale, bias[i]) - lse[b]) * LOG2E) : 0.0f;
+                  const float pr = id[i] >= 0 && lse[b] != -INFINITY ? exp2_fast((fmaf(dot, p.scale, bias) - lse[b]) * LOG2E) : 0.0f;
                   const float w = pr * dp;
+                  const F2 ww = f2(w, w), pp = f2(pr, pr);
                   s.delta[b] += w;
 #pragma unroll
                   for (int t = 0; t < NV; t++)
 #pragma unroll
-                     for (int j = 0; j < W; j++) {
-                        s.a[b][t][j] = fmaf(w, k[t][j], s.a[b][t][j]);
-                        s.b[b][t][j] = fmaf(pr, k[t][j], s.b[b][t][j]);
+                     for (int j = 0; j < P; j++) {
+                        s.a[b][t][j] = fma2(ww, k[t][j], s.a[b][t][j]);
+                        s.b[b][t][j] = fma2(pp, k[t][j], s.b[b][t][j]);
                      }
                }
             }
          }
       }
-      for (int x = G * p.slot_heads; x < 32; x <<= 1) {
+      for (int x2 = G * p.slot_heads; x2 < 32; x2 <<= 1) {
 #pragma unroll
          for (int b = 0; b < QB; b++) {
-            s.delta[b] += __shfl_xor_sync(FULL, s.delta[b], x);
+            s.delta[b] += __shfl_xor_sync(FULL, s.delta[b], x2);
 #pragma unroll
             for (int t = 0; t < NV; t++)
 #pragma unroll
-               for (int j = 0; j < W; j++) {
-                  s.a[b][t][j] += __shfl_xor_sync(FULL, s.a[b][t][j], x);
-                  s.b[b][t][j] += __shfl_xor_sync(FULL, s.b[b][t][j], x);
+               for (int j = 0; j < P; j++) {
+                  s.a[b][t][j] = add2(s.a[b][t][j], shfl_xor_pair(s.a[b][t][j], x2));
+                  s.b[b][t][j] = add2(s.b[b][t][j], shfl_xor_pair(s.b[b][t][j], x2));
                }
          }
       }
@@ -499,13 +550,13 @@ struct BackwardRows {
       for (int b = 0; b < QB; b++) {
 #pragma unroll
          for (int t = 0; t < NV; t++) {
-            float x[W];
-            get_floats<W>(from + (b * 2 * NV + t) * W * G, x);
+            F2 x[P];
+            get_pairs<P>(from + (b * 2 * NV + t) * W * G, x);
 #pragma unroll
-            for (int j = 0; j < W; j++) s.a[b][t][j] += x[j];
-            get_floats<W>(from + ((b * 2 + 1) * NV + t) * W * G, x);
+            for (int j = 0; j < P; j++) s.a[b][t][j] = add2(s.a[b][t][j], x[j]);
+            get_pairs<P>(from + ((b * 2 + 1) * NV + t) * W * G, x);
 #pragma unroll
-            for (int j = 0; j < W; j++) s.b[b][t][j] += x[j];
+            for (int j = 0; j < P; j++) s.b[b][t][j] = add2(s.b[b][t][j], x[j]);
          }
          s.delta[b] += unit[QB * 2 * NV * W * G + (b * G + at.in_slot) * 2];
       }
@@ -517,8 +568,8 @@ struct BackwardRows {
       for (int b = 0; b < QB; b++) {
 #pragma unroll
          for (int t = 0; t < NV; t++) {
-            put_floats<W>(to + (b * 2 * NV + t) * W * G, s.a[b][t]);
-            put_floats<W>(to + ((b * 2 + 1) * NV + t) * W * G, s.b[b][t]);
+            put_pairs<P>(to + (b * 2 * NV + t) * W * G, s.a[b][t]);
+            put_pairs<P>(to + ((b * 2 + 1) * NV + t) * W * G, s.b[b][t]);
          }
          unit[QB * 2 * NV * W * G + (b * G + at.in_slot) * 2] = s.delta[b];
       }
@@ -535,10 +586,12 @@ struct BackwardRows {
 #pragma unroll
          for (int t = 0; t < NV; t++) {
             const int x = (at.in_half + (G / 2) * t) * W;
-            float o[W];
+            float a[W], c[W];
+            unpair(s.a[b][t], a);
+            unpair(s.b[b][t], c);
 #pragma unroll
-            for (int j = 0; j < W; j++) o[j] = factor * fmaf(-s.delta[b], s.b[b][t][j], s.a[b][t][j]);
-            st_row<T, VECTOR>(static_cast<T *>(p.out) + (rh * 2 + at.half) * p.d + x, o, p.d - x);
+            for (int j = 0; j < W; j++) a[j] = factor * fmaf(-s.delta[b], c[j], a[j]);
+            st_row<T, FORM != PIECES>(static_cast<T *>(p.out) + (rh * 2 + at.half) * p.d + x, a, p.d - x);
          }
          if (at.in_half == 0) {
             p.stats[rh * 2 + at.half] = make_float2(__ldg(p.lse + rh * 2 + at.half), s.delta[b]);
@@ -551,14 +604,14 @@ struct BackwardRows {
 // ---------------------------------------------------------------------------------------------------------------------
 // backward over the columns: dk and dv.  A unit is a kv head; every edge counts once for each query head of its group.
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int G, int NV, int QB, bool VECTOR>
+template <typename T, int G, int NV, int QB, int FORM>
 struct BackwardColumns {
-   static constexpr int W = Elt<T>::W, U = NV > 1 ? 1 : 2;
+   static constexpr int W = Elt<T>::W, P = W / 2, U = 2;
+   static constexpr int KSKIP = (G / 2) * W, VSKIP = G * W;
    static constexpr int LANE_FLOATS = 2 * NV * W;
    struct State {
-      float dk[NV][W], dv[NV][W];
+      F2 dk[NV][P], dv[NV][P];
    };
-   float k[NV][W], v[NV][W];
    State s;
 
    static __device__ __forceinline__ void clear(State &s)
@@ -566,93 +619,87 @@ struct BackwardColumns {
 #pragma unroll
       for (int t = 0; t < NV; t++)
 #pragma unroll
-         for (int j = 0; j < W; j++) s.dk[t][j] = s.dv[t][j] = 0.0f;
+         for (int j = 0; j < P; j++) s.dk[t][j] = s.dv[t][j] = 0;
    }
 
-   __device__ __forceinline__ void run(const AttnParams &p, const Place &at, long long col, long long e0, long long e1, int warp, int warps)
+   __device__ __forceinline__ void run(const AttnParams &p, const Place &at, EdgeStream &edges, long long col, long long e0, long long e1,
+                                       int warp, int warps)
    {
       clear(s);
+      if (e0 + 32 * warp >= e1) return;
       const int kv = at.unit;
-#pragma unroll
-      for (int t = 0; t < NV; t++) {
-         const int x = (at.in_half + (G / 2) * t) * W, y = (at.in_slot + G * t) * W;
-         Elt<T>::unpack(ld_row<T, VECTOR>(static_cast<const T *>(p.k) + col * p.ldk + kv * p.hsk + at.half * p.d + x, p.d - x, p.step), k[t]);
-         Elt<T>::unpack(ld_row<T, VECTOR>(static_cast<const T *>(p.v) + col * p.ldv + kv * p.hsv + y, p.dv - y, p.step), v[t]);
-      }
+      const int x = at.in_half * W, y = at.in_slot * W;
+      F2 k[NV][P], v[NV][P];
+      Gather<T, NV, FORM>(p.k, p.ldk, kv * p.hsk + at.half * p.d, x, p.d).template load_pairs<KSKIP>(col, k, p.step);
+      Gather<T, NV, FORM>(p.v, p.ldv, kv * p.hsv, y, p.dv).template load_pairs<VSKIP>(col, v, p.step);
       for (long long base = e0 + 32 * warp; base < e1; base += 32 * warps) {
-         EdgeBatch batch;
-         batch.load(p, base + at.lane, e1);
+         const int my_id = edges.take(p, base, e1, at.lane);
+         const float my_bias = edges.bias;
+         edges.fetch(p, base + 32 * warps < e1 ? base + 32 * warps : e1 + 32 * warp, at.lane);
          const int count = static_cast<int>(e1 - base < 32 ? e1 - base : 32);
          for (int first = 0; first < count; first += U * at.edge_slots) {
-            long long id[U];
+            int id[U];
             float bias[U];
 #pragma unroll
             for (int i = 0; i < U; i++) {
-               const int from = first + i * at.edge_slots + at.edge_slot;
-               id[i] = __shfl_sync(FULL, batch.id, from);
-               bias[i] = __shfl_sync(FULL, batch.bias, from);
+               id[i] = __shfl_sync(FULL, my_id, first + i * at.edge_slots + at.edge_slot);
+               bias[i] = p.bias ? __shfl_sync(FULL, my_bias, first + i * at.edge_slots + at.edge_slot) : 0.0f;
             }
             for (int g = 0; g < p.group; g++) {
                const int head = kv * p.group + g;
+               const Gather<T, NV, FORM> qg(p.q, p.ldq, head * p.hsq + at.half * p.d, x, p.d), dg(p.dout, p.ldo, head * p.hso, y, p.dv);
                uint4 qr[U][NV], dr[U][NV];
                float2 stat[U];
                float lam[U];
 #pragma unroll
                for (int i = 0; i < U; i++) {
-                  const bool live = id[i] >= 0;
-                  stat[i] = make_float2(0.0f, 0.0f);
+                  stat[i] = make_float2(-INFINITY, 0.0f);
                   lam[i] = 0.0f;
-                  if (live) {
-                     stat[i] = __ldg(p.stats + (id[i] * p.heads + head) * 2 + at.half);
+                  if (id[i] >= 0) {
+                     stat[i] = __ldg(p.stats + (static_cast<long long>(id[i]) * p.heads + head) * 2 + at.half);
                      lam[i] = __ldg(p.lam + id[i] * p.ldlam + head);
                   }
-#pragma unroll
-                  for (int t = 0; t < NV; t++) {
-                     const int x = (at.in_half + (G / 2) * t) * W, y = (at.in_slot + G * t) * W;
-                     qr[i][t] = ld_row<T, VECTOR>(static_cast<const T *>(p.q) + id[i] * p.ldq + head * p.hsq + at.half * p.d + x,
-                                                  live ? p.d - x : 0, p.step);
-                     dr[i][t] = ld_row<T, VECTOR>(static_cast<const T *>(p.dout) + id[i] * p.ldo + head * p.hso + y,
-                                                  live ? p.dv - y : 0, p.step);
-                  }
+                  qg.template load<KSKIP>(id[i], qr[i], p.step);
+                  dg.template load<VSKIP>(id[i], dr[i], p.step);
                }
 #pragma unroll
                for (int i = 0; i < U; i++) {
-                  float q[NV][W], dout[NV][W], dot = 0.0f, dp = 0.0f;
+                  F2 q[NV][P], dout[NV][P], dots = 0, dps = 0;
 #pragma unroll
                   for (int t = 0; t < NV; t++) {
-                     Elt<T>::unpack(qr[i][t], q[t]);
-                     Elt<T>::unpack(dr[i][t], dout[t]);
+                     unpack_pairs<T>(qr[i][t], q[t]);
+                     unpack_pairs<T>(dr[i][t], dout[t]);
 #pragma unroll
-                     for (int j = 0; j < W; j++) {
-                        dot = fmaf(q[t][j], k[t][j], dot);
-                        dp = fmaf(dout[t][j], v[t][j], dp);
+                     for (int j = 0; j < P; j++) {
+                        dots = fma2(q[t][j], k[t][j], dots);
+                        dps = fma2(dout[t][j], v[t][j], dps);
                      }
                   }
-                  dot = add_over<G / 2>(dot);
-                  dp = add_over<G>(dp);
-                  const bool live = id[i] >= 0 && stat[i].x != -INFINITY;
-                  const float pr = live ? exp2f((fmaf(dot, p.scale, bias[i]) - stat[i].x) * LOG2E) : 0.0f;
+                  const float dot = add_over<G / 2>(sum2(dots)), dp = add_over<G>(sum2(dps));
+                  const bool live = stat[i].x != -INFINITY;  // an edge, and of a row that has any
+                  const float pr = live ? exp2_fast((fmaf(dot, p.scale, bias[i]) - stat[i].x) * LOG2E) : 0.0f;
                   const float mine = live ? (at.half ? -lam[i] : 1.0f) * pr : 0.0f;  // this map's part of the weight
                   const float w = mine + __shfl_xor_sync(FULL, mine, G / 2);
                   const float ds = live ? mine * (dp - stat[i].y) : 0.0f;
+                  const F2 ww = f2(w, w), dd = f2(ds, ds);
 #pragma unroll
                   for (int t = 0; t < NV; t++)
 #pragma unroll
-                     for (int j = 0; j < W; j++) {
-                        s.dk[t][j] = fmaf(ds, q[t][j], s.dk[t][j]);
-                        s.dv[t][j] = fmaf(w, dout[t][j], s.dv[t][j]);
+                     for (int j = 0; j < P; j++) {
+                        s.dk[t][j] = fma2(dd, q[t][j], s.dk[t][j]);
+                        s.dv[t][j] = fma2(ww, dout[t][j], s.dv[t][j]);
                      }
                }
             }
          }
       }
-      for (int x = G * p.slot_heads; x < 32; x <<= 1) {
+      for (int x2 = G * p.slot_heads; x2 < 32; x2 <<= 1) {
 #pragma unroll
          for (int t = 0; t < NV; t++)
 #pragma unroll
-            for (int j = 0; j < W; j++) {
-               s.dk[t][j] += __shfl_xor_sync(FULL, s.dk[t][j], x);
-               s.dv[t][j] += __shfl_xor_sync(FULL, s.dv[t][j], x);
+            for (int j = 0; j < P; j++) {
+               s.dk[t][j] = add2(s.dk[t][j], shfl_xor_pair(s.dk[t][j], x2));
+               s.dv[t][j] = add2(s.dv[t][j], shfl_xor_pair(s.dv[t][j], x2));
             }
       }
    }
@@ -661,13 +708,13 @@ struct BackwardColumns {
       const float *from = unit + at.in_slot * W;
 #pragma unroll
       for (int t = 0; t < NV; t++) {
-         float x[W];
-         get_floats<W>(from + t * W * G, x);
+         F2 x[P];
+         get_pairs<P>(from + t * W * G, x);
 #pragma unroll
-         for (int j = 0; j < W; j++) s.dk[t][j] += x[j];
-         get_floats<W>(from + (NV + t) * W * G, x);
+         for (int j = 0; j < P; j++) s.dk[t][j] = add2(s.dk[t][j], x[j]);
+         get_pairs<P>(from + (NV + t) * W * G, x);
 #pragma unroll
-         for (int j = 0; j < W; j++) s.dv[t][j] += x[j];
+         for (int j = 0; j < P; j++) s.dv[t][j] = add2(s.dv[t][j], x[j]);
       }
    }
    __device__ __forceinline__ void put(float *unit, const Place &at) const
@@ -675,8 +722,8 @@ struct BackwardColumns {
       float *to = unit + at.in_slot * W;
 #pragma unroll
       for (int t = 0; t < NV; t++) {
-         put_floats<W>(to + t * W * G, s.dk[t]);
-         put_floats<W>(to + (NV + t) * W * G, s.dv[t]);
+         put_pairs<P>(to + t * W * G, s.dk[t]);
+         put_pairs<P>(to + (NV + t) * W * G, s.dv[t]);
       }
    }
 
@@ -687,11 +734,13 @@ struct BackwardColumns {
 #pragma unroll
       for (int t = 0; t < NV; t++) {
          const int x = (at.in_half + (G / 2) * t) * W, y = (at.in_slot + G * t) * W;
-         float o[W];
+         float o[W], v[W];
+         unpair(s.dk[t], o);
+         unpair(s.dv[t], v);
 #pragma unroll
-         for (int j = 0; j < W; j++) o[j] = s.dk[t][j] * p.scale;
-         st_row<T, VECTOR>(static_cast<T *>(p.out) + (rh * 2 + at.half) * p.d + x, o, p.d - x);
-         st_row<T, VECTOR>(static_cast<T *>(p.out2) + rh * p.dv + y, s.dv[t], p.dv - y);
+         for (int j = 0; j < W; j++) o[j] *= p.scale;
+         st_row<T, FORM != PIECES>(static_cast<T *>(p.out) + (rh * 2 + at.half) * p.d + x, o, p.d - x);
+         st_row<T, FORM != PIECES>(static_cast<T *>(p.out2) + rh * p.dv + y, v, p.dv - y);
       }
    }
 };
@@ -719,12 +768,12 @@ __device__ __forceinline__ void join_warps(Op &op, const Place &at, float *share
    if (at.warp > 0) op.put(mine + (at.warp - 1) * STRIDE, at);
    __syncthreads();
    if (at.warp == 0)
-      for (int w = 1; w < PIECE_WARPS; w++) op.join_from(mine + (w - 1) * STRIDE, at);
+      for (int w = 1; w < JOINT_WARPS; w++) op.join_from(mine + (w - 1) * STRIDE, at);
 }
 
 // TOGETHER: the warps of a block share every row (few, long rows), else each warp has a piece of its own.
 template <typename Op, int G, bool TOGETHER>
-__global__ void __launch_bounds__(PIECE_WARPS * 32) walk_kernel(const AttnParams p)
+__global__ void __launch_bounds__((TOGETHER ? JOINT_WARPS : PIECE_WARPS) * 32) walk_kernel(const AttnParams p)
 {
    extern __shared__ __align__(16) float shared[];
    const int warp = threadIdx.x >> 5;
@@ -736,23 +785,33 @@ __global__ void __launch_bounds__(PIECE_WARPS * 32) walk_kernel(const AttnParams
    const long long lo = piece * p.piece, hi = lo + p.piece;
    long long u = rows.lower_bound(lo, at.lane);
    const bool teller = at.lane == 0 && (!TOGETHER || warp == 0) && job == piece * p.unit_blocks;
+   const int share = TOGETHER ? warp : 0, shares = TOGETHER ? JOINT_WARPS : 1;
    long long begun = -1;
    Op op;
+   EdgeStream edges;
+   // row pointers 32 at a time, one to a lane
+   long long from = u > 0 ? u - 1 : 0;
+   long long mine = rows.begin(from + at.lane < p.m ? from + at.lane : p.m);
    if (u > 0) {  // the row before may reach into this piece
-      const long long b = rows.begin(u - 1), e = rows.begin(u), fb = b - rows.first + ROW_ITEMS * (u - 1), fe = e - rows.first + ROW_ITEMS * u;
+      const long long b = __shfl_sync(FULL, mine, 0), e = __shfl_sync(FULL, mine, 1);
+      const long long fb = b - rows.first + ROW_ITEMS * (u - 1), fe = e - rows.first + ROW_ITEMS * u;
       if (fe > lo && fe - fb > p.row_limit) {
          long long e0 = b + (lo - fb - ROW_ITEMS), e1 = b + (hi - fb - ROW_ITEMS);
          e0 = e0 < b ? b : e0;
          e1 = e1 > e ? e : e1 < e0 ? e0 : e1;
-         op.run(p, at, u - 1, e0, e1, TOGETHER ? warp : 0, TOGETHER ? PIECE_WARPS : 1);
+         op.run(p, at, edges, u - 1, e0, e1, share, shares);
          if (TOGETHER) join_warps<Op, G>(op, at, shared);
          if ((!TOGETHER || warp == 0) && at.edge_slot == 0) op.put(part_at<Op, G>(p, at, 2 * piece), at);
       }
    }
    for (; u < p.m; u++) {
-      const long long b = rows.begin(u), fb = b - rows.first + ROW_ITEMS * u;
+      if (u + 1 - from > 31) {
+         from = u;
+         mine = rows.begin(from + at.lane < p.m ? from + at.lane : p.m);
+      }
+      const long long b = __shfl_sync(FULL, mine, static_cast<int>(u - from)), fb = b - rows.first + ROW_ITEMS * u;
       if (fb >= hi) break;
-      long long e = rows.begin(u + 1);
+      long long e = __shfl_sync(FULL, mine, static_cast<int>(u + 1 - from));
       const long long fe = e - rows.first + ROW_ITEMS * (u + 1);
       const bool cut = fe - fb > p.row_limit;
       if (cut) {
@@ -760,7 +819,7 @@ __global__ void __launch_bounds__(PIECE_WARPS * 32) walk_kernel(const AttnParams
          e = e1 > e ? e : e1 < b ? b : e1;
          begun = u;
       }
-      op.run(p, at, u, b, e, TOGETHER ? warp : 0, TOGETHER ? PIECE_WARPS : 1);
+      op.run(p, at, edges, u, b, e, share, shares);
       if (TOGETHER) join_warps<Op, G>(op, at, shared);
       if (!TOGETHER || warp == 0) {
          if (!cut) op.finish(p, at, u);
@@ -773,7 +832,7 @@ __global__ void __launch_bounds__(PIECE_WARPS * 32) walk_kernel(const AttnParams
 
 // The parts of the long rows that begin in this block's pieces; a row's parts go to the warps in runs, joined in order.
 template <typename Op, int G>
-__global__ void __launch_bounds__(PIECE_WARPS * 32) join_kernel(const AttnParams p)
+__global__ void __launch_bounds__(JOINT_WARPS * 32) join_kernel(const AttnParams p)
 {
    extern __shared__ __align__(16) float shared[];
    const int warp = threadIdx.x >> 5;
@@ -785,7 +844,7 @@ __global__ void __launch_bounds__(PIECE_WARPS * 32) join_kernel(const AttnParams
       const long long u = p.long_row[piece];
       if (u < 0) continue;
       const long long last = (rows.items(u + 1) - 1) / p.piece, parts = last - piece + 1;
-      const long long each = (parts + PIECE_WARPS - 1) / PIECE_WARPS;
+      const long long each = (parts + JOINT_WARPS - 1) / JOINT_WARPS;
       Op::clear(op.s);
       for (long long i = warp * each; i < (warp + 1) * each && i < parts; i++)
          op.join_from(part_at<Op, G>(p, at, 2 * (piece + i) + (i == 0 ? 1 : 0)), at);
@@ -798,50 +857,54 @@ __global__ void __launch_bounds__(PIECE_WARPS * 32) join_kernel(const AttnParams
 // launchers: one instantiation per walk, storage type, slot, vectors of a lane, heads of a unit
 // ---------------------------------------------------------------------------------------------------------------------
 struct WalkShape {
-   int g = 0, nv = 0, qb = 1;
-   bool vector = true, together = false;
+   int g = 0, nv = 0, qb = 1, form = PIECES;
+   bool together = false;
 };
 
 template <typename Op, int G>
 int launch_op(const AttnParams &p, bool together, cudaStream_t st)
 {
-   const int bytes = (PIECE_WARPS - 1) * 32 * Op::LANE_FLOATS * static_cast<int>(sizeof(float));
+   const int bytes = (JOINT_WARPS - 1) * 32 * Op::LANE_FLOATS * static_cast<int>(sizeof(float));
    if (cudaFuncSetAttribute(join_kernel<Op, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -1;
    const long long jobs = p.pieces * p.unit_blocks;
    if (together) {
       if (cudaFuncSetAttribute(walk_kernel<Op, G, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -1;
-      walk_kernel<Op, G, true><<<static_cast<unsigned>(jobs), PIECE_WARPS * 32, bytes, st>>>(p);
+      walk_kernel<Op, G, true><<<static_cast<unsigned>(jobs), JOINT_WARPS * 32, bytes, st>>>(p);
    } else {
       walk_kernel<Op, G, false><<<static_cast<unsigned>((jobs + PIECE_WARPS - 1) / PIECE_WARPS), PIECE_WARPS * 32, 0, st>>>(p);
    }
    const long long groups = (p.pieces + JOIN_PIECES - 1) / JOIN_PIECES;
-   join_kernel<Op, G><<<static_cast<unsigned>(groups * p.unit_blocks), PIECE_WARPS * 32, bytes, st>>>(p);
+   join_kernel<Op, G><<<static_cast<unsigned>(groups * p.unit_blocks), JOINT_WARPS * 32, bytes, st>>>(p);
    return 0;
 }
 
-template <typename T, int G, int NV, template <typename, int, int, int, bool> class Op, bool COLUMNS>
+// query heads that a unit may hold: registers decide (a lane holds 2 NV W sums and NV W numbers of q for each)
+template <typename T, bool COLUMNS>
+constexpr int max_heads() { return COLUMNS ? 1 : sizeof(T) == 4 ? 4 : 2; }
+
+template <typename T, int G, int NV, template <typename, int, int, int, int> class Op, bool COLUMNS>
 int launch_slot(const WalkShape &s, const AttnParams &p, cudaStream_t st)
 {
-   if (!s.vector) return launch_op<Op<T, G, NV, 1, false>, G>(p, s.together, st);
-   if constexpr (!COLUMNS) {
-      if (s.qb == 4) return launch_op<Op<T, G, NV, 4, true>, G>(p, s.together, st);
-      if (s.qb == 2) return launch_op<Op<T, G, NV, 2, true>, G>(p, s.together, st);
-   }
-   return launch_op<Op<T, G, NV, 1, true>, G>(p, s.together, st);
+   if (s.form == PIECES) return launch_op<Op<T, G, NV, 1, PIECES>, G>(p, s.together, st);
+   if (s.form == RAGGED) return launch_op<Op<T, G, NV, 1, RAGGED>, G>(p, s.together, st);
+   if constexpr (max_heads<T, COLUMNS>() >= 4)
+      if (s.qb == 4) return launch_op<Op<T, G, NV, 4, EXACT>, G>(p, s.together, st);
+   if constexpr (max_heads<T, COLUMNS>() >= 2)
+      if (s.qb == 2) return launch_op<Op<T, G, NV, 2, EXACT>, G>(p, s.together, st);
+   return launch_op<Op<T, G, NV, 1, EXACT>, G>(p, s.together, st);
 }
 
 // -1: no such instantiation
-template <typename T, template <typename, int, int, int, bool> class Op, bool COLUMNS>
+template <typename T, template <typename, int, int, int, int> class Op, bool COLUMNS>
 int launch_walk(const WalkShape &s, const AttnParams &p, cudaStream_t st)
 {
-   if (s.nv == 1) {
-      if (s.g == 4) return launch_slot<T, 4, 1, Op, COLUMNS>(s, p, st);
-      if (s.g == 8) return launch_slot<T, 8, 1, Op, COLUMNS>(s, p, st);
-      if (s.g == 16) return launch_slot<T, 16, 1, Op, COLUMNS>(s, p, st);
-      if (s.g == 32) return launch_slot<T, 32, 1, Op, COLUMNS>(s, p, st);
-   }
+   if (s.nv == 1 && s.g == 4) return launch_slot<T, 4, 1, Op, COLUMNS>(s, p, st);
+   if (s.nv != 2) return -1;
+   if (s.g == 4) return launch_slot<T, 4, 2, Op, COLUMNS>(s, p, st);
+   if (s.g == 8) return launch_slot<T, 8, 2, Op, COLUMNS>(s, p, st);
+   if (s.g == 16) return launch_slot<T, 16, 2, Op, COLUMNS>(s, p, st);
    if constexpr (sizeof(T) == 4)
-      if (s.nv == 2 && s.g == 32) return launch_slot<T, 32, 2, Op, COLUMNS>(s, p, st);
+      if (s.g == 32) return launch_slot<T, 32, 2, Op, COLUMNS>(s, p, st);
    return -1;
 }
 

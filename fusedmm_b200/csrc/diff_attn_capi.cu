@@ -33,6 +33,16 @@ __global__ void __launch_bounds__(256) lam_sum_kernel(const float *in, long long
    }
 }
 
+// the bias of the edges in the order of the transposed pattern
+__global__ void __launch_bounds__(256) permute_bias_kernel(const float *bias, const int *t_edge, long long nnz, const void *t_rowptr,
+                                                           int ptr64, long long n, float *out)
+{
+   const long long t = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+   if (t >= nnz || t >= load_index(t_rowptr, ptr64, n)) return;  // behind the last column t_edge names no edge of a column
+   const int e = __ldg(t_edge + t);
+   out[t] = e >= 0 && e < nnz ? __ldg(bias + e) : -INFINITY;
+}
+
 namespace {
 
 enum Walk { FORWARD, ROWS, COLUMNS };
@@ -51,11 +61,12 @@ Shape choose_shape(Walk w, int dtype, bool vector, long long rows, long long edg
    Shape s;
    const int width = dtype == DT_F32 ? 4 : 8;
    const int nk = 2 * ((d + width - 1) / width), nvv = (dv + width - 1) / width, need = nk > nvv ? nk : nvv;
-   s.walk.g = need <= 4 ? 4 : need <= 8 ? 8 : need <= 16 ? 16 : 32;
-   s.walk.nv = need <= 32 ? 1 : 2;
-   s.walk.vector = vector;
-   const int group = heads / kv_heads;
-   s.walk.qb = w == COLUMNS || !vector ? 1 : group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+   s.walk.g = need <= 8 ? 4 : need <= 16 ? 8 : need <= 32 ? 16 : 32;
+   s.walk.nv = need <= 4 ? 1 : 2;
+   const int vectors = s.walk.g * s.walk.nv;
+   s.walk.form = !vector ? PIECES : nk == vectors && nvv == vectors ? EXACT : RAGGED;
+   const int group = heads / kv_heads, most = w == COLUMNS || s.walk.form != EXACT ? 1 : dtype == DT_F32 ? 4 : 2;
+   s.walk.qb = most >= 4 && group % 4 == 0 ? 4 : most >= 2 && group % 2 == 0 ? 2 : 1;
    s.units = w == COLUMNS ? kv_heads : heads / s.walk.qb;
    s.slot_heads = 1;
    while (2 * s.slot_heads <= 32 / s.walk.g && s.units % (2 * s.slot_heads) == 0) s.slot_heads *= 2;
@@ -102,8 +113,16 @@ int check_sizes(int32_t dtype, int64_t m, int64_t n, int64_t nnz, int32_t heads,
    if (m < 0 || n < 0 || nnz < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || d < 1 || dv < 1) return FUSEDMM_B200_ERR_ARG;
    if (d > FUSEDMM_B200_ATTN_MAX_WIDTH / 2 || dv > FUSEDMM_B200_ATTN_MAX_WIDTH || heads > FUSEDMM_B200_ATTN_MAX_HEADS)
       return FUSEDMM_B200_ERR_LIMIT;
-   if (m > (1LL << 48) || nnz > (1LL << 48)) return FUSEDMM_B200_ERR_LIMIT;
+   if (m > (1LL << 48) || nnz > (1LL << 48) || n >= INT_MAX) return FUSEDMM_B200_ERR_LIMIT;
    return 0;
+}
+
+// the kernels form the address of a row as base + id * stride with 32-bit factors
+bool strides_fit(int32_t dtype, std::initializer_list<int64_t> strides)
+{
+   for (int64_t s : strides)
+      if (s < 0 || s * (dtype == DT_F32 ? 4 : 2) >= INT_MAX) return false;
+   return true;
 }
 
 // elements that one load of these rows may take at once; 16 bytes' worth: whole vectors
@@ -128,8 +147,12 @@ long long walk_scratch(Walk w, int dtype, long long rows, long long edges, int h
                  choose_shape(w, dtype, false, rows, edges, heads, kv_heads, d, dv, sms).scratch_bytes());
 }
 
-// scratch of the backward pass in front of the walks': stats, dlam of every row, the sums of runs of rows
-long long backward_front(long long m, int heads) { return round256(m * heads * 16) + round256(m * heads * 4) + round256(LAM_BLOCKS * heads * 4LL); }
+// scratch of the backward pass in front of the walks': stats, dlam of every row, the sums of runs of rows,
+// and the bias in the columns' order
+long long backward_front(long long m, int heads, long long nnz)
+{
+   return round256(m * heads * 16) + round256(m * heads * 4) + round256(LAM_BLOCKS * heads * 4LL) + round256(nnz * 4);
+}
 
 }  // namespace
 }  // namespace attn
@@ -146,7 +169,7 @@ int64_t fusedmm_b200_diff_attention_workspace(int32_t backward, int32_t dtype, i
    int sms = 0;
    if (int s = sm_count(&sms)) return s;
    if (!backward) return walk_scratch(FORWARD, dtype, m, nnz, heads, kv_heads, d, dv, sms);
-   return backward_front(m, heads) + max_ll(walk_scratch(ROWS, dtype, m, nnz, heads, kv_heads, d, dv, sms),
+   return backward_front(m, heads, nnz) + max_ll(walk_scratch(ROWS, dtype, m, nnz, heads, kv_heads, d, dv, sms),
                                             walk_scratch(COLUMNS, dtype, n, nnz, heads, kv_heads, d, dv, sms));
 }
 
@@ -158,6 +181,7 @@ int fusedmm_b200_diff_attention(int32_t dtype, int32_t ptr_bits, int32_t idx_bit
 {
    if ((ptr_bits != 32 && ptr_bits != 64) || (idx_bits != 32 && idx_bits != 64)) return FUSEDMM_B200_ERR_ARG;
    if (int s = check_sizes(dtype, m, n, nnz, heads, kv_heads, d, dv)) return s;
+   if (!strides_fit(dtype, {ldq, hsq, ldk, hsk, ldv, hsv, ldlam})) return FUSEDMM_B200_ERR_LIMIT;
    if (m == 0) return 0;
    const bool gathers = nnz > 0 && n > 0;
    if (!rowptr || !q || !lam || !out || (nnz > 0 && !colidx) || (gathers && (!k || !v))) return FUSEDMM_B200_ERR_ARG;
@@ -198,7 +222,8 @@ int fusedmm_b200_diff_attention_backward(int32_t dtype, int32_t ptr_bits, int32_
 {
    if ((ptr_bits != 32 && ptr_bits != 64) || (idx_bits != 32 && idx_bits != 64)) return FUSEDMM_B200_ERR_ARG;
    if (int s = check_sizes(dtype, m, n, nnz, heads, kv_heads, d, dv)) return s;
-   if (m >= INT_MAX || n >= INT_MAX || nnz >= INT_MAX) return FUSEDMM_B200_ERR_LIMIT;
+   if (m >= INT_MAX || nnz >= INT_MAX) return FUSEDMM_B200_ERR_LIMIT;
+   if (!strides_fit(dtype, {ldq, hsq, ldk, hsk, ldv, hsv, lddo, hsdo, ldlam})) return FUSEDMM_B200_ERR_LIMIT;
    if (!dlam || (m > 0 && (!rowptr || !q || !lam || !lse || !dout || !dq)) || (n > 0 && (!k || !v || !dk || !dv_out || !t_rowptr)) ||
        (nnz > 0 && (!colidx || !t_row || (bias && !t_edge))))
       return FUSEDMM_B200_ERR_ARG;
@@ -216,7 +241,7 @@ int fusedmm_b200_diff_attention_backward(int32_t dtype, int32_t ptr_bits, int32_
    char *ws = static_cast<char *>(workspace);
    float *row_dlam = reinterpret_cast<float *>(ws + round256(m * heads * 16));
    float *lam_part = reinterpret_cast<float *>(ws + round256(m * heads * 16) + round256(m * heads * 4));
-   char *scratch = ws + backward_front(m, heads);
+   char *scratch = ws + backward_front(m, heads, nnz);
    Step step(dtype);
    step.with(q, ldq, hsq, d);
    step.with(k, ldk, hsk, d);
@@ -252,7 +277,12 @@ int fusedmm_b200_diff_attention_backward(int32_t dtype, int32_t ptr_bits, int32_
       }
    }
    if (n > 0) {
-      p.rowptr = t_rowptr; p.colidx = t_row; p.idx64 = 0; p.m = n; p.n = m; p.nnz = nnz; p.out = dk; p.out2 = dv_out; p.edge_of = t_edge;
+      p.rowptr = t_rowptr; p.colidx = t_row; p.idx64 = 0; p.m = n; p.n = m; p.nnz = nnz; p.out = dk; p.out2 = dv_out;
+      if (bias && nnz > 0) {
+         float *moved = lam_part + round256(LAM_BLOCKS * heads * 4LL) / 4;
+         permute_bias_kernel<<<static_cast<unsigned>((nnz + 255) / 256), 256, 0, st>>>(bias, t_edge, nnz, t_rowptr, p.ptr64, n, moved);
+         p.bias = moved;
+      }
       const Shape s = choose_shape(COLUMNS, dtype, step.vector(), n, p.nnz, heads, kv_heads, d, dv, sms);
       apply(p, s, scratch);
       if (int r = launch(COLUMNS, dtype, s, p, st)) return r;
