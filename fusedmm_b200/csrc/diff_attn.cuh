@@ -49,6 +49,8 @@ struct AttnParams {
    int heads, kv_heads, group, d, dv, step;
    float scale;
    int units, unit_blocks, slot_heads;  // head units of QB heads; warps (blocks) that share them; slots of a warp across units
+   // the walks on the matrix units: kv heads of a unit, query heads of each of them, units that share a kv head
+   int unit_kv, unit_heads, head_blocks;
    long long piece, row_limit, pieces;
    float *partial;
    long long *long_row;          // [pieces]: the long row that begins in a piece, or -1
@@ -226,7 +228,7 @@ __device__ __forceinline__ void unpair(const F2 (&f)[N], float (&o)[2 * N])
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int G, int NV, int QB, int FORM>
 struct Forward {
-   static constexpr int W = Elt<T>::W, P = W / 2, U = 2;
+   static constexpr int W = Elt<T>::W, P = W / 2, U = 2, BLOCKS = QB * NV * W > 16 ? 2 : 4;
    static constexpr int KSKIP = (G / 2) * W, VSKIP = G * W;
    static constexpr int LANE_FLOATS = QB * (2 * NV * W + 2);  // partial state of a lane
    struct State {
@@ -234,7 +236,9 @@ struct Forward {
       float top[QB], sum[QB];  // of this half's map
    };
    State s;
+   static constexpr bool lost = false;  // no sum reaches another head's
 
+   __device__ __forceinline__ void setup(const AttnParams &, const Place &) {}
    static __device__ __forceinline__ void clear(State &s)
    {
 #pragma unroll
@@ -251,7 +255,7 @@ struct Forward {
    }
 
    __device__ __forceinline__ void run(const AttnParams &p, const Place &at, EdgeStream &edges, long long row, long long e0, long long e1,
-                                       int warp, int warps)
+                                       int warp, int warps, int)
    {
       clear(s);
       if (e0 + 32 * warp >= e1) return;
@@ -398,7 +402,7 @@ struct Forward {
       }
       join(s, o, at, false);
    }
-   __device__ __forceinline__ void put(float *unit, const Place &at) const
+   __device__ __forceinline__ void put(float *unit, const Place &at, int) const
    {
       float *to = unit + at.in_slot * W;
 #pragma unroll
@@ -411,7 +415,7 @@ struct Forward {
       }
    }
 
-   __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long row)
+   __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long row, int)
    {
 #pragma unroll
       for (int b = 0; b < QB; b++) {
@@ -442,7 +446,7 @@ struct Forward {
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int G, int NV, int QB, int FORM>
 struct BackwardRows {
-   static constexpr int W = Elt<T>::W, P = W / 2, U = 2;
+   static constexpr int W = Elt<T>::W, P = W / 2, U = 2, BLOCKS = QB * NV * W > 16 ? 2 : 4;
    static constexpr int KSKIP = (G / 2) * W, VSKIP = G * W;
    static constexpr int LANE_FLOATS = QB * (2 * NV * W + 2);
    struct State {
@@ -450,7 +454,9 @@ struct BackwardRows {
       float delta[QB];
    };
    State s;
+   static constexpr bool lost = false;  // no sum reaches another head's
 
+   __device__ __forceinline__ void setup(const AttnParams &, const Place &) {}
    static __device__ __forceinline__ void clear(State &s)
    {
 #pragma unroll
@@ -464,7 +470,7 @@ struct BackwardRows {
    }
 
    __device__ __forceinline__ void run(const AttnParams &p, const Place &at, EdgeStream &edges, long long row, long long e0, long long e1,
-                                       int warp, int warps)
+                                       int warp, int warps, int)
    {
       clear(s);
       if (e0 + 32 * warp >= e1) return;
@@ -561,7 +567,7 @@ struct BackwardRows {
          s.delta[b] += unit[QB * 2 * NV * W * G + (b * G + at.in_slot) * 2];
       }
    }
-   __device__ __forceinline__ void put(float *unit, const Place &at) const
+   __device__ __forceinline__ void put(float *unit, const Place &at, int) const
    {
       float *to = unit + at.in_slot * W;
 #pragma unroll
@@ -575,7 +581,7 @@ struct BackwardRows {
       }
    }
 
-   __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long row)
+   __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long row, int)
    {
       if (at.edge_slot != 0) return;
 #pragma unroll
@@ -606,14 +612,16 @@ struct BackwardRows {
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int G, int NV, int QB, int FORM>
 struct BackwardColumns {
-   static constexpr int W = Elt<T>::W, P = W / 2, U = 2;
+   static constexpr int W = Elt<T>::W, P = W / 2, U = 2, BLOCKS = W == 4 ? 4 : 3;
    static constexpr int KSKIP = (G / 2) * W, VSKIP = G * W;
    static constexpr int LANE_FLOATS = 2 * NV * W;
    struct State {
       F2 dk[NV][P], dv[NV][P];
    };
    State s;
+   static constexpr bool lost = false;  // no sum reaches another head's
 
+   __device__ __forceinline__ void setup(const AttnParams &, const Place &) {}
    static __device__ __forceinline__ void clear(State &s)
    {
 #pragma unroll
@@ -623,7 +631,7 @@ struct BackwardColumns {
    }
 
    __device__ __forceinline__ void run(const AttnParams &p, const Place &at, EdgeStream &edges, long long col, long long e0, long long e1,
-                                       int warp, int warps)
+                                       int warp, int warps, int)
    {
       clear(s);
       if (e0 + 32 * warp >= e1) return;
@@ -717,7 +725,7 @@ struct BackwardColumns {
          for (int j = 0; j < P; j++) s.dv[t][j] = add2(s.dv[t][j], x[j]);
       }
    }
-   __device__ __forceinline__ void put(float *unit, const Place &at) const
+   __device__ __forceinline__ void put(float *unit, const Place &at, int) const
    {
       float *to = unit + at.in_slot * W;
 #pragma unroll
@@ -727,7 +735,7 @@ struct BackwardColumns {
       }
    }
 
-   __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long col)
+   __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long col, int)
    {
       if (at.edge_slot != 0) return;
       const long long rh = col * p.kv_heads + at.unit;
@@ -765,15 +773,34 @@ __device__ __forceinline__ void join_warps(Op &op, const Place &at, float *share
    constexpr int STRIDE = Op::LANE_FLOATS * 32;  // slots side by side, as in scratch
    float *mine = shared + (at.lane / G) * part_floats<Op, G>;
    __syncthreads();
-   if (at.warp > 0) op.put(mine + (at.warp - 1) * STRIDE, at);
+   if (at.warp > 0) op.put(mine + (at.warp - 1) * STRIDE, at, -1);
    __syncthreads();
    if (at.warp == 0)
       for (int w = 1; w < JOINT_WARPS; w++) op.join_from(mine + (w - 1) * STRIDE, at);
 }
 
+// Edges [e0, e1) of a row: to the result, or (part >= 0) to the scratch of that part.  Where an operator computes several
+// heads in one product and a sum came out as no number, a 0 of one head may have met an infinity or NaN of another's: the
+// heads are then computed one by one.
+template <typename Op, int G, bool TOGETHER>
+__device__ __forceinline__ void walk_row(Op &op, const AttnParams &p, const Place &at, EdgeStream &edges, float *shared, long long row,
+                                         long long e0, long long e1, long long part)
+{
+   for (int only = -1; only < p.unit_kv; only++) {
+      op.run(p, at, edges, row, e0, e1, TOGETHER ? at.warp : 0, TOGETHER ? JOINT_WARPS : 1, only);
+      if (only < 0 && p.unit_kv > 1 && (TOGETHER ? __syncthreads_or(op.lost) : __any_sync(FULL, op.lost))) continue;
+      if (TOGETHER) join_warps<Op, G>(op, at, shared);
+      if (!TOGETHER || at.warp == 0) {
+         if (part < 0) op.finish(p, at, row, only);
+         else if (at.edge_slot == 0) op.put(part_at<Op, G>(p, at, part), at, only);
+      }
+      if (only < 0) break;
+   }
+}
+
 // TOGETHER: the warps of a block share every row (few, long rows), else each warp has a piece of its own.
 template <typename Op, int G, bool TOGETHER>
-__global__ void __launch_bounds__((TOGETHER ? JOINT_WARPS : PIECE_WARPS) * 32) walk_kernel(const AttnParams p)
+__global__ void __launch_bounds__((TOGETHER ? JOINT_WARPS : PIECE_WARPS) * 32, TOGETHER ? 1 : Op::BLOCKS) walk_kernel(const AttnParams p)
 {
    extern __shared__ __align__(16) float shared[];
    const int warp = threadIdx.x >> 5;
@@ -785,24 +812,17 @@ __global__ void __launch_bounds__((TOGETHER ? JOINT_WARPS : PIECE_WARPS) * 32) w
    const long long lo = piece * p.piece, hi = lo + p.piece;
    long long u = rows.lower_bound(lo, at.lane);
    const bool teller = at.lane == 0 && (!TOGETHER || warp == 0) && job == piece * p.unit_blocks;
-   const int share = TOGETHER ? warp : 0, shares = TOGETHER ? JOINT_WARPS : 1;
    long long begun = -1;
    Op op;
+   op.setup(p, at);
    EdgeStream edges;
    // row pointers 32 at a time, one to a lane
    long long from = u > 0 ? u - 1 : 0;
    long long mine = rows.begin(from + at.lane < p.m ? from + at.lane : p.m);
-   if (u > 0) {  // the row before may reach into this piece
+   if (u > 0) {  // the row before may reach into this piece: then it is this loop's first
       const long long b = __shfl_sync(FULL, mine, 0), e = __shfl_sync(FULL, mine, 1);
       const long long fb = b - rows.first + ROW_ITEMS * (u - 1), fe = e - rows.first + ROW_ITEMS * u;
-      if (fe > lo && fe - fb > p.row_limit) {
-         long long e0 = b + (lo - fb - ROW_ITEMS), e1 = b + (hi - fb - ROW_ITEMS);
-         e0 = e0 < b ? b : e0;
-         e1 = e1 > e ? e : e1 < e0 ? e0 : e1;
-         op.run(p, at, edges, u - 1, e0, e1, share, shares);
-         if (TOGETHER) join_warps<Op, G>(op, at, shared);
-         if ((!TOGETHER || warp == 0) && at.edge_slot == 0) op.put(part_at<Op, G>(p, at, 2 * piece), at);
-      }
+      if (fe > lo && fe - fb > p.row_limit) u--;
    }
    for (; u < p.m; u++) {
       if (u + 1 - from > 31) {
@@ -811,21 +831,18 @@ __global__ void __launch_bounds__((TOGETHER ? JOINT_WARPS : PIECE_WARPS) * 32) w
       }
       const long long b = __shfl_sync(FULL, mine, static_cast<int>(u - from)), fb = b - rows.first + ROW_ITEMS * u;
       if (fb >= hi) break;
-      long long e = __shfl_sync(FULL, mine, static_cast<int>(u + 1 - from));
+      const long long e = __shfl_sync(FULL, mine, static_cast<int>(u + 1 - from));
       const long long fe = e - rows.first + ROW_ITEMS * (u + 1);
-      const bool cut = fe - fb > p.row_limit;
-      if (cut) {
-         const long long e1 = b + (hi - fb - ROW_ITEMS);
-         e = e1 > e ? e : e1 < b ? b : e1;
-         begun = u;
+      long long e0 = b, e1 = e, part = -1;
+      if (fe - fb > p.row_limit) {  // a long row: this piece's part of it
+         e0 = b + (lo - fb - ROW_ITEMS);
+         e1 = b + (hi - fb - ROW_ITEMS);
+         e0 = e0 < b ? b : e0;
+         e1 = e1 > e ? e : e1 < e0 ? e0 : e1;
+         part = 2 * piece + (fb >= lo);
+         if (fb >= lo) begun = u;
       }
-      op.run(p, at, edges, u, b, e, share, shares);
-      if (TOGETHER) join_warps<Op, G>(op, at, shared);
-      if (!TOGETHER || warp == 0) {
-         if (!cut) op.finish(p, at, u);
-         else if (at.edge_slot == 0) op.put(part_at<Op, G>(p, at, 2 * piece + 1), at);
-      }
-      if (cut) break;  // it reaches beyond this piece
+      walk_row<Op, G, TOGETHER>(op, p, at, edges, shared, u, e0, e1, part);
    }
    if (teller) p.long_row[piece] = begun;
 }
@@ -840,6 +857,7 @@ __global__ void __launch_bounds__(JOINT_WARPS * 32) join_kernel(const AttnParams
    const Place at = Place::make<G>(p, static_cast<int>(blockIdx.x - group * p.unit_blocks));
    const Rows rows(p);
    Op op;
+   op.setup(p, at);
    for (long long piece = group * JOIN_PIECES; piece < (group + 1) * JOIN_PIECES && piece < p.pieces; piece++) {
       const long long u = p.long_row[piece];
       if (u < 0) continue;
@@ -849,7 +867,7 @@ __global__ void __launch_bounds__(JOINT_WARPS * 32) join_kernel(const AttnParams
       for (long long i = warp * each; i < (warp + 1) * each && i < parts; i++)
          op.join_from(part_at<Op, G>(p, at, 2 * (piece + i) + (i == 0 ? 1 : 0)), at);
       join_warps<Op, G>(op, at, shared);
-      if (warp == 0) op.finish(p, at, u);
+      if (warp == 0) op.finish(p, at, u, -1);
    }
 }
 
@@ -858,6 +876,7 @@ __global__ void __launch_bounds__(JOINT_WARPS * 32) join_kernel(const AttnParams
 // ---------------------------------------------------------------------------------------------------------------------
 struct WalkShape {
    int g = 0, nv = 0, qb = 1, form = PIECES;
+   int width = 0;  // > 0: a walk on the matrix units, for d up to this and dv up to twice this
    bool together = false;
 };
 

@@ -49,7 +49,7 @@ enum Walk { FORWARD, ROWS, COLUMNS };
 
 struct Shape {
    WalkShape walk;
-   int units = 0, unit_blocks = 0, slot_heads = 0;
+   int units = 0, unit_blocks = 0, slot_heads = 0, unit_kv = 1, unit_heads = 1, head_blocks = 1;
    long long piece = 0, row_limit = 0, pieces = 0, part_bytes = 0;
    long long scratch_bytes() const { return (pieces * 2 * units * part_bytes + 255) / 256 * 256 + (pieces * 8 + 255) / 256 * 256; }
 };
@@ -61,18 +61,33 @@ Shape choose_shape(Walk w, int dtype, bool vector, long long rows, long long edg
    Shape s;
    const int width = dtype == DT_F32 ? 4 : 8;
    const int nk = 2 * ((d + width - 1) / width), nvv = (dv + width - 1) / width, need = nk > nvv ? nk : nvv;
-   s.walk.g = need <= 8 ? 4 : need <= 16 ? 8 : need <= 32 ? 16 : 32;
-   s.walk.nv = need <= 4 ? 1 : 2;
-   const int vectors = s.walk.g * s.walk.nv;
-   s.walk.form = !vector ? PIECES : nk == vectors && nvv == vectors ? EXACT : RAGGED;
-   const int group = heads / kv_heads, most = w == COLUMNS || s.walk.form != EXACT ? 1 : dtype == DT_F32 ? 4 : 2;
-   s.walk.qb = most >= 4 && group % 4 == 0 ? 4 : most >= 2 && group % 2 == 0 ? 2 : 1;
-   s.units = w == COLUMNS ? kv_heads : heads / s.walk.qb;
-   s.slot_heads = 1;
-   while (2 * s.slot_heads <= 32 / s.walk.g && s.units % (2 * s.slot_heads) == 0) s.slot_heads *= 2;
+   const int group = heads / kv_heads;
+   int lane_floats;
+   if (dtype == DT_BF16 || (dtype == DT_F16 && w == FORWARD)) {
+      s.walk.width = need <= 4 ? 16 : need <= 8 ? 32 : need <= 16 ? 64 : 128;
+      s.walk.form = !vector ? PIECES : d == s.walk.width && dv == 2 * d ? EXACT : RAGGED;
+      s.head_blocks = w == COLUMNS ? 1 : (group + 3) / 4;
+      s.unit_heads = w == COLUMNS ? 1 : (group + s.head_blocks - 1) / s.head_blocks;
+      s.unit_kv = 1;
+      while (s.unit_kv * 2 * s.unit_heads <= 4 && kv_heads % (s.unit_kv * 2) == 0) s.unit_kv *= 2;
+      s.units = kv_heads / s.unit_kv * s.head_blocks;
+      s.slot_heads = 1;
+      lane_floats = w == FORWARD ? s.walk.width / 2 + 4 : w == ROWS ? s.walk.width / 2 + 2 : s.walk.width;
+      s.part_bytes = static_cast<long long>(lane_floats) * 32 * 4;
+   } else {
+      s.walk.g = need <= 8 ? 4 : need <= 16 ? 8 : need <= 32 ? 16 : 32;
+      s.walk.nv = need <= 4 ? 1 : 2;
+      const int vectors = s.walk.g * s.walk.nv;
+      s.walk.form = !vector ? PIECES : nk == vectors && nvv == vectors ? EXACT : RAGGED;
+      const int most = w == COLUMNS || s.walk.form != EXACT ? 1 : dtype == DT_F32 ? 4 : 2;
+      s.walk.qb = most >= 4 && group % 4 == 0 ? 4 : most >= 2 && group % 2 == 0 ? 2 : 1;
+      s.units = w == COLUMNS ? kv_heads : heads / s.walk.qb;
+      s.slot_heads = 1;
+      while (2 * s.slot_heads <= 32 / s.walk.g && s.units % (2 * s.slot_heads) == 0) s.slot_heads *= 2;
+      lane_floats = w == COLUMNS ? 2 * s.walk.nv * width : s.walk.qb * (2 * s.walk.nv * width + 2);
+      s.part_bytes = static_cast<long long>(lane_floats) * s.walk.g * 4;
+   }
    s.unit_blocks = s.units / s.slot_heads;
-   const int lane_floats = w == COLUMNS ? 2 * s.walk.nv * width : s.walk.qb * (2 * s.walk.nv * width + 2);
-   s.part_bytes = static_cast<long long>(lane_floats) * s.walk.g * 4;
    const long long items = edges + ROW_ITEMS * rows, mean = edges / rows;
    const bool few = rows * s.unit_blocks < 8LL * sms;
    s.walk.together = mean >= 256 || (few && mean >= 64);
@@ -91,6 +106,7 @@ Shape choose_shape(Walk w, int dtype, bool vector, long long rows, long long edg
 void apply(AttnParams &p, const Shape &s, char *scratch)
 {
    p.units = s.units; p.unit_blocks = s.unit_blocks; p.slot_heads = s.slot_heads;
+   p.unit_kv = s.unit_kv; p.unit_heads = s.unit_heads; p.head_blocks = s.head_blocks;
    p.piece = s.piece; p.row_limit = s.row_limit; p.pieces = s.pieces;
    p.partial = reinterpret_cast<float *>(scratch);
    p.long_row = reinterpret_cast<long long *>(scratch + (s.pieces * 2 * s.units * s.part_bytes + 255) / 256 * 256);

@@ -1,10 +1,10 @@
 // the forward walk of differential attention, bf16
-#include "diff_attn.cuh"
+#include "diff_attn_mma.cuh"
 
 namespace fmm {
 namespace attn {
 
-int walk_forward_bf16(const WalkShape &s, const AttnParams &p, cudaStream_t st) { return launch_walk<__nv_bfloat16, Forward, false>(s, p, st); }
+int walk_forward_bf16(const WalkShape &s, const AttnParams &p, cudaStream_t st) { return launch_mma<__nv_bfloat16, ForwardMma>(s, p, st); }
 
 }  // namespace attn
 }  // namespace fmm

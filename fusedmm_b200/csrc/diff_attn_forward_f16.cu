@@ -1,10 +1,10 @@
 // the forward walk of differential attention, f16
-#include "diff_attn.cuh"
+#include "diff_attn_mma.cuh"
 
 namespace fmm {
 namespace attn {
 
-int walk_forward_f16(const WalkShape &s, const AttnParams &p, cudaStream_t st) { return launch_walk<__half, Forward, false>(s, p, st); }
+int walk_forward_f16(const WalkShape &s, const AttnParams &p, cudaStream_t st) { return launch_mma<__half, ForwardMma>(s, p, st); }
 
 }  // namespace attn
 }  // namespace fmm

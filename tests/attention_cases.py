@@ -8,6 +8,10 @@ HALF_STEP = {torch.float64: 0.0, torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 
 # rounding is off by up to half of that whatever the value
 HALF_SUBNORMAL = {torch.float64: 0.0, torch.float32: 2.0 ** -150, torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}
 E32 = 2.0 ** -24
+# For 16-bit types the weights enter the second product as the sum of two numbers of the type: the first is off by up to half
+# a step, the second holds what is missing up to half a step of that.  The matrix units' sums may drop digits, so that each
+# addition is off by a whole step and not by half of one.
+SPLIT = {torch.float64: 0.0, torch.float32: 0.0, torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -22}
 
 
 def random_pattern(gen, m, n, mean, ptr=torch.int64, idx=torch.int32, hub=0, empty=0.2):
@@ -27,6 +31,7 @@ def attention_reference(rowptr, colidx, bias, q, k, v, lam, scale, dout=None):
     c = lambda t: None if t is None else t.detach().cpu().double()
     rowptr, colidx = rowptr.cpu().long(), colidx.cpu().long()
     half, tiny = HALF_STEP[q.dtype], HALF_SUBNORMAL[q.dtype] + 1e-30
+    split, E32 = SPLIT[q.dtype], 2.0 ** -24 if q.dtype == torch.float32 else 2.0 ** -23
     q, k, v, lam, bias, dout = c(q), c(k), c(v), c(lam), c(bias), c(dout)
     m, heads, _, d = q.shape
     n, kvh, dv = v.shape
@@ -57,7 +62,7 @@ def attention_reference(rowptr, colidx, bias, q, k, v, lam, scale, dout=None):
     smax = zeros(m, heads, 2).scatter_reduce(0, row[:, None, None].expand_as(s), serr, "amax")
     # relative error of p: the score's and the sum's (which holds the scores' again), the exponentials' (2 units), the sums'
     perr = 2 * smax + E32 * (16 + deg)[:, None, None]
-    perr = perr.amax(-1)
+    perr = perr.amax(-1) + split
     w = pr[..., 0] - lam_rows[row] * pr[..., 1]
     wabs = pr[..., 0] + lam_rows[row].abs() * pr[..., 1]
     out = zeros(m, heads, dv).index_add(0, row, w[..., None] * ve)
@@ -75,7 +80,7 @@ def attention_reference(rowptr, colidx, bias, q, k, v, lam, scale, dout=None):
     ds = sign * pr * (dp[..., None] - delta[row])
     dsabs = sign.abs() * pr * (dpabs[..., None] + dabs[row])
     # what a ds loses against its parts' sizes: p, the dot of dv products, the sum over the row
-    rel = (2 * perr + E32 * (dv + deg + 16)[:, None])[row]
+    rel = (2 * perr + split + E32 * (dv + deg + 16)[:, None])[row]
     dq = zeros(m, heads, 2, d).index_add(0, row, scale * ds[..., None] * ke)
     dqb = zeros(m, heads, 2, d).index_add(0, row, abs(scale) * (rel[..., None] * dsabs)[..., None] * ke.abs())
     group = heads // kvh
