@@ -44,13 +44,18 @@ struct AttnParams {
    void *out;                    // forward [m,H,Dv]; dq [m,H,2,D]; dk [n,Hk,2,D]
    void *out2;                   // dv [n,Hk,Dv]
    float *lse;                   // [m,H,2]
-   float2 *stats;                // [m,H,2]: lse and D of a map
+   float4 *stats;                // [m,H,2]: lse and D of a map, its factor in the weight (1 or -lam)
    float *dlam;                  // [m,H]
    int heads, kv_heads, group, d, dv, step;
    float scale;
    int units, unit_blocks, slot_heads;  // head units of QB heads; warps (blocks) that share them; slots of a warp across units
    // the walks on the matrix units: kv heads of a unit, query heads of each of them, units that share a kv head
    int unit_kv, unit_heads, head_blocks;
+   // ... and the two gathered arrays there: bytes from row to row and from head to head, elements of a row (of one map for
+   // the first); the groups of heads that a unit takes one after the other, and the heads of a group for one kv head (log2)
+   unsigned a_stride, b_stride;
+   long long a_head, b_head;
+   int a_width, b_width, subs, kv_log2;
    long long piece, row_limit, pieces;
    float *partial;
    long long *long_row;          // [pieces]: the long row that begins in a piece, or -1
@@ -76,10 +81,9 @@ struct Rows {
       return b < first ? first : b > p.nnz ? p.nnz : b;
    }
    __device__ __forceinline__ long long items(long long u) const { return begin(u) - first + ROW_ITEMS * u; }
-   // first row u in [0, m] with items(u) >= at; the whole warp takes part
-   __device__ __forceinline__ long long lower_bound(long long at, int lane) const
+   // first row u in [lo, hi) with items(u) >= at, or hi; the whole warp takes part
+   __device__ __forceinline__ long long lower_bound(long long at, long long lo, long long hi, int lane) const
    {
-      long long lo = 0, hi = p.m;
       while (lo < hi) {
          const long long step = (hi - lo + 31) / 32;
          const long long u = lo + step * lane;
@@ -236,9 +240,7 @@ struct Forward {
       float top[QB], sum[QB];  // of this half's map
    };
    State s;
-   static constexpr bool lost = false;  // no sum reaches another head's
 
-   __device__ __forceinline__ void setup(const AttnParams &, const Place &) {}
    static __device__ __forceinline__ void clear(State &s)
    {
 #pragma unroll
@@ -255,7 +257,7 @@ struct Forward {
    }
 
    __device__ __forceinline__ void run(const AttnParams &p, const Place &at, EdgeStream &edges, long long row, long long e0, long long e1,
-                                       int warp, int warps, int)
+                                       int warp, int warps)
    {
       clear(s);
       if (e0 + 32 * warp >= e1) return;
@@ -402,7 +404,7 @@ struct Forward {
       }
       join(s, o, at, false);
    }
-   __device__ __forceinline__ void put(float *unit, const Place &at, int) const
+   __device__ __forceinline__ void put(float *unit, const Place &at) const
    {
       float *to = unit + at.in_slot * W;
 #pragma unroll
@@ -415,7 +417,7 @@ struct Forward {
       }
    }
 
-   __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long row, int)
+   __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long row)
    {
 #pragma unroll
       for (int b = 0; b < QB; b++) {
@@ -454,9 +456,7 @@ struct BackwardRows {
       float delta[QB];
    };
    State s;
-   static constexpr bool lost = false;  // no sum reaches another head's
 
-   __device__ __forceinline__ void setup(const AttnParams &, const Place &) {}
    static __device__ __forceinline__ void clear(State &s)
    {
 #pragma unroll
@@ -470,7 +470,7 @@ struct BackwardRows {
    }
 
    __device__ __forceinline__ void run(const AttnParams &p, const Place &at, EdgeStream &edges, long long row, long long e0, long long e1,
-                                       int warp, int warps, int)
+                                       int warp, int warps)
    {
       clear(s);
       if (e0 + 32 * warp >= e1) return;
@@ -567,7 +567,7 @@ struct BackwardRows {
          s.delta[b] += unit[QB * 2 * NV * W * G + (b * G + at.in_slot) * 2];
       }
    }
-   __device__ __forceinline__ void put(float *unit, const Place &at, int) const
+   __device__ __forceinline__ void put(float *unit, const Place &at) const
    {
       float *to = unit + at.in_slot * W;
 #pragma unroll
@@ -581,14 +581,14 @@ struct BackwardRows {
       }
    }
 
-   __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long row, int)
+   __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long row)
    {
       if (at.edge_slot != 0) return;
 #pragma unroll
       for (int b = 0; b < QB; b++) {
          const int head = at.unit * QB + b;
          const long long rh = row * p.heads + head;
-         const float factor = at.half ? -__ldg(p.lam + row * p.ldlam + head) * p.scale : p.scale;
+         const float sign = at.half ? -__ldg(p.lam + row * p.ldlam + head) : 1.0f, factor = sign * p.scale;
 #pragma unroll
          for (int t = 0; t < NV; t++) {
             const int x = (at.in_half + (G / 2) * t) * W;
@@ -600,7 +600,7 @@ struct BackwardRows {
             st_row<T, FORM != PIECES>(static_cast<T *>(p.out) + (rh * 2 + at.half) * p.d + x, a, p.d - x);
          }
          if (at.in_half == 0) {
-            p.stats[rh * 2 + at.half] = make_float2(__ldg(p.lse + rh * 2 + at.half), s.delta[b]);
+            p.stats[rh * 2 + at.half] = make_float4(__ldg(p.lse + rh * 2 + at.half), s.delta[b], sign, 0.0f);
             if (at.half == 1) p.dlam[rh] = -s.delta[b];
          }
       }
@@ -619,9 +619,7 @@ struct BackwardColumns {
       F2 dk[NV][P], dv[NV][P];
    };
    State s;
-   static constexpr bool lost = false;  // no sum reaches another head's
 
-   __device__ __forceinline__ void setup(const AttnParams &, const Place &) {}
    static __device__ __forceinline__ void clear(State &s)
    {
 #pragma unroll
@@ -631,7 +629,7 @@ struct BackwardColumns {
    }
 
    __device__ __forceinline__ void run(const AttnParams &p, const Place &at, EdgeStream &edges, long long col, long long e0, long long e1,
-                                       int warp, int warps, int)
+                                       int warp, int warps)
    {
       clear(s);
       if (e0 + 32 * warp >= e1) return;
@@ -657,16 +655,11 @@ struct BackwardColumns {
                const int head = kv * p.group + g;
                const Gather<T, NV, FORM> qg(p.q, p.ldq, head * p.hsq + at.half * p.d, x, p.d), dg(p.dout, p.ldo, head * p.hso, y, p.dv);
                uint4 qr[U][NV], dr[U][NV];
-               float2 stat[U];
-               float lam[U];
+               float4 stat[U];
 #pragma unroll
                for (int i = 0; i < U; i++) {
-                  stat[i] = make_float2(-INFINITY, 0.0f);
-                  lam[i] = 0.0f;
-                  if (id[i] >= 0) {
-                     stat[i] = __ldg(p.stats + (static_cast<long long>(id[i]) * p.heads + head) * 2 + at.half);
-                     lam[i] = __ldg(p.lam + id[i] * p.ldlam + head);
-                  }
+                  stat[i] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+                  if (id[i] >= 0) stat[i] = __ldg(p.stats + (static_cast<long long>(id[i]) * p.heads + head) * 2 + at.half);
                   qg.template load<KSKIP>(id[i], qr[i], p.step);
                   dg.template load<VSKIP>(id[i], dr[i], p.step);
                }
@@ -686,7 +679,7 @@ struct BackwardColumns {
                   const float dot = add_over<G / 2>(sum2(dots)), dp = add_over<G>(sum2(dps));
                   const bool live = stat[i].x != -INFINITY;  // an edge, and of a row that has any
                   const float pr = live ? exp2_fast((fmaf(dot, p.scale, bias[i]) - stat[i].x) * LOG2E) : 0.0f;
-                  const float mine = live ? (at.half ? -lam[i] : 1.0f) * pr : 0.0f;  // this map's part of the weight
+                  const float mine = live ? stat[i].z * pr : 0.0f;  // this map's part of the weight
                   const float w = mine + __shfl_xor_sync(FULL, mine, G / 2);
                   const float ds = live ? mine * (dp - stat[i].y) : 0.0f;
                   const F2 ww = f2(w, w), dd = f2(ds, ds);
@@ -725,7 +718,7 @@ struct BackwardColumns {
          for (int j = 0; j < P; j++) s.dv[t][j] = add2(s.dv[t][j], x[j]);
       }
    }
-   __device__ __forceinline__ void put(float *unit, const Place &at, int) const
+   __device__ __forceinline__ void put(float *unit, const Place &at) const
    {
       float *to = unit + at.in_slot * W;
 #pragma unroll
@@ -735,7 +728,7 @@ struct BackwardColumns {
       }
    }
 
-   __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long col, int)
+   __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long col)
    {
       if (at.edge_slot != 0) return;
       const long long rh = col * p.kv_heads + at.unit;
@@ -773,29 +766,10 @@ __device__ __forceinline__ void join_warps(Op &op, const Place &at, float *share
    constexpr int STRIDE = Op::LANE_FLOATS * 32;  // slots side by side, as in scratch
    float *mine = shared + (at.lane / G) * part_floats<Op, G>;
    __syncthreads();
-   if (at.warp > 0) op.put(mine + (at.warp - 1) * STRIDE, at, -1);
+   if (at.warp > 0) op.put(mine + (at.warp - 1) * STRIDE, at);
    __syncthreads();
    if (at.warp == 0)
       for (int w = 1; w < JOINT_WARPS; w++) op.join_from(mine + (w - 1) * STRIDE, at);
-}
-
-// Edges [e0, e1) of a row: to the result, or (part >= 0) to the scratch of that part.  Where an operator computes several
-// heads in one product and a sum came out as no number, a 0 of one head may have met an infinity or NaN of another's: the
-// heads are then computed one by one.
-template <typename Op, int G, bool TOGETHER>
-__device__ __forceinline__ void walk_row(Op &op, const AttnParams &p, const Place &at, EdgeStream &edges, float *shared, long long row,
-                                         long long e0, long long e1, long long part)
-{
-   for (int only = -1; only < p.unit_kv; only++) {
-      op.run(p, at, edges, row, e0, e1, TOGETHER ? at.warp : 0, TOGETHER ? JOINT_WARPS : 1, only);
-      if (only < 0 && p.unit_kv > 1 && (TOGETHER ? __syncthreads_or(op.lost) : __any_sync(FULL, op.lost))) continue;
-      if (TOGETHER) join_warps<Op, G>(op, at, shared);
-      if (!TOGETHER || at.warp == 0) {
-         if (part < 0) op.finish(p, at, row, only);
-         else if (at.edge_slot == 0) op.put(part_at<Op, G>(p, at, part), at, only);
-      }
-      if (only < 0) break;
-   }
 }
 
 // TOGETHER: the warps of a block share every row (few, long rows), else each warp has a piece of its own.
@@ -810,11 +784,10 @@ __global__ void __launch_bounds__((TOGETHER ? JOINT_WARPS : PIECE_WARPS) * 32, T
    const Place at = Place::make<G>(p, static_cast<int>(job - piece * p.unit_blocks));
    const Rows rows(p);
    const long long lo = piece * p.piece, hi = lo + p.piece;
-   long long u = rows.lower_bound(lo, at.lane);
+   long long u = rows.lower_bound(lo, 0, p.m, at.lane);
    const bool teller = at.lane == 0 && (!TOGETHER || warp == 0) && job == piece * p.unit_blocks;
    long long begun = -1;
    Op op;
-   op.setup(p, at);
    EdgeStream edges;
    // row pointers 32 at a time, one to a lane
    long long from = u > 0 ? u - 1 : 0;
@@ -842,7 +815,12 @@ __global__ void __launch_bounds__((TOGETHER ? JOINT_WARPS : PIECE_WARPS) * 32, T
          part = 2 * piece + (fb >= lo);
          if (fb >= lo) begun = u;
       }
-      walk_row<Op, G, TOGETHER>(op, p, at, edges, shared, u, e0, e1, part);
+      op.run(p, at, edges, u, e0, e1, TOGETHER ? warp : 0, TOGETHER ? JOINT_WARPS : 1);
+      if (TOGETHER) join_warps<Op, G>(op, at, shared);
+      if (!TOGETHER || warp == 0) {
+         if (part < 0) op.finish(p, at, u);
+         else if (at.edge_slot == 0) op.put(part_at<Op, G>(p, at, part), at);
+      }
    }
    if (teller) p.long_row[piece] = begun;
 }
@@ -857,7 +835,6 @@ __global__ void __launch_bounds__(JOINT_WARPS * 32) join_kernel(const AttnParams
    const Place at = Place::make<G>(p, static_cast<int>(blockIdx.x - group * p.unit_blocks));
    const Rows rows(p);
    Op op;
-   op.setup(p, at);
    for (long long piece = group * JOIN_PIECES; piece < (group + 1) * JOIN_PIECES && piece < p.pieces; piece++) {
       const long long u = p.long_row[piece];
       if (u < 0) continue;
@@ -867,7 +844,7 @@ __global__ void __launch_bounds__(JOINT_WARPS * 32) join_kernel(const AttnParams
       for (long long i = warp * each; i < (warp + 1) * each && i < parts; i++)
          op.join_from(part_at<Op, G>(p, at, 2 * (piece + i) + (i == 0 ? 1 : 0)), at);
       join_warps<Op, G>(op, at, shared);
-      if (warp == 0) op.finish(p, at, u, -1);
+      if (warp == 0) op.finish(p, at, u);
    }
 }
 

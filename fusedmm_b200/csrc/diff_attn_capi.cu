@@ -66,10 +66,16 @@ Shape choose_shape(Walk w, int dtype, bool vector, long long rows, long long edg
    if (dtype == DT_BF16 || (dtype == DT_F16 && w == FORWARD)) {
       s.walk.width = need <= 4 ? 16 : need <= 8 ? 32 : need <= 16 ? 64 : 128;
       s.walk.form = !vector ? PIECES : d == s.walk.width && dv == 2 * d ? EXACT : RAGGED;
-      s.head_blocks = w == COLUMNS ? 1 : (group + 3) / 4;
-      s.unit_heads = w == COLUMNS ? 1 : (group + s.head_blocks - 1) / s.head_blocks;
+      // a product has columns for four heads of each map: query heads of one kv head first, then neighbouring kv heads
       s.unit_kv = 1;
-      while (s.unit_kv * 2 * s.unit_heads <= 4 && kv_heads % (s.unit_kv * 2) == 0) s.unit_kv *= 2;
+      if (w == COLUMNS) {
+         s.unit_heads = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+      } else {
+         s.head_blocks = (group + 3) / 4;
+         s.unit_heads = (group + s.head_blocks - 1) / s.head_blocks;
+      }
+      if (s.unit_heads == group)
+         while (s.unit_kv * 2 * s.unit_heads <= 4 && kv_heads % (s.unit_kv * 2) == 0) s.unit_kv *= 2;
       s.units = kv_heads / s.unit_kv * s.head_blocks;
       s.slot_heads = 1;
       lane_floats = w == FORWARD ? s.walk.width / 2 + 4 : w == ROWS ? s.walk.width / 2 + 2 : s.walk.width;
@@ -112,8 +118,18 @@ void apply(AttnParams &p, const Shape &s, char *scratch)
    p.long_row = reinterpret_cast<long long *>(scratch + (s.pieces * 2 * s.units * s.part_bytes + 255) / 256 * 256);
 }
 
-int launch(Walk w, int dtype, const Shape &s, const AttnParams &p, cudaStream_t st)
+int launch(Walk w, int dtype, const Shape &s, AttnParams &p, cudaStream_t st)
 {
+   const long long b = dtype == DT_F32 ? 4 : 2;
+   const bool columns = w == COLUMNS;
+   p.a_stride = static_cast<unsigned>((columns ? p.ldq : p.ldk) * b);
+   p.b_stride = static_cast<unsigned>((columns ? p.ldo : p.ldv) * b);
+   p.a_head = (columns ? p.hsq : p.hsk) * b;
+   p.b_head = (columns ? p.hso : p.hsv) * b;
+   p.a_width = p.d;
+   p.b_width = p.dv;
+   p.subs = columns ? p.group / s.unit_heads : 1;
+   p.kv_log2 = columns ? s.unit_heads >> 1 : 0;  // 1, 2, 4 -> 0, 1, 2
    int r = -1;
    if (w == FORWARD) r = dtype == DT_F32 ? walk_forward_f32(s.walk, p, st) : dtype == DT_BF16 ? walk_forward_bf16(s.walk, p, st) : walk_forward_f16(s.walk, p, st);
    if (w == ROWS) r = dtype == DT_F32 ? walk_rows_f32(s.walk, p, st) : dtype == DT_BF16 ? walk_rows_bf16(s.walk, p, st) : walk_rows_f16(s.walk, p, st);
@@ -167,7 +183,7 @@ long long walk_scratch(Walk w, int dtype, long long rows, long long edges, int h
 // and the bias in the columns' order
 long long backward_front(long long m, int heads, long long nnz)
 {
-   return round256(m * heads * 16) + round256(m * heads * 4) + round256(LAM_BLOCKS * heads * 4LL) + round256(nnz * 4);
+   return round256(m * heads * 32) + round256(m * heads * 4) + round256(LAM_BLOCKS * heads * 4LL) + round256(nnz * 4);
 }
 
 }  // namespace
@@ -255,8 +271,8 @@ int fusedmm_b200_diff_attention_backward(int32_t dtype, int32_t ptr_bits, int32_
    if (int s = sm_count(&sms)) return s;
    cudaStream_t st = static_cast<cudaStream_t>(stream);
    char *ws = static_cast<char *>(workspace);
-   float *row_dlam = reinterpret_cast<float *>(ws + round256(m * heads * 16));
-   float *lam_part = reinterpret_cast<float *>(ws + round256(m * heads * 16) + round256(m * heads * 4));
+   float *row_dlam = reinterpret_cast<float *>(ws + round256(m * heads * 32));
+   float *lam_part = reinterpret_cast<float *>(ws + round256(m * heads * 32) + round256(m * heads * 4));
    char *scratch = ws + backward_front(m, heads, nnz);
    Step step(dtype);
    step.with(q, ldq, hsq, d);
@@ -271,7 +287,7 @@ int fusedmm_b200_diff_attention_backward(int32_t dtype, int32_t ptr_bits, int32_
    p.q = q; p.k = k; p.v = v; p.lam = lam; p.dout = dout;
    p.ldq = ldq; p.hsq = hsq; p.ldk = ldk; p.hsk = hsk; p.ldv = ldv; p.hsv = hsv; p.ldo = lddo; p.hso = hsdo; p.ldlam = ldlam;
    p.lse = const_cast<float *>(lse);
-   p.stats = reinterpret_cast<float2 *>(ws);
+   p.stats = reinterpret_cast<float4 *>(ws);
    p.dlam = ldlam ? dlam : row_dlam;
    p.heads = heads; p.kv_heads = kv_heads; p.group = heads / kv_heads; p.d = d; p.dv = dv; p.step = step.step;
    p.scale = static_cast<float>(scale);

@@ -1,21 +1,22 @@
 // diff_attn_mma.cuh -- the walks of diff_attn.cuh for 16-bit types on the matrix units.
 //
-// A step takes 16 pairs (edge, kv head): HS neighbouring kv heads of 16/HS edges, HS x (query heads of a kv head) <= 4.
-// The two products of the forward walk are mma m16n8k16 with 32-bit sums:
+// The edges of a piece are one run, whatever rows they belong to.  A warp streams them through a ring of its own in shared
+// memory: a block of the ring holds 16 gathered pairs (edge, head), `slots` neighbouring heads of 16/slots edges, and is
+// filled by cp.async several blocks ahead of its use, so that the latency of the gathers, of the column ids before them and
+// of the rows' ends is hidden however few edges a row has.  Blocks are swizzled so that ldmatrix meets no bank twice; the same
+// block serves as operand with its elements as inner index (ldmatrix) and with the pairs as inner index (ldmatrix.trans).
+//
+// The products are mma m16n8k16 with 32-bit sums.  Forward:
 //   scores  [16 pairs x 8 columns], column = (map, query head): A = gathered k, B = q.  A pair and a query head of
-//           different kv heads give numbers nobody uses (HS > 1): at these sizes a wasted column costs less than the
-//           conversions and lane sums of a product on the ordinary units.
-//   output  [8 rows x dv] over k = 16 pairs: A = weights, 0 where the heads differ, B = gathered v.
+//           different kv heads give numbers nobody uses: at these sizes a wasted column costs less than the conversions and
+//           lane sums of a product on the ordinary units.
+//   output  [8 rows x dv] over the 16 pairs: A = weights, 0 where the heads differ or the edge is another row's,
+//           B = gathered v.
 // Weights are split into two 16-bit numbers whose sum has 16 bits (bf16) or 22 (half) of the 32-bit value; the second lies in
-// the rows 8..15 of A that the first leaves free, so the split costs no product.
-// The order of a product's inner index is free as long as both operands share it: every lane loads 8 consecutive elements
-// of a gathered row as they are, no shared memory and no transposition; where an operand has the pairs as inner index
-// two rows' elements are put side by side with byte permutes.  The weights change from "pair by column" to "row by pair"
-// with movmatrix.
+// the rows 8..15 of A that the first leaves free, so the split costs no product.  They change from "pair by column" to "row
+// by pair" with movmatrix.
 // Why not tcgen05: a tile there has 64 or 128 rows that share one operand; here a gathered row meets at most 8 rows of q,
 // and consecutive rows of the pattern gather different rows.
-//
-// Measured against the walks on the ordinary units see the choice of the shape in diff_attn_capi.cu.
 #pragma once
 #include "diff_attn.cuh"
 
@@ -25,7 +26,7 @@ namespace attn {
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1)
 {
-   if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
+   if constexpr (std::is_same<T, __half>::value)
       asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                    : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
    else
@@ -38,6 +39,23 @@ __device__ __forceinline__ unsigned transpose8x8(unsigned v)
    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
    return r;
 }
+__device__ __forceinline__ void ldmatrix4(unsigned (&r)[4], unsigned at)
+{
+   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(unsigned (&r)[4], unsigned at)
+{
+   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+// `there` bytes from global memory, zeros behind them (0: nothing is read)
+template <int BYTES>
+__device__ __forceinline__ void copy_async(unsigned to, const void *from, int there)
+{
+   if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there) : "memory");
+   else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(there) : "memory");
+}
 // v as the sum of two numbers of T, for two neighbours
 template <typename T>
 __device__ __forceinline__ void split2(float a, float b, unsigned &hi, unsigned &lo)
@@ -48,119 +66,165 @@ __device__ __forceinline__ void split2(float a, float b, unsigned &hi, unsigned 
    lo = Elt<T>::pack2(a - x, b - y);
 }
 
-// E elements (2, 4 or 8) at p, `left` of them there
-template <typename T, int E, int FORM>
-__device__ __forceinline__ void load_part(const T *p, int left, int step, unsigned (&r)[E / 2])
+// two elements of a row, those of them that are there
+template <typename T, int FORM>
+__device__ __forceinline__ unsigned load_two(const T *p, int left, int step)
 {
-   if constexpr (FORM == PIECES) {
-      const uint4 v = ld_pieces(p, left < E ? left : E, step < E ? step : E);
-      r[0] = v.x;
-      if constexpr (E >= 4) r[1] = v.y;
-      if constexpr (E == 8) { r[2] = v.z; r[3] = v.w; }
+   if (FORM == EXACT || (left >= 2 && (FORM == RAGGED || step >= 2))) return __ldg(reinterpret_cast<const unsigned *>(p));
+   const unsigned short *u = reinterpret_cast<const unsigned short *>(p);
+   return (left > 0 ? __ldg(u) : 0u) | (left > 1 ? static_cast<unsigned>(__ldg(u + 1)) << 16 : 0u);
+}
+// a row as the B operand of this lane's column: elements 2c, 2c + 1 of every 8
+template <typename T, int WIDTH, int FORM>
+__device__ __forceinline__ void load_operand(const T *row, int c, int width, int step, unsigned (&r)[WIDTH / 8])
+{
+#pragma unroll
+   for (int i = 0; i < WIDTH / 8; i++) r[i] = load_two<T, FORM>(row + 8 * i + 2 * c, width - 8 * i - 2 * c, step);
+}
+template <typename T, int FORM>
+__device__ __forceinline__ void store_two(T *p, float a, float b, int left)
+{
+   if (FORM != PIECES) {
+      if (left > 0) *reinterpret_cast<unsigned *>(p) = Elt<T>::pack2(a, b);
    } else {
-      const bool there = FORM == EXACT || left > 0;
-      if constexpr (E == 8) {
-         const uint4 v = there ? ldg16(p) : make_uint4(0u, 0u, 0u, 0u);
-         r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
-      } else if constexpr (E == 4) {
-         const uint2 v = there ? __ldg(reinterpret_cast<const uint2 *>(p)) : make_uint2(0u, 0u);
-         r[0] = v.x; r[1] = v.y;
-      } else {
-         r[0] = there ? __ldg(reinterpret_cast<const unsigned *>(p)) : 0u;
-      }
+      if (left > 0) p[0] = Elt<T>::down(a);
+      if (left > 1) p[1] = Elt<T>::down(b);
    }
 }
 
-// A row of WIDTH elements as the lanes hold it when its elements are the inner index: lane c (of 4) has the elements
-// 4 E s + E c .. + E - 1 of every set s; two registers make a step of 16 elements.
-template <typename T, int WIDTH>
-struct Inner {
-   static constexpr int E = WIDTH / 4 < 8 ? WIDTH / 4 : 8, SETS = WIDTH / (4 * E), REGS = WIDTH / 8, STEPS = WIDTH / 16;
-   template <int FORM>
-   static __device__ __forceinline__ void load(const T *row, int c, int width, bool live, int step, unsigned (&r)[REGS])
-   {
-#pragma unroll
-      for (int s = 0; s < SETS; s++) {
-         const int x = 4 * E * s + E * c;
-         unsigned part[E / 2];
-         load_part<T, E, FORM>(row + x, live ? width - x : 0, step, part);
-#pragma unroll
-         for (int i = 0; i < E / 2; i++) r[s * (E / 2) + i] = part[i];
-      }
-   }
-};
-// ... and when its elements are rows or columns of the product: lane group g (of 8) has the elements 8 E s + E g .. + E - 1.
-template <typename T, int WIDTH>
-struct Outer {
-   static constexpr int E = WIDTH / 8 < 8 ? WIDTH / 8 : 8, SETS = WIDTH / (8 * E), REGS = WIDTH / 16;
-   template <int FORM>
-   static __device__ __forceinline__ void load(const T *row, int g, int width, bool live, int step, unsigned (&r)[REGS])
-   {
-#pragma unroll
-      for (int s = 0; s < SETS; s++) {
-         const int x = 8 * E * s + E * g;
-         unsigned part[E / 2];
-         load_part<T, E, FORM>(row + x, live ? width - x : 0, step, part);
-#pragma unroll
-         for (int i = 0; i < E / 2; i++) r[s * (E / 2) + i] = part[i];
-      }
-   }
-   // E consecutive results of this lane's rows to memory
-   template <bool VECTOR>
-   static __device__ __forceinline__ void store(T *p, const float (&f)[E], int left)
-   {
-      if constexpr (VECTOR) {
-         if (left <= 0) return;
-         unsigned r[E / 2];
-#pragma unroll
-         for (int i = 0; i < E / 2; i++) r[i] = Elt<T>::pack2(f[2 * i], f[2 * i + 1]);
-         if constexpr (E == 8) *reinterpret_cast<uint4 *>(p) = make_uint4(r[0], r[1], r[2], r[3]);
-         else if constexpr (E == 4) *reinterpret_cast<uint2 *>(p) = make_uint2(r[0], r[1]);
-         else *reinterpret_cast<unsigned *>(p) = r[0];
-      } else {
-#pragma unroll
-         for (int i = 0; i < E; i++)
-            if (i < left) p[i] = Elt<T>::down(f[i]);
-      }
-   }
-};
-__device__ __forceinline__ unsigned low_halves(unsigned a, unsigned b) { return __byte_perm(a, b, 0x5410); }
-__device__ __forceinline__ unsigned high_halves(unsigned a, unsigned b) { return __byte_perm(a, b, 0x7632); }
-
-// a gathered array: pointers of this lane's head, byte stride of rows
-template <typename T>
-struct Source {
-   const char *base;
-   unsigned stride;
-   __device__ __forceinline__ void set(const void *array, long long ld, long long offset)
-   {
-      base = static_cast<const char *>(array) + offset * static_cast<long long>(sizeof(T));
-      stride = static_cast<unsigned>(ld * static_cast<long long>(sizeof(T)));
-   }
-   template <int FORM>
-   __device__ __forceinline__ const T *row(int id) const
-   {
-      const T *r = reinterpret_cast<const T *>(base + static_cast<unsigned long long>(static_cast<unsigned>(id)) * stride);
-      return FORM == EXACT && id < 0 ? reinterpret_cast<const T *>(zero_row) : r;
-   }
-};
-
-// Lane geometry that the three walks share.  Lane = 4 r + c.  As an operand's row (or column) r: the query head and map of
-// column n = r; as a result: the pairs r and r + 8, the columns 2c and 2c + 1.
+// Lane geometry that the three walks share.  Lane = 4 r + c.  As an operand's row (or column) r: column n = r of the scores,
+// map r / 4, slot r % 4; as a result: the pairs r and r + 8, the columns 2c and 2c + 1.
 struct Lanes {
-   int r, c, hs, hs_log2, kv0, pair_head;  // pair_head: which of the unit's kv heads the pairs r and r + 8 are of
-   __device__ __forceinline__ void set(const AttnParams &p, const Place &at)
+   int r, c, slots, slots_log2, pair_slot;  // pair_slot: of the pairs r and r + 8
+   __device__ __forceinline__ void set(const Place &at, int slots_)
    {
       r = at.lane >> 2;
       c = at.lane & 3;
-      hs = p.unit_kv;
-      hs_log2 = hs >> 1;  // 1, 2, 4 -> 0, 1, 2
-      kv0 = (at.unit / p.head_blocks) * hs;
-      pair_head = r & (hs - 1);
+      slots = slots_;
+      slots_log2 = slots_ >> 1;  // 1, 2, 4 -> 0, 1, 2
+      pair_slot = r & (slots - 1);
    }
-   // the edge, counted from the step's first, of a pair
-   __device__ __forceinline__ int edge(int pair) const { return pair >> hs_log2; }
 };
+
+// The ring of a warp: STAGES blocks of 16 pairs, each of two gathered rows of 2 DK elements (k of both maps and v, or q and
+// do), 16 biases and, where the walk wants them, 16 records of 32 bytes.
+template <typename T, int DK, int FORM, int STAGES_, bool RECORDS>
+struct Ring {
+   static constexpr int STAGES = STAGES_, ROW = 4 * DK, CHUNKS = DK / 4, REGION = 16 * ROW;
+   static constexpr int BIAS = 2 * REGION, RECORD = BIAS + 64, STAGE = RECORD + (RECORDS ? 16 * 32 : 0);
+   const char *a, *b;       // the two arrays at the unit's first head; strides are in AttnParams
+   const char *records;     // [row][head][32 bytes], of the unit's first head
+   EdgeStream edges;
+   unsigned ring;           // shared address
+   long long first, end;    // the run of edges
+   int issued, current;     // blocks
+   int only;                // the only kv head of the unit whose pairs are gathered, or -1
+
+   // byte offset of a chunk of 8 elements
+   static __device__ __forceinline__ unsigned at(int pair, int chunk)
+   {
+      const int key = CHUNKS >= 8 ? pair & 7 : (pair >> 1) & 3;
+      return pair * ROW + ((chunk ^ key) << 4);
+   }
+   __device__ __forceinline__ unsigned slot_of(int block) const { return ring + (block % STAGES) * STAGE; }
+
+   __device__ __forceinline__ void chunk_in(unsigned to, const T *from, int left, int step) const
+   {
+      if constexpr (FORM != PIECES) {
+         copy_async<16>(to, from, left > 0 ? 16 : 0);
+      } else {
+         if (step >= 4) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) copy_async<8>(to + 8 * i, left > 4 * i ? from + 4 * i : from, left > 4 * i ? 8 : 0);
+         } else if (step >= 2) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) copy_async<4>(to + 4 * i, left > 2 * i ? from + 2 * i : from, left > 2 * i ? 4 : 0);
+         } else {
+            const uint4 v = ld_pieces(from, left, 1);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+         }
+      }
+   }
+
+   // gathers the next block, if there is one; always closes a group of copies
+   __device__ __forceinline__ void issue(const AttnParams &p, const Lanes &l, int lane)
+   {
+      const int per_block = 16 >> l.slots_log2;
+      const int edge_block = p.subs == 1 ? issued : issued / p.subs, sub = p.subs == 1 ? 0 : issued - edge_block * p.subs;
+      const long long e = first + static_cast<long long>(edge_block) * per_block;
+      if (e < end) {
+         const long long batch = first + (e - first) / 32 * 32;
+         const int off = static_cast<int>(e - batch);
+         const int my_id = edges.take(p, batch, end, lane);
+         const float my_bias = my_id >= 0 ? edges.bias : -INFINITY;
+         const unsigned to = slot_of(issued);
+         const float bias = __shfl_sync(FULL, my_bias, off + (lane & (per_block - 1)));
+         if (lane < per_block) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + BIAS + 4 * lane), "f"(bias) : "memory");
+         constexpr int TIMES = CHUNKS / 2, PER = 32 / CHUNKS;  // pairs of one round
+         const int x = lane % CHUNKS, pair0 = lane / CHUNKS;
+         // first array: chunk x of both maps' elements; second: chunk x
+         const int map = x / (CHUNKS / 2), xa = (x % (CHUNKS / 2)) * 8, xb = x * 8;
+         const int left_a = p.a_width - xa, left_b = p.b_width - xb;
+         const int head0 = sub << p.kv_log2;
+#pragma unroll
+         for (int i = 0; i < TIMES; i++) {
+            const int pair = i * PER + pair0, s = (PER >= 4 ? pair0 : pair) & (l.slots - 1);
+            int id = __shfl_sync(FULL, my_id, off + (pair >> l.slots_log2));
+            if (only >= 0 && (s >> p.kv_log2) != only) id = -1;
+            const bool live = id >= 0;
+            const unsigned row = live ? id : 0;
+            const T *ra = reinterpret_cast<const T *>(a + static_cast<unsigned long long>(row) * p.a_stride + (s + head0) * p.a_head);
+            const T *rb = reinterpret_cast<const T *>(b + static_cast<unsigned long long>(row) * p.b_stride + (s + head0) * p.b_head);
+            const unsigned place = to + at(pair, x);
+            chunk_in(place, ra + map * p.a_width + xa, live ? left_a : 0, p.step);
+            chunk_in(place + REGION, rb + xb, live ? left_b : 0, p.step);
+         }
+         if constexpr (RECORDS) {
+            const int pair = lane >> 1, s = pair & (l.slots - 1);
+            const int id = __shfl_sync(FULL, my_id, off + (pair >> l.slots_log2));
+            const unsigned row = id >= 0 ? id : 0;
+            copy_async<16>(to + RECORD + lane * 16, records + static_cast<unsigned long long>(row) * (p.heads * 32u) + (s + head0) * 32 + (lane & 1) * 16,
+                           id >= 0 ? 16 : 0);
+         }
+         // the last block of a batch of ids: the next batch sets out
+         if (off + per_block == 32 && sub == p.subs - 1) edges.fetch(p, batch + 32, lane);
+      }
+      issued++;
+      asm volatile("cp.async.commit_group;" ::: "memory");
+   }
+   __device__ __forceinline__ void begin(const AttnParams &p, const Lanes &l, int lane, long long from, long long to, int only_kv)
+   {
+      drain();
+      first = from;
+      end = to;
+      only = only_kv;
+      issued = 0;
+      current = -1;
+#pragma unroll 1
+      for (int i = 0; i < STAGES - 1; i++) issue(p, l, lane);
+   }
+   // the next block; the one before it may be overwritten
+   __device__ __forceinline__ void advance(const AttnParams &p, const Lanes &l, int lane)
+   {
+      __syncwarp();  // every lane is done with the block before
+      issue(p, l, lane);
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+      __syncwarp();  // every lane's copies are there
+      current++;
+   }
+   __device__ __forceinline__ void drain()
+   {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
+   }
+};
+
+__device__ __forceinline__ float shared_float(unsigned at)
+{
+   float f;
+   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(at) : "memory");
+   return f;
+}
 
 // value of column n = r from the lanes that hold the columns 2c and 2c + 1 (the same in all r)
 __device__ __forceinline__ float of_column(float x0, float x1, int r)
@@ -181,26 +245,27 @@ __device__ __forceinline__ float max_pairs(float v)
    return fmaxf(v, __shfl_xor_sync(FULL, v, 16));
 }
 
-// The query heads of the row walks' columns: column n = 4 map + s, s = (kv head of the unit) * per_kv + (query head of it).
+// The query heads of the row walks' columns: column n = 4 map + s, s = (kv head of the unit) * unit_heads + (query head of it).
 struct QueryHeads {
-   int head;       // of column n = r, clamped to a head that exists
-   bool live;      // column n = r is one
-   bool valid[2];  // the pairs r and r + 8 belong to the columns 2c, 2c + 1
-   int col_head[2];
-   int kv;         // which of the unit's kv heads column n = r is of
-   __device__ __forceinline__ void set(const AttnParams &p, const Place &at, const Lanes &l)
+   int head;        // of column n = r, one that exists if that column is none
+   bool live;       // column n = r is one
+   int kv;          // which of the unit's kv heads column n = r is of
+   bool valid[2];   // the pairs r and r + 8 belong to the columns 2c, 2c + 1
+   int col_head[2], col_kv[2];
+   __device__ __forceinline__ void set(const AttnParams &p, const Place &at, const Lanes &l, int kv0)
    {
-      const int block = at.unit % p.head_blocks, first = block * p.unit_heads, rest = p.group - first;
+      const int first = (at.unit % p.head_blocks) * p.unit_heads, rest = p.group - first;
       const int heads = rest < p.unit_heads ? rest : p.unit_heads;
       const int s = l.r & 3, g = s % p.unit_heads;
       kv = s / p.unit_heads;
-      live = kv < l.hs && g < heads;
-      head = live ? (l.kv0 + kv) * p.group + first + g : l.kv0 * p.group + first;
+      live = kv < l.slots && g < heads;
+      head = live ? (kv0 + kv) * p.group + first + g : kv0 * p.group + first;
 #pragma unroll
       for (int x = 0; x < 2; x++) {
-         const int sx = (2 * l.c + x) & 3, kx = sx / p.unit_heads, gx = sx % p.unit_heads;
-         valid[x] = kx == l.pair_head && gx < heads;
-         col_head[x] = valid[x] ? (l.kv0 + kx) * p.group + first + gx : head;
+         const int sx = (2 * l.c + x) & 3, gx = sx % p.unit_heads;
+         col_kv[x] = sx / p.unit_heads;
+         valid[x] = col_kv[x] == l.pair_slot && gx < heads;
+         col_head[x] = valid[x] ? (kv0 + col_kv[x]) * p.group + first + gx : head;
       }
    }
 };
@@ -209,29 +274,41 @@ struct QueryHeads {
 // row's scaling is done once as a rule.  32-bit sums and 16-bit weights (half: up to 65504) hold e^5 with room.
 constexpr float SLACK = 5.0f;
 
+// warps of a block and blocks of a multiprocessor: registers and rings decide (a warp's ring is STAGES x 128 DK bytes)
+template <int DK>
+struct Budget {
+   static constexpr int STAGES = DK == 16 ? 4 : DK == 32 ? 3 : 2;
+   static constexpr int SOLO = DK == 128 ? 2 : 4, JOINT = DK == 128 ? 4 : 8;
+   static constexpr int BLOCKS = DK <= 32 ? 4 : 3;
+   static constexpr bool AHEAD = DK <= 32;  // a row's own operands are fetched during the row before (wider: no registers left)
+};
+
 // ---------------------------------------------------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int DK, int DV, int FORM>
+template <typename T, int DK, int FORM>
 struct ForwardMma {
-   static constexpr int BLOCKS = DV <= 64 ? 4 : DV <= 128 ? 3 : 2;
-   static constexpr int TILES = DV / 8;
-   static constexpr int LANE_FLOATS = 2 * TILES + 4;
-   using KIn = Inner<T, DK>;
-   using VOut = Outer<T, DV>;
+   static constexpr int DV = 2 * DK, TILES = DV / 8, LANE_FLOATS = 2 * TILES + 4;
+   using Gathered = Ring<T, DK, FORM, Budget<DK>::STAGES, false>;
+   using Width = Budget<DK>;
    struct State {
-      float acc[TILES][2];   // rows n = r: sums of weights times v
-      float top[2], sum[2];  // columns 2c, 2c + 1; sum: of this lane's pairs until the end of run()
+      float acc[TILES][2];   // rows n = r: sums of weights times v, columns 8t + 2c, + 1
+      float top[2], sum[2];  // columns 2c, 2c + 1
    };
    State s;
    Lanes l;
    QueryHeads heads;
+   int kv0;
+   unsigned next[DK / 8];
    bool lost;  // run() met a number that is none
 
-   __device__ __forceinline__ void setup(const AttnParams &p, const Place &at)
+   __device__ __forceinline__ void setup(const AttnParams &p, const Place &at, Gathered &ring)
    {
-      l.set(p, at);
-      heads.set(p, at, l);
+      l.set(at, p.unit_kv);
+      kv0 = (at.unit / p.head_blocks) * p.unit_kv;
+      heads.set(p, at, l, kv0);
+      ring.a = static_cast<const char *>(p.k) + kv0 * p.a_head;
+      ring.b = static_cast<const char *>(p.v) + kv0 * p.b_head;
    }
    static __device__ __forceinline__ void clear(State &s)
    {
@@ -240,71 +317,62 @@ struct ForwardMma {
       s.top[0] = s.top[1] = -INFINITY;
       s.sum[0] = s.sum[1] = 0.0f;
    }
-
-   __device__ __forceinline__ void run(const AttnParams &p, const Place &at, EdgeStream &edges, long long row, long long e0, long long e1,
-                                       int warp, int warps, int only)
+   // the row's own operand, ahead of run()
+   __device__ __forceinline__ void fetch(const AttnParams &p, long long row)
    {
-      lost = false;
-      clear(s);
-      if (e0 + 32 * warp >= e1) return;
+      load_operand<T, DK, FORM>(static_cast<const T *>(p.q) + row * p.ldq + heads.head * p.hsq + (l.r >> 2) * p.d, l.c, p.d, p.step, next);
+   }
+
+   // edges [e0, e1) of the ring's run; `follow`: the row to fetch for, or -1
+   __device__ __forceinline__ void run(const AttnParams &p, const Place &at, Gathered &ring, int e0, int e1, long long follow)
+   {
       float acc[TILES][4];
 #pragma unroll
       for (int t = 0; t < TILES; t++) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.0f;
-      unsigned q[KIn::REGS];
-      KIn::template load<FORM>(static_cast<const T *>(p.q) + row * p.ldq + heads.head * p.hsq + (l.r >> 2) * p.d, l.c, p.d, true, p.step, q);
-      Source<T> kg, vg[2];
-      kg.set(p.k, p.ldk, (l.kv0 + l.pair_head) * p.hsk);
-      const int even = (2 * l.c) & (l.hs - 1), odd = (2 * l.c + 1) & (l.hs - 1);
-      vg[0].set(p.v, p.ldv, (l.kv0 + even) * p.hsv);
-      vg[1].set(p.v, p.ldv, (l.kv0 + odd) * p.hsv);
-      const bool skip[2] = {only >= 0 && even != only, only >= 0 && odd != only};
-      const int per_step = 16 >> l.hs_log2;
-      for (long long base = e0 + 32 * warp; base < e1; base += 32 * warps) {
-         const int my_id = edges.take(p, base, e1, at.lane);
-         const float my_bias = edges.bias;
-         edges.fetch(p, base + 32 * warps < e1 ? base + 32 * warps : e1 + 32 * warp, at.lane);
-         const int count = static_cast<int>(e1 - base < 32 ? e1 - base : 32);
-         for (int first = 0; first < count; first += per_step) {
-            // gathered rows: k of the pairs r and r + 8, v of the pairs 2c, 2c + 1, 2c + 8, 2c + 9
-            int id[2];
-            unsigned k[2][2][KIn::REGS], v[4][VOut::REGS];
+      s.top[0] = s.top[1] = -INFINITY;
+      s.sum[0] = s.sum[1] = 0.0f;
+      unsigned q[DK / 8];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-               id[h] = __shfl_sync(FULL, my_id, first + l.edge(l.r + 8 * h));
-               const T *src = kg.template row<FORM>(id[h]);
-               KIn::template load<FORM>(src, l.c, p.d, id[h] >= 0, p.step, k[0][h]);
-               KIn::template load<FORM>(FORM == EXACT && id[h] < 0 ? src : src + p.d, l.c, p.d, id[h] >= 0, p.step, k[1][h]);
+      for (int i = 0; i < DK / 8; i++) q[i] = next[i];
+      if (Width::AHEAD && follow >= 0) fetch(p, follow);
+      const int per_log2 = 4 - l.slots_log2;
+      // rows of ldmatrix: lane's pair and chunk parity
+      const int pair = at.lane & 15, high = at.lane >> 4;
+      for (int e = e0; e < e1;) {
+         const int block = e >> per_log2;
+         if (block != ring.current) ring.advance(p, l, at.lane);
+         const int lo = e - (block << per_log2), left = e1 - (block << per_log2), hi = left < (1 << per_log2) ? left : 1 << per_log2;
+         const unsigned slot = ring.slot_of(block);
+         float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+         for (int i = 0; i < DK / 16; i++) {
+            unsigned k[4];
+            ldmatrix4(k, slot + Gathered::at(pair, 2 * i + high));
+            mma16816<T>(s0, k[0], k[1], k[2], k[3], q[2 * i], q[2 * i + 1]);
+            ldmatrix4(k, slot + Gathered::at(pair, DK / 8 + 2 * i + high));
+            mma16816<T>(s1, k[0], k[1], k[2], k[3], q[2 * i], q[2 * i + 1]);
+         }
+         float score[2][2];
+#pragma unroll
+         for (int h = 0; h < 2; h++) {
+            const int edge = (l.r + 8 * h) >> l.slots_log2;
+            const float bias = shared_float(slot + Gathered::BIAS + 4 * edge);
+            const bool live = edge >= lo && edge < hi && bias != -INFINITY;
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+               const float dot = l.c < 2 ? s0[2 * h + x] : s1[2 * h + x];
+               score[h][x] = heads.valid[x] && live ? fmaf(dot, p.scale, bias) : -INFINITY;
             }
-#pragma unroll
-            for (int h = 0; h < 4; h++) {
-               int vid = __shfl_sync(FULL, my_id, first + l.edge(2 * l.c + (h & 1) + 8 * (h >> 1)));
-               if (skip[h & 1]) vid = -1;
-               VOut::template load<FORM>(vg[h & 1].template row<FORM>(vid), l.r, p.dv, vid >= 0, p.step, v[h]);
-            }
-            float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < KIn::STEPS; i++) {
-               mma16816<T>(s0, k[0][0][2 * i], k[0][1][2 * i], k[0][0][2 * i + 1], k[0][1][2 * i + 1], q[2 * i], q[2 * i + 1]);
-               mma16816<T>(s1, k[1][0][2 * i], k[1][1][2 * i], k[1][0][2 * i + 1], k[1][1][2 * i + 1], q[2 * i], q[2 * i + 1]);
-            }
-            float score[2][2];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-               const float bias = p.bias ? __shfl_sync(FULL, my_bias, first + l.edge(l.r + 8 * h)) : 0.0f;
-#pragma unroll
-               for (int x = 0; x < 2; x++) {
-                  const float dot = l.c < 2 ? s0[2 * h + x] : s1[2 * h + x];
-                  score[h][x] = heads.valid[x] && id[h] >= 0 ? fmaf(dot, p.scale, bias) : -INFINITY;
-               }
-            }
-            const float m0 = fmaxf(score[0][0], score[1][0]), m1 = fmaxf(score[0][1], score[1][1]);
-            if (__any_sync(FULL, m0 > s.top[0] + SLACK || m1 > s.top[1] + SLACK)) {
-               const float t0 = fmaxf(s.top[0], max_pairs(m0)), t1 = fmaxf(s.top[1], max_pairs(m1));
-               const float f0 = t0 == -INFINITY ? 1.0f : exp2_fast((s.top[0] - t0) * LOG2E);
-               const float f1 = t1 == -INFINITY ? 1.0f : exp2_fast((s.top[1] - t1) * LOG2E);
+         }
+         const float m0 = fmaxf(score[0][0], score[1][0]), m1 = fmaxf(score[0][1], score[1][1]);
+         if (__any_sync(FULL, m0 > s.top[0] + SLACK || m1 > s.top[1] + SLACK)) {
+            const float t0 = fmaxf(s.top[0], max_pairs(m0)), t1 = fmaxf(s.top[1], max_pairs(m1));
+            const float f0 = t0 == -INFINITY ? 1.0f : exp2_fast((s.top[0] - t0) * LOG2E);
+            const float f1 = t1 == -INFINITY ? 1.0f : exp2_fast((s.top[1] - t1) * LOG2E);
+            s.top[0] = t0;
+            s.top[1] = t1;
+            if (e != e0) {
                const float f = of_column(f0, f1, l.r);
-               s.top[0] = t0;
-               s.top[1] = t1;
                s.sum[0] *= f0;
                s.sum[1] *= f1;
 #pragma unroll
@@ -312,35 +380,38 @@ struct ForwardMma {
 #pragma unroll
                   for (int i = 0; i < 4; i++) acc[t][i] *= f;
             }
-            // a row that has met no edge yet has the maximum -inf: its differences are taken from 0
-            const float ref0 = s.top[0] == -INFINITY ? 0.0f : s.top[0], ref1 = s.top[1] == -INFINITY ? 0.0f : s.top[1];
-            unsigned a[4];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-               // the difference is taken before the factor: scores near the type's largest numbers keep their order
-               const float p0 = exp2_fast((score[h][0] - ref0) * LOG2E), p1 = exp2_fast((score[h][1] - ref1) * LOG2E);
-               s.sum[0] += p0;
-               s.sum[1] += p1;
-               unsigned hi, lo;
-               split2<T>(p0, p1, hi, lo);
-               a[2 * h] = transpose8x8(hi);
-               a[2 * h + 1] = transpose8x8(lo);
-            }
-#pragma unroll
-            for (int t = 0; t < VOut::REGS; t++) {
-               mma16816<T>(acc[2 * t], a[0], a[1], a[2], a[3], low_halves(v[0][t], v[1][t]), low_halves(v[2][t], v[3][t]));
-               mma16816<T>(acc[2 * t + 1], a[0], a[1], a[2], a[3], high_halves(v[0][t], v[1][t]), high_halves(v[2][t], v[3][t]));
-            }
          }
+         // a row that has met no edge yet has the maximum -inf: its differences are taken from 0
+         const float ref0 = s.top[0] == -INFINITY ? 0.0f : s.top[0], ref1 = s.top[1] == -INFINITY ? 0.0f : s.top[1];
+         unsigned a[4];
+#pragma unroll
+         for (int h = 0; h < 2; h++) {
+            // the difference is taken before the factor: scores near the type's largest numbers keep their order
+            const float p0 = exp2_fast((score[h][0] - ref0) * LOG2E), p1 = exp2_fast((score[h][1] - ref1) * LOG2E);
+            s.sum[0] += p0;
+            s.sum[1] += p1;
+            unsigned up, low;
+            split2<T>(p0, p1, up, low);
+            a[2 * h] = transpose8x8(up);
+            a[2 * h + 1] = transpose8x8(low);
+         }
+#pragma unroll
+         for (int t = 0; t < TILES; t += 2) {
+            unsigned v[4];
+            ldmatrix4_trans(v, slot + Gathered::REGION + Gathered::at(pair, t + high));
+            mma16816<T>(acc[t], a[0], a[1], a[2], a[3], v[0], v[1]);
+            mma16816<T>(acc[t + 1], a[0], a[1], a[2], a[3], v[2], v[3]);
+         }
+         e = (block << per_log2) + hi;
       }
-      bool bad = false;
+      float all = 0.0f;
 #pragma unroll
       for (int t = 0; t < TILES; t++) {
          s.acc[t][0] = acc[t][0] + acc[t][2];
          s.acc[t][1] = acc[t][1] + acc[t][3];
-         bad |= s.acc[t][0] != s.acc[t][0] || s.acc[t][1] != s.acc[t][1];
+         all += s.acc[t][0] * 0.0f + s.acc[t][1] * 0.0f;  // 0, or NaN once anything is infinite or NaN
       }
-      lost = bad;
+      lost = all != all;
       s.sum[0] = sum_pairs(s.sum[0]);
       s.sum[1] = sum_pairs(s.sum[1]);
    }
@@ -374,30 +445,44 @@ struct ForwardMma {
 #pragma unroll
          for (int t = 0; t < TILES; t++) to[32 * t] = make_float2(s.acc[t][0], s.acc[t][1]);
       }
-      to[32 * TILES] = make_float2(s.top[0], s.top[1]);
-      to[32 * (TILES + 1)] = make_float2(s.sum[0], s.sum[1]);
+      float *top = reinterpret_cast<float *>(to + 32 * TILES), *sum = reinterpret_cast<float *>(to + 32 * (TILES + 1));
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+         if (only < 0 || heads.col_kv[x] == only) {
+            top[x] = s.top[x];
+            sum[x] = s.sum[x];
+         }
    }
 
    __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long row, int only)
    {
       const float sum = of_column(s.sum[0], s.sum[1], l.r), top = of_column(s.top[0], s.top[1], l.r);
       const bool mine = heads.live && (only < 0 || heads.kv == only);
-      const float lam = __ldg(p.lam + row * p.ldlam + heads.head), f = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const float lam = __ldg(p.lam + row * p.ldlam + heads.head), f = sum == 0.0f ? 0.0f : __frcp_rn(sum);
       const long long rh = row * p.heads + heads.head;
+      T *out = static_cast<T *>(p.out) + rh * p.dv + 2 * l.c;
 #pragma unroll
-      for (int set = 0; set < VOut::SETS; set++)
+      for (int t = 0; t < TILES; t++) {
+         float o[2];
 #pragma unroll
          for (int x = 0; x < 2; x++) {
-            float o[VOut::E];
-#pragma unroll
-            for (int j = 0; j < VOut::E; j++) {
-               const float v = s.acc[set * VOut::E + j][x] * f;
-               o[j] = v - lam * __shfl_xor_sync(FULL, v, 16);
-            }
-            const int y = 8 * VOut::E * set + VOut::E * (2 * l.c + x);
-            if (mine && l.r < 4) VOut::template store<FORM != PIECES>(static_cast<T *>(p.out) + rh * p.dv + y, o, p.dv - y);
+            const float v = s.acc[t][x] * f;
+            o[x] = v - lam * __shfl_xor_sync(FULL, v, 16);
          }
+         if (mine && l.r < 4) store_two<T, FORM>(out + 8 * t, o[0], o[1], p.dv - 8 * t - 2 * l.c);
+      }
       if (mine && l.c == 0 && p.lse) p.lse[rh * 2 + (l.r >> 2)] = top + LN2 * log2f(sum);
+   }
+   __device__ __forceinline__ void finish_empty(const AttnParams &p, const Place &at, long long row)
+   {
+      if (!heads.live) return;
+      const long long rh = row * p.heads + heads.head;
+      T *out = static_cast<T *>(p.out) + rh * p.dv + 2 * l.c;
+      if (l.r < 4) {
+#pragma unroll
+         for (int t = 0; t < TILES; t++) store_two<T, FORM>(out + 8 * t, 0.0f, 0.0f, p.dv - 8 * t - 2 * l.c);
+      }
+      if (l.c == 0 && p.lse) p.lse[rh * 2 + (l.r >> 2)] = -INFINITY;
    }
 };
 
@@ -405,14 +490,11 @@ struct ForwardMma {
 // backward over the rows (the sums A = sum p dP k, B = sum p k, D = sum p dP of BackwardRows).  For map 0 the rows of A's
 // operand are w = p dP of the columns 0..3 and p of the same, for map 1 the other way round.
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int DK, int DV, int FORM>
+template <typename T, int DK, int FORM>
 struct BackwardRowsMma {
-   static constexpr int BLOCKS = DV <= 64 ? 4 : DV <= 128 ? 3 : 2;
-   static constexpr int TILES = DK / 8;
-   static constexpr int LANE_FLOATS = 4 * TILES + 2;
-   using KIn = Inner<T, DK>;
-   using KOut = Outer<T, DK>;
-   using VIn = Inner<T, DV>;
+   static constexpr int DV = 2 * DK, TILES = DK / 8, LANE_FLOATS = 4 * TILES + 2;
+   using Gathered = Ring<T, DK, FORM, Budget<DK>::STAGES, false>;
+   using Width = Budget<DK>;
    struct State {
       float acc[2][TILES][2];
       float delta[2];  // columns 2c, 2c + 1
@@ -420,12 +502,18 @@ struct BackwardRowsMma {
    State s;
    Lanes l;
    QueryHeads heads;
+   int kv0;
+   unsigned next[DK / 8], next_out[DV / 8];
+   float next_lse[2];
    bool lost;
 
-   __device__ __forceinline__ void setup(const AttnParams &p, const Place &at)
+   __device__ __forceinline__ void setup(const AttnParams &p, const Place &at, Gathered &ring)
    {
-      l.set(p, at);
-      heads.set(p, at, l);
+      l.set(at, p.unit_kv);
+      kv0 = (at.unit / p.head_blocks) * p.unit_kv;
+      heads.set(p, at, l, kv0);
+      ring.a = static_cast<const char *>(p.k) + kv0 * p.a_head;
+      ring.b = static_cast<const char *>(p.v) + kv0 * p.b_head;
    }
    static __device__ __forceinline__ void clear(State &s)
    {
@@ -435,112 +523,101 @@ struct BackwardRowsMma {
          for (int t = 0; t < TILES; t++) s.acc[m][t][0] = s.acc[m][t][1] = 0.0f;
       s.delta[0] = s.delta[1] = 0.0f;
    }
-
-   __device__ __forceinline__ void run(const AttnParams &p, const Place &at, EdgeStream &edges, long long row, long long e0, long long e1,
-                                       int warp, int warps, int only)
+   __device__ __forceinline__ void fetch(const AttnParams &p, long long row)
    {
-      lost = false;
-      clear(s);
-      if (e0 + 32 * warp >= e1) return;
+      load_operand<T, DK, FORM>(static_cast<const T *>(p.q) + row * p.ldq + heads.head * p.hsq + (l.r >> 2) * p.d, l.c, p.d, p.step, next);
+      load_operand<T, DV, FORM>(static_cast<const T *>(p.dout) + row * p.ldo + heads.head * p.hso, l.c, p.dv, p.step, next_out);
+#pragma unroll
+      for (int x = 0; x < 2; x++) next_lse[x] = __ldg(p.lse + (row * p.heads + heads.col_head[x]) * 2 + (l.c >> 1));
+   }
+
+   __device__ __forceinline__ void run(const AttnParams &p, const Place &at, Gathered &ring, int e0, int e1, long long follow)
+   {
       float acc[2][TILES][4];
 #pragma unroll
       for (int m = 0; m < 2; m++)
 #pragma unroll
          for (int t = 0; t < TILES; t++) acc[m][t][0] = acc[m][t][1] = acc[m][t][2] = acc[m][t][3] = 0.0f;
-      unsigned q[KIn::REGS], dout[VIn::REGS];
-      KIn::template load<FORM>(static_cast<const T *>(p.q) + row * p.ldq + heads.head * p.hsq + (l.r >> 2) * p.d, l.c, p.d, true, p.step, q);
-      VIn::template load<FORM>(static_cast<const T *>(p.dout) + row * p.ldo + heads.head * p.hso, l.c, p.dv, true, p.step, dout);
-      float lse[2];
+      s.delta[0] = s.delta[1] = 0.0f;
+      unsigned q[DK / 8], dout[DV / 8];
+      float lse[2] = {next_lse[0], next_lse[1]};
 #pragma unroll
-      for (int x = 0; x < 2; x++) lse[x] = __ldg(p.lse + (row * p.heads + heads.col_head[x]) * 2 + (l.c >> 1));
-      Source<T> kg, vg, ko[2];
-      kg.set(p.k, p.ldk, (l.kv0 + l.pair_head) * p.hsk);
-      vg.set(p.v, p.ldv, (l.kv0 + l.pair_head) * p.hsv);
-      const int even = (2 * l.c) & (l.hs - 1), odd = (2 * l.c + 1) & (l.hs - 1);
-      ko[0].set(p.k, p.ldk, (l.kv0 + even) * p.hsk);
-      ko[1].set(p.k, p.ldk, (l.kv0 + odd) * p.hsk);
-      const bool skip[2] = {only >= 0 && even != only, only >= 0 && odd != only};
-      const int per_step = 16 >> l.hs_log2;
-      for (long long base = e0 + 32 * warp; base < e1; base += 32 * warps) {
-         const int my_id = edges.take(p, base, e1, at.lane);
-         const float my_bias = edges.bias;
-         edges.fetch(p, base + 32 * warps < e1 ? base + 32 * warps : e1 + 32 * warp, at.lane);
-         const int count = static_cast<int>(e1 - base < 32 ? e1 - base : 32);
-         for (int first = 0; first < count; first += per_step) {
-            int id[2];
-            unsigned k[2][2][KIn::REGS], v[2][VIn::REGS];
+      for (int i = 0; i < DK / 8; i++) q[i] = next[i];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-               id[h] = __shfl_sync(FULL, my_id, first + l.edge(l.r + 8 * h));
-               const T *src = kg.template row<FORM>(id[h]);
-               KIn::template load<FORM>(src, l.c, p.d, id[h] >= 0, p.step, k[0][h]);
-               KIn::template load<FORM>(FORM == EXACT && id[h] < 0 ? src : src + p.d, l.c, p.d, id[h] >= 0, p.step, k[1][h]);
-               VIn::template load<FORM>(vg.template row<FORM>(id[h]), l.c, p.dv, id[h] >= 0, p.step, v[h]);
-            }
-            float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int i = 0; i < DV / 8; i++) dout[i] = next_out[i];
+      if (Width::AHEAD && follow >= 0) fetch(p, follow);
+      const int per_log2 = 4 - l.slots_log2;
+      const int pair = at.lane & 15, high = at.lane >> 4;
+      for (int e = e0; e < e1;) {
+         const int block = e >> per_log2;
+         if (block != ring.current) ring.advance(p, l, at.lane);
+         const int lo = e - (block << per_log2), left = e1 - (block << per_log2), hi = left < (1 << per_log2) ? left : 1 << per_log2;
+         const unsigned slot = ring.slot_of(block);
+         float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < KIn::STEPS; i++) {
-               mma16816<T>(s0, k[0][0][2 * i], k[0][1][2 * i], k[0][0][2 * i + 1], k[0][1][2 * i + 1], q[2 * i], q[2 * i + 1]);
-               mma16816<T>(s1, k[1][0][2 * i], k[1][1][2 * i], k[1][0][2 * i + 1], k[1][1][2 * i + 1], q[2 * i], q[2 * i + 1]);
-            }
-#pragma unroll
-            for (int i = 0; i < VIn::STEPS; i++)
-               mma16816<T>(dp, v[0][2 * i], v[1][2 * i], v[0][2 * i + 1], v[1][2 * i + 1], dout[2 * i], dout[2 * i + 1]);
-            // the same rows of k once more, as columns of the second product
-            unsigned kt[2][4][KOut::REGS];
-#pragma unroll
-            for (int h = 0; h < 4; h++) {
-               int kid = __shfl_sync(FULL, my_id, first + l.edge(2 * l.c + (h & 1) + 8 * (h >> 1)));
-               if (skip[h & 1]) kid = -1;
-               const T *src = ko[h & 1].template row<FORM>(kid);
-               KOut::template load<FORM>(src, l.r, p.d, kid >= 0, p.step, kt[0][h]);
-               KOut::template load<FORM>(FORM == EXACT && kid < 0 ? src : src + p.d, l.r, p.d, kid >= 0, p.step, kt[1][h]);
-            }
-            unsigned a0[4], a1[4];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-               const float bias = p.bias ? __shfl_sync(FULL, my_bias, first + l.edge(l.r + 8 * h)) : 0.0f;
-               float pr[2], w[2];
-#pragma unroll
-               for (int x = 0; x < 2; x++) {
-                  const float dot = l.c < 2 ? s0[2 * h + x] : s1[2 * h + x];
-                  // an edge that is masked has p = 0, and so has a row without edges (its lse is -inf)
-                  const bool live = heads.valid[x] && id[h] >= 0 && lse[x] != -INFINITY;
-                  pr[x] = live ? exp2_fast((fmaf(dot, p.scale, bias) - lse[x]) * LOG2E) : 0.0f;
-                  w[x] = live ? pr[x] * dp[2 * h + x] : 0.0f;
-                  s.delta[x] += w[x];
-               }
-               unsigned wh, wl, ph, pl;
-               split2<T>(w[0], w[1], wh, wl);
-               split2<T>(pr[0], pr[1], ph, pl);
-               wh = transpose8x8(wh);
-               wl = transpose8x8(wl);
-               ph = __shfl_xor_sync(FULL, transpose8x8(ph), 16);
-               pl = __shfl_xor_sync(FULL, transpose8x8(pl), 16);
-               a0[2 * h] = l.r < 4 ? wh : ph;
-               a0[2 * h + 1] = l.r < 4 ? wl : pl;
-               a1[2 * h] = l.r < 4 ? ph : wh;
-               a1[2 * h + 1] = l.r < 4 ? pl : wl;
-            }
-#pragma unroll
-            for (int t = 0; t < KOut::REGS; t++) {
-               mma16816<T>(acc[0][2 * t], a0[0], a0[1], a0[2], a0[3], low_halves(kt[0][0][t], kt[0][1][t]), low_halves(kt[0][2][t], kt[0][3][t]));
-               mma16816<T>(acc[0][2 * t + 1], a0[0], a0[1], a0[2], a0[3], high_halves(kt[0][0][t], kt[0][1][t]), high_halves(kt[0][2][t], kt[0][3][t]));
-               mma16816<T>(acc[1][2 * t], a1[0], a1[1], a1[2], a1[3], low_halves(kt[1][0][t], kt[1][1][t]), low_halves(kt[1][2][t], kt[1][3][t]));
-               mma16816<T>(acc[1][2 * t + 1], a1[0], a1[1], a1[2], a1[3], high_halves(kt[1][0][t], kt[1][1][t]), high_halves(kt[1][2][t], kt[1][3][t]));
-            }
+         for (int i = 0; i < DK / 16; i++) {
+            unsigned k[4];
+            ldmatrix4(k, slot + Gathered::at(pair, 2 * i + high));
+            mma16816<T>(s0, k[0], k[1], k[2], k[3], q[2 * i], q[2 * i + 1]);
+            ldmatrix4(k, slot + Gathered::at(pair, DK / 8 + 2 * i + high));
+            mma16816<T>(s1, k[0], k[1], k[2], k[3], q[2 * i], q[2 * i + 1]);
          }
+#pragma unroll
+         for (int i = 0; i < DV / 16; i++) {
+            unsigned v[4];
+            ldmatrix4(v, slot + Gathered::REGION + Gathered::at(pair, 2 * i + high));
+            mma16816<T>(dp, v[0], v[1], v[2], v[3], dout[2 * i], dout[2 * i + 1]);
+         }
+         unsigned a0[4], a1[4];
+#pragma unroll
+         for (int h = 0; h < 2; h++) {
+            const int edge = (l.r + 8 * h) >> l.slots_log2;
+            const float bias = shared_float(slot + Gathered::BIAS + 4 * edge);
+            const bool there = edge >= lo && edge < hi && bias != -INFINITY;
+            float pr[2], w[2];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+               const float dot = l.c < 2 ? s0[2 * h + x] : s1[2 * h + x];
+               // an edge that is masked has p = 0, and so has a row without edges (its lse is -inf)
+               const bool live = heads.valid[x] && there && lse[x] != -INFINITY;
+               pr[x] = live ? exp2_fast((fmaf(dot, p.scale, bias) - lse[x]) * LOG2E) : 0.0f;
+               w[x] = live ? pr[x] * dp[2 * h + x] : 0.0f;
+               s.delta[x] += w[x];
+            }
+            unsigned wh, wl, ph, pl;
+            split2<T>(w[0], w[1], wh, wl);
+            split2<T>(pr[0], pr[1], ph, pl);
+            wh = transpose8x8(wh);
+            wl = transpose8x8(wl);
+            ph = __shfl_xor_sync(FULL, transpose8x8(ph), 16);
+            pl = __shfl_xor_sync(FULL, transpose8x8(pl), 16);
+            a0[2 * h] = l.r < 4 ? wh : ph;
+            a0[2 * h + 1] = l.r < 4 ? wl : pl;
+            a1[2 * h] = l.r < 4 ? ph : wh;
+            a1[2 * h + 1] = l.r < 4 ? pl : wl;
+         }
+#pragma unroll
+         for (int t = 0; t < TILES; t += 2) {
+            unsigned k[4];
+            ldmatrix4_trans(k, slot + Gathered::at(pair, t + high));
+            mma16816<T>(acc[0][t], a0[0], a0[1], a0[2], a0[3], k[0], k[1]);
+            mma16816<T>(acc[0][t + 1], a0[0], a0[1], a0[2], a0[3], k[2], k[3]);
+            ldmatrix4_trans(k, slot + Gathered::at(pair, DK / 8 + t + high));
+            mma16816<T>(acc[1][t], a1[0], a1[1], a1[2], a1[3], k[0], k[1]);
+            mma16816<T>(acc[1][t + 1], a1[0], a1[1], a1[2], a1[3], k[2], k[3]);
+         }
+         e = (block << per_log2) + hi;
       }
-      bool bad = false;
+      float all = 0.0f;
 #pragma unroll
       for (int m = 0; m < 2; m++)
 #pragma unroll
          for (int t = 0; t < TILES; t++) {
             s.acc[m][t][0] = acc[m][t][0] + acc[m][t][2];
             s.acc[m][t][1] = acc[m][t][1] + acc[m][t][3];
-            bad |= s.acc[m][t][0] != s.acc[m][t][0] || s.acc[m][t][1] != s.acc[m][t][1];
+            all += s.acc[m][t][0] * 0.0f + s.acc[m][t][1] * 0.0f;
          }
-      lost = bad;
+      lost = all != all;
       s.delta[0] = sum_pairs(s.delta[0]);
       s.delta[1] = sum_pairs(s.delta[1]);
    }
@@ -569,7 +646,10 @@ struct BackwardRowsMma {
 #pragma unroll
             for (int t = 0; t < TILES; t++) to[32 * (m * TILES + t)] = make_float2(s.acc[m][t][0], s.acc[m][t][1]);
       }
-      to[64 * TILES] = make_float2(s.delta[0], s.delta[1]);
+      float *delta = reinterpret_cast<float *>(to + 64 * TILES);
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+         if (only < 0 || heads.col_kv[x] == only) delta[x] = s.delta[x];
    }
 
    __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long row, int only)
@@ -578,51 +658,67 @@ struct BackwardRowsMma {
       const bool mine = heads.live && (only < 0 || heads.kv == only);
       const int map = l.r >> 2;
       const long long rh = row * p.heads + heads.head;
-      const float factor = map ? -__ldg(p.lam + row * p.ldlam + heads.head) * p.scale : p.scale;
+      const float sign = map ? -__ldg(p.lam + row * p.ldlam + heads.head) : 1.0f, factor = sign * p.scale;
+      T *out = static_cast<T *>(p.out) + (rh * 2 + map) * p.d + 2 * l.c;
 #pragma unroll
-      for (int set = 0; set < KOut::SETS; set++)
+      for (int t = 0; t < TILES; t++) {
+         float o[2];
 #pragma unroll
          for (int x = 0; x < 2; x++) {
-            float o[KOut::E];
-#pragma unroll
-            for (int j = 0; j < KOut::E; j++) {
-               const int t = set * KOut::E + j;
-               // rows 0..3 hold A of map 0 and B of map 1, rows 4..7 B of map 0 and A of map 1
-               const float b = __shfl_xor_sync(FULL, map ? s.acc[0][t][x] : s.acc[1][t][x], 16);
-               o[j] = factor * fmaf(-delta, b, map ? s.acc[1][t][x] : s.acc[0][t][x]);
-            }
-            const int y = 8 * KOut::E * set + KOut::E * (2 * l.c + x);
-            if (mine) KOut::template store<FORM != PIECES>(static_cast<T *>(p.out) + (rh * 2 + map) * p.d + y, o, p.d - y);
+            // rows 0..3 hold A of map 0 and B of map 1, rows 4..7 B of map 0 and A of map 1
+            const float b = __shfl_xor_sync(FULL, map ? s.acc[0][t][x] : s.acc[1][t][x], 16);
+            o[x] = factor * fmaf(-delta, b, map ? s.acc[1][t][x] : s.acc[0][t][x]);
          }
+         if (mine) store_two<T, FORM>(out + 8 * t, o[0], o[1], p.d - 8 * t - 2 * l.c);
+      }
       if (mine && l.c == 0) {
-         p.stats[rh * 2 + map] = make_float2(__ldg(p.lse + rh * 2 + map), delta);
+         p.stats[rh * 2 + map] = make_float4(__ldg(p.lse + rh * 2 + map), delta, sign, 0.0f);
          if (map) p.dlam[rh] = -delta;
       }
+   }
+   __device__ __forceinline__ void finish_empty(const AttnParams &p, const Place &at, long long row)
+   {
+      if (!heads.live) return;
+      const int map = l.r >> 2;
+      const long long rh = row * p.heads + heads.head;
+      T *out = static_cast<T *>(p.out) + (rh * 2 + map) * p.d + 2 * l.c;
+#pragma unroll
+      for (int t = 0; t < TILES; t++) store_two<T, FORM>(out + 8 * t, 0.0f, 0.0f, p.d - 8 * t - 2 * l.c);
+      if (l.c == 0 && map) p.dlam[rh] = 0.0f;  // nobody gathers the row: its record is not read
    }
 };
 
 // ---------------------------------------------------------------------------------------------------------------------
-// backward over the columns: dk and dv.  Columns of the products are (map, kv head of the unit); a pair is an edge with a
-// kv head, taken once for every query head of the group.  dk and dv are [16 elements x 8] products: the inner index is the
-// pairs, the columns 0..3 take the upper and 4..7 the lower part of the split ds (or weight) of the unit's kv heads.
+// backward over the columns: dk and dv.  A pair is an edge with a query head; the columns of the products are (map, kv head of
+// the unit).  dk and dv are [16 elements x 8] products over the pairs: the columns 0..3 take the upper and 4..7 the lower part
+// of the split ds (or weight) of the unit's kv heads.
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int DK, int DV, int FORM>
+template <typename T, int DK, int FORM>
 struct BackwardColumnsMma {
-   static constexpr int BLOCKS = DV <= 64 ? 4 : DV <= 128 ? 3 : 2;
-   using KIn = Inner<T, DK>;
-   using KOut = Outer<T, DK>;
-   using VIn = Inner<T, DV>;
-   using VOut = Outer<T, DV>;
-   static constexpr int KT = KOut::REGS, VT = VOut::REGS;
-   static constexpr int LANE_FLOATS = 4 * (2 * KT + VT);
+   static constexpr int DV = 2 * DK, KT = DK / 16, VT = DV / 16, LANE_FLOATS = 4 * (2 * KT + VT);
+   using Gathered = Ring<T, DK, FORM, Budget<DK>::STAGES, true>;
+   using Width = Budget<DK>;
    struct State {
       float dk[2][KT][4], dv[VT][4];
    };
    State s;
    Lanes l;
+   int kv0, per_kv;       // query heads of a kv head that a block holds
+   int pair_kv;           // which of the unit's kv heads the pairs r and r + 8 are of
+   unsigned next[DK / 8], next_v[DV / 8];
    bool lost;
 
-   __device__ __forceinline__ void setup(const AttnParams &p, const Place &at) { l.set(p, at); }
+   __device__ __forceinline__ void setup(const AttnParams &p, const Place &at, Gathered &ring)
+   {
+      l.set(at, p.unit_kv * p.unit_heads);
+      kv0 = at.unit * p.unit_kv;
+      per_kv = p.unit_heads;
+      pair_kv = l.pair_slot / per_kv;
+      const long long head = kv0 * p.group;
+      ring.a = static_cast<const char *>(p.q) + head * p.a_head;
+      ring.b = static_cast<const char *>(p.dout) + head * p.b_head;
+      ring.records = reinterpret_cast<const char *>(p.stats + head * 2);
+   }
    static __device__ __forceinline__ void clear(State &s)
    {
 #pragma unroll
@@ -634,126 +730,100 @@ struct BackwardColumnsMma {
 #pragma unroll
          for (int i = 0; i < 4; i++) s.dv[t][i] = 0.0f;
    }
-
-   __device__ __forceinline__ void run(const AttnParams &p, const Place &at, EdgeStream &edges, long long col, long long e0, long long e1,
-                                       int warp, int warps, int only)
+   __device__ __forceinline__ void fetch(const AttnParams &p, long long col)
    {
-      lost = false;
-      clear(s);
-      if (e0 + 32 * warp >= e1) return;
       // column n = r: map r / 4, kv head r % 4 of the unit (one that exists stands for those beyond)
-      const int n_head = l.kv0 + ((l.r & 3) < l.hs ? l.r & 3 : 0);
-      unsigned k[KIn::REGS], v[VIn::REGS];
-      KIn::template load<FORM>(static_cast<const T *>(p.k) + col * p.ldk + n_head * p.hsk + (l.r >> 2) * p.d, l.c, p.d, true, p.step, k);
-      VIn::template load<FORM>(static_cast<const T *>(p.v) + col * p.ldv + n_head * p.hsv, l.c, p.dv, true, p.step, v);
-      const int even = (2 * l.c) & (l.hs - 1), odd = (2 * l.c + 1) & (l.hs - 1);
-      const bool skip[2] = {only >= 0 && even != only, only >= 0 && odd != only};
-      const int per_step = 16 >> l.hs_log2;
+      const int head = kv0 + ((l.r & 3) < p.unit_kv ? l.r & 3 : 0);
+      load_operand<T, DK, FORM>(static_cast<const T *>(p.k) + col * p.ldk + head * p.hsk + (l.r >> 2) * p.d, l.c, p.d, p.step, next);
+      load_operand<T, DV, FORM>(static_cast<const T *>(p.v) + col * p.ldv + head * p.hsv, l.c, p.dv, p.step, next_v);
+   }
+
+   __device__ __forceinline__ void run(const AttnParams &p, const Place &at, Gathered &ring, int e0, int e1, long long follow)
+   {
+      clear(s);
+      unsigned k[DK / 8], v[DV / 8];
+#pragma unroll
+      for (int i = 0; i < DK / 8; i++) k[i] = next[i];
+#pragma unroll
+      for (int i = 0; i < DV / 8; i++) v[i] = next_v[i];
+      if (Width::AHEAD && follow >= 0) fetch(p, follow);
+      const int per_log2 = 4 - l.slots_log2;
+      const int pair = at.lane & 15, high = at.lane >> 4;
       // of the columns 2c, 2c + 1 at most one is of the pairs' kv head
-      const bool valid = (l.c & 1) == l.pair_head >> 1;
-      const int x = l.pair_head & 1, map = l.c >> 1;
-      for (long long base = e0 + 32 * warp; base < e1; base += 32 * warps) {
-         const int my_id = edges.take(p, base, e1, at.lane);
-         const float my_bias = edges.bias;
-         edges.fetch(p, base + 32 * warps < e1 ? base + 32 * warps : e1 + 32 * warp, at.lane);
-         const int count = static_cast<int>(e1 - base < 32 ? e1 - base : 32);
-         for (int first = 0; first < count; first += per_step) {
-            int id[2];
-            float bias[2];
+      const bool valid = (l.c & 1) == pair_kv >> 1;
+      const int x = pair_kv & 1, map = l.c >> 1;
+      for (int e = e0; e < e1;) {
+         const int edges = e >> per_log2;
+         const int lo = e - (edges << per_log2), left = e1 - (edges << per_log2), hi = left < (1 << per_log2) ? left : 1 << per_log2;
+         for (int sub = 0; sub < p.subs; sub++) {
+            const int block = edges * p.subs + sub;
+            if (block != ring.current) ring.advance(p, l, at.lane);
+            const unsigned slot = ring.slot_of(block);
+            float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < DK / 16; i++) {
+               unsigned q[4];
+               ldmatrix4(q, slot + Gathered::at(pair, 2 * i + high));
+               mma16816<T>(s0, q[0], q[1], q[2], q[3], k[2 * i], k[2 * i + 1]);
+               ldmatrix4(q, slot + Gathered::at(pair, DK / 8 + 2 * i + high));
+               mma16816<T>(s1, q[0], q[1], q[2], q[3], k[2 * i], k[2 * i + 1]);
+            }
+#pragma unroll
+            for (int i = 0; i < DV / 16; i++) {
+               unsigned d[4];
+               ldmatrix4(d, slot + Gathered::REGION + Gathered::at(pair, 2 * i + high));
+               mma16816<T>(dp, d[0], d[1], d[2], d[3], v[2 * i], v[2 * i + 1]);
+            }
+            unsigned b0[2], b1[2], bw[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-               id[h] = __shfl_sync(FULL, my_id, first + l.edge(l.r + 8 * h));
-               bias[h] = p.bias ? __shfl_sync(FULL, my_bias, first + l.edge(l.r + 8 * h)) : 0.0f;
+               const int edge = (l.r + 8 * h) >> l.slots_log2;
+               const float bias = shared_float(slot + Gathered::BIAS + 4 * edge);
+               float lse, delta, sign, none;
+               asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(lse), "=f"(delta), "=f"(sign), "=f"(none)
+                            : "r"(slot + Gathered::RECORD + (l.r + 8 * h) * 32 + map * 16) : "memory");
+               // an edge of this column, of a row that has any, and this lane's column is the pair's
+               const bool live = valid && edge >= lo && edge < hi && bias != -INFINITY && lse != -INFINITY;
+               const float dot = map ? (x ? s1[2 * h + 1] : s1[2 * h]) : (x ? s0[2 * h + 1] : s0[2 * h]);
+               const float pr = live ? exp2_fast((fmaf(dot, p.scale, bias) - lse) * LOG2E) : 0.0f;
+               const float part = live ? sign * pr : 0.0f;  // this map's part of the weight
+               const float w = part + __shfl_xor_sync(FULL, part, 2);
+               const float ds = live ? part * ((x ? dp[2 * h + 1] : dp[2 * h]) - delta) : 0.0f;
+               unsigned up, low, wh, wl;
+               split2<T>(x ? 0.0f : ds, x ? ds : 0.0f, up, low);
+               split2<T>(x ? 0.0f : w, x ? w : 0.0f, wh, wl);
+               const unsigned got = __shfl_xor_sync(FULL, l.c < 2 ? low : up, 2);
+               b0[h] = transpose8x8(l.c < 2 ? up : got);
+               b1[h] = transpose8x8(l.c < 2 ? got : low);
+               bw[h] = transpose8x8(l.c < 2 ? wh : wl);
             }
-            int pair_id[4];
 #pragma unroll
-            for (int h = 0; h < 4; h++) {
-               pair_id[h] = __shfl_sync(FULL, my_id, first + l.edge(2 * l.c + (h & 1) + 8 * (h >> 1)));
-               if (skip[h & 1]) pair_id[h] = -1;
+            for (int t = 0; t < KT; t++) {
+               unsigned q[4];
+               ldmatrix4_trans(q, slot + Gathered::at(pair, 2 * t + high));
+               mma16816<T>(s.dk[0][t], q[0], q[2], q[1], q[3], b0[0], b0[1]);
+               ldmatrix4_trans(q, slot + Gathered::at(pair, DK / 8 + 2 * t + high));
+               mma16816<T>(s.dk[1][t], q[0], q[2], q[1], q[3], b1[0], b1[1]);
             }
-            for (int g = 0; g < p.group; g++) {
-               const int head = (l.kv0 + l.pair_head) * p.group + g;
-               Source<T> qg, dg;
-               qg.set(p.q, p.ldq, head * p.hsq);
-               dg.set(p.dout, p.ldo, head * p.hso);
-               unsigned q[2][2][KIn::REGS], dout[2][VIn::REGS];
-               float2 stat[2];
-               float lam[2];
 #pragma unroll
-               for (int h = 0; h < 2; h++) {
-                  const T *src = qg.template row<FORM>(id[h]);
-                  KIn::template load<FORM>(src, l.c, p.d, id[h] >= 0, p.step, q[0][h]);
-                  KIn::template load<FORM>(FORM == EXACT && id[h] < 0 ? src : src + p.d, l.c, p.d, id[h] >= 0, p.step, q[1][h]);
-                  VIn::template load<FORM>(dg.template row<FORM>(id[h]), l.c, p.dv, id[h] >= 0, p.step, dout[h]);
-                  stat[h] = make_float2(-INFINITY, 0.0f);
-                  lam[h] = 0.0f;
-                  if (id[h] >= 0 && valid) {
-                     stat[h] = __ldg(p.stats + (static_cast<long long>(id[h]) * p.heads + head) * 2 + map);
-                     lam[h] = __ldg(p.lam + id[h] * p.ldlam + head);
-                  }
-               }
-               float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-               for (int i = 0; i < KIn::STEPS; i++) {
-                  mma16816<T>(s0, q[0][0][2 * i], q[0][1][2 * i], q[0][0][2 * i + 1], q[0][1][2 * i + 1], k[2 * i], k[2 * i + 1]);
-                  mma16816<T>(s1, q[1][0][2 * i], q[1][1][2 * i], q[1][0][2 * i + 1], q[1][1][2 * i + 1], k[2 * i], k[2 * i + 1]);
-               }
-#pragma unroll
-               for (int i = 0; i < VIn::STEPS; i++)
-                  mma16816<T>(dp, dout[0][2 * i], dout[1][2 * i], dout[0][2 * i + 1], dout[1][2 * i + 1], v[2 * i], v[2 * i + 1]);
-               unsigned qt[2][4][KT], dt[4][VT];
-#pragma unroll
-               for (int h = 0; h < 4; h++) {
-                  const int other = (l.kv0 + (h & 1 ? odd : even)) * p.group + g;
-                  Source<T> qo, dd;
-                  qo.set(p.q, p.ldq, other * p.hsq);
-                  dd.set(p.dout, p.ldo, other * p.hso);
-                  const T *src = qo.template row<FORM>(pair_id[h]);
-                  KOut::template load<FORM>(src, l.r, p.d, pair_id[h] >= 0, p.step, qt[0][h]);
-                  KOut::template load<FORM>(FORM == EXACT && pair_id[h] < 0 ? src : src + p.d, l.r, p.d, pair_id[h] >= 0, p.step, qt[1][h]);
-                  VOut::template load<FORM>(dd.template row<FORM>(pair_id[h]), l.r, p.dv, pair_id[h] >= 0, p.step, dt[h]);
-               }
-               unsigned b0[2], b1[2], bw[2];
-#pragma unroll
-               for (int h = 0; h < 2; h++) {
-                  const bool live = stat[h].x != -INFINITY;  // an edge of a row that has any, and this lane's column is the pair's
-                  const float dot = map ? (x ? s1[2 * h + 1] : s1[2 * h]) : (x ? s0[2 * h + 1] : s0[2 * h]);
-                  const float pr = live ? exp2_fast((fmaf(dot, p.scale, bias[h]) - stat[h].x) * LOG2E) : 0.0f;
-                  const float part = live ? (map ? -lam[h] : 1.0f) * pr : 0.0f;  // this map's part of the weight
-                  const float w = part + __shfl_xor_sync(FULL, part, 2);
-                  const float ds = live ? part * ((x ? dp[2 * h + 1] : dp[2 * h]) - stat[h].y) : 0.0f;
-                  unsigned hi, lo, wh, wl;
-                  split2<T>(x ? 0.0f : ds, x ? ds : 0.0f, hi, lo);
-                  split2<T>(x ? 0.0f : w, x ? w : 0.0f, wh, wl);
-                  const unsigned got = __shfl_xor_sync(FULL, l.c < 2 ? lo : hi, 2);
-                  b0[h] = transpose8x8(l.c < 2 ? hi : got);
-                  b1[h] = transpose8x8(l.c < 2 ? got : lo);
-                  bw[h] = transpose8x8(l.c < 2 ? wh : wl);
-               }
-#pragma unroll
-               for (int t = 0; t < KT; t++) {
-                  mma16816<T>(s.dk[0][t], low_halves(qt[0][0][t], qt[0][1][t]), high_halves(qt[0][0][t], qt[0][1][t]),
-                              low_halves(qt[0][2][t], qt[0][3][t]), high_halves(qt[0][2][t], qt[0][3][t]), b0[0], b0[1]);
-                  mma16816<T>(s.dk[1][t], low_halves(qt[1][0][t], qt[1][1][t]), high_halves(qt[1][0][t], qt[1][1][t]),
-                              low_halves(qt[1][2][t], qt[1][3][t]), high_halves(qt[1][2][t], qt[1][3][t]), b1[0], b1[1]);
-               }
-#pragma unroll
-               for (int t = 0; t < VT; t++)
-                  mma16816<T>(s.dv[t], low_halves(dt[0][t], dt[1][t]), high_halves(dt[0][t], dt[1][t]), low_halves(dt[2][t], dt[3][t]),
-                              high_halves(dt[2][t], dt[3][t]), bw[0], bw[1]);
+            for (int t = 0; t < VT; t++) {
+               unsigned d[4];
+               ldmatrix4_trans(d, slot + Gathered::REGION + Gathered::at(pair, 2 * t + high));
+               mma16816<T>(s.dv[t], d[0], d[2], d[1], d[3], bw[0], bw[1]);
             }
          }
+         e = (edges << per_log2) + hi;
       }
-      bool bad = false;
+      float all = 0.0f;
 #pragma unroll
       for (int t = 0; t < KT; t++)
 #pragma unroll
-         for (int i = 0; i < 4; i++) bad |= s.dk[0][t][i] != s.dk[0][t][i] || s.dk[1][t][i] != s.dk[1][t][i];
+         for (int i = 0; i < 4; i++) all += s.dk[0][t][i] * 0.0f + s.dk[1][t][i] * 0.0f;
 #pragma unroll
       for (int t = 0; t < VT; t++)
 #pragma unroll
-         for (int i = 0; i < 4; i++) bad |= s.dv[t][i] != s.dv[t][i];
-      lost = bad;
+         for (int i = 0; i < 4; i++) all += s.dv[t][i] * 0.0f;
+      lost = all != all;
    }
 
    __device__ __forceinline__ void join_from(const float *unit, const Place &at)
@@ -784,43 +854,221 @@ struct BackwardColumnsMma {
       }
    }
 
-   template <typename Out, int REGS>
-   __device__ __forceinline__ void write(const float (&f)[REGS][4], T *row, long long head_step, int width, float factor, int only)
+   template <int TILES>
+   __device__ __forceinline__ void write(const float (&f)[TILES][4], T *row, long long head_step, int width, float factor, int only)
    {
 #pragma unroll
-      for (int set = 0; set < Out::SETS; set++)
+      for (int t = 0; t < TILES; t++)
 #pragma unroll
          for (int x = 0; x < 2; x++) {
-            float o[Out::E];
-#pragma unroll
-            for (int j = 0; j < Out::E / 2; j++) {
-               const float lo = f[set * (Out::E / 2) + j][x], hi = f[set * (Out::E / 2) + j][2 + x];
-               o[2 * j] = factor * (lo + __shfl_xor_sync(FULL, lo, 2));
-               o[2 * j + 1] = factor * (hi + __shfl_xor_sync(FULL, hi, 2));
-            }
-            const int kv = 2 * l.c + x, y = 8 * Out::E * set + Out::E * l.r;
-            if (l.c < 2 && kv < l.hs && (only < 0 || kv == only))
-               Out::template store<FORM != PIECES>(row + kv * head_step + y, o, width - y);
+            // elements 16t + r and 16t + 8 + r; neighbouring r trade one so that each has two consecutive elements
+            const float a = factor * (f[t][x] + __shfl_xor_sync(FULL, f[t][x], 2));
+            const float b = factor * (f[t][2 + x] + __shfl_xor_sync(FULL, f[t][2 + x], 2));
+            const bool odd = l.r & 1;
+            const float got = __shfl_xor_sync(FULL, odd ? a : b, 4);
+            const int kv = 2 * l.c + x, y = 16 * t + (odd ? 8 + l.r - 1 : l.r);
+            if (l.c < 2 && (only < 0 ? kv * per_kv < l.slots : kv == only))
+               store_two<T, FORM>(row + kv * head_step + y, odd ? got : a, odd ? b : got, width - y);
          }
    }
    __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long col, int only)
    {
-      const long long rh = col * p.kv_heads + l.kv0;
-      write<KOut, KT>(s.dk[0], static_cast<T *>(p.out) + rh * 2 * p.d, 2 * p.d, p.d, p.scale, only);
-      write<KOut, KT>(s.dk[1], static_cast<T *>(p.out) + rh * 2 * p.d + p.d, 2 * p.d, p.d, p.scale, only);
-      write<VOut, VT>(s.dv, static_cast<T *>(p.out2) + rh * p.dv, p.dv, p.dv, 1.0f, only);
+      const long long rh = col * p.kv_heads + kv0;
+      write<KT>(s.dk[0], static_cast<T *>(p.out) + rh * 2 * p.d, 2 * p.d, p.d, p.scale, only);
+      write<KT>(s.dk[1], static_cast<T *>(p.out) + rh * 2 * p.d + p.d, 2 * p.d, p.d, p.scale, only);
+      write<VT>(s.dv, static_cast<T *>(p.out2) + rh * p.dv, p.dv, p.dv, 1.0f, only);
+   }
+   __device__ __forceinline__ void finish_empty(const AttnParams &p, const Place &at, long long col)
+   {
+      const long long rh = col * p.kv_heads + kv0;
+      T *dk = static_cast<T *>(p.out) + rh * 2 * p.d, *dv = static_cast<T *>(p.out2) + rh * p.dv;
+      for (int i = 2 * at.lane; i < p.unit_kv * 2 * p.d; i += 64) store_two<T, FORM>(dk + i, 0.0f, 0.0f, p.unit_kv * 2 * p.d - i);
+      for (int i = 2 * at.lane; i < p.unit_kv * p.dv; i += 64) store_two<T, FORM>(dv + i, 0.0f, 0.0f, p.unit_kv * p.dv - i);
    }
 };
 
-template <typename T, int DK, template <typename, int, int, int> class Op>
-int launch_mma_width(const WalkShape &s, const AttnParams &p, cudaStream_t st)
+// ---------------------------------------------------------------------------------------------------------------------
+// the walk
+// ---------------------------------------------------------------------------------------------------------------------
+// the warps of a block that shared a row: warp 0 takes the others' states in order; the rings serve as the place
+template <typename Op>
+__device__ __forceinline__ void join_ring_warps(Op &op, const Place &at, float *shared)
 {
-   if (s.form == EXACT) return launch_op<Op<T, DK, 2 * DK, EXACT>, 32>(p, s.together, st);
-   if (s.form == RAGGED) return launch_op<Op<T, DK, 2 * DK, RAGGED>, 32>(p, s.together, st);
-   return launch_op<Op<T, DK, 2 * DK, PIECES>, 32>(p, s.together, st);
+   constexpr int STRIDE = Op::LANE_FLOATS * 32;
+   __syncthreads();
+   if (at.warp > 0) op.put(shared + (at.warp - 1) * STRIDE, at, -1);
+   __syncthreads();
+   if (at.warp == 0)
+      for (int w = 1; w < Op::Width::JOINT; w++) op.join_from(shared + (w - 1) * STRIDE, at);
 }
 
-template <typename T, template <typename, int, int, int> class Op>
+// Where several heads are computed in one product and a sum came out infinite or as no number, a 0 of one head may have met an
+// infinity or NaN of another's: the edges are then taken once more, each kv head by itself.
+template <typename Op, bool TOGETHER>
+__device__ __forceinline__ void ring_segment(Op &op, typename Op::Gathered &ring, const AttnParams &p, const Place &at, float *shared,
+                                             long long row, long long e0, long long e1, long long part, long long follow, long long run_end)
+{
+   long long w0 = e0, w1 = e1;
+   if (TOGETHER) {  // equal runs of whole blocks
+      const int per_log2 = 4 - op.l.slots_log2;
+      const long long blocks = (e1 - e0 + (1 << per_log2) - 1) >> per_log2, each = (blocks + Op::Width::JOINT - 1) / Op::Width::JOINT;
+      w0 = e0 + ((at.warp * each) << per_log2);
+      w1 = w0 + (each << per_log2);
+      w0 = w0 < e1 ? w0 : e1;
+      w1 = w1 < e1 ? w1 : e1;
+      ring.begin(p, op.l, at.lane, w0, w1, -1);
+   }
+   // (row pointers that decrease must not lead out of the ring)
+   w0 = w0 < ring.first ? ring.first : w0;
+   w1 = w1 < w0 ? w0 : w1;
+   op.run(p, at, ring, static_cast<int>(w0 - ring.first), static_cast<int>(w1 - ring.first), follow);
+   const bool lost = p.unit_kv > 1 && (TOGETHER ? __syncthreads_or(op.lost) : __any_sync(FULL, op.lost));
+   for (int only = lost ? 0 : -1; only < (lost ? p.unit_kv : 0); only++) {
+      if (lost) {
+         op.fetch(p, row);
+         ring.begin(p, op.l, at.lane, w0, w1, only);
+         op.run(p, at, ring, 0, static_cast<int>(w1 - w0), only == p.unit_kv - 1 ? follow : -1);
+      }
+      if (TOGETHER) {
+         ring.drain();
+         join_ring_warps(op, at, shared);
+      }
+      if (!TOGETHER || at.warp == 0) {
+         if (part < 0) op.finish(p, at, row, only);
+         else op.put(part_at<Op, 32>(p, at, part), at, only);
+      }
+      if (TOGETHER) __syncthreads();
+   }
+   if (lost && !TOGETHER && p.subs == 1) ring.begin(p, op.l, at.lane, e1, run_end, -1);
+}
+
+template <typename Op, bool TOGETHER>
+__global__ void __launch_bounds__((TOGETHER ? Op::Width::JOINT : Op::Width::SOLO) * 32, TOGETHER ? 1 : Op::Width::BLOCKS)
+ring_walk_kernel(const AttnParams p)
+{
+   extern __shared__ __align__(128) float shared[];
+   constexpr int WARPS = TOGETHER ? Op::Width::JOINT : Op::Width::SOLO;
+   const int warp = threadIdx.x >> 5;
+   const long long job = TOGETHER ? blockIdx.x : static_cast<long long>(blockIdx.x) * WARPS + warp;
+   const long long piece = job / p.unit_blocks;
+   if (piece >= p.pieces) return;
+   const Place at = Place::make<32>(p, static_cast<int>(job - piece * p.unit_blocks));
+   const Rows rows(p);
+   const long long lo = piece * p.piece, hi = lo + p.piece;
+   Op op;
+   typename Op::Gathered ring;
+   ring.ring = static_cast<unsigned>(__cvta_generic_to_shared(shared)) + warp * (Op::Gathered::STAGES * Op::Gathered::STAGE);
+   op.setup(p, at, ring);
+   long long u = rows.lower_bound(lo, 0, p.m, at.lane);
+   // the rows that begin in this piece end before `last`: a row is ROW_ITEMS items at least
+   const long long most = u + p.piece / ROW_ITEMS + 1;
+   const long long last = rows.lower_bound(hi, u, most < p.m ? most : p.m, at.lane);
+   long long begun = -1;
+   if (u > 0) {  // the row before may reach into this piece: then it is this loop's first
+      const long long fb = rows.items(u - 1), fe = rows.items(u);
+      if (fe > lo && fe - fb > p.row_limit) u--;
+   }
+   // the run of edges: up to the last row's end, or where it is cut
+   auto part_of = [&](long long row, long long b, long long e, long long &e0, long long &e1) {
+      const long long fb = b - rows.first + ROW_ITEMS * row, fe = e - rows.first + ROW_ITEMS * (row + 1);
+      e0 = b;
+      e1 = e > b ? e : b;
+      if (fe - fb <= p.row_limit) return -1LL;
+      e0 = b + (lo - fb - ROW_ITEMS);
+      e1 = b + (hi - fb - ROW_ITEMS);
+      e0 = e0 < b ? b : e0;
+      e1 = e1 > e ? e : e1 < e0 ? e0 : e1;
+      return 2 * piece + (fb >= lo);
+   };
+   if (u < last) {
+      long long run_begin, run_end, x;
+      part_of(u, rows.begin(u), rows.begin(u + 1), run_begin, x);
+      part_of(last - 1, rows.begin(last - 1), rows.begin(last), x, run_end);
+      // (where a row's edges are taken once for each of several groups of heads, every row is a run of its own)
+      if (!TOGETHER && p.subs == 1) ring.begin(p, op.l, at.lane, run_begin, run_end, -1);
+      // rows 31 at a time, their pointers one to a lane; rows with edges are found by their bits
+      for (long long from = u; from < last; from += 31) {
+         const int here = static_cast<int>(last - from < 31 ? last - from : 31);
+         const long long mine = rows.begin(from + at.lane < p.m ? from + at.lane : p.m);
+         const long long behind = __shfl_down_sync(FULL, mine, 1);
+         long long m0 = 0, m1 = 0, part = -1;
+         if (at.lane < here) part = part_of(from + at.lane, mine, behind, m0, m1);
+         const unsigned busy = __ballot_sync(FULL, at.lane < here && (m1 > m0 || part >= 0));
+         const unsigned starts = __ballot_sync(FULL, part >= 0 && (part & 1));
+         if (starts) begun = from + __ffs(starts) - 1;
+         for (unsigned none = ~busy & ((1u << here) - 1); none; none &= none - 1)
+            if (!TOGETHER || warp == 0) op.finish_empty(p, at, from + __ffs(none) - 1);
+         if (Op::Width::AHEAD && busy) op.fetch(p, from + __ffs(busy) - 1);
+         for (unsigned todo = busy; todo;) {
+            const int i = __ffs(todo) - 1;
+            todo &= todo - 1;
+            const long long e0 = __shfl_sync(FULL, m0, i), e1 = __shfl_sync(FULL, m1, i), pt = __shfl_sync(FULL, part, i);
+            if (!TOGETHER && p.subs != 1) ring.begin(p, op.l, at.lane, e0, e1, -1);
+            if (!Op::Width::AHEAD) op.fetch(p, from + i);
+            ring_segment<Op, TOGETHER>(op, ring, p, at, shared, from + i, e0, e1, pt, todo ? from + __ffs(todo) - 1 : -1, run_end);
+         }
+      }
+   }
+   ring.drain();
+   if (at.lane == 0 && (!TOGETHER || warp == 0) && job == piece * p.unit_blocks) p.long_row[piece] = begun;
+}
+
+// the parts of the long rows, as join_kernel
+template <typename Op>
+__global__ void __launch_bounds__(Op::Width::JOINT * 32) ring_join_kernel(const AttnParams p)
+{
+   extern __shared__ __align__(16) float shared[];
+   const int warp = threadIdx.x >> 5;
+   const long long group = blockIdx.x / p.unit_blocks;
+   const Place at = Place::make<32>(p, static_cast<int>(blockIdx.x - group * p.unit_blocks));
+   const Rows rows(p);
+   Op op;
+   typename Op::Gathered ring;
+   op.setup(p, at, ring);
+   for (long long piece = group * JOIN_PIECES; piece < (group + 1) * JOIN_PIECES && piece < p.pieces; piece++) {
+      const long long u = p.long_row[piece];
+      if (u < 0) continue;
+      const long long last = (rows.items(u + 1) - 1) / p.piece, parts = last - piece + 1;
+      const long long each = (parts + Op::Width::JOINT - 1) / Op::Width::JOINT;
+      Op::clear(op.s);
+      for (long long i = warp * each; i < (warp + 1) * each && i < parts; i++)
+         op.join_from(part_at<Op, 32>(p, at, 2 * (piece + i) + (i == 0 ? 1 : 0)), at);
+      join_ring_warps(op, at, shared);
+      if (warp == 0) op.finish(p, at, u, -1);
+   }
+}
+
+template <typename Op>
+int launch_ring(const AttnParams &p, bool together, cudaStream_t st)
+{
+   constexpr int RING = Op::Gathered::STAGES * Op::Gathered::STAGE;
+   constexpr int JOIN = (Op::Width::JOINT - 1) * 32 * Op::LANE_FLOATS * static_cast<int>(sizeof(float));
+   static_assert(JOIN <= Op::Width::JOINT * RING, "the rings serve as the place where warps meet");
+   const long long jobs = p.pieces * p.unit_blocks;
+   if (together) {
+      constexpr int bytes = Op::Width::JOINT * RING;
+      if (cudaFuncSetAttribute(ring_walk_kernel<Op, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -1;
+      ring_walk_kernel<Op, true><<<static_cast<unsigned>(jobs), Op::Width::JOINT * 32, bytes, st>>>(p);
+   } else {
+      constexpr int bytes = Op::Width::SOLO * RING;
+      if (cudaFuncSetAttribute(ring_walk_kernel<Op, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -1;
+      ring_walk_kernel<Op, false><<<static_cast<unsigned>((jobs + Op::Width::SOLO - 1) / Op::Width::SOLO), Op::Width::SOLO * 32, bytes, st>>>(p);
+   }
+   if (cudaFuncSetAttribute(ring_join_kernel<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, JOIN) != cudaSuccess) return -1;
+   const long long groups = (p.pieces + JOIN_PIECES - 1) / JOIN_PIECES;
+   ring_join_kernel<Op><<<static_cast<unsigned>(groups * p.unit_blocks), Op::Width::JOINT * 32, JOIN, st>>>(p);
+   return 0;
+}
+
+template <typename T, int DK, template <typename, int, int> class Op>
+int launch_mma_width(const WalkShape &s, const AttnParams &p, cudaStream_t st)
+{
+   if (s.form == EXACT) return launch_ring<Op<T, DK, EXACT>>(p, s.together, st);
+   if (s.form == RAGGED) return launch_ring<Op<T, DK, RAGGED>>(p, s.together, st);
+   return launch_ring<Op<T, DK, PIECES>>(p, s.together, st);
+}
+
+template <typename T, template <typename, int, int> class Op>
 int launch_mma(const WalkShape &s, const AttnParams &p, cudaStream_t st)
 {
    if (s.width == 16) return launch_mma_width<T, 16, Op>(s, p, st);
