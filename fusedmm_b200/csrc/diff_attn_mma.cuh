@@ -107,26 +107,41 @@ struct Lanes {
 };
 
 // The ring of a warp: STAGES blocks of 16 pairs, each of two gathered rows of 2 DK elements (k of both maps and v, or q and
-// do), 16 biases and, where the walk wants them, 16 records of 32 bytes.
+// do), 16 biases and, where the walk wants them, 16 records of 32 bytes.  What a block costs beside its products is mostly
+// the addresses of its copies: everything that a lane's copies share is worked out once (Lane pointers, places).
 template <typename T, int DK, int FORM, int STAGES_, bool RECORDS>
 struct Ring {
    static constexpr int STAGES = STAGES_, ROW = 4 * DK, CHUNKS = DK / 4, REGION = 16 * ROW;
-   static constexpr int BIAS = 2 * REGION, RECORD = BIAS + 64, STAGE = RECORD + (RECORDS ? 16 * 32 : 0);
-   const char *a, *b;       // the two arrays at the unit's first head; strides are in AttnParams
+   static constexpr int BIAS = 2 * REGION, RECORD = BIAS + 128, USED = RECORD + (RECORDS ? 16 * 32 : 0);
+   static constexpr int STAGE = (USED + ROW - 1) / ROW * ROW;  // rows are aligned to their size, so that chunks can be named by exclusive or
+   // one round of copies: 32 lanes take PER pairs of CHUNKS chunks of 8 elements
+   static constexpr int PER = 32 / CHUNKS, ROUNDS = CHUNKS / 2;
+   const char *a, *b;       // the two arrays at the lane's chunk of the unit's head 0 (of the lane's slot, if that is the same in all rounds)
    const char *records;     // [row][head][32 bytes], of the unit's first head
    EdgeStream edges;
-   unsigned ring;           // shared address
+   int batch_id;            // the present 32 edges
+   float batch_bias;
+   unsigned ring, place;    // shared addresses: block 0; the lane's chunk in a block
+   unsigned fill, slot;     // block to fill next, block in use
    long long first, end;    // the run of edges
    int issued, current;     // blocks
    int only;                // the only kv head of the unit whose pairs are gathered, or -1
 
-   // byte offset of a chunk of 8 elements
-   static __device__ __forceinline__ unsigned at(int pair, int chunk)
+   // byte offset of a chunk of 8 elements of a pair.  The chunk is exchanged by bits of the pair, so that the 8 pairs that
+   // ldmatrix reads at one chunk lie in 8 different groups of banks; offset(pair, chunk ^ x) = offset(pair, chunk) ^ (x << 4).
+   static __device__ __forceinline__ unsigned offset(int pair, int chunk)
    {
       const int key = CHUNKS >= 8 ? pair & 7 : (pair >> 1) & 3;
       return pair * ROW + ((chunk ^ key) << 4);
    }
-   __device__ __forceinline__ unsigned slot_of(int block) const { return ring + (block % STAGES) * STAGE; }
+   __device__ __forceinline__ void setup(const AttnParams &p, const Lanes &l, int lane, const void *array_a, const void *array_b, int head)
+   {
+      const int x = lane % CHUNKS, pair = lane / CHUNKS, s = PER >= 4 ? pair & (l.slots - 1) : 0;
+      const int map = x / (CHUNKS / 2), xa = (x % (CHUNKS / 2)) * 8, xb = x * 8;
+      a = static_cast<const char *>(array_a) + (head + s) * p.a_head + static_cast<long long>(map * p.a_width + xa) * sizeof(T);
+      b = static_cast<const char *>(array_b) + (head + s) * p.b_head + static_cast<long long>(xb) * sizeof(T);
+      place = ring + offset(pair, x);
+   }
 
    __device__ __forceinline__ void chunk_in(unsigned to, const T *from, int left, int step) const
    {
@@ -149,47 +164,59 @@ struct Ring {
    // gathers the next block, if there is one; always closes a group of copies
    __device__ __forceinline__ void issue(const AttnParams &p, const Lanes &l, int lane)
    {
-      const int per_block = 16 >> l.slots_log2;
+      const int per_log2 = 4 - l.slots_log2;
       const int edge_block = p.subs == 1 ? issued : issued / p.subs, sub = p.subs == 1 ? 0 : issued - edge_block * p.subs;
-      const long long e = first + static_cast<long long>(edge_block) * per_block;
-      if (e < end) {
-         const long long batch = first + (e - first) / 32 * 32;
-         const int off = static_cast<int>(e - batch);
-         const int my_id = edges.take(p, batch, end, lane);
-         const float my_bias = my_id >= 0 ? edges.bias : -INFINITY;
-         const unsigned to = slot_of(issued);
-         const float bias = __shfl_sync(FULL, my_bias, off + (lane & (per_block - 1)));
-         if (lane < per_block) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + BIAS + 4 * lane), "f"(bias) : "memory");
-         constexpr int TIMES = CHUNKS / 2, PER = 32 / CHUNKS;  // pairs of one round
-         const int x = lane % CHUNKS, pair0 = lane / CHUNKS;
-         // first array: chunk x of both maps' elements; second: chunk x
-         const int map = x / (CHUNKS / 2), xa = (x % (CHUNKS / 2)) * 8, xb = x * 8;
-         const int left_a = p.a_width - xa, left_b = p.b_width - xb;
-         const int head0 = sub << p.kv_log2;
+      const int e = edge_block << per_log2;  // from the run's start
+      if (first + e < end) {
+         const int off = e & 31;
+         if (off == 0 && sub == 0) {  // a new batch of ids; the one after it sets out
+            batch_id = edges.take(p, first + e, end, lane);
+            batch_bias = batch_id >= 0 ? edges.bias : -INFINITY;
+            edges.fetch(p, first + e + 32, lane);
+         }
+         const unsigned to = fill - ring;
+         const float bias = __shfl_sync(FULL, batch_bias, off + (lane & ((1 << per_log2) - 1)));
+         if ((lane >> per_log2) == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(fill + BIAS + 4 * lane), "f"(bias) : "memory");
+         const int pair0 = lane / CHUNKS;
+         int left_a = 1, left_b = 1;  // EXACT: every lane's chunk is there
+         if constexpr (FORM != EXACT) {
+            const int x = lane % CHUNKS;
+            left_a = p.a_width - (x % (CHUNKS / 2)) * 8;
+            left_b = p.b_width - x * 8;
+         }
+         const char *la = a, *lb = b;
+         if (sub > 0) {
+            la += (sub << p.kv_log2) * p.a_head;
+            lb += (sub << p.kv_log2) * p.b_head;
+         }
 #pragma unroll
-         for (int i = 0; i < TIMES; i++) {
-            const int pair = i * PER + pair0, s = (PER >= 4 ? pair0 : pair) & (l.slots - 1);
-            int id = __shfl_sync(FULL, my_id, off + (pair >> l.slots_log2));
-            if (only >= 0 && (s >> p.kv_log2) != only) id = -1;
+         for (int i = 0; i < ROUNDS; i++) {
+            const int pair = i * PER + pair0;
+            int id = __shfl_sync(FULL, batch_id, off + (pair >> l.slots_log2));
+            if (only >= 0 && ((pair & (l.slots - 1)) >> p.kv_log2) != only) id = -1;
             const bool live = id >= 0;
             const unsigned row = live ? id : 0;
-            const T *ra = reinterpret_cast<const T *>(a + static_cast<unsigned long long>(row) * p.a_stride + (s + head0) * p.a_head);
-            const T *rb = reinterpret_cast<const T *>(b + static_cast<unsigned long long>(row) * p.b_stride + (s + head0) * p.b_head);
-            const unsigned place = to + at(pair, x);
-            chunk_in(place, ra + map * p.a_width + xa, live ? left_a : 0, p.step);
-            chunk_in(place + REGION, rb + xb, live ? left_b : 0, p.step);
+            const char *ra = la + static_cast<unsigned long long>(row) * p.a_stride, *rb = lb + static_cast<unsigned long long>(row) * p.b_stride;
+            if constexpr (PER < 4) {
+               const int s = pair & (l.slots - 1);
+               ra += s * p.a_head;
+               rb += s * p.b_head;
+            }
+            // the pair's bits that change from round to round, as in offset()
+            const unsigned at = to + ((place + i * PER * ROW) ^ (CHUNKS >= 8 ? ((i * PER) & 7) << 4 : 0));
+            chunk_in(at, reinterpret_cast<const T *>(ra), live ? left_a : 0, p.step);
+            chunk_in(at + REGION, reinterpret_cast<const T *>(rb), live ? left_b : 0, p.step);
          }
          if constexpr (RECORDS) {
-            const int pair = lane >> 1, s = pair & (l.slots - 1);
-            const int id = __shfl_sync(FULL, my_id, off + (pair >> l.slots_log2));
+            const int pair = lane >> 1, s = (pair & (l.slots - 1)) + (sub << p.kv_log2);
+            const int id = __shfl_sync(FULL, batch_id, off + (pair >> l.slots_log2));
             const unsigned row = id >= 0 ? id : 0;
-            copy_async<16>(to + RECORD + lane * 16, records + static_cast<unsigned long long>(row) * (p.heads * 32u) + (s + head0) * 32 + (lane & 1) * 16,
+            copy_async<16>(fill + RECORD + lane * 16, records + static_cast<unsigned long long>(row) * (p.heads * 32u) + (s * 32 + (lane & 1) * 16),
                            id >= 0 ? 16 : 0);
          }
-         // the last block of a batch of ids: the next batch sets out
-         if (off + per_block == 32 && sub == p.subs - 1) edges.fetch(p, batch + 32, lane);
       }
       issued++;
+      fill = fill == ring + (STAGES - 1) * STAGE ? ring : fill + STAGE;
       asm volatile("cp.async.commit_group;" ::: "memory");
    }
    __device__ __forceinline__ void begin(const AttnParams &p, const Lanes &l, int lane, long long from, long long to, int only_kv)
@@ -200,6 +227,8 @@ struct Ring {
       only = only_kv;
       issued = 0;
       current = -1;
+      fill = ring;
+      slot = ring + (STAGES - 1) * STAGE;
 #pragma unroll 1
       for (int i = 0; i < STAGES - 1; i++) issue(p, l, lane);
    }
@@ -211,6 +240,7 @@ struct Ring {
       asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
       __syncwarp();  // every lane's copies are there
       current++;
+      slot = slot == ring + (STAGES - 1) * STAGE ? ring : slot + STAGE;
    }
    __device__ __forceinline__ void drain()
    {
@@ -307,8 +337,7 @@ struct ForwardMma {
       l.set(at, p.unit_kv);
       kv0 = (at.unit / p.head_blocks) * p.unit_kv;
       heads.set(p, at, l, kv0);
-      ring.a = static_cast<const char *>(p.k) + kv0 * p.a_head;
-      ring.b = static_cast<const char *>(p.v) + kv0 * p.b_head;
+      ring.setup(p, l, at.lane, p.k, p.v, kv0);
    }
    static __device__ __forceinline__ void clear(State &s)
    {
@@ -336,20 +365,19 @@ struct ForwardMma {
       for (int i = 0; i < DK / 8; i++) q[i] = next[i];
       if (Width::AHEAD && follow >= 0) fetch(p, follow);
       const int per_log2 = 4 - l.slots_log2;
-      // rows of ldmatrix: lane's pair and chunk parity
-      const int pair = at.lane & 15, high = at.lane >> 4;
+      const unsigned mine = Gathered::offset(at.lane & 15, at.lane >> 4);  // the lane's row of ldmatrix; chunks by exclusive or
       for (int e = e0; e < e1;) {
          const int block = e >> per_log2;
          if (block != ring.current) ring.advance(p, l, at.lane);
          const int lo = e - (block << per_log2), left = e1 - (block << per_log2), hi = left < (1 << per_log2) ? left : 1 << per_log2;
-         const unsigned slot = ring.slot_of(block);
+         const unsigned slot = ring.slot;
          float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
          for (int i = 0; i < DK / 16; i++) {
             unsigned k[4];
-            ldmatrix4(k, slot + Gathered::at(pair, 2 * i + high));
+            ldmatrix4(k, (slot + mine) ^ ((2 * i) << 4));
             mma16816<T>(s0, k[0], k[1], k[2], k[3], q[2 * i], q[2 * i + 1]);
-            ldmatrix4(k, slot + Gathered::at(pair, DK / 8 + 2 * i + high));
+            ldmatrix4(k, (slot + mine) ^ ((DK / 8 + 2 * i) << 4));
             mma16816<T>(s1, k[0], k[1], k[2], k[3], q[2 * i], q[2 * i + 1]);
          }
          float score[2][2];
@@ -398,7 +426,7 @@ struct ForwardMma {
 #pragma unroll
          for (int t = 0; t < TILES; t += 2) {
             unsigned v[4];
-            ldmatrix4_trans(v, slot + Gathered::REGION + Gathered::at(pair, t + high));
+            ldmatrix4_trans(v, (slot + mine + Gathered::REGION) ^ ((t) << 4));
             mma16816<T>(acc[t], a[0], a[1], a[2], a[3], v[0], v[1]);
             mma16816<T>(acc[t + 1], a[0], a[1], a[2], a[3], v[2], v[3]);
          }
@@ -512,8 +540,7 @@ struct BackwardRowsMma {
       l.set(at, p.unit_kv);
       kv0 = (at.unit / p.head_blocks) * p.unit_kv;
       heads.set(p, at, l, kv0);
-      ring.a = static_cast<const char *>(p.k) + kv0 * p.a_head;
-      ring.b = static_cast<const char *>(p.v) + kv0 * p.b_head;
+      ring.setup(p, l, at.lane, p.k, p.v, kv0);
    }
    static __device__ __forceinline__ void clear(State &s)
    {
@@ -547,25 +574,25 @@ struct BackwardRowsMma {
       for (int i = 0; i < DV / 8; i++) dout[i] = next_out[i];
       if (Width::AHEAD && follow >= 0) fetch(p, follow);
       const int per_log2 = 4 - l.slots_log2;
-      const int pair = at.lane & 15, high = at.lane >> 4;
+      const unsigned mine = Gathered::offset(at.lane & 15, at.lane >> 4);  // the lane's row of ldmatrix; chunks by exclusive or
       for (int e = e0; e < e1;) {
          const int block = e >> per_log2;
          if (block != ring.current) ring.advance(p, l, at.lane);
          const int lo = e - (block << per_log2), left = e1 - (block << per_log2), hi = left < (1 << per_log2) ? left : 1 << per_log2;
-         const unsigned slot = ring.slot_of(block);
+         const unsigned slot = ring.slot;
          float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
          for (int i = 0; i < DK / 16; i++) {
             unsigned k[4];
-            ldmatrix4(k, slot + Gathered::at(pair, 2 * i + high));
+            ldmatrix4(k, (slot + mine) ^ ((2 * i) << 4));
             mma16816<T>(s0, k[0], k[1], k[2], k[3], q[2 * i], q[2 * i + 1]);
-            ldmatrix4(k, slot + Gathered::at(pair, DK / 8 + 2 * i + high));
+            ldmatrix4(k, (slot + mine) ^ ((DK / 8 + 2 * i) << 4));
             mma16816<T>(s1, k[0], k[1], k[2], k[3], q[2 * i], q[2 * i + 1]);
          }
 #pragma unroll
          for (int i = 0; i < DV / 16; i++) {
             unsigned v[4];
-            ldmatrix4(v, slot + Gathered::REGION + Gathered::at(pair, 2 * i + high));
+            ldmatrix4(v, (slot + mine + Gathered::REGION) ^ ((2 * i) << 4));
             mma16816<T>(dp, v[0], v[1], v[2], v[3], dout[2 * i], dout[2 * i + 1]);
          }
          unsigned a0[4], a1[4];
@@ -599,10 +626,10 @@ struct BackwardRowsMma {
 #pragma unroll
          for (int t = 0; t < TILES; t += 2) {
             unsigned k[4];
-            ldmatrix4_trans(k, slot + Gathered::at(pair, t + high));
+            ldmatrix4_trans(k, (slot + mine) ^ ((t) << 4));
             mma16816<T>(acc[0][t], a0[0], a0[1], a0[2], a0[3], k[0], k[1]);
             mma16816<T>(acc[0][t + 1], a0[0], a0[1], a0[2], a0[3], k[2], k[3]);
-            ldmatrix4_trans(k, slot + Gathered::at(pair, DK / 8 + t + high));
+            ldmatrix4_trans(k, (slot + mine) ^ ((DK / 8 + t) << 4));
             mma16816<T>(acc[1][t], a1[0], a1[1], a1[2], a1[3], k[0], k[1]);
             mma16816<T>(acc[1][t + 1], a1[0], a1[1], a1[2], a1[3], k[2], k[3]);
          }
@@ -715,8 +742,7 @@ struct BackwardColumnsMma {
       per_kv = p.unit_heads;
       pair_kv = l.pair_slot / per_kv;
       const long long head = kv0 * p.group;
-      ring.a = static_cast<const char *>(p.q) + head * p.a_head;
-      ring.b = static_cast<const char *>(p.dout) + head * p.b_head;
+      ring.setup(p, l, at.lane, p.q, p.dout, kv0 * p.group);
       ring.records = reinterpret_cast<const char *>(p.stats + head * 2);
    }
    static __device__ __forceinline__ void clear(State &s)
@@ -748,7 +774,7 @@ struct BackwardColumnsMma {
       for (int i = 0; i < DV / 8; i++) v[i] = next_v[i];
       if (Width::AHEAD && follow >= 0) fetch(p, follow);
       const int per_log2 = 4 - l.slots_log2;
-      const int pair = at.lane & 15, high = at.lane >> 4;
+      const unsigned mine = Gathered::offset(at.lane & 15, at.lane >> 4);  // the lane's row of ldmatrix; chunks by exclusive or
       // of the columns 2c, 2c + 1 at most one is of the pairs' kv head
       const bool valid = (l.c & 1) == pair_kv >> 1;
       const int x = pair_kv & 1, map = l.c >> 1;
@@ -758,20 +784,20 @@ struct BackwardColumnsMma {
          for (int sub = 0; sub < p.subs; sub++) {
             const int block = edges * p.subs + sub;
             if (block != ring.current) ring.advance(p, l, at.lane);
-            const unsigned slot = ring.slot_of(block);
+            const unsigned slot = ring.slot;
             float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < DK / 16; i++) {
                unsigned q[4];
-               ldmatrix4(q, slot + Gathered::at(pair, 2 * i + high));
+               ldmatrix4(q, (slot + mine) ^ ((2 * i) << 4));
                mma16816<T>(s0, q[0], q[1], q[2], q[3], k[2 * i], k[2 * i + 1]);
-               ldmatrix4(q, slot + Gathered::at(pair, DK / 8 + 2 * i + high));
+               ldmatrix4(q, (slot + mine) ^ ((DK / 8 + 2 * i) << 4));
                mma16816<T>(s1, q[0], q[1], q[2], q[3], k[2 * i], k[2 * i + 1]);
             }
 #pragma unroll
             for (int i = 0; i < DV / 16; i++) {
                unsigned d[4];
-               ldmatrix4(d, slot + Gathered::REGION + Gathered::at(pair, 2 * i + high));
+               ldmatrix4(d, (slot + mine + Gathered::REGION) ^ ((2 * i) << 4));
                mma16816<T>(dp, d[0], d[1], d[2], d[3], v[2 * i], v[2 * i + 1]);
             }
             unsigned b0[2], b1[2], bw[2];
@@ -800,15 +826,15 @@ struct BackwardColumnsMma {
 #pragma unroll
             for (int t = 0; t < KT; t++) {
                unsigned q[4];
-               ldmatrix4_trans(q, slot + Gathered::at(pair, 2 * t + high));
+               ldmatrix4_trans(q, (slot + mine) ^ ((2 * t) << 4));
                mma16816<T>(s.dk[0][t], q[0], q[2], q[1], q[3], b0[0], b0[1]);
-               ldmatrix4_trans(q, slot + Gathered::at(pair, DK / 8 + 2 * t + high));
+               ldmatrix4_trans(q, (slot + mine) ^ ((DK / 8 + 2 * t) << 4));
                mma16816<T>(s.dk[1][t], q[0], q[2], q[1], q[3], b1[0], b1[1]);
             }
 #pragma unroll
             for (int t = 0; t < VT; t++) {
                unsigned d[4];
-               ldmatrix4_trans(d, slot + Gathered::REGION + Gathered::at(pair, 2 * t + high));
+               ldmatrix4_trans(d, (slot + mine + Gathered::REGION) ^ ((2 * t) << 4));
                mma16816<T>(s.dv[t], d[0], d[2], d[1], d[3], bw[0], bw[1]);
             }
          }
@@ -942,6 +968,8 @@ __device__ __forceinline__ void ring_segment(Op &op, typename Op::Gathered &ring
    if (lost && !TOGETHER && p.subs == 1) ring.begin(p, op.l, at.lane, e1, run_end, -1);
 }
 
+constexpr int RING_ALIGN = 512;  // the longest row of a ring
+
 template <typename Op, bool TOGETHER>
 __global__ void __launch_bounds__((TOGETHER ? Op::Width::JOINT : Op::Width::SOLO) * 32, TOGETHER ? 1 : Op::Width::BLOCKS)
 ring_walk_kernel(const AttnParams p)
@@ -957,7 +985,7 @@ ring_walk_kernel(const AttnParams p)
    const long long lo = piece * p.piece, hi = lo + p.piece;
    Op op;
    typename Op::Gathered ring;
-   ring.ring = static_cast<unsigned>(__cvta_generic_to_shared(shared)) + warp * (Op::Gathered::STAGES * Op::Gathered::STAGE);
+   ring.ring = ((static_cast<unsigned>(__cvta_generic_to_shared(shared)) + RING_ALIGN - 1) & ~(RING_ALIGN - 1u)) + warp * (Op::Gathered::STAGES * Op::Gathered::STAGE);
    op.setup(p, at, ring);
    long long u = rows.lower_bound(lo, 0, p.m, at.lane);
    // the rows that begin in this piece end before `last`: a row is ROW_ITEMS items at least
@@ -1046,11 +1074,11 @@ int launch_ring(const AttnParams &p, bool together, cudaStream_t st)
    static_assert(JOIN <= Op::Width::JOINT * RING, "the rings serve as the place where warps meet");
    const long long jobs = p.pieces * p.unit_blocks;
    if (together) {
-      constexpr int bytes = Op::Width::JOINT * RING;
+      constexpr int bytes = Op::Width::JOINT * RING + RING_ALIGN;
       if (cudaFuncSetAttribute(ring_walk_kernel<Op, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -1;
       ring_walk_kernel<Op, true><<<static_cast<unsigned>(jobs), Op::Width::JOINT * 32, bytes, st>>>(p);
    } else {
-      constexpr int bytes = Op::Width::SOLO * RING;
+      constexpr int bytes = Op::Width::SOLO * RING + RING_ALIGN;
       if (cudaFuncSetAttribute(ring_walk_kernel<Op, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -1;
       ring_walk_kernel<Op, false><<<static_cast<unsigned>((jobs + Op::Width::SOLO - 1) / Op::Width::SOLO), Op::Width::SOLO * 32, bytes, st>>>(p);
    }
