@@ -4,7 +4,7 @@
 namespace fmm {
 namespace attn {
 
-int walk_forward_f16(const WalkShape &s, const AttnParams &p, cudaStream_t st) { return launch_mma<__half, ForwardMma>(s, p, st); }
+int walk_forward_f16(const WalkShape &s, const AttnParams &p, cudaStream_t st) { return launch_mma<__half, true, ForwardMma>(s, p, st); }
 
 }  // namespace attn
 }  // namespace fmm

@@ -33,6 +33,24 @@ __device__ __forceinline__ void mma16816(float (&c)[4], unsigned a0, unsigned a1
       asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                    : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// ... the first product of a sum
+template <typename T>
+__device__ __forceinline__ void mma16816_first(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1)
+{
+   const float z = 0.0f;
+   if constexpr (std::is_same<T, __half>::value)
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                   : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(z));
+   else
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                   : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(z));
+}
+template <typename T>
+__device__ __forceinline__ void mma16816_at(bool start, float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1)
+{
+   if (start) mma16816_first<T>(c, a[0], a[1], a[2], a[3], b0, b1);
+   else mma16816<T>(c, a[0], a[1], a[2], a[3], b0, b1);
+}
 __device__ __forceinline__ unsigned transpose8x8(unsigned v)
 {
    unsigned r;
@@ -123,9 +141,10 @@ struct Ring {
    float batch_bias;
    unsigned ring, place;    // shared addresses: block 0; the lane's chunk in a block
    unsigned fill, slot;     // block to fill next, block in use
-   long long first, end;    // the run of edges
+   long long first;         // the run of edges
+   int length;
    int issued, current;     // blocks
-   int only;                // the only kv head of the unit whose pairs are gathered, or -1
+   unsigned on;             // bit i: the lane's pair of round i is gathered (all, but where the kv heads are taken one by one)
 
    // byte offset of a chunk of 8 elements of a pair.  The chunk is exchanged by bits of the pair, so that the 8 pairs that
    // ldmatrix reads at one chunk lie in 8 different groups of banks; offset(pair, chunk ^ x) = offset(pair, chunk) ^ (x << 4).
@@ -167,10 +186,10 @@ struct Ring {
       const int per_log2 = 4 - l.slots_log2;
       const int edge_block = p.subs == 1 ? issued : issued / p.subs, sub = p.subs == 1 ? 0 : issued - edge_block * p.subs;
       const int e = edge_block << per_log2;  // from the run's start
-      if (first + e < end) {
+      if (e < length) {
          const int off = e & 31;
          if (off == 0 && sub == 0) {  // a new batch of ids; the one after it sets out
-            batch_id = edges.take(p, first + e, end, lane);
+            batch_id = edges.take(p, first + e, first + length, lane);
             batch_bias = batch_id >= 0 ? edges.bias : -INFINITY;
             edges.fetch(p, first + e + 32, lane);
          }
@@ -192,9 +211,8 @@ struct Ring {
 #pragma unroll
          for (int i = 0; i < ROUNDS; i++) {
             const int pair = i * PER + pair0;
-            int id = __shfl_sync(FULL, batch_id, off + (pair >> l.slots_log2));
-            if (only >= 0 && ((pair & (l.slots - 1)) >> p.kv_log2) != only) id = -1;
-            const bool live = id >= 0;
+            const int id = __shfl_sync(FULL, batch_id, off + (pair >> l.slots_log2));
+            const bool live = id >= 0 && (on >> i & 1);
             const unsigned row = live ? id : 0;
             const char *ra = la + static_cast<unsigned long long>(row) * p.a_stride, *rb = lb + static_cast<unsigned long long>(row) * p.b_stride;
             if constexpr (PER < 4) {
@@ -223,8 +241,11 @@ struct Ring {
    {
       drain();
       first = from;
-      end = to;
-      only = only_kv;
+      length = static_cast<int>(to - from);
+      on = ~0u;
+      if (only_kv >= 0)
+         for (int i = 0; i < ROUNDS; i++)
+            if ((((i * PER + lane / CHUNKS) & (l.slots - 1)) >> p.kv_log2) != only_kv) on &= ~(1u << i);
       issued = 0;
       current = -1;
       fill = ring;
@@ -256,32 +277,64 @@ __device__ __forceinline__ float shared_float(unsigned at)
    return f;
 }
 
-// value of column n = r from the lanes that hold the columns 2c and 2c + 1 (the same in all r)
-__device__ __forceinline__ float of_column(float x0, float x1, int r)
-{
-   const float a = __shfl_sync(FULL, x0, r >> 1), b = __shfl_sync(FULL, x1, r >> 1);
-   return r & 1 ? b : a;
-}
-__device__ __forceinline__ float sum_pairs(float v)
-{
-   v += __shfl_xor_sync(FULL, v, 4);
-   v += __shfl_xor_sync(FULL, v, 8);
-   return v + __shfl_xor_sync(FULL, v, 16);
-}
-__device__ __forceinline__ float max_pairs(float v)
-{
-   v = fmaxf(v, __shfl_xor_sync(FULL, v, 4));
-   v = fmaxf(v, __shfl_xor_sync(FULL, v, 8));
-   return fmaxf(v, __shfl_xor_sync(FULL, v, 16));
-}
+// What a lane knows of the score columns.  A product has 8 columns, (map, slot); with four kv heads to a unit a pair has one
+// column of each map that counts, so a lane has at most one (ONE); otherwise it has the columns 2c and 2c + 1.
+template <bool ONE>
+struct Columns {
+   static constexpr int N = ONE ? 1 : 2;
+   // value of column n = r from the lanes that hold it
+   static __device__ __forceinline__ float of_row(const float (&x)[N], int r)
+   {
+      if constexpr (ONE) return __shfl_sync(FULL, x[0], 4 * (r & 3) + 2 * (r >> 2) + ((r >> 1) & 1));
+      const float a = __shfl_sync(FULL, x[0], r >> 1), b = __shfl_sync(FULL, x[N - 1], r >> 1);
+      return r & 1 ? b : a;
+   }
+   // over all pairs
+   static __device__ __forceinline__ float sum(float v)
+   {
+      if constexpr (!ONE) {
+         v += __shfl_xor_sync(FULL, v, 4);
+         v += __shfl_xor_sync(FULL, v, 8);
+      }
+      return v + __shfl_xor_sync(FULL, v, 16);
+   }
+   static __device__ __forceinline__ float max(float v)
+   {
+      if constexpr (!ONE) {
+         v = fmaxf(v, __shfl_xor_sync(FULL, v, 4));
+         v = fmaxf(v, __shfl_xor_sync(FULL, v, 8));
+      }
+      return fmaxf(v, __shfl_xor_sync(FULL, v, 16));
+   }
+   // the scores of pair r + 8h that count, of the two maps' products
+   static __device__ __forceinline__ float pick(const float (&s0)[4], const float (&s1)[4], int h, int x, const Lanes &l)
+   {
+      if constexpr (ONE) return l.pair_slot & 1 ? (l.c < 2 ? s0[2 * h + 1] : s1[2 * h + 1]) : (l.c < 2 ? s0[2 * h] : s1[2 * h]);
+      return l.c < 2 ? s0[2 * h + x] : s1[2 * h + x];
+   }
+   static __device__ __forceinline__ float pick(const float (&s)[4], int h, int x, const Lanes &l)
+   {
+      if constexpr (ONE) return l.pair_slot & 1 ? s[2 * h + 1] : s[2 * h];
+      return s[2 * h + x];
+   }
+   // the weights of pair r + 8h at the columns 2c, 2c + 1, split
+   template <typename T>
+   static __device__ __forceinline__ void split(const float (&w)[N], const Lanes &l, unsigned &hi, unsigned &lo)
+   {
+      if constexpr (ONE) split2<T>(l.pair_slot & 1 ? 0.0f : w[0], l.pair_slot & 1 ? w[0] : 0.0f, hi, lo);
+      else split2<T>(w[0], w[N - 1], hi, lo);
+   }
+};
 
 // The query heads of the row walks' columns: column n = 4 map + s, s = (kv head of the unit) * unit_heads + (query head of it).
+template <bool ONE>
 struct QueryHeads {
+   static constexpr int N = ONE ? 1 : 2;
    int head;        // of column n = r, one that exists if that column is none
    bool live;       // column n = r is one
    int kv;          // which of the unit's kv heads column n = r is of
-   bool valid[2];   // the pairs r and r + 8 belong to the columns 2c, 2c + 1
-   int col_head[2], col_kv[2];
+   bool valid[N];   // the pairs r and r + 8 belong to this lane's columns
+   int col_head[N], col_kv[N];
    __device__ __forceinline__ void set(const AttnParams &p, const Place &at, const Lanes &l, int kv0)
    {
       const int first = (at.unit % p.head_blocks) * p.unit_heads, rest = p.group - first;
@@ -291,8 +344,8 @@ struct QueryHeads {
       live = kv < l.slots && g < heads;
       head = live ? (kv0 + kv) * p.group + first + g : kv0 * p.group + first;
 #pragma unroll
-      for (int x = 0; x < 2; x++) {
-         const int sx = (2 * l.c + x) & 3, gx = sx % p.unit_heads;
+      for (int x = 0; x < N; x++) {
+         const int sx = (2 * l.c + (ONE ? l.pair_slot & 1 : x)) & 3, gx = sx % p.unit_heads;
          col_kv[x] = sx / p.unit_heads;
          valid[x] = col_kv[x] == l.pair_slot && gx < heads;
          col_head[x] = valid[x] ? (kv0 + col_kv[x]) * p.group + first + gx : head;
@@ -316,18 +369,20 @@ struct Budget {
 // ---------------------------------------------------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int DK, int FORM>
+template <typename T, int DK, int FORM, bool ONE>
 struct ForwardMma {
+   using Cols = Columns<ONE>;
+   static constexpr int N = Cols::N;
    static constexpr int DV = 2 * DK, TILES = DV / 8, LANE_FLOATS = 2 * TILES + 4;
    using Gathered = Ring<T, DK, FORM, Budget<DK>::STAGES, false>;
    using Width = Budget<DK>;
    struct State {
       float acc[TILES][2];   // rows n = r: sums of weights times v, columns 8t + 2c, + 1
-      float top[2], sum[2];  // columns 2c, 2c + 1
+      float top[N], sum[N];  // of this lane's columns
    };
    State s;
    Lanes l;
-   QueryHeads heads;
+   QueryHeads<ONE> heads;
    int kv0;
    unsigned next[DK / 8];
    bool lost;  // run() met a number that is none
@@ -343,8 +398,11 @@ struct ForwardMma {
    {
 #pragma unroll
       for (int t = 0; t < TILES; t++) s.acc[t][0] = s.acc[t][1] = 0.0f;
-      s.top[0] = s.top[1] = -INFINITY;
-      s.sum[0] = s.sum[1] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < N; x++) {
+         s.top[x] = -INFINITY;
+         s.sum[x] = 0.0f;
+      }
    }
    // the row's own operand, ahead of run()
    __device__ __forceinline__ void fetch(const AttnParams &p, long long row)
@@ -358,8 +416,11 @@ struct ForwardMma {
       float acc[TILES][4];
 #pragma unroll
       for (int t = 0; t < TILES; t++) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.0f;
-      s.top[0] = s.top[1] = -INFINITY;
-      s.sum[0] = s.sum[1] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < N; x++) {
+         s.top[x] = -INFINITY;
+         s.sum[x] = 0.0f;
+      }
       unsigned q[DK / 8];
 #pragma unroll
       for (int i = 0; i < DK / 8; i++) q[i] = next[i];
@@ -371,55 +432,60 @@ struct ForwardMma {
          if (block != ring.current) ring.advance(p, l, at.lane);
          const int lo = e - (block << per_log2), left = e1 - (block << per_log2), hi = left < (1 << per_log2) ? left : 1 << per_log2;
          const unsigned slot = ring.slot;
-         float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+         float s0[4], s1[4];
 #pragma unroll
          for (int i = 0; i < DK / 16; i++) {
             unsigned k[4];
             ldmatrix4(k, (slot + mine) ^ ((2 * i) << 4));
-            mma16816<T>(s0, k[0], k[1], k[2], k[3], q[2 * i], q[2 * i + 1]);
+            mma16816_at<T>(i == 0, s0, k, q[2 * i], q[2 * i + 1]);
             ldmatrix4(k, (slot + mine) ^ ((DK / 8 + 2 * i) << 4));
-            mma16816<T>(s1, k[0], k[1], k[2], k[3], q[2 * i], q[2 * i + 1]);
+            mma16816_at<T>(i == 0, s1, k, q[2 * i], q[2 * i + 1]);
          }
-         float score[2][2];
+         float score[2][N], high[N];
+         bool grown = false;
 #pragma unroll
          for (int h = 0; h < 2; h++) {
             const int edge = (l.r + 8 * h) >> l.slots_log2;
             const float bias = shared_float(slot + Gathered::BIAS + 4 * edge);
             const bool live = edge >= lo && edge < hi && bias != -INFINITY;
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-               const float dot = l.c < 2 ? s0[2 * h + x] : s1[2 * h + x];
-               score[h][x] = heads.valid[x] && live ? fmaf(dot, p.scale, bias) : -INFINITY;
-            }
+            for (int x = 0; x < N; x++) score[h][x] = heads.valid[x] && live ? fmaf(Cols::pick(s0, s1, h, x, l), p.scale, bias) : -INFINITY;
          }
-         const float m0 = fmaxf(score[0][0], score[1][0]), m1 = fmaxf(score[0][1], score[1][1]);
-         if (__any_sync(FULL, m0 > s.top[0] + SLACK || m1 > s.top[1] + SLACK)) {
-            const float t0 = fmaxf(s.top[0], max_pairs(m0)), t1 = fmaxf(s.top[1], max_pairs(m1));
-            const float f0 = t0 == -INFINITY ? 1.0f : exp2_fast((s.top[0] - t0) * LOG2E);
-            const float f1 = t1 == -INFINITY ? 1.0f : exp2_fast((s.top[1] - t1) * LOG2E);
-            s.top[0] = t0;
-            s.top[1] = t1;
+#pragma unroll
+         for (int x = 0; x < N; x++) {
+            high[x] = fmaxf(score[0][x], score[1][x]);
+            grown |= high[x] > s.top[x] + SLACK;
+         }
+         if (__any_sync(FULL, grown)) {
+            float f[N];
+#pragma unroll
+            for (int x = 0; x < N; x++) {
+               const float t = fmaxf(s.top[x], Cols::max(high[x]));
+               f[x] = t == -INFINITY ? 1.0f : exp2_fast((s.top[x] - t) * LOG2E);
+               s.top[x] = t;
+               s.sum[x] *= f[x];
+            }
             if (e != e0) {
-               const float f = of_column(f0, f1, l.r);
-               s.sum[0] *= f0;
-               s.sum[1] *= f1;
+               const float fr = Cols::of_row(f, l.r);
 #pragma unroll
                for (int t = 0; t < TILES; t++)
 #pragma unroll
-                  for (int i = 0; i < 4; i++) acc[t][i] *= f;
+                  for (int i = 0; i < 4; i++) acc[t][i] *= fr;
             }
          }
-         // a row that has met no edge yet has the maximum -inf: its differences are taken from 0
-         const float ref0 = s.top[0] == -INFINITY ? 0.0f : s.top[0], ref1 = s.top[1] == -INFINITY ? 0.0f : s.top[1];
          unsigned a[4];
 #pragma unroll
          for (int h = 0; h < 2; h++) {
-            // the difference is taken before the factor: scores near the type's largest numbers keep their order
-            const float p0 = exp2_fast((score[h][0] - ref0) * LOG2E), p1 = exp2_fast((score[h][1] - ref1) * LOG2E);
-            s.sum[0] += p0;
-            s.sum[1] += p1;
+            float w[N];
+#pragma unroll
+            for (int x = 0; x < N; x++) {
+               // a row that has met no edge yet has the maximum -inf: its differences are taken from 0.
+               // The difference is taken before the factor: scores near the type's largest numbers keep their order.
+               w[x] = exp2_fast((score[h][x] - (s.top[x] == -INFINITY ? 0.0f : s.top[x])) * LOG2E);
+               s.sum[x] += w[x];
+            }
             unsigned up, low;
-            split2<T>(p0, p1, up, low);
+            Cols::template split<T>(w, l, up, low);
             a[2 * h] = transpose8x8(up);
             a[2 * h + 1] = transpose8x8(low);
          }
@@ -440,17 +506,17 @@ struct ForwardMma {
          all += s.acc[t][0] * 0.0f + s.acc[t][1] * 0.0f;  // 0, or NaN once anything is infinite or NaN
       }
       lost = all != all;
-      s.sum[0] = sum_pairs(s.sum[0]);
-      s.sum[1] = sum_pairs(s.sum[1]);
+#pragma unroll
+      for (int x = 0; x < N; x++) s.sum[x] = Cols::sum(s.sum[x]);
    }
 
    __device__ __forceinline__ void join_from(const float *unit, const Place &at)
    {
       const float2 *from = reinterpret_cast<const float2 *>(unit) + at.lane;
       const float2 top = from[32 * TILES], sum = from[32 * (TILES + 1)];
-      float f[2], g[2];
+      float f[N], g[N];
 #pragma unroll
-      for (int x = 0; x < 2; x++) {
+      for (int x = 0; x < N; x++) {
          const float ot = x ? top.y : top.x, os = x ? sum.y : sum.x;
          const float t = fmaxf(s.top[x], ot), ref = t == -INFINITY ? 0.0f : t;
          f[x] = exp2_fast((s.top[x] - ref) * LOG2E);
@@ -458,7 +524,7 @@ struct ForwardMma {
          s.sum[x] = s.sum[x] * f[x] + os * g[x];
          s.top[x] = t;
       }
-      const float fr = of_column(f[0], f[1], l.r), gr = of_column(g[0], g[1], l.r);
+      const float fr = Cols::of_row(f, l.r), gr = Cols::of_row(g, l.r);
 #pragma unroll
       for (int t = 0; t < TILES; t++) {
          const float2 o = from[32 * t];
@@ -475,7 +541,7 @@ struct ForwardMma {
       }
       float *top = reinterpret_cast<float *>(to + 32 * TILES), *sum = reinterpret_cast<float *>(to + 32 * (TILES + 1));
 #pragma unroll
-      for (int x = 0; x < 2; x++)
+      for (int x = 0; x < N; x++)
          if (only < 0 || heads.col_kv[x] == only) {
             top[x] = s.top[x];
             sum[x] = s.sum[x];
@@ -484,22 +550,25 @@ struct ForwardMma {
 
    __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long row, int only)
    {
-      const float sum = of_column(s.sum[0], s.sum[1], l.r), top = of_column(s.top[0], s.top[1], l.r);
+      const float sum = Cols::of_row(s.sum, l.r), top = Cols::of_row(s.top, l.r);
       const bool mine = heads.live && (only < 0 || heads.kv == only);
       const float lam = __ldg(p.lam + row * p.ldlam + heads.head), f = sum == 0.0f ? 0.0f : __frcp_rn(sum);
       const long long rh = row * p.heads + heads.head;
-      T *out = static_cast<T *>(p.out) + rh * p.dv + 2 * l.c;
+      // rows 0..3 hold map 0, rows 4..7 map 1: these take the even, those the odd tiles of the result
+      const int odd = l.r >> 2;
+      T *out = static_cast<T *>(p.out) + rh * p.dv + 8 * odd + 2 * l.c;
 #pragma unroll
-      for (int t = 0; t < TILES; t++) {
+      for (int t = 0; t < TILES; t += 2) {
          float o[2];
 #pragma unroll
          for (int x = 0; x < 2; x++) {
-            const float v = s.acc[t][x] * f;
-            o[x] = v - lam * __shfl_xor_sync(FULL, v, 16);
+            const float keep = f * (odd ? s.acc[t + 1][x] : s.acc[t][x]), give = f * (odd ? s.acc[t][x] : s.acc[t + 1][x]);
+            const float got = __shfl_xor_sync(FULL, give, 16);
+            o[x] = odd ? got - lam * keep : keep - lam * got;
          }
-         if (mine && l.r < 4) store_two<T, FORM>(out + 8 * t, o[0], o[1], p.dv - 8 * t - 2 * l.c);
+         if (mine) store_two<T, FORM>(out + 8 * t, o[0], o[1], p.dv - 8 * (t + odd) - 2 * l.c);
       }
-      if (mine && l.c == 0 && p.lse) p.lse[rh * 2 + (l.r >> 2)] = top + LN2 * log2f(sum);
+      if (mine && l.c == 0 && p.lse) p.lse[rh * 2 + odd] = top + LN2 * log2f(sum);
    }
    __device__ __forceinline__ void finish_empty(const AttnParams &p, const Place &at, long long row)
    {
@@ -518,21 +587,23 @@ struct ForwardMma {
 // backward over the rows (the sums A = sum p dP k, B = sum p k, D = sum p dP of BackwardRows).  For map 0 the rows of A's
 // operand are w = p dP of the columns 0..3 and p of the same, for map 1 the other way round.
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int DK, int FORM>
+template <typename T, int DK, int FORM, bool ONE>
 struct BackwardRowsMma {
+   using Cols = Columns<ONE>;
+   static constexpr int N = Cols::N;
    static constexpr int DV = 2 * DK, TILES = DK / 8, LANE_FLOATS = 4 * TILES + 2;
    using Gathered = Ring<T, DK, FORM, Budget<DK>::STAGES, false>;
    using Width = Budget<DK>;
    struct State {
       float acc[2][TILES][2];
-      float delta[2];  // columns 2c, 2c + 1
+      float delta[N];  // of this lane's columns
    };
    State s;
    Lanes l;
-   QueryHeads heads;
+   QueryHeads<ONE> heads;
    int kv0;
    unsigned next[DK / 8], next_out[DV / 8];
-   float next_lse[2];
+   float next_lse[N];
    bool lost;
 
    __device__ __forceinline__ void setup(const AttnParams &p, const Place &at, Gathered &ring)
@@ -548,14 +619,15 @@ struct BackwardRowsMma {
       for (int m = 0; m < 2; m++)
 #pragma unroll
          for (int t = 0; t < TILES; t++) s.acc[m][t][0] = s.acc[m][t][1] = 0.0f;
-      s.delta[0] = s.delta[1] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < N; x++) s.delta[x] = 0.0f;
    }
    __device__ __forceinline__ void fetch(const AttnParams &p, long long row)
    {
       load_operand<T, DK, FORM>(static_cast<const T *>(p.q) + row * p.ldq + heads.head * p.hsq + (l.r >> 2) * p.d, l.c, p.d, p.step, next);
       load_operand<T, DV, FORM>(static_cast<const T *>(p.dout) + row * p.ldo + heads.head * p.hso, l.c, p.dv, p.step, next_out);
 #pragma unroll
-      for (int x = 0; x < 2; x++) next_lse[x] = __ldg(p.lse + (row * p.heads + heads.col_head[x]) * 2 + (l.c >> 1));
+      for (int x = 0; x < N; x++) next_lse[x] = __ldg(p.lse + (row * p.heads + heads.col_head[x]) * 2 + (l.c >> 1));
    }
 
    __device__ __forceinline__ void run(const AttnParams &p, const Place &at, Gathered &ring, int e0, int e1, long long follow)
@@ -565,9 +637,12 @@ struct BackwardRowsMma {
       for (int m = 0; m < 2; m++)
 #pragma unroll
          for (int t = 0; t < TILES; t++) acc[m][t][0] = acc[m][t][1] = acc[m][t][2] = acc[m][t][3] = 0.0f;
-      s.delta[0] = s.delta[1] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < N; x++) s.delta[x] = 0.0f;
       unsigned q[DK / 8], dout[DV / 8];
-      float lse[2] = {next_lse[0], next_lse[1]};
+      float lse[N];
+#pragma unroll
+      for (int x = 0; x < N; x++) lse[x] = next_lse[x];
 #pragma unroll
       for (int i = 0; i < DK / 8; i++) q[i] = next[i];
 #pragma unroll
@@ -580,20 +655,20 @@ struct BackwardRowsMma {
          if (block != ring.current) ring.advance(p, l, at.lane);
          const int lo = e - (block << per_log2), left = e1 - (block << per_log2), hi = left < (1 << per_log2) ? left : 1 << per_log2;
          const unsigned slot = ring.slot;
-         float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+         float s0[4], s1[4], dp[4];
 #pragma unroll
          for (int i = 0; i < DK / 16; i++) {
             unsigned k[4];
             ldmatrix4(k, (slot + mine) ^ ((2 * i) << 4));
-            mma16816<T>(s0, k[0], k[1], k[2], k[3], q[2 * i], q[2 * i + 1]);
+            mma16816_at<T>(i == 0, s0, k, q[2 * i], q[2 * i + 1]);
             ldmatrix4(k, (slot + mine) ^ ((DK / 8 + 2 * i) << 4));
-            mma16816<T>(s1, k[0], k[1], k[2], k[3], q[2 * i], q[2 * i + 1]);
+            mma16816_at<T>(i == 0, s1, k, q[2 * i], q[2 * i + 1]);
          }
 #pragma unroll
          for (int i = 0; i < DV / 16; i++) {
             unsigned v[4];
             ldmatrix4(v, (slot + mine + Gathered::REGION) ^ ((2 * i) << 4));
-            mma16816<T>(dp, v[0], v[1], v[2], v[3], dout[2 * i], dout[2 * i + 1]);
+            mma16816_at<T>(i == 0, dp, v, dout[2 * i], dout[2 * i + 1]);
          }
          unsigned a0[4], a1[4];
 #pragma unroll
@@ -601,19 +676,18 @@ struct BackwardRowsMma {
             const int edge = (l.r + 8 * h) >> l.slots_log2;
             const float bias = shared_float(slot + Gathered::BIAS + 4 * edge);
             const bool there = edge >= lo && edge < hi && bias != -INFINITY;
-            float pr[2], w[2];
+            float pr[N], w[N];
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-               const float dot = l.c < 2 ? s0[2 * h + x] : s1[2 * h + x];
+            for (int x = 0; x < N; x++) {
                // an edge that is masked has p = 0, and so has a row without edges (its lse is -inf)
                const bool live = heads.valid[x] && there && lse[x] != -INFINITY;
-               pr[x] = live ? exp2_fast((fmaf(dot, p.scale, bias) - lse[x]) * LOG2E) : 0.0f;
-               w[x] = live ? pr[x] * dp[2 * h + x] : 0.0f;
+               pr[x] = live ? exp2_fast((fmaf(Cols::pick(s0, s1, h, x, l), p.scale, bias) - lse[x]) * LOG2E) : 0.0f;
+               w[x] = live ? pr[x] * Cols::pick(dp, h, x, l) : 0.0f;
                s.delta[x] += w[x];
             }
             unsigned wh, wl, ph, pl;
-            split2<T>(w[0], w[1], wh, wl);
-            split2<T>(pr[0], pr[1], ph, pl);
+            Cols::template split<T>(w, l, wh, wl);
+            Cols::template split<T>(pr, l, ph, pl);
             wh = transpose8x8(wh);
             wl = transpose8x8(wl);
             ph = __shfl_xor_sync(FULL, transpose8x8(ph), 16);
@@ -645,8 +719,8 @@ struct BackwardRowsMma {
             all += s.acc[m][t][0] * 0.0f + s.acc[m][t][1] * 0.0f;
          }
       lost = all != all;
-      s.delta[0] = sum_pairs(s.delta[0]);
-      s.delta[1] = sum_pairs(s.delta[1]);
+#pragma unroll
+      for (int x = 0; x < N; x++) s.delta[x] = Cols::sum(s.delta[x]);
    }
 
    __device__ __forceinline__ void join_from(const float *unit, const Place &at)
@@ -662,7 +736,7 @@ struct BackwardRowsMma {
          }
       const float2 d = from[64 * TILES];
       s.delta[0] += d.x;
-      s.delta[1] += d.y;
+      if constexpr (!ONE) s.delta[N - 1] += d.y;
    }
    __device__ __forceinline__ void put(float *unit, const Place &at, int only) const
    {
@@ -675,13 +749,13 @@ struct BackwardRowsMma {
       }
       float *delta = reinterpret_cast<float *>(to + 64 * TILES);
 #pragma unroll
-      for (int x = 0; x < 2; x++)
+      for (int x = 0; x < N; x++)
          if (only < 0 || heads.col_kv[x] == only) delta[x] = s.delta[x];
    }
 
    __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long row, int only)
    {
-      const float delta = of_column(s.delta[0], s.delta[1], l.r);
+      const float delta = Cols::of_row(s.delta, l.r);
       const bool mine = heads.live && (only < 0 || heads.kv == only);
       const int map = l.r >> 2;
       const long long rh = row * p.heads + heads.head;
@@ -720,7 +794,7 @@ struct BackwardRowsMma {
 // the unit).  dk and dv are [16 elements x 8] products over the pairs: the columns 0..3 take the upper and 4..7 the lower part
 // of the split ds (or weight) of the unit's kv heads.
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int DK, int FORM>
+template <typename T, int DK, int FORM, bool>
 struct BackwardColumnsMma {
    static constexpr int DV = 2 * DK, KT = DK / 16, VT = DV / 16, LANE_FLOATS = 4 * (2 * KT + VT);
    using Gathered = Ring<T, DK, FORM, Budget<DK>::STAGES, true>;
@@ -785,20 +859,20 @@ struct BackwardColumnsMma {
             const int block = edges * p.subs + sub;
             if (block != ring.current) ring.advance(p, l, at.lane);
             const unsigned slot = ring.slot;
-            float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f}, dp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float s0[4], s1[4], dp[4];
 #pragma unroll
             for (int i = 0; i < DK / 16; i++) {
                unsigned q[4];
                ldmatrix4(q, (slot + mine) ^ ((2 * i) << 4));
-               mma16816<T>(s0, q[0], q[1], q[2], q[3], k[2 * i], k[2 * i + 1]);
+               mma16816_at<T>(i == 0, s0, q, k[2 * i], k[2 * i + 1]);
                ldmatrix4(q, (slot + mine) ^ ((DK / 8 + 2 * i) << 4));
-               mma16816<T>(s1, q[0], q[1], q[2], q[3], k[2 * i], k[2 * i + 1]);
+               mma16816_at<T>(i == 0, s1, q, k[2 * i], k[2 * i + 1]);
             }
 #pragma unroll
             for (int i = 0; i < DV / 16; i++) {
                unsigned d[4];
                ldmatrix4(d, (slot + mine + Gathered::REGION) ^ ((2 * i) << 4));
-               mma16816<T>(dp, d[0], d[1], d[2], d[3], v[2 * i], v[2 * i + 1]);
+               mma16816_at<T>(i == 0, dp, d, v[2 * i], v[2 * i + 1]);
             }
             unsigned b0[2], b1[2], bw[2];
 #pragma unroll
@@ -1088,21 +1162,28 @@ int launch_ring(const AttnParams &p, bool together, cudaStream_t st)
    return 0;
 }
 
-template <typename T, int DK, template <typename, int, int> class Op>
-int launch_mma_width(const WalkShape &s, const AttnParams &p, cudaStream_t st)
+template <typename T, int DK, bool ONE, template <typename, int, int, bool> class Op>
+int launch_mma_form(const WalkShape &s, const AttnParams &p, cudaStream_t st)
 {
-   if (s.form == EXACT) return launch_ring<Op<T, DK, EXACT>>(p, s.together, st);
-   if (s.form == RAGGED) return launch_ring<Op<T, DK, RAGGED>>(p, s.together, st);
-   return launch_ring<Op<T, DK, PIECES>>(p, s.together, st);
+   if (s.form == EXACT) return launch_ring<Op<T, DK, EXACT, ONE>>(p, s.together, st);
+   if (s.form == RAGGED) return launch_ring<Op<T, DK, RAGGED, ONE>>(p, s.together, st);
+   return launch_ring<Op<T, DK, PIECES, ONE>>(p, s.together, st);
 }
 
-template <typename T, template <typename, int, int> class Op>
+// ONES: the walk has a form of its own for four kv heads to a unit
+template <typename T, bool ONES, template <typename, int, int, bool> class Op>
 int launch_mma(const WalkShape &s, const AttnParams &p, cudaStream_t st)
 {
-   if (s.width == 16) return launch_mma_width<T, 16, Op>(s, p, st);
-   if (s.width == 32) return launch_mma_width<T, 32, Op>(s, p, st);
-   if (s.width == 64) return launch_mma_width<T, 64, Op>(s, p, st);
-   if (s.width == 128) return launch_mma_width<T, 128, Op>(s, p, st);
+   if (ONES && p.unit_kv == 4) {
+      if (s.width == 16) return launch_mma_form<T, 16, ONES, Op>(s, p, st);
+      if (s.width == 32) return launch_mma_form<T, 32, ONES, Op>(s, p, st);
+      if (s.width == 64) return launch_mma_form<T, 64, ONES, Op>(s, p, st);
+      if (s.width == 128) return launch_mma_form<T, 128, ONES, Op>(s, p, st);
+   }
+   if (s.width == 16) return launch_mma_form<T, 16, false, Op>(s, p, st);
+   if (s.width == 32) return launch_mma_form<T, 32, false, Op>(s, p, st);
+   if (s.width == 64) return launch_mma_form<T, 64, false, Op>(s, p, st);
+   if (s.width == 128) return launch_mma_form<T, 128, false, Op>(s, p, st);
    return -1;
 }
 

@@ -4,7 +4,7 @@
 namespace fmm {
 namespace attn {
 
-int walk_rows_bf16(const WalkShape &s, const AttnParams &p, cudaStream_t st) { return launch_mma<__nv_bfloat16, BackwardRowsMma>(s, p, st); }
+int walk_rows_bf16(const WalkShape &s, const AttnParams &p, cudaStream_t st) { return launch_mma<__nv_bfloat16, true, BackwardRowsMma>(s, p, st); }
 
 }  // namespace attn
 }  // namespace fmm
