@@ -281,8 +281,6 @@ class Plan:
 
 
 # ---- attention over the edges of a CSR (torch CUDA tensors only; see include/fusedmm_b200.h) ---------------------------
-_DT = {"torch.float32": 0, "torch.bfloat16": 2, "torch.float16": 3}
-_POS = {"torch.int32": 0, "torch.int64": 1, "torch.float32": 2, "torch.float64": 3}
 LEGACY_STREAM = 1  # cudaStreamLegacy: enqueues on the default stream, where NULL would also wait for it
 _attn_fns = {}
 
@@ -301,6 +299,25 @@ _ROTARY_IN = (_i, _l, _i, _i, _i, _p, _l, _l, _p, _l, _l, _i, _p, _p, _i, _d, _i
 _ATTN_IN = (_i, _i, _i, _l, _l, _l, _p, _p, _p, _i, _i, _i, _i, _p, _l, _l, _p, _l, _l, _p, _l, _l, _p, _l, _d)
 
 
+class _Codes(dict):
+    """torch dtype -> code of the C ABI or None; filled by the dtypes' names, so that this module needs no torch."""
+
+    def __init__(self, **names):
+        super().__init__()
+        self._names = names
+
+    def __missing__(self, dtype):
+        code = self[dtype] = self._names.get(str(dtype)[6:])
+        return code
+
+
+_DT = _Codes(float32=0, bfloat16=2, float16=3)
+_POS = _Codes(int32=0, int64=1, float32=2, float64=3)
+_BITS = _Codes(int32=32, int64=64)
+_F32 = _Codes(float32=0)
+_F64 = _Codes(float64=0)
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -314,32 +331,29 @@ def _rows(t, name):
     """Strides (rows, heads) of a tensor whose axes behind the heads are dense."""
     shape, stride = t.shape, t.stride()
     dense = 1
-    for size, st in zip(reversed(shape[2:]), reversed(stride[2:])):
-        if size > 1 and st != dense:
+    for i in range(len(shape) - 1, 1, -1):
+        if stride[i] != dense and shape[i] > 1:
             raise ValueError(f"{name}: the axes behind the heads must be dense")
-        dense *= size
+        dense *= shape[i]
     # the stride of an axis of one entry is never used; one that breaks no alignment stands for it
     return (stride[0] if shape[0] > 1 else dense * shape[1]), (stride[1] if shape[1] > 1 else dense)
 
 
-def _same_place(tensors):
-    dev = None
-    for name, t in tensors:
-        if t is None:
-            continue
-        _require(t.is_cuda, f"{name} must be a CUDA tensor")
-        if dev is None:
-            dev = t.device
-        _require(t.device == dev, f"{name} is on {t.device}, the first tensor on {dev}")
-    return dev
+def _same_place(names, *tensors):
+    dev = tensors[0].device
+    for name, t in zip(names.split(), tensors):
+        if t is not None and (t.device != dev or not t.is_cuda):
+            _require(t.is_cuda, f"{name} must be a CUDA tensor")
+            _require(False, f"{name} is on {t.device}, the first tensor on {dev}")
 
 
-def _rotary_args(q, k, q_weight, k_weight, pos, freq, eps, interleaved):
-    """Checks, then the arguments that both directions share."""
-    _require(str(q.dtype) in _DT, "q must be float32, bfloat16 or float16")
+def rotary_args(q, k, q_weight, k_weight, pos, freq, eps, interleaved):
+    """Checks the arguments of the norm and rotation (ValueError) and lays out what both directions pass to the C ABI."""
+    dtype = _DT[q.dtype]
+    _require(dtype is not None, "q must be float32, bfloat16 or float16")
     _require(q.dim() == 3, "q must be [rows, heads, d]")
     rows, hq, d = q.shape
-    hk = 0
+    hk = ldk = hsk = 0
     if k is not None:
         _require(k.dtype == q.dtype, "q and k must share one type")
         _require(k.dim() == 3 and k.shape[0] == rows and k.shape[2] == d, "k must be [rows, heads, d] with the rows and d of q")
@@ -351,123 +365,129 @@ def _rotary_args(q, k, q_weight, k_weight, pos, freq, eps, interleaved):
         if w is None:
             continue
         _require(eps is not None, f"{name} without eps: no norm is asked for")
-        _require(w.dim() == 1 and w.shape[0] == d and w.stride(0) == 1, f"{name} must be dense, of d entries")
-        _require(str(w.dtype) == "torch.float32" or w.dtype == q.dtype, f"{name} must be float32 or of the type of q")
+        _require(w.dim() == 1 and w.shape[0] == d and (d == 1 or w.stride(0) == 1), f"{name} must be dense, of d entries")
+        _require(w.dtype == q.dtype or _F32[w.dtype] is not None, f"{name} must be float32 or of the type of q")
         _require(wt is None or wt == w.dtype, "q_weight and k_weight must share one type")
         wt = w.dtype
-    _require(not (k_weight is not None and k is None), "k_weight without k")
+    _require(k_weight is None or k is not None, "k_weight without k")
     _require(eps is None or eps >= 0, "eps must not be negative")
-    pt, ldp, asp, axes, pairs = 0, 0, 0, 0, 0
+    pt = ldp = asp = axes = pairs = 0
     if pos is not None:
-        _require(str(pos.dtype) in _POS, "pos must be int32, int64, float32 or float64")
+        pt = _POS[pos.dtype]
+        _require(pt is not None, "pos must be int32, int64, float32 or float64")
+        flat = pos.dim() == 1
         _require(pos.dim() in (1, 2) and pos.shape[0] == rows, "pos must be [rows] or [rows, axes]")
-        axes = 1 if pos.dim() == 1 else pos.shape[1]
+        axes = 1 if flat else pos.shape[1]
         _require(1 <= axes <= 4, "there must be one to four axes")
-        _require(str(freq.dtype) == "torch.float64", "freq must be float64 (angles of far positions need its digits)")
+        _require(_F64[freq.dtype] is not None, "freq must be float64 (angles of far positions need its digits)")
         _require(freq.dim() in (1, 2) and (1 if freq.dim() == 1 else freq.shape[0]) == axes and freq.is_contiguous(),
                  "freq must be dense [axes, pairs], or [pairs] with one axis")
         pairs = freq.shape[-1]
         _require(2 * pairs <= d, "freq has more pairs than half of d")
-        pt, ldp, asp = _POS[str(pos.dtype)], pos.stride(0), pos.stride(1) if pos.dim() == 2 else 0
+        ldp, asp = pos.stride(0), 0 if flat else pos.stride(1)
     ldq, hsq = _rows(q, "q")
-    ldk, hsk = _rows(k, "k") if k is not None else (0, 0)
-    dev = _same_place((("q", q), ("k", k), ("q_weight", q_weight), ("k_weight", k_weight), ("pos", pos), ("freq", freq)))
-    return dev, (_DT[str(q.dtype)], rows, hq, hk, d, _ptr(q), ldq, hsq, _ptr(k), ldk, hsk, 0 if wt is None else _DT[str(wt)],
-                 _ptr(q_weight), _ptr(k_weight), int(eps is not None), 0.0 if eps is None else float(eps), pt, _ptr(pos), ldp,
-                 asp, axes, _ptr(freq), pairs, int(bool(interleaved)))
+    if k is not None:
+        ldk, hsk = _rows(k, "k")
+    _same_place("q k q_weight k_weight pos freq", q, k, q_weight, k_weight, pos, freq)
+    return (dtype, rows, hq, hk, d, q.data_ptr(), ldq, hsq, _ptr(k), ldk, hsk, 0 if wt is None else _DT[wt], _ptr(q_weight),
+            _ptr(k_weight), 0 if eps is None else 1, 0.0 if eps is None else float(eps), pt, _ptr(pos), ldp, asp, axes, _ptr(freq),
+            pairs, 1 if interleaved else 0)
 
 
-def qk_norm_rotary(q, k, q_weight, k_weight, pos, freq, eps, interleaved, q_out, k_out, stream=LEGACY_STREAM):
-    """``fusedmm_b200_qk_norm_rotary`` on torch CUDA tensors of the current device; returns the status code."""
-    _, args = _rotary_args(q, k, q_weight, k_weight, pos, freq, eps, interleaved)
-    fn = _attn_fn("qk_norm_rotary", C.c_int, *_ROTARY_IN, _p, _p, _p)
-    return fn(*args, _ptr(q_out), _ptr(k_out), stream)
+def qk_norm_rotary(args, q_out, k_out, stream=LEGACY_STREAM):
+    """``fusedmm_b200_qk_norm_rotary`` with what :func:`rotary_args` laid out, on the current device; returns the status code."""
+    return _attn_fn("qk_norm_rotary", C.c_int, *_ROTARY_IN, _p, _p, _p)(*args, _ptr(q_out), _ptr(k_out), stream)
 
 
 def qk_norm_rotary_backward_workspace(rows, d):
     return _attn_fn("qk_norm_rotary_backward_workspace", _l, _l, _i)(rows, d)
 
 
-def qk_norm_rotary_backward(q, k, q_weight, k_weight, pos, freq, eps, interleaved, dq_out, dk_out, dq, dk, dwq, dwk, workspace,
-                            stream=LEGACY_STREAM):
-    """``fusedmm_b200_qk_norm_rotary_backward`` on torch CUDA tensors of the current device; returns the status code."""
-    _, args = _rotary_args(q, k, q_weight, k_weight, pos, freq, eps, interleaved)
+def qk_norm_rotary_backward(args, q, k, dq_out, dk_out, dq, dk, dwq, dwk, workspace, stream=LEGACY_STREAM):
+    """``fusedmm_b200_qk_norm_rotary_backward`` likewise; ``dq_out``, ``dk_out`` are the gradients of its results."""
     _require(dq_out.shape == q.shape and dq_out.dtype == q.dtype, "the gradient of q's result must have its shape and type")
     _require(k is None or (dk_out.shape == k.shape and dk_out.dtype == k.dtype), "the gradient of k's result must have its shape and type")
+    _same_place("q dq_out dk_out", q, dq_out, dk_out)
     lddq, hsdq = _rows(dq_out, "the gradient of q's result")
     lddk, hsdk = _rows(dk_out, "the gradient of k's result") if k is not None else (0, 0)
     fn = _attn_fn("qk_norm_rotary_backward", C.c_int, *_ROTARY_IN, _p, _l, _l, _p, _l, _l, _p, _p, _p, _p, _p, _l, _p)
     return fn(*args, _ptr(dq_out), lddq, hsdq, _ptr(dk_out) if k is not None else None, lddk, hsdk, _ptr(dq), _ptr(dk), _ptr(dwq),
-              _ptr(dwk), _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), stream)
+              _ptr(dwk), _ptr(workspace), 0 if workspace is None else workspace.nbytes, stream)
 
 
-def _pattern_args(rowptr, colidx):
-    for name, t in (("rowptr", rowptr), ("colidx", colidx)):
-        _require(str(t.dtype) in ("torch.int32", "torch.int64"), f"{name} must be int32 or int64")
-        _require(t.dim() == 1 and t.is_contiguous(), f"{name} must be a dense vector")
-    _require(rowptr.numel() >= 1, "rowptr must have rows + 1 entries")
-    return rowptr.element_size() * 8, colidx.element_size() * 8
+def _pattern_bits(rowptr, colidx):
+    pb, ib = _BITS[rowptr.dtype], _BITS[colidx.dtype]
+    _require(pb is not None, "rowptr must be int32 or int64")
+    _require(ib is not None, "colidx must be int32 or int64")
+    _require(rowptr.dim() == 1 and rowptr.is_contiguous(), "rowptr must be a dense vector")
+    _require(colidx.dim() == 1 and colidx.is_contiguous(), "colidx must be a dense vector")
+    _require(rowptr.shape[0] >= 1, "rowptr must have rows + 1 entries")
+    return pb, ib
 
 
-def _attention_args(rowptr, colidx, bias, q, k, v, lam, scale):
-    """Checks, then the arguments that both directions share."""
-    pb, ib = _pattern_args(rowptr, colidx)
-    _require(str(q.dtype) in _DT, "q must be float32, bfloat16 or float16")
+def attention_args(rowptr, colidx, bias, q, k, v, lam, scale):
+    """Checks the arguments of differential attention (ValueError) and lays out what both directions pass to the C ABI."""
+    pb, ib = _pattern_bits(rowptr, colidx)
+    dtype = _DT[q.dtype]
+    _require(dtype is not None, "q must be float32, bfloat16 or float16")
     _require(k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v must share one type")
     _require(q.dim() == 4 and q.shape[2] == 2, "q must be [rows, heads, 2, d]")
     m, heads, _, d = q.shape
-    _require(rowptr.numel() == m + 1, "rowptr must have one entry more than q has rows")
+    _require(rowptr.shape[0] == m + 1, "rowptr must have one entry more than q has rows")
     _require(k.dim() == 4 and k.shape[2] == 2 and k.shape[3] == d, "k must be [columns, kv_heads, 2, d] with the d of q")
-    n, kv_heads = k.shape[:2]
+    n, kv_heads = k.shape[0], k.shape[1]
     _require(v.dim() == 3 and v.shape[0] == n and v.shape[1] == kv_heads, "v must be [columns, kv_heads, dv]")
     dv = v.shape[2]
     _require(heads >= 1 and kv_heads >= 1 and heads % kv_heads == 0, "the heads of q must be a multiple of the heads of k")
     _require(1 <= d <= 128 and 1 <= dv <= 256, "d must be between 1 and 128, dv between 1 and 256")
-    _require(str(lam.dtype) == "torch.float32", "lam must be float32")
+    _require(_F32[lam.dtype] is not None, "lam must be float32")
     if lam.dim() == 1:
         _require(lam.shape[0] == heads and (heads == 1 or lam.stride(0) == 1), "lam must be dense [heads], or [rows, heads]")
         ldlam = 0
     else:
-        _require(lam.dim() == 2 and tuple(lam.shape) == (m, heads) and (heads == 1 or lam.stride(1) == 1) and
+        _require(lam.dim() == 2 and lam.shape[0] == m and lam.shape[1] == heads and (heads == 1 or lam.stride(1) == 1) and
                  (m <= 1 or lam.stride(0) >= heads), "lam must be [heads], or [rows, heads] with dense rows")
         ldlam = lam.stride(0) if m > 1 else heads
+    nnz = colidx.shape[0]
     if bias is not None:
-        _require(str(bias.dtype) == "torch.float32" and bias.dim() == 1 and bias.is_contiguous() and
-                 bias.numel() == colidx.numel(), "bias must be dense float32 with an entry for each edge")
-    qs, ks, vs = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
-    dev = _same_place((("rowptr", rowptr), ("colidx", colidx), ("bias", bias), ("q", q), ("k", k), ("v", v), ("lam", lam)))
-    return dev, (_DT[str(q.dtype)], pb, ib, m, n, colidx.numel(), _ptr(rowptr), _ptr(colidx), _ptr(bias), heads, kv_heads, d, dv,
-                 _ptr(q), *qs, _ptr(k), *ks, _ptr(v), *vs, _ptr(lam), ldlam, float(scale))
+        _require(_F32[bias.dtype] is not None and bias.dim() == 1 and bias.is_contiguous() and bias.shape[0] == nnz,
+                 "bias must be dense float32 with an entry for each edge")
+    ldq, hsq = _rows(q, "q")
+    ldk, hsk = _rows(k, "k")
+    ldv, hsv = _rows(v, "v")
+    _same_place("rowptr colidx bias q k v lam", rowptr, colidx, bias, q, k, v, lam)
+    return (dtype, pb, ib, m, n, nnz, rowptr.data_ptr(), colidx.data_ptr(), _ptr(bias), heads, kv_heads, d, dv, q.data_ptr(), ldq, hsq,
+            k.data_ptr(), ldk, hsk, v.data_ptr(), ldv, hsv, lam.data_ptr(), ldlam, float(scale))
 
 
-def diff_attention_workspace(backward, q, k, v, nnz):
-    """Bytes of workspace (``fusedmm_b200_diff_attention_workspace``)."""
+def diff_attention_workspace(backward, args):
+    """Bytes of workspace (``fusedmm_b200_diff_attention_workspace``) of a call with these arguments."""
     fn = _attn_fn("diff_attention_workspace", _l, _i, _i, _l, _l, _l, _i, _i, _i, _i)
-    return fn(int(backward), _DT[str(q.dtype)], q.shape[0], k.shape[0], nnz, q.shape[1], k.shape[1], q.shape[3], v.shape[2])
+    return fn(int(backward), args[0], args[3], args[4], args[5], args[9], args[10], args[11], args[12])
 
 
-def diff_attention(rowptr, colidx, bias, q, k, v, lam, scale, out, lse, workspace, stream=LEGACY_STREAM):
-    """``fusedmm_b200_diff_attention`` on torch CUDA tensors of the current device; returns the status code."""
-    _, args = _attention_args(rowptr, colidx, bias, q, k, v, lam, scale)
+def diff_attention(args, out, lse, workspace, stream=LEGACY_STREAM):
+    """``fusedmm_b200_diff_attention`` with what :func:`attention_args` laid out, on the current device; returns the status code."""
     fn = _attn_fn("diff_attention", C.c_int, *_ATTN_IN, _p, _p, _p, _l, _p)
-    return fn(*args, _ptr(out), _ptr(lse), _ptr(workspace), workspace.numel() * workspace.element_size(), stream)
+    return fn(*args, _ptr(out), _ptr(lse), _ptr(workspace), workspace.nbytes, stream)
 
 
-def diff_attention_backward(rowptr, colidx, bias, q, k, v, lam, scale, lse, dout, t_rowptr, t_row, t_edge, dq, dk, dv, dlam,
-                            workspace, stream=LEGACY_STREAM):
-    """``fusedmm_b200_diff_attention_backward`` on torch CUDA tensors of the current device; returns the status code."""
-    _, args = _attention_args(rowptr, colidx, bias, q, k, v, lam, scale)
-    _require(tuple(dout.shape) == (q.shape[0], q.shape[1], v.shape[2]) and dout.dtype == q.dtype, "dout must have the shape and type of the result")
-    _require(t_rowptr.dtype == rowptr.dtype and t_rowptr.numel() == k.shape[0] + 1 and t_rowptr.is_contiguous(),
+def diff_attention_backward(args, q, k, v, lse, dout, transposed, dq, dk, dv, dlam, workspace, stream=LEGACY_STREAM):
+    """``fusedmm_b200_diff_attention_backward`` likewise; ``transposed``: what :func:`csr_transpose` wrote."""
+    t_rowptr, t_row, t_edge = transposed
+    _require(dout.dim() == 3 and dout.shape[0] == q.shape[0] and dout.shape[1] == q.shape[1] and dout.shape[2] == v.shape[2] and
+             dout.dtype == q.dtype, "dout must have the shape and type of the result")
+    _require(_BITS[t_rowptr.dtype] == args[1] and t_rowptr.shape[0] == k.shape[0] + 1 and t_rowptr.is_contiguous(),
              "the transposed row pointers must have the type of rowptr and an entry more than k has rows")
     for t in (t_row, t_edge):
-        _require(t is None or (str(t.dtype) == "torch.int32" and t.is_contiguous() and t.numel() == colidx.numel()),
+        _require(t is None or (_BITS[t.dtype] == 32 and t.is_contiguous() and t.shape[0] == args[5]),
                  "the transposed pattern must have an int32 entry for each edge")
-    _require(bias is None or t_edge is not None, "a bias needs the edges' positions in the transposed pattern")
-    _same_place((("q", q), ("dout", dout), ("transposed", t_rowptr), ("transposed", t_row), ("transposed", t_edge)))
+    _require(args[8] is None or t_edge is not None, "a bias needs the edges' positions in the transposed pattern")
+    _same_place("q dout transposed transposed transposed lse", q, dout, t_rowptr, t_row, t_edge, lse)
+    lddo, hsdo = _rows(dout, "dout")
     fn = _attn_fn("diff_attention_backward", C.c_int, *_ATTN_IN, _p, _p, _l, _l, _p, _p, _p, _p, _p, _p, _p, _p, _l, _p)
-    return fn(*args, _ptr(lse), _ptr(dout), *_rows(dout, "dout"), _ptr(t_rowptr), _ptr(t_row), _ptr(t_edge), _ptr(dq), _ptr(dk),
-              _ptr(dv), _ptr(dlam), _ptr(workspace), workspace.numel() * workspace.element_size(), stream)
+    return fn(*args, _ptr(lse), _ptr(dout), lddo, hsdo, _ptr(t_rowptr), _ptr(t_row), _ptr(t_edge), _ptr(dq), _ptr(dk), _ptr(dv),
+              _ptr(dlam), _ptr(workspace), workspace.nbytes, stream)
 
 
 def csr_transpose_workspace(m, n, nnz):
@@ -476,8 +496,8 @@ def csr_transpose_workspace(m, n, nnz):
 
 def csr_transpose(rowptr, colidx, n, t_rowptr, t_row, t_edge, workspace, stream=LEGACY_STREAM):
     """``fusedmm_b200_csr_transpose`` on torch CUDA tensors of the current device; returns the status code."""
-    pb, ib = _pattern_args(rowptr, colidx)
-    _same_place((("rowptr", rowptr), ("colidx", colidx)))
+    pb, ib = _pattern_bits(rowptr, colidx)
+    _same_place("rowptr colidx", rowptr, colidx)
     fn = _attn_fn("csr_transpose", C.c_int, _i, _i, _l, _l, _l, _p, _p, _p, _p, _p, _p, _l, _p)
-    return fn(pb, ib, rowptr.numel() - 1, n, colidx.numel(), _ptr(rowptr), _ptr(colidx), _ptr(t_rowptr), _ptr(t_row),
-              _ptr(t_edge), _ptr(workspace), workspace.numel() * workspace.element_size(), stream)
+    return fn(pb, ib, rowptr.shape[0] - 1, n, colidx.shape[0], _ptr(rowptr), _ptr(colidx), _ptr(t_rowptr), _ptr(t_row),
+              _ptr(t_edge), _ptr(workspace), workspace.nbytes, stream)

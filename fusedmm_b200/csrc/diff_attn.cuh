@@ -857,14 +857,17 @@ struct WalkShape {
    bool together = false;
 };
 
+// Lets a kernel have this much shared memory on the current device (kept by the runtime per kernel and device: asked once)
+bool allow_shared(const void *kernel, int bytes);
+
 template <typename Op, int G>
 int launch_op(const AttnParams &p, bool together, cudaStream_t st)
 {
    const int bytes = (JOINT_WARPS - 1) * 32 * Op::LANE_FLOATS * static_cast<int>(sizeof(float));
-   if (cudaFuncSetAttribute(join_kernel<Op, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -1;
+   if (!allow_shared(reinterpret_cast<const void *>(join_kernel<Op, G>), bytes)) return -1;
    const long long jobs = p.pieces * p.unit_blocks;
    if (together) {
-      if (cudaFuncSetAttribute(walk_kernel<Op, G, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -1;
+      if (!allow_shared(reinterpret_cast<const void *>(walk_kernel<Op, G, true>), bytes)) return -1;
       walk_kernel<Op, G, true><<<static_cast<unsigned>(jobs), JOINT_WARPS * 32, bytes, st>>>(p);
    } else {
       walk_kernel<Op, G, false><<<static_cast<unsigned>((jobs + PIECE_WARPS - 1) / PIECE_WARPS), PIECE_WARPS * 32, 0, st>>>(p);

@@ -4,12 +4,28 @@
 #include "diff_attn.cuh"
 
 #include <climits>
-#include <cstdlib>
+#include <mutex>
+#include <set>
+#include <utility>
 
 namespace fmm {
 namespace attn {
 
 constexpr int LAM_BLOCKS = 256;
+
+bool allow_shared(const void *kernel, int bytes)
+{
+   if (bytes <= 48 << 10) return true;
+   static std::mutex mu;
+   static std::set<std::pair<const void *, int>> *done = new std::set<std::pair<const void *, int>>;
+   int dev = 0;
+   if (cudaGetDevice(&dev) != cudaSuccess) return false;
+   std::lock_guard<std::mutex> lock(mu);
+   if (done->count({kernel, dev})) return true;
+   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+   done->insert({kernel, dev});
+   return true;
+}
 
 // dlam[h] = sum over the rows: each block a run of rows, then one block the blocks' sums
 __global__ void __launch_bounds__(256) lam_sum_kernel(const float *in, long long rows, int heads, float *out, long long each)

@@ -27,10 +27,10 @@ template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1)
 {
    if constexpr (std::is_same<T, __half>::value)
-      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                    : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
    else
-      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                    : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // ... the first product of a sum
@@ -39,10 +39,10 @@ __device__ __forceinline__ void mma16816_first(float (&c)[4], unsigned a0, unsig
 {
    const float z = 0.0f;
    if constexpr (std::is_same<T, __half>::value)
-      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                    : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(z));
    else
-      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                    : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(z));
 }
 template <typename T>
@@ -54,7 +54,7 @@ __device__ __forceinline__ void mma16816_at(bool start, float (&c)[4], const uns
 __device__ __forceinline__ unsigned transpose8x8(unsigned v)
 {
    unsigned r;
-   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
    return r;
 }
 __device__ __forceinline__ void ldmatrix4(unsigned (&r)[4], unsigned at)
@@ -203,6 +203,7 @@ struct Ring {
             left_a = p.a_width - (x % (CHUNKS / 2)) * 8;
             left_b = p.b_width - x * 8;
          }
+         if (PER >= 4 && on == 0) left_a = left_b = 0;  // a lane whose pairs are all of one slot
          const char *la = a, *lb = b;
          if (sub > 0) {
             la += (sub << p.kv_log2) * p.a_head;
@@ -212,8 +213,9 @@ struct Ring {
          for (int i = 0; i < ROUNDS; i++) {
             const int pair = i * PER + pair0;
             const int id = __shfl_sync(FULL, batch_id, off + (pair >> l.slots_log2));
-            const bool live = id >= 0 && (on >> i & 1);
+            const bool live = id >= 0;
             const unsigned row = live ? id : 0;
+            const bool here = PER >= 4 ? live : live && (on >> i & 1);
             const char *ra = la + static_cast<unsigned long long>(row) * p.a_stride, *rb = lb + static_cast<unsigned long long>(row) * p.b_stride;
             if constexpr (PER < 4) {
                const int s = pair & (l.slots - 1);
@@ -222,8 +224,8 @@ struct Ring {
             }
             // the pair's bits that change from round to round, as in offset()
             const unsigned at = to + ((place + i * PER * ROW) ^ (CHUNKS >= 8 ? ((i * PER) & 7) << 4 : 0));
-            chunk_in(at, reinterpret_cast<const T *>(ra), live ? left_a : 0, p.step);
-            chunk_in(at + REGION, reinterpret_cast<const T *>(rb), live ? left_b : 0, p.step);
+            chunk_in(at, reinterpret_cast<const T *>(ra), here ? left_a : 0, p.step);
+            chunk_in(at + REGION, reinterpret_cast<const T *>(rb), here ? left_b : 0, p.step);
          }
          if constexpr (RECORDS) {
             const int pair = lane >> 1, s = (pair & (l.slots - 1)) + (sub << p.kv_log2);
@@ -244,7 +246,7 @@ struct Ring {
       length = static_cast<int>(to - from);
       on = ~0u;
       if (only_kv >= 0)
-         for (int i = 0; i < ROUNDS; i++)
+         for (int i = 0; i < 32; i++)  // (with PER >= 4 all rounds are alike)
             if ((((i * PER + lane / CHUNKS) & (l.slots - 1)) >> p.kv_log2) != only_kv) on &= ~(1u << i);
       issued = 0;
       current = -1;
@@ -358,11 +360,15 @@ struct QueryHeads {
 constexpr float SLACK = 5.0f;
 
 // warps of a block and blocks of a multiprocessor: registers and rings decide (a warp's ring is STAGES x 128 DK bytes)
-template <int DK>
+enum { WALK_FORWARD, WALK_ROWS, WALK_COLUMNS };
+template <int DK, int WALK>
 struct Budget {
    static constexpr int STAGES = DK == 16 ? 4 : DK == 32 ? 3 : 2;
    static constexpr int SOLO = DK == 128 ? 2 : 4, JOINT = DK == 128 ? 4 : 8;
-   static constexpr int BLOCKS = DK <= 32 ? 4 : 3;
+   // The backward walks run faster with fewer warps and their registers: R-MAT training at d 32 columns 2.45 ms with four
+   // blocks, 2.19 with three, rows 1.84 and 1.57 (forward 1.26 and 1.30); window training at d 64 columns 419 us with three blocks,
+   // 375 with two, rows 102 and 98 (forward 82 and 89).
+   static constexpr int BLOCKS = DK == 16 ? 4 : DK == 32 ? (WALK == WALK_FORWARD ? 4 : 3) : DK == 64 ? (WALK == WALK_FORWARD ? 3 : 2) : 3;
    static constexpr bool AHEAD = DK <= 32;  // a row's own operands are fetched during the row before (wider: no registers left)
 };
 
@@ -374,8 +380,8 @@ struct ForwardMma {
    using Cols = Columns<ONE>;
    static constexpr int N = Cols::N;
    static constexpr int DV = 2 * DK, TILES = DV / 8, LANE_FLOATS = 2 * TILES + 4;
-   using Gathered = Ring<T, DK, FORM, Budget<DK>::STAGES, false>;
-   using Width = Budget<DK>;
+   using Gathered = Ring<T, DK, FORM, Budget<DK, WALK_FORWARD>::STAGES, false>;
+   using Width = Budget<DK, WALK_FORWARD>;
    struct State {
       float acc[TILES][2];   // rows n = r: sums of weights times v, columns 8t + 2c, + 1
       float top[N], sum[N];  // of this lane's columns
@@ -592,8 +598,8 @@ struct BackwardRowsMma {
    using Cols = Columns<ONE>;
    static constexpr int N = Cols::N;
    static constexpr int DV = 2 * DK, TILES = DK / 8, LANE_FLOATS = 4 * TILES + 2;
-   using Gathered = Ring<T, DK, FORM, Budget<DK>::STAGES, false>;
-   using Width = Budget<DK>;
+   using Gathered = Ring<T, DK, FORM, Budget<DK, WALK_ROWS>::STAGES, false>;
+   using Width = Budget<DK, WALK_ROWS>;
    struct State {
       float acc[2][TILES][2];
       float delta[N];  // of this lane's columns
@@ -655,7 +661,7 @@ struct BackwardRowsMma {
          if (block != ring.current) ring.advance(p, l, at.lane);
          const int lo = e - (block << per_log2), left = e1 - (block << per_log2), hi = left < (1 << per_log2) ? left : 1 << per_log2;
          const unsigned slot = ring.slot;
-         float s0[4], s1[4], dp[4];
+         float s0[4], s1[4], dp[4], dp2[4];
 #pragma unroll
          for (int i = 0; i < DK / 16; i++) {
             unsigned k[4];
@@ -668,8 +674,10 @@ struct BackwardRowsMma {
          for (int i = 0; i < DV / 16; i++) {
             unsigned v[4];
             ldmatrix4(v, (slot + mine + Gathered::REGION) ^ ((2 * i) << 4));
-            mma16816_at<T>(i == 0, dp, v, dout[2 * i], dout[2 * i + 1]);
+            mma16816_at<T>(i < 2, i & 1 ? dp2 : dp, v, dout[2 * i], dout[2 * i + 1]);  // two sums side by side
          }
+#pragma unroll
+         for (int i = 0; i < 4; i++) dp[i] += dp2[i];
          unsigned a0[4], a1[4];
 #pragma unroll
          for (int h = 0; h < 2; h++) {
@@ -797,8 +805,8 @@ struct BackwardRowsMma {
 template <typename T, int DK, int FORM, bool>
 struct BackwardColumnsMma {
    static constexpr int DV = 2 * DK, KT = DK / 16, VT = DV / 16, LANE_FLOATS = 4 * (2 * KT + VT);
-   using Gathered = Ring<T, DK, FORM, Budget<DK>::STAGES, true>;
-   using Width = Budget<DK>;
+   using Gathered = Ring<T, DK, FORM, Budget<DK, WALK_COLUMNS>::STAGES, true>;
+   using Width = Budget<DK, WALK_COLUMNS>;
    struct State {
       float dk[2][KT][4], dv[VT][4];
    };
@@ -859,7 +867,7 @@ struct BackwardColumnsMma {
             const int block = edges * p.subs + sub;
             if (block != ring.current) ring.advance(p, l, at.lane);
             const unsigned slot = ring.slot;
-            float s0[4], s1[4], dp[4];
+            float s0[4], s1[4], dp[4], dp2[4];
 #pragma unroll
             for (int i = 0; i < DK / 16; i++) {
                unsigned q[4];
@@ -872,8 +880,10 @@ struct BackwardColumnsMma {
             for (int i = 0; i < DV / 16; i++) {
                unsigned d[4];
                ldmatrix4(d, (slot + mine + Gathered::REGION) ^ ((2 * i) << 4));
-               mma16816_at<T>(i == 0, dp, d, v[2 * i], v[2 * i + 1]);
+               mma16816_at<T>(i < 2, i & 1 ? dp2 : dp, d, v[2 * i], v[2 * i + 1]);  // two sums side by side
             }
+#pragma unroll
+            for (int i = 0; i < 4; i++) dp[i] += dp2[i];
             unsigned b0[2], b1[2], bw[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -1002,8 +1012,8 @@ __device__ __forceinline__ void join_ring_warps(Op &op, const Place &at, float *
       for (int w = 1; w < Op::Width::JOINT; w++) op.join_from(shared + (w - 1) * STRIDE, at);
 }
 
-// Where several heads are computed in one product and a sum came out infinite or as no number, a 0 of one head may have met an
-// infinity or NaN of another's: the edges are then taken once more, each kv head by itself.
+// Where a sum came out infinite or as no number, a weight of 0 may have met an infinity or NaN of another row's edge in the same
+// block, or of another head: the row's edges are then taken once more, in blocks of their own and each kv head by itself.
 template <typename Op, bool TOGETHER>
 __device__ __forceinline__ void ring_segment(Op &op, typename Op::Gathered &ring, const AttnParams &p, const Place &at, float *shared,
                                              long long row, long long e0, long long e1, long long part, long long follow, long long run_end)
@@ -1022,7 +1032,7 @@ __device__ __forceinline__ void ring_segment(Op &op, typename Op::Gathered &ring
    w0 = w0 < ring.first ? ring.first : w0;
    w1 = w1 < w0 ? w0 : w1;
    op.run(p, at, ring, static_cast<int>(w0 - ring.first), static_cast<int>(w1 - ring.first), follow);
-   const bool lost = p.unit_kv > 1 && (TOGETHER ? __syncthreads_or(op.lost) : __any_sync(FULL, op.lost));
+   const bool lost = TOGETHER ? p.unit_kv > 1 && __syncthreads_or(op.lost) : __any_sync(FULL, op.lost);
    for (int only = lost ? 0 : -1; only < (lost ? p.unit_kv : 0); only++) {
       if (lost) {
          op.fetch(p, row);
@@ -1149,14 +1159,14 @@ int launch_ring(const AttnParams &p, bool together, cudaStream_t st)
    const long long jobs = p.pieces * p.unit_blocks;
    if (together) {
       constexpr int bytes = Op::Width::JOINT * RING + RING_ALIGN;
-      if (cudaFuncSetAttribute(ring_walk_kernel<Op, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -1;
+      if (!allow_shared(reinterpret_cast<const void *>(ring_walk_kernel<Op, true>), bytes)) return -1;
       ring_walk_kernel<Op, true><<<static_cast<unsigned>(jobs), Op::Width::JOINT * 32, bytes, st>>>(p);
    } else {
       constexpr int bytes = Op::Width::SOLO * RING + RING_ALIGN;
-      if (cudaFuncSetAttribute(ring_walk_kernel<Op, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -1;
+      if (!allow_shared(reinterpret_cast<const void *>(ring_walk_kernel<Op, false>), bytes)) return -1;
       ring_walk_kernel<Op, false><<<static_cast<unsigned>((jobs + Op::Width::SOLO - 1) / Op::Width::SOLO), Op::Width::SOLO * 32, bytes, st>>>(p);
    }
-   if (cudaFuncSetAttribute(ring_join_kernel<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, JOIN) != cudaSuccess) return -1;
+   if (!allow_shared(reinterpret_cast<const void *>(ring_join_kernel<Op>), JOIN)) return -1;
    const long long groups = (p.pieces + JOIN_PIECES - 1) / JOIN_PIECES;
    ring_join_kernel<Op><<<static_cast<unsigned>(groups * p.unit_blocks), Op::Width::JOINT * 32, JOIN, st>>>(p);
    return 0;

@@ -61,113 +61,152 @@ _lib.define("diff_attention_backward(Tensor rowptr, Tensor colidx, Tensor? bias,
 _lib.define("csr_transpose(Tensor rowptr, Tensor colidx, int n) -> (Tensor, Tensor, Tensor)")
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream or api.LEGACY_STREAM
-
-
 def _check(status, name):
     if status != 0:
         raise api.FusedMMError(f"{name} failed: {api.status_string(status)} ({status})")
 
 
-def _scratch(size, name, device):
-    if size < 0:
-        _check(size, name)
-    return torch.empty(max(size, 1), dtype=torch.uint8, device=device)
+class _On:
+    """Makes a tensor's device the current one for a call (nothing to do as a rule) and gives torch's stream on it."""
+    __slots__ = ("device", "index", "guard", "stream")
+
+    def __init__(self, device):
+        self.device, self.index, self.guard = device, device.index, None
+
+    def __enter__(self):
+        if self.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.index)
+            self.guard.__enter__()
+        self.stream = torch._C._cuda_getCurrentRawStream(self.index) or api.LEGACY_STREAM
+        return self
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+    def empty(self, shape, dtype):
+        return torch.empty(shape, dtype=dtype, device=self.device)
+
+    def scratch(self, size, name):
+        if size < 0:
+            _check(size, name)
+        return torch.empty(size or 1, dtype=torch.uint8, device=self.device)
 
 
 def _rotary_cuda(q, k, pos, freq, q_weight, k_weight, eps, interleaved):
-    with torch.cuda.device(q.device):
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = torch.empty(k.shape if k is not None else (0,), dtype=q.dtype, device=q.device)
-        _check(api.qk_norm_rotary(q, k, q_weight, k_weight, pos, freq, eps, interleaved, q_out, k_out if k is not None else None,
-                                  _stream(q.device)), "qk_norm_rotary")
+    args = api.rotary_args(q, k, q_weight, k_weight, pos, freq, eps, interleaved)
+    with _On(q.device) as on:
+        q_out = on.empty(q.shape, q.dtype)
+        k_out = on.empty(k.shape if k is not None else 0, q.dtype)
+        _check(api.qk_norm_rotary(args, q_out, k_out if k is not None else None, on.stream), "qk_norm_rotary")
     return q_out, k_out
 
 
 def _rotary_backward_cuda(q, k, pos, freq, q_weight, k_weight, eps, interleaved, dq_out, dk_out):
-    dev = q.device
-    with torch.cuda.device(dev):
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        dk = torch.empty(k.shape if k is not None else (0,), dtype=q.dtype, device=dev)
-        dw = [torch.empty(q.shape[2] if w is not None else 0, dtype=torch.float32, device=dev) for w in (q_weight, k_weight)]
-        weights = q_weight is not None or k_weight is not None
-        ws = _scratch(api.qk_norm_rotary_backward_workspace(q.shape[0], q.shape[2]), "qk_norm_rotary_backward", dev) if weights else None
-        _check(api.qk_norm_rotary_backward(q, k, q_weight, k_weight, pos, freq, eps, interleaved, dq_out, dk_out, dq,
-                                           dk if k is not None else None, dw[0] if q_weight is not None else None,
-                                           dw[1] if k_weight is not None else None, ws, _stream(dev)), "qk_norm_rotary_backward")
-    return dq, dk, dw[0], dw[1]
+    args = api.rotary_args(q, k, q_weight, k_weight, pos, freq, eps, interleaved)
+    with _On(q.device) as on:
+        dq = on.empty(q.shape, q.dtype)
+        dk = on.empty(k.shape if k is not None else 0, q.dtype)
+        dwq = on.empty(q.shape[2], torch.float32) if q_weight is not None else None
+        dwk = on.empty(q.shape[2], torch.float32) if k_weight is not None else None
+        ws = None
+        if dwq is not None or dwk is not None:
+            ws = on.scratch(api.qk_norm_rotary_backward_workspace(q.shape[0], q.shape[2]), "qk_norm_rotary_backward")
+        _check(api.qk_norm_rotary_backward(args, q, k, dq_out, dk_out, dq, dk if k is not None else None, dwq, dwk, ws, on.stream),
+               "qk_norm_rotary_backward")
+        none = None if dwq is not None and dwk is not None else on.empty(0, torch.float32)
+    return dq, dk, none if dwq is None else dwq, none if dwk is None else dwk
 
 
-def _attention_cuda(rowptr, colidx, bias, q, k, v, lam, scale, t_rowptr=None, t_row=None, t_edge=None):
-    api._attention_args(rowptr, colidx, bias, q, k, v, lam, scale)  # before anything is sized by its shapes
-    dev = q.device
-    with torch.cuda.device(dev):
-        m, heads = q.shape[:2]
-        out = torch.empty((m, heads, v.shape[2]), dtype=q.dtype, device=dev)
-        lse = torch.empty((m, heads, 2), dtype=torch.float32, device=dev)
-        ws = _scratch(api.diff_attention_workspace(False, q, k, v, colidx.numel()), "diff_attention", dev)
-        _check(api.diff_attention(rowptr, colidx, bias, q, k, v, lam, scale, out, lse, ws, _stream(dev)), "diff_attention")
+def _attention_forward(rowptr, colidx, bias, q, k, v, lam, scale, want_lse):
+    args = api.attention_args(rowptr, colidx, bias, q, k, v, lam, scale)
+    with _On(q.device) as on:
+        m, heads = q.shape[0], q.shape[1]
+        out = on.empty((m, heads, v.shape[2]), q.dtype)
+        lse = on.empty((m, heads, 2), torch.float32) if want_lse else None
+        ws = on.scratch(api.diff_attention_workspace(False, args), "diff_attention")
+        _check(api.diff_attention(args, out, lse, ws, on.stream), "diff_attention")
     return out, lse
 
 
+def _attention_cuda(rowptr, colidx, bias, q, k, v, lam, scale, t_rowptr=None, t_row=None, t_edge=None):
+    return _attention_forward(rowptr, colidx, bias, q, k, v, lam, scale, True)
+
+
 def _attention_backward_cuda(rowptr, colidx, bias, q, k, v, lam, scale, lse, dout, t_rowptr, t_row, t_edge):
-    dev = q.device
-    with torch.cuda.device(dev):
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
-        dv = torch.empty(v.shape, dtype=v.dtype, device=dev)
-        dlam = torch.empty(lam.shape, dtype=torch.float32, device=dev)
-        ws = _scratch(api.diff_attention_workspace(True, q, k, v, colidx.numel()), "diff_attention_backward", dev)
-        _check(api.diff_attention_backward(rowptr, colidx, bias, q, k, v, lam, scale, lse, dout, t_rowptr, t_row, t_edge, dq, dk,
-                                           dv, dlam, ws, _stream(dev)), "diff_attention_backward")
+    args = api.attention_args(rowptr, colidx, bias, q, k, v, lam, scale)
+    with _On(q.device) as on:
+        dq, dk, dv = on.empty(q.shape, q.dtype), on.empty(k.shape, k.dtype), on.empty(v.shape, v.dtype)
+        dlam = on.empty(lam.shape, torch.float32)
+        ws = on.scratch(api.diff_attention_workspace(True, args), "diff_attention_backward")
+        _check(api.diff_attention_backward(args, q, k, v, lse, dout, (t_rowptr, t_row, t_edge), dq, dk, dv, dlam, ws, on.stream),
+               "diff_attention_backward")
     return dq, dk, dv, dlam
 
 
 def _transpose_cuda(rowptr, colidx, n):
-    api._pattern_args(rowptr, colidx)
-    dev, nnz = rowptr.device, colidx.numel()
-    with torch.cuda.device(dev):
-        ws = _scratch(api.csr_transpose_workspace(rowptr.numel() - 1, n, nnz), "csr_transpose", dev)
-        t_rowptr = torch.empty(n + 1, dtype=rowptr.dtype, device=dev)
-        t_row, t_edge = torch.empty(nnz, dtype=torch.int32, device=dev), torch.empty(nnz, dtype=torch.int32, device=dev)
-        _check(api.csr_transpose(rowptr, colidx, n, t_rowptr, t_row, t_edge, ws, _stream(dev)), "csr_transpose")
+    api._pattern_bits(rowptr, colidx)
+    nnz = colidx.shape[0]
+    with _On(rowptr.device) as on:
+        ws = on.scratch(api.csr_transpose_workspace(rowptr.shape[0] - 1, n, nnz), "csr_transpose")
+        t_rowptr, t_row, t_edge = on.empty(n + 1, rowptr.dtype), on.empty(nnz, torch.int32), on.empty(nnz, torch.int32)
+        _check(api.csr_transpose(rowptr, colidx, n, t_rowptr, t_row, t_edge, ws, on.stream), "csr_transpose")
     return t_rowptr, t_row, t_edge
 
 
 def _dense_rows(t):
-    """A gradient whose last axes are not dense (an expanded one, say) is laid out anew."""
-    return t if t.stride(-1) == 1 and t.stride(0) != 0 and t.stride(1) != 0 else t.contiguous()
+    """A gradient whose last axis is not dense, or whose rows coincide (an expanded one), is laid out anew."""
+    stride = t.stride()
+    return t if stride[-1] == 1 and stride[0] != 0 and stride[1] != 0 else t.contiguous()
+
+
+def _plain(*tensors):
+    """True if these are ordinary CUDA tensors and nothing watches torch's operators: the call may then go straight to the
+    library, without a round through the dispatcher (some 30 us)."""
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack():
+        return False
+    for t in tensors:
+        if t is not None and ((type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter) or not t.is_cuda):
+            return False
+    return torch._C._functorch.peek_interpreter_stack() is None
+
+
+def _below(op, *args):
+    """A call of an operator from its own autograd layer."""
+    with torch._C._AutoDispatchBelowAutograd():
+        return op(*args)
 
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, pos, freq, q_weight, k_weight, eps, interleaved):
-        with torch._C._AutoDispatchBelowAutograd():
-            out = torch.ops.fusedmm_b200.qk_norm_rotary(q, k, pos, freq, q_weight, k_weight, eps, interleaved)
         ctx.save_for_backward(q, k, pos, freq, q_weight, k_weight)
         ctx.args = eps, interleaved
-        return out
+        args = (q, k, pos, freq, q_weight, k_weight, eps, interleaved)
+        return _rotary_cuda(*args) if _plain(q) else _below(torch.ops.fusedmm_b200.qk_norm_rotary, *args)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq_out, dk_out):
         q, k, pos, freq, q_weight, k_weight = ctx.saved_tensors
-        if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
+        need = ctx.needs_input_grad
+        if need[2] or need[3]:
             raise api.FusedMMError("qk_norm_rotary has no gradient for pos and freq")
         eps, interleaved = ctx.args
-        dq, dk, dwq, dwk = torch.ops.fusedmm_b200.qk_norm_rotary_backward(
-            q, k, pos, freq, q_weight, k_weight, eps, interleaved, _dense_rows(dq_out), None if k is None else _dense_rows(dk_out))
-        need = ctx.needs_input_grad
-        return (dq if need[0] else None, dk if k is not None and need[1] else None, None, None,
-                dwq.to(q_weight.dtype) if need[4] else None, dwk.to(k_weight.dtype) if need[5] else None, None, None)
+        run = _rotary_backward_cuda if _plain(q, dq_out) else torch.ops.fusedmm_b200.qk_norm_rotary_backward
+        dq, dk, dwq, dwk = run(q, k, pos, freq, q_weight, k_weight, eps, interleaved, _dense_rows(dq_out),
+                               None if k is None else _dense_rows(dk_out))
+        return (dq if need[0] else None, dk if need[1] else None, None, None, dwq.to(q_weight.dtype) if need[4] else None,
+                dwk.to(k_weight.dtype) if need[5] else None, None, None)
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rowptr, colidx, bias, q, k, v, lam, scale, t_rowptr, t_row, t_edge):
-        with torch._C._AutoDispatchBelowAutograd():
-            out, lse = torch.ops.fusedmm_b200.diff_attention(rowptr, colidx, bias, q, k, v, lam, scale, t_rowptr, t_row, t_edge)
+        if _plain(q):
+            out, lse = _attention_forward(rowptr, colidx, bias, q, k, v, lam, scale, True)
+        else:
+            out, lse = _below(torch.ops.fusedmm_b200.diff_attention, rowptr, colidx, bias, q, k, v, lam, scale, t_rowptr, t_row, t_edge)
         ctx.save_for_backward(rowptr, colidx, bias, q, k, v, lam, lse, t_rowptr, t_row, t_edge)
         ctx.scale = scale
         ctx.mark_non_differentiable(lse)
@@ -177,13 +216,15 @@ class _Attention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _):
         rowptr, colidx, bias, q, k, v, lam, lse, t_rowptr, t_row, t_edge = ctx.saved_tensors
-        if ctx.needs_input_grad[2]:
+        need = ctx.needs_input_grad
+        if need[2]:
             raise api.FusedMMError("diff_attention has no gradient for bias")
+        plain = _plain(q, dout)
         if t_rowptr is None:
-            t_rowptr, t_row, t_edge = torch.ops.fusedmm_b200.csr_transpose(rowptr, colidx, k.shape[0])
-        grads = torch.ops.fusedmm_b200.diff_attention_backward(rowptr, colidx, bias, q, k, v, lam, ctx.scale, lse,
-                                                               _dense_rows(dout), t_rowptr, t_row, t_edge)
-        return (None, None, None, *[g if need else None for g, need in zip(grads, ctx.needs_input_grad[3:7])], None, None, None, None)
+            t_rowptr, t_row, t_edge = (_transpose_cuda if plain else torch.ops.fusedmm_b200.csr_transpose)(rowptr, colidx, k.shape[0])
+        run = _attention_backward_cuda if plain else torch.ops.fusedmm_b200.diff_attention_backward
+        grads = run(rowptr, colidx, bias, q, k, v, lam, ctx.scale, lse, _dense_rows(dout), t_rowptr, t_row, t_edge)
+        return (None, None, None, *[g if n else None for g, n in zip(grads, need[3:7])], None, None, None, None)
 
 
 _lib.impl("qk_norm_rotary", _rotary_cuda, "CUDA")
@@ -231,7 +272,13 @@ def qk_norm_rotary(q, k=None, pos=None, freq=None, *, q_weight=None, k_weight=No
     ``q_weight`` / ``k_weight`` [d] (ones if left out).  With ``pos`` [rows] or [rows, axes] (up to four axes; integers or
     coordinates) and ``freq`` [axes, pairs] (float64) the pairs (i, i + pairs), or (2i, 2i + 1) with ``interleaved``, turn
     by ``pos @ freq``; a pair that belongs to one axis has zeros on the others; elements behind the pairs pass."""
-    q_out, k_out = torch.ops.fusedmm_b200.qk_norm_rotary(q, k, pos, freq, q_weight, k_weight, eps, interleaved)
+    args = (q, k, pos, freq, q_weight, k_weight, eps, interleaved)
+    if not _plain(q, k, pos, freq, q_weight, k_weight):
+        q_out, k_out = torch.ops.fusedmm_b200.qk_norm_rotary(*args)
+    elif torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, pos, freq, q_weight, k_weight)):
+        q_out, k_out = _Rotary.apply(*args)
+    else:
+        q_out, k_out = _rotary_cuda(*args)
     return q_out if k is None else (q_out, k_out)
 
 
@@ -245,11 +292,17 @@ def diff_attention(rowptr, colidx, q, k, v, lam, *, bias=None, scale=None, trans
     ``scale`` is 1/sqrt(d) if left out.  ``transposed``: what :func:`csr_transpose` made of this pattern; without it a
     backward pass makes it again.  With ``return_lse`` also the logarithms of the maps' sums, [m, heads, 2]."""
     t = (None, None, None) if transposed is None else transposed
-    out, lse = torch.ops.fusedmm_b200.diff_attention(rowptr, colidx, bias, q, k, v, lam, q.shape[-1] ** -0.5 if scale is None else scale, *t)
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    if not _plain(rowptr, colidx, bias, q, k, v, lam, *t):
+        out, lse = torch.ops.fusedmm_b200.diff_attention(rowptr, colidx, bias, q, k, v, lam, scale, *t)
+    elif torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, lam, bias)):
+        out, lse = _Attention.apply(rowptr, colidx, bias, q, k, v, lam, scale, *t)
+    else:
+        out, lse = _attention_forward(rowptr, colidx, bias, q, k, v, lam, scale, return_lse)
     return (out, lse) if return_lse else out
 
 
 def csr_transpose(rowptr, colidx, n):
     """The transposed pattern of a CSR with ``n`` columns: row pointers of the columns, the rows of their edges and the
     edges' positions in ``colidx`` (edges outside [0, n) left out).  What ``diff_attention(transposed=...)`` takes."""
-    return torch.ops.fusedmm_b200.csr_transpose(rowptr, colidx, n)
+    return _transpose_cuda(rowptr, colidx, n) if _plain(rowptr, colidx) else torch.ops.fusedmm_b200.csr_transpose(rowptr, colidx, n)

@@ -9,7 +9,7 @@ from fusedmm_b200 import api, torch_op
 I, L, P, D = C.c_int32, C.c_int64, C.c_void_p, C.c_double
 
 
-def attention_args(m=4, n=5, nnz=7, heads=4, kvh=2, d=8, dv=16, dtype=torch.float32):
+def good_attention(m=4, n=5, nnz=7, heads=4, kvh=2, d=8, dv=16, dtype=torch.float32):
     return dict(rowptr=torch.tensor([0, nnz] + [nnz] * (m - 1), dtype=torch.int32), colidx=torch.zeros(nnz, dtype=torch.int32),
                 bias=None, q=torch.zeros(m, heads, 2, d, dtype=dtype), k=torch.zeros(n, kvh, 2, d, dtype=dtype),
                 v=torch.zeros(n, kvh, dv, dtype=dtype), lam=torch.zeros(heads), scale=1.0)
@@ -38,10 +38,10 @@ def attention_args(m=4, n=5, nnz=7, heads=4, kvh=2, d=8, dv=16, dtype=torch.floa
 ])
 def test_attention_refuses(change, text):
     with pytest.raises(ValueError, match=text):
-        api._attention_args(**{**attention_args(), **change})
+        api.attention_args(**{**good_attention(), **change})
 
 
-def rotary_args(**change):
+def good_rotary(**change):
     return {**dict(q=torch.zeros(6, 3, 16), k=torch.zeros(6, 1, 16), q_weight=None, k_weight=None, pos=torch.zeros(6, 2),
                    freq=torch.zeros(2, 8, dtype=torch.float64), eps=1e-6, interleaved=False), **change}
 
@@ -70,7 +70,7 @@ def rotary_args(**change):
 ])
 def test_rotary_refuses(change, text):
     with pytest.raises(ValueError, match=text):
-        api._rotary_args(**rotary_args(**change))
+        api.rotary_args(**good_rotary(**change))
 
 
 def test_c_entries_check_their_arguments_first():
@@ -116,7 +116,7 @@ def test_c_entries_check_their_arguments_first():
 
 
 def test_host_tensors_have_no_kernel():
-    a = attention_args()
+    a = good_attention()
     with pytest.raises(NotImplementedError):
         torch_op.diff_attention(a["rowptr"], a["colidx"], a["q"], a["k"], a["v"], a["lam"])
     with pytest.raises(NotImplementedError):

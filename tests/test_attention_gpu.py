@@ -150,17 +150,38 @@ def test_bias_of_the_lowest_value(cuda_device):
     assert bool(lse[0].isfinite().all())
 
 
-def test_nan_in_an_edge_that_counts_shows(cuda_device):
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("heads,kvh", [(2, 2), (4, 4), (4, 1), (6, 3)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_a_bad_number_shows_where_it_counts_and_nowhere_else(cuda_device, dtype, heads, kvh, bad, where):
+    """One NaN or infinity in k or v of one kv head: rows that have the edge, at heads of that kv head, and no others differ."""
     gen = gen_of(9)
-    rowptr, colidx = random_pattern(gen, 6, 12, 6, torch.int32, torch.int32, empty=0.0)
-    t = make(gen, F32, rowptr, colidx, 6, 12, 2, 2, 8, 8)
-    hit = int(colidx[int(rowptr[2])])
-    t["k"][hit, 0, 0, 3] = math.nan
-    out = torch_op.diff_attention(t["rowptr"], t["colidx"], t["q"], t["k"], t["v"], t["lam"])
-    rows = torch.repeat_interleave(torch.arange(6), (rowptr[1:] - rowptr[:-1]).long())
-    touched = torch.zeros(6, dtype=torch.bool)
+    m, n, d = 60, 40, 8
+    rowptr, colidx = random_pattern(gen, m, n, 4, torch.int32, torch.int32, empty=0.1)
+    t = make(gen, dtype, rowptr, colidx, m, n, heads, kvh, d, 16)
+    hit = int(colidx[int(rowptr[20])])
+    dout = randn(gen, dtype, m, heads, 16).cuda()
+    # Rows that share a block with the bad number are summed once more by themselves, in another order: they need not keep their
+    # bits.  The bounds of the 64-bit evaluation hold for every order of a row's sums.
+    want = attention_reference(t["rowptr"], t["colidx"], None, t["q"], t["k"], t["v"], t["lam"], 0.3, dout)
+    t[where][hit, 0].reshape(-1)[3] = bad
+    got = run_all(t, 0.3, dout)
+    rows = torch.repeat_interleave(torch.arange(m), (rowptr[1:] - rowptr[:-1]).long())
+    touched = torch.zeros(m, dtype=torch.bool)
     touched[rows[colidx == hit]] = True
-    assert torch.equal(out[:, 0].isnan().all(-1).cpu(), touched) and not out[:, 1].isnan().any()
+    near = torch.zeros(n, dtype=torch.bool)  # columns with an edge of a touched row
+    near[colidx[touched[rows]].long()] = True
+    mine = torch.arange(heads) < heads // kvh
+    for name, first, own in (("out", touched, mine), ("dq", touched, mine), ("dk", near, torch.arange(kvh) < 1), ("dv", near, torch.arange(kvh) < 1)):
+        value, bound = want[name]
+        for part in ((~first, slice(None)), (slice(None), ~own)):
+            check(got[name].cpu()[part[0]][:, part[1]], (value[part[0]][:, part[1]], bound[part[0]][:, part[1]]), name)
+    shown = got["out"][touched][:, mine]
+    if where == "k" and bad == math.nan:
+        assert bool(shown.isnan().all())
+    elif where == "v":
+        assert bool((~shown[..., 3].isfinite()).all()) and bool(shown[..., :3].isfinite().all())
 
 
 def test_views_of_a_packed_projection_and_a_gradient_that_is_expanded(cuda_device):
@@ -284,12 +305,12 @@ def test_synchronous_call_of_the_c_entry(cuda_device):
     t = make(gen, F32, rowptr, colidx, 30, 40, 2, 2, 8, 16)
     want = torch_op.diff_attention(t["rowptr"], t["colidx"], t["q"], t["k"], t["v"], t["lam"], scale=0.5)
     out = torch.empty_like(want)
-    ws = torch.empty(api.diff_attention_workspace(False, t["q"], t["k"], t["v"], colidx.numel()), dtype=torch.uint8, device="cuda")
+    args = api.attention_args(t["rowptr"], t["colidx"], None, t["q"], t["k"], t["v"], t["lam"], 0.5)
+    ws = torch.empty(api.diff_attention_workspace(False, args), dtype=torch.uint8, device="cuda")
     torch.cuda.synchronize()
-    assert api.diff_attention(t["rowptr"], t["colidx"], None, t["q"], t["k"], t["v"], t["lam"], 0.5, out, None, ws, None) == 0
+    assert api.diff_attention(args, out, None, ws, None) == 0
     assert torch.equal(out, want)
-    small = ws[: ws.numel() - 1]
-    assert api.diff_attention(t["rowptr"], t["colidx"], None, t["q"], t["k"], t["v"], t["lam"], 0.5, out, None, small, None) == -3
+    assert api.diff_attention(args, out, None, ws[: ws.numel() - 1], None) == -3
 
 
 @pytest.mark.parametrize("m,n,mean,ptr,idx", [(1, 1, 3, torch.int32, torch.int32), (300, 250, 9, torch.int64, torch.int32),
@@ -461,3 +482,33 @@ def test_no_gradient_for_masks_and_positions(cuda_device):
     y = torch_op.qk_norm_rotary(t["k"][:, :, 0], None, pos, torch.ones(1, 2, dtype=torch.float64, device="cuda"))
     with pytest.raises(api.FusedMMError, match="pos"):
         y.sum().backward()
+
+
+def test_shapes_of_gradients_for_a_compiler(cuda_device):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        q = torch.empty(6, 4, 2, 8, dtype=BF16, device="cuda", requires_grad=True)
+        k, v = torch.empty(9, 2, 2, 8, dtype=BF16, device="cuda"), torch.empty(9, 2, 12, dtype=BF16, device="cuda")
+        rowptr, colidx = torch.empty(7, dtype=torch.int64, device="cuda"), torch.empty(30, dtype=torch.int32, device="cuda")
+        out = torch_op.diff_attention(rowptr, colidx, q, k, v, torch.empty(4, device="cuda"))
+        assert torch.autograd.grad(out, q, torch.empty_like(out))[0].shape == q.shape
+        x = torch.empty(6, 4, 8, device="cuda", requires_grad=True)
+        y = torch_op.qk_norm_rotary(x, eps=1e-6)
+        assert torch.autograd.grad(y, x, torch.empty_like(y))[0].shape == x.shape
+
+
+def test_operators_of_torch_and_functions_agree(cuda_device):
+    """torch.ops.fusedmm_b200.* (the way of a compiled program) and the module's functions make the same calls."""
+    gen = gen_of(18)
+    rowptr, colidx = random_pattern(gen, 20, 30, 6, torch.int64, torch.int32)
+    t = make(gen, BF16, rowptr, colidx, 20, 30, 4, 2, 16, 32)
+    dout = randn(gen, BF16, 20, 4, 32).cuda()
+    want = run_all(t, 0.25, dout)
+    leaves = [t[a].detach().requires_grad_() for a in ("q", "k", "v", "lam")]
+    out, lse = torch.ops.fusedmm_b200.diff_attention(t["rowptr"], t["colidx"], None, *leaves, 0.25, None, None, None)
+    grads = torch.autograd.grad(out, leaves, dout)
+    for a, b in zip((out, lse, *grads), (want[n] for n in ("out", "lse", "dq", "dk", "dv", "dlam"))):
+        assert torch.equal(a, b)
+    x, w = t["k"][:, :, 0].contiguous(), torch.rand(16, generator=gen).cuda()
+    assert torch.equal(torch_op.qk_norm_rotary(x, q_weight=w, eps=1e-6),
+                       torch.ops.fusedmm_b200.qk_norm_rotary(x, None, None, None, w, None, 1e-6, False)[0])
