@@ -5,11 +5,12 @@
 //   (y_lo, y_hi) -> (y_lo cos - y_hi sin, y_hi cos + y_lo sin) for the pairs i < P; what lies behind the pairs passes.
 //   backward, g = dy turned back:  dw = sum_rows,heads g x r;  dx = r (w g - x r mean(w g x r)), r the root's reciprocal.
 //
-// Bound: bytes; every element is read and written once, the arithmetic is ~10 instructions an element.  A head is cut into
-// units of two vectors that hold the two halves of the same pairs, one unit to a lane, so the rotation needs no exchange
-// between lanes and the norm one butterfly over the lanes of the head.  The angles of a row are shared by all heads:
-// a block takes a few rows, computes their sines once (in 64 bits up to the turn's fraction: 2^20 positions times a
-// frequency leave no digit of the angle in 32) and keeps them in shared memory.
+// Bound: bytes; every element is read and written once, and the arithmetic (some 6 instructions an element with the conversions)
+// has to stay out of the way.  A head is cut into units of two vectors that hold the two halves of the same pairs, one unit to
+// a lane, so the rotation needs no exchange between lanes and the norm one butterfly over the lanes of the head.  A group of
+// lanes (a slot) takes a row and goes through its heads: a lane's sines and weights stay in its registers, and the next
+// heads are on their way from memory.  Angles are formed in 64 bits up to the fraction of a turn (2^20 positions times a
+// frequency leave no digit of the angle in 32).
 #include "../../include/fusedmm_b200.h"
 #include "attn_common.cuh"
 #include "attn_host.h"
@@ -17,8 +18,10 @@
 namespace fmm {
 namespace attn {
 
+// Heads of a row on their way from memory: one 262 us, two 249, three 232, four 230 (65536 x 40 heads of 128, bf16; the bytes need
+// 205), and four take the registers of a quarter of the warps from float (100003 x 8 heads of 40: 67, 65, 63, 77 us).
+constexpr int ROT_AHEAD = 3;
 constexpr int ROT_THREADS = 256;
-constexpr int ROT_TABLE = 2048;  // sine/cosine pairs a block keeps
 constexpr int ROT_SCALAR_UNITS = 4;  // units of a lane in the element-wise form: 32 lanes x 4 units x 2 elements = 256
 
 struct RotaryParams {
@@ -33,7 +36,7 @@ struct RotaryParams {
    const double *freq;   // [axes][pairs]
    float *dw_partial;    // [blocks][2][d]
    long long rows;
-   int d, pairs, axes, pos_type, w_f32, interleaved, norm, tile, lanes_log2, units;
+   int d, pairs, axes, pos_type, w_f32, interleaved, norm, lanes_log2, units, splits;
    float eps;
 };
 
@@ -48,20 +51,16 @@ __device__ __forceinline__ double position(const RotaryParams &p, long long row,
    }
 }
 
-// sines and cosines of the tile's rows into shared memory
-__device__ __forceinline__ void fill_table(const RotaryParams &p, long long row0, int nrows, float2 *table)
+// cosine and sine of pair i of a row
+__device__ __forceinline__ void angle_of(const RotaryParams &p, const double (&pos)[FUSEDMM_B200_ROTARY_MAX_AXES], int i, float &c, float &s)
 {
-   for (int t = threadIdx.x; t < nrows * p.pairs; t += ROT_THREADS) {
-      const int r = t / p.pairs, i = t - r * p.pairs;
-      double angle = 0.0;
-      for (int a = 0; a < p.axes; a++) angle = fma(position(p, row0 + r, a), __ldg(p.freq + a * p.pairs + i), angle);
-      const double half_turns = angle * 0.31830988618379067154;  // 1/pi
-      // only the fraction of a turn matters; it fits 32 bits once the whole turns are gone
-      const float rest = static_cast<float>(half_turns - 2.0 * rint(half_turns * 0.5));
-      float s, c;
-      sincospif(rest, &s, &c);
-      table[t] = make_float2(c, s);
-   }
+   double angle = 0.0;
+#pragma unroll
+   for (int a = 0; a < FUSEDMM_B200_ROTARY_MAX_AXES; a++)
+      if (a < p.axes) angle = fma(pos[a], __ldg(p.freq + a * p.pairs + i), angle);
+   const double half_turns = angle * 0.31830988618379067154;  // 1/pi
+   // only the fraction of a turn matters; it fits 32 bits once the whole turns are gone
+   sincospif(static_cast<float>(half_turns - 2.0 * rint(half_turns * 0.5)), &s, &c);
 }
 
 // One unit: 2W elements in two vectors.  Unit u < pairs/W of the halves form holds elements [uW, uW+W) and
@@ -86,173 +85,237 @@ struct Unit {
    }
 };
 
-template <int W>
-__device__ __forceinline__ void turn(float (&lo)[W], float (&hi)[W], const float2 *cs, bool interleaved, float sign)
+// Turns a unit, back with BACK.  c, s: cosines and sines of its pairs, two to a register pair.
+template <int W, bool INTER, bool BACK>
+__device__ __forceinline__ void turn(F2 (&lo)[(W + 1) / 2], F2 (&hi)[(W + 1) / 2], const F2 (&c)[(W + 1) / 2], const F2 (&s)[(W + 1) / 2])
 {
-   if (interleaved && W > 1) {
-      // the two vectors are consecutive: pair j is elements 2j, 2j+1 of their 2W
+   if constexpr (INTER && W > 1) {
+      // the two vectors are consecutive: pair j is elements 2j, 2j + 1 of their 2W, one register pair
 #pragma unroll
       for (int j = 0; j < W; j++) {
-         const float2 t = cs[j];
-         float &a = 2 * j < W ? lo[(2 * j) % W] : hi[(2 * j) % W];
-         float &b = 2 * j < W ? lo[(2 * j + 1) % W] : hi[(2 * j + 1) % W];
-         const float s = sign * t.y, a0 = a;
-         a = fmaf(a0, t.x, -b * s);
-         b = fmaf(b, t.x, a0 * s);
+         F2 &x = j < W / 2 ? lo[j % (W / 2)] : hi[j % (W / 2)];
+         const float2 v = f2_parts(x), cc = f2_parts(c[j / 2]), ss = f2_parts(s[j / 2]);
+         const float cj = j & 1 ? cc.y : cc.x, sj = BACK ? -(j & 1 ? ss.y : ss.x) : (j & 1 ? ss.y : ss.x);
+         x = f2(fmaf(v.x, cj, -v.y * sj), fmaf(v.y, cj, v.x * sj));
       }
    } else {
+      const F2 minus = f2(-1.0f, -1.0f);
 #pragma unroll
-      for (int j = 0; j < W; j++) {
-         const float2 t = cs[j];
-         const float s = sign * t.y, a0 = lo[j];
-         lo[j] = fmaf(a0, t.x, -hi[j] * s);
-         hi[j] = fmaf(hi[j], t.x, a0 * s);
+      for (int j = 0; j < (W + 1) / 2; j++) {
+         const F2 negative = mul2(s[j], minus), up = BACK ? negative : s[j], down = BACK ? s[j] : negative;
+         const F2 a = fma2(lo[j], c[j], mul2(hi[j], down));
+         hi[j] = fma2(hi[j], c[j], mul2(lo[j], up));
+         lo[j] = a;
       }
    }
 }
 
+// A unit's two vectors as they come from memory, and as numbers.
 template <typename T, int W>
-__device__ __forceinline__ void load_part(const T *base, int at, float (&f)[W])
-{
-   if constexpr (W == 1) {
-      f[0] = at >= 0 ? Elt<T>::up(base[at]) : 0.0f;
-   } else {
-      const uint4 r = at >= 0 ? ldg16(base + at) : make_uint4(0u, 0u, 0u, 0u);
-      Elt<T>::unpack(r, f);
+struct Unpacked {
+   static constexpr int P = (W + 1) / 2;
+   uint4 r[2];  // (W = 1: the number's bits)
+   __device__ __forceinline__ void load(const T *base, const Unit<W> &u, bool live)
+   {
+#pragma unroll
+      for (int s = 0; s < 2; s++) {
+         const bool there = live && u.at[s] >= 0;
+         if constexpr (W == 1) r[s].x = there ? __float_as_uint(Elt<T>::up(base[u.at[s]])) : 0u;
+         else r[s] = there ? ldg16(base + u.at[s]) : make_uint4(0u, 0u, 0u, 0u);
+      }
    }
-}
+   __device__ __forceinline__ void unpack(F2 (&f)[2][P]) const
+   {
+#pragma unroll
+      for (int s = 0; s < 2; s++) {
+         if constexpr (W == 1) f[s][0] = f2(__uint_as_float(r[s].x), 0.0f);
+         else unpack_pairs<T>(r[s], f[s]);
+      }
+   }
+};
 template <typename T, int W>
-__device__ __forceinline__ void store_part(T *base, int at, const float (&f)[W])
+__device__ __forceinline__ void store_part(T *base, int at, const F2 (&f)[(W + 1) / 2])
 {
    if (at < 0) return;
-   if constexpr (W == 1) base[at] = Elt<T>::down(f[0]);
-   else *reinterpret_cast<uint4 *>(base + at) = Elt<T>::pack(f);
-}
-template <typename T, int W>
-__device__ __forceinline__ void load_weight(const RotaryParams &p, int which, int at, float (&f)[W])
-{
+   if constexpr (W == 1) {
+      base[at] = Elt<T>::down(f2_parts(f[0]).x);
+   } else {
+      float o[W];
 #pragma unroll
-   for (int j = 0; j < W; j++) {
-      f[j] = 1.0f;
-      if (at >= 0 && p.w[which])
-         f[j] = p.w_f32 ? __ldg(static_cast<const float *>(p.w[which]) + at + j) : Elt<T>::up(static_cast<const T *>(p.w[which])[at + j]);
+      for (int i = 0; i < W / 2; i++) {
+         const float2 v = f2_parts(f[i]);
+         o[2 * i] = v.x;
+         o[2 * i + 1] = v.y;
+      }
+      *reinterpret_cast<uint4 *>(base + at) = Elt<T>::pack(o);
    }
 }
 
+// LOG2: a slot has 2^LOG2 lanes, or 2^p.lanes_log2 with -1
+template <int LOG2>
 __device__ __forceinline__ float sum_over(float v, int lanes_log2)
 {
-   for (int s = 0; s < lanes_log2; s++) v += __shfl_xor_sync(FULL, v, 1 << s);
+   if constexpr (LOG2 >= 0) {
+#pragma unroll
+      for (int s = 0; s < LOG2; s++) v += __shfl_xor_sync(FULL, v, 1 << s);
+   } else {
+      for (int s = 0; s < lanes_log2; s++) v += __shfl_xor_sync(FULL, v, 1 << s);
+   }
    return v;
 }
 
-// NU: units of a lane (1 with vectors).  A slot of 2^lanes_log2 lanes takes one head of one row at a time.
-template <typename T, int W, int NU, bool BACKWARD>
+// NU: units of a lane (1 with vectors).  INTER: pairs side by side.  AHEAD heads of a row are on their way from memory.
+template <typename T, int W, int NU, int LOG2, bool INTER, bool BACKWARD>
 __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotaryParams p)
 {
-   __shared__ float2 table[ROT_TABLE];
+   constexpr int P = (W + 1) / 2, AHEAD = NU > 1 ? 1 : ROT_AHEAD;
    __shared__ float sums[BACKWARD ? ROT_THREADS * NU * 2 * W : 1];
-   const int lanes = 1 << p.lanes_log2;
-   const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x >> p.lanes_log2, slots = ROT_THREADS >> p.lanes_log2;
+   const int lanes_log2 = LOG2 >= 0 ? LOG2 : p.lanes_log2, lanes = 1 << lanes_log2;
+   const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x >> lanes_log2, slots = ROT_THREADS >> lanes_log2;
    Unit<W> unit[NU];
 #pragma unroll
    for (int i = 0; i < NU; i++) unit[i].place(p, lane + i * 32);
-   float dw[2][NU][2][W] = {};
+   F2 dw[BACKWARD ? 2 : 1][NU][2][P] = {};
    const float inv_d = 1.0f / p.d;
-   const long long tiles = (p.rows + p.tile - 1) / p.tile;
-   for (long long tl = blockIdx.x; tl < tiles; tl += gridDim.x) {
-      const long long row0 = tl * p.tile;
-      const int nrows = static_cast<int>(min(static_cast<long long>(p.tile), p.rows - row0));
-      __syncthreads();  // the table's last readers
-      if (p.pairs > 0) fill_table(p, row0, nrows, table);
-      __syncthreads();
+   // the block's part of the heads
+   const int part = blockIdx.y;
+   int h0[2], h1[2];
+#pragma unroll
+   for (int which = 0; which < 2; which++) {
+      h0[which] = static_cast<int>(static_cast<long long>(p.heads[which]) * part / p.splits);
+      h1[which] = static_cast<int>(static_cast<long long>(p.heads[which]) * (part + 1) / p.splits);
+   }
+   for (long long row0 = static_cast<long long>(blockIdx.x) * slots; row0 < p.rows; row0 += static_cast<long long>(gridDim.x) * slots) {
+      // every lane of a warp runs every round: the butterflies need them all
+      const bool live = row0 + slot < p.rows;
+      const long long row = live ? row0 + slot : row0;
+      F2 c[NU][P], s[NU][P];
+      bool turned = false;
 #pragma unroll
       for (int which = 0; which < 2; which++) {
-         const int heads = p.heads[which], tasks = nrows * heads;
-         if (tasks == 0) continue;
-         float w[NU][2][W];
-#pragma unroll
-         for (int i = 0; i < NU; i++) {
-            load_weight<T, W>(p, which, unit[i].at[0], w[i][0]);
-            load_weight<T, W>(p, which, unit[i].at[1], w[i][1]);
-         }
-         // every lane of a warp runs every round: the butterflies need them all
-         const int rounds = (tasks + slots - 1) / slots;
-         for (int n = 0; n < rounds; n++) {
-            const int task = n * slots + slot;
-            const bool live = task < tasks;
-            const int r = live ? task / heads : 0, h = live ? task - r * heads : 0;
-            const long long row = row0 + r;
-            const T *x = static_cast<const T *>(p.x[which]) + row * p.ldx[which] + h * p.hsx[which];
-            T *y = static_cast<T *>(p.y[which]) + (row * heads + h) * p.d;
-            float v[NU][2][W];
+         const int heads = h1[which] - h0[which];
+         if (heads <= 0) continue;
+         Unpacked<T, W> x[AHEAD][NU], dy[BACKWARD ? AHEAD : 1][NU];
+         const T *src = static_cast<const T *>(p.x[which]) + row * p.ldx[which] + h0[which] * p.hsx[which], *dsrc = nullptr;
+         if constexpr (BACKWARD) dsrc = static_cast<const T *>(p.dy[which]) + row * p.ldd[which] + h0[which] * p.hsd[which];
+         T *y = static_cast<T *>(p.y[which]) + (row * p.heads[which] + h0[which]) * p.d;
+         auto fetch = [&](int k, bool there) {
 #pragma unroll
             for (int i = 0; i < NU; i++) {
-               load_part<T, W>(x, live ? unit[i].at[0] : -1, v[i][0]);
-               load_part<T, W>(x, live ? unit[i].at[1] : -1, v[i][1]);
+               x[k][i].load(src, unit[i], there);
+               if constexpr (BACKWARD) dy[BACKWARD ? k : 0][i].load(dsrc, unit[i], there);
             }
-            float rr = 1.0f;
-            if (p.norm) {
-               float ss = 0.0f;
+            src += p.hsx[which];
+            if constexpr (BACKWARD) dsrc += p.hsd[which];
+         };
 #pragma unroll
-               for (int i = 0; i < NU; i++)
+         for (int k = 0; k < AHEAD; k++) fetch(k, live && k < heads);
+         if (!turned) {  // while the first heads are on their way
+            turned = true;
+            double pos[FUSEDMM_B200_ROTARY_MAX_AXES];
 #pragma unroll
-                  for (int j = 0; j < W; j++) ss = fmaf(v[i][0][j], v[i][0][j], fmaf(v[i][1][j], v[i][1][j], ss));
-               ss = sum_over(ss, p.lanes_log2);
-               rr = rsqrtf(fmaf(ss, inv_d, p.eps));
-            }
-            if constexpr (!BACKWARD) {
+            for (int a = 0; a < FUSEDMM_B200_ROTARY_MAX_AXES; a++) pos[a] = p.pairs > 0 && a < p.axes ? position(p, row, a) : 0.0;
 #pragma unroll
-               for (int i = 0; i < NU; i++) {
-                  if (p.norm) {
+            for (int i = 0; i < NU; i++)
 #pragma unroll
-                     for (int j = 0; j < W; j++) {
-                        v[i][0][j] = v[i][0][j] * rr * w[i][0][j];
-                        v[i][1][j] = v[i][1][j] * rr * w[i][1][j];
+               for (int j = 0; j < P; j++) {
+                  float cc[2] = {1.0f, 1.0f}, ss[2] = {0.0f, 0.0f};
+#pragma unroll
+                  for (int o = 0; o < (W == 1 ? 1 : 2); o++)
+                     if (unit[i].pair >= 0) angle_of(p, pos, unit[i].pair + 2 * j + o, cc[o], ss[o]);
+                  c[i][j] = f2(cc[0], cc[1]);
+                  s[i][j] = f2(ss[0], ss[1]);
+               }
+         }
+         F2 w[NU][2][P];
+#pragma unroll
+         for (int i = 0; i < NU; i++)
+#pragma unroll
+            for (int v = 0; v < 2; v++)
+#pragma unroll
+               for (int j = 0; j < P; j++) {
+                  float e[2] = {1.0f, 1.0f};
+#pragma unroll
+                  for (int o = 0; o < (W == 1 ? 1 : 2); o++)
+                     if (p.w[which] && unit[i].at[v] >= 0) {
+                        const int at = unit[i].at[v] + 2 * j + o;
+                        e[o] = p.w_f32 ? __ldg(static_cast<const float *>(p.w[which]) + at) : Elt<T>::up(static_cast<const T *>(p.w[which])[at]);
                      }
-                  }
-                  if (unit[i].pair >= 0) turn<W>(v[i][0], v[i][1], table + r * p.pairs + unit[i].pair, p.interleaved, 1.0f);
-                  if (live) {
-                     store_part<T, W>(y, unit[i].at[0], v[i][0]);
-                     store_part<T, W>(y, unit[i].at[1], v[i][1]);
-                  }
+                  w[i][v][j] = f2(e[0], e[1]);
                }
-            } else {
-               const T *dy = static_cast<const T *>(p.dy[which]) + row * p.ldd[which] + h * p.hsd[which];
-               float g[NU][2][W], dot = 0.0f;
+         for (int n = 0; n < heads; n += AHEAD) {
+#pragma unroll
+            for (int k = 0; k < AHEAD; k++) {
+               if (n + k >= heads) break;
+               F2 v[NU][2][P], g[BACKWARD ? NU : 1][2][P];
 #pragma unroll
                for (int i = 0; i < NU; i++) {
-                  load_part<T, W>(dy, live ? unit[i].at[0] : -1, g[i][0]);
-                  load_part<T, W>(dy, live ? unit[i].at[1] : -1, g[i][1]);
-                  if (unit[i].pair >= 0) turn<W>(g[i][0], g[i][1], table + r * p.pairs + unit[i].pair, p.interleaved, -1.0f);
-                  if (p.norm) {
-#pragma unroll
-                     for (int s = 0; s < 2; s++)
-#pragma unroll
-                        for (int j = 0; j < W; j++) {
-                           v[i][s][j] *= rr;
-                           // a slot without a task has zeros here, times a weight that may be infinite: adds nothing
-                           if (live) dw[which][i][s][j] = fmaf(g[i][s][j], v[i][s][j], dw[which][i][s][j]);
-                           g[i][s][j] *= w[i][s][j];
-                           dot = fmaf(g[i][s][j], v[i][s][j], dot);
-                        }
-                  }
+                  x[k][i].unpack(v[i]);
+                  if constexpr (BACKWARD) dy[BACKWARD ? k : 0][i].unpack(g[BACKWARD ? i : 0]);
                }
+               fetch(k, live && n + k + AHEAD < heads);
+               F2 rr = f2(1.0f, 1.0f);
                if (p.norm) {
-                  dot = sum_over(dot, p.lanes_log2) * inv_d;
+                  F2 squares = 0;
 #pragma unroll
                   for (int i = 0; i < NU; i++)
 #pragma unroll
-                     for (int s = 0; s < 2; s++)
-#pragma unroll
-                        for (int j = 0; j < W; j++) g[i][s][j] = rr * fmaf(-v[i][s][j], dot, g[i][s][j]);
+                     for (int j = 0; j < P; j++) squares = fma2(v[i][0][j], v[i][0][j], fma2(v[i][1][j], v[i][1][j], squares));
+                  const float r = rsqrtf(fmaf(sum_over<LOG2>(sum2(squares), lanes_log2), inv_d, p.eps));
+                  rr = f2(r, r);
                }
-               if (live) {
+               if constexpr (!BACKWARD) {
 #pragma unroll
                   for (int i = 0; i < NU; i++) {
-                     store_part<T, W>(y, unit[i].at[0], g[i][0]);
-                     store_part<T, W>(y, unit[i].at[1], g[i][1]);
+                     if (p.norm) {
+#pragma unroll
+                        for (int o = 0; o < 2; o++)
+#pragma unroll
+                           for (int j = 0; j < P; j++) v[i][o][j] = mul2(mul2(v[i][o][j], rr), w[i][o][j]);
+                     }
+                     if (unit[i].pair >= 0) turn<W, INTER, false>(v[i][0], v[i][1], c[i], s[i]);
+                     if (live) {
+                        store_part<T, W>(y, unit[i].at[0], v[i][0]);
+                        store_part<T, W>(y, unit[i].at[1], v[i][1]);
+                     }
+                  }
+               } else {
+                  F2 dots = 0;
+#pragma unroll
+                  for (int i = 0; i < NU; i++) {
+                     if (unit[i].pair >= 0) turn<W, INTER, true>(g[i][0], g[i][1], c[i], s[i]);
+                     if (p.norm) {
+#pragma unroll
+                        for (int o = 0; o < 2; o++)
+#pragma unroll
+                           for (int j = 0; j < P; j++) {
+                              v[i][o][j] = mul2(v[i][o][j], rr);
+                              // (a slot without a row has zeros, but with eps 0 the root of nothing is infinite)
+                              if (live) dw[BACKWARD ? which : 0][i][o][j] = fma2(g[i][o][j], v[i][o][j], dw[BACKWARD ? which : 0][i][o][j]);
+                              g[i][o][j] = mul2(g[i][o][j], w[i][o][j]);
+                              dots = fma2(g[i][o][j], v[i][o][j], dots);
+                           }
+                     }
+                  }
+                  if (p.norm) {
+                     const float dot = -sum_over<LOG2>(sum2(dots), lanes_log2) * inv_d;
+                     const F2 dd = f2(dot, dot);
+#pragma unroll
+                     for (int i = 0; i < NU; i++)
+#pragma unroll
+                        for (int o = 0; o < 2; o++)
+#pragma unroll
+                           for (int j = 0; j < P; j++) g[i][o][j] = mul2(rr, fma2(v[i][o][j], dd, g[i][o][j]));
+                  }
+                  if (live) {
+#pragma unroll
+                     for (int i = 0; i < NU; i++) {
+                        store_part<T, W>(y, unit[i].at[0], g[i][0]);
+                        store_part<T, W>(y, unit[i].at[1], g[i][1]);
+                     }
                   }
                }
+               y += p.d;
             }
          }
       }
@@ -260,41 +323,50 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotaryParams 
    if constexpr (BACKWARD) {
       if (!p.dw_partial) return;
       // the block's share of the weight gradients: every slot's sums side by side, added in the order of the slots
+      const long long block = static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x;
 #pragma unroll
       for (int which = 0; which < 2; which++) {
          __syncthreads();
 #pragma unroll
          for (int i = 0; i < NU; i++)
 #pragma unroll
-            for (int s = 0; s < 2; s++)
-               if (unit[i].at[s] >= 0)
+            for (int o = 0; o < 2; o++)
+               if (unit[i].at[o] >= 0)
 #pragma unroll
-                  for (int j = 0; j < W; j++) sums[slot * p.d + unit[i].at[s] + j] = dw[which][i][s][j];
+                  for (int j = 0; j < W; j++) {
+                     const float2 v = f2_parts(dw[which][i][o][j / 2]);
+                     sums[slot * p.d + unit[i].at[o] + j] = j & 1 ? v.y : v.x;
+                  }
          __syncthreads();
          for (int e = threadIdx.x; e < p.d; e += ROT_THREADS) {
             float t = 0.0f;
-            for (int s = 0; s < slots; s++) t += sums[s * p.d + e];
-            p.dw_partial[(static_cast<long long>(blockIdx.x) * 2 + which) * p.d + e] = t;
+            for (int s2 = 0; s2 < slots; s2++) t += sums[s2 * p.d + e];
+            p.dw_partial[(block * 2 + which) * p.d + e] = t;
          }
       }
    }
 }
 
-// dw[which][e] = sum over the blocks; 32 columns to a block, its 8 warps take the partial rows in turn
-__global__ void __launch_bounds__(256) rotary_dw_kernel(const float *partial, int blocks, int d, float *dwq, float *dwk)
+// dw[which][e] = sum over the blocks; 32 columns to a block, its 32 warps take the partial rows in turn
+__global__ void __launch_bounds__(1024) rotary_dw_kernel(const float *partial, int blocks, int d, float *dwq, float *dwk)
 {
-   __shared__ float part[8][33];
-   const int col = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
+   __shared__ float part[32][33];
+   const int lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane, w = threadIdx.x >> 5;
    float t = 0.0f;
-   if (col < 2 * d)
-      for (int b = w; b < blocks; b += 8) t += partial[static_cast<long long>(b) * 2 * d + col];
-   part[w][threadIdx.x & 31] = t;
+   if (col < 2 * d) {
+#pragma unroll 4
+      for (int b = w; b < blocks; b += 32) t += partial[static_cast<long long>(b) * 2 * d + col];
+   }
+   part[w][lane] = t;
    __syncthreads();
-   if (w == 0 && col < 2 * d) {
-      float s = 0.0f;
-      for (int i = 0; i < 8; i++) s += part[i][threadIdx.x];
-      float *out = col < d ? dwq : dwk;
-      if (out) out[col < d ? col : col - d] = s;
+   // warp w adds up column w of the 32
+   float s = part[lane][w];
+#pragma unroll
+   for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(FULL, s, x);
+   const int mine = blockIdx.x * 32 + w;
+   if (lane == 0 && mine < 2 * d) {
+      float *out = mine < d ? dwq : dwk;
+      if (out) out[mine < d ? mine : mine - d] = s;
    }
 }
 
@@ -307,21 +379,27 @@ int ceil_log2(int n)
    return l;
 }
 
-// rows of a block: enough heads for four rounds of its slots, so that the sines are shared and loads of several rounds
-// overlap, but no more than the sine table holds, and fewer when there are too few rows to give every SM work
-void choose_tile(RotaryParams &p, int sm_count)
-{
-   const int slots = ROT_THREADS >> p.lanes_log2, heads = p.heads[0] + p.heads[1];
-   long long tile = (4LL * slots + heads - 1) / heads;
-   if (p.pairs > 0) tile = tile < ROT_TABLE / p.pairs ? tile : ROT_TABLE / p.pairs;
-   const long long spread = p.rows / (4LL * sm_count);
-   if (tile > spread) tile = spread;
-   if (tile > 64) tile = 64;
-   p.tile = static_cast<int>(tile < 1 ? 1 : tile);
-}
-
 constexpr int ROT_BACKWARD_BLOCKS_PER_SM = 4;
 
+// Heads of a row go to one slot, which forms the row's sines once, unless there are too few rows to give every SM this many
+// warps (16384 rows of 20 heads of 64: 19 us with 12, 24 with 24, which forms the sines twice).
+constexpr int ROT_WARPS = 12;
+int choose_splits(const RotaryParams &p, int sm_count)
+{
+   const long long warps = ((p.rows << p.lanes_log2) + 31) / 32, wanted = static_cast<long long>(ROT_WARPS) * sm_count;
+   const int most = p.heads[0] > p.heads[1] ? p.heads[0] : p.heads[1];
+   const long long splits = (wanted + warps - 1) / warps;
+   return static_cast<int>(splits < 1 ? 1 : splits > most ? most : splits);
+}
+
+template <typename T, int W, int NU, int LOG2, bool BACKWARD>
+void launch_form(const RotaryParams &p, dim3 grid, cudaStream_t st)
+{
+   if (p.interleaved || W == 1) rotary_kernel<T, W, NU, LOG2, true, BACKWARD><<<grid, ROT_THREADS, 0, st>>>(p);
+   else rotary_kernel<T, W, NU, LOG2, false, BACKWARD><<<grid, ROT_THREADS, 0, st>>>(p);
+}
+
+// returns the number of blocks
 template <typename T, bool BACKWARD>
 int launch(RotaryParams &p, bool vectors, int sm_count, cudaStream_t st)
 {
@@ -330,13 +408,19 @@ int launch(RotaryParams &p, bool vectors, int sm_count, cudaStream_t st)
    const int behind = (p.d - 2 * p.pairs) / width;
    p.units = p.pairs / width + (behind + 1) / 2;
    p.lanes_log2 = vectors ? ceil_log2(p.units) : 5;
-   choose_tile(p, sm_count);
-   const long long tiles = (p.rows + p.tile - 1) / p.tile;
-   const long long cap = BACKWARD ? static_cast<long long>(sm_count) * ROT_BACKWARD_BLOCKS_PER_SM : 0x7fffffffLL;
-   const unsigned grid = static_cast<unsigned>(tiles < cap ? tiles : cap);
-   if (vectors) rotary_kernel<T, W, 1, BACKWARD><<<grid, ROT_THREADS, 0, st>>>(p);
-   else rotary_kernel<T, 1, ROT_SCALAR_UNITS, BACKWARD><<<grid, ROT_THREADS, 0, st>>>(p);
-   return static_cast<int>(grid);
+   p.splits = choose_splits(p, sm_count);
+   const int slots = ROT_THREADS >> p.lanes_log2;
+   const long long blocks = (p.rows + slots - 1) / slots;
+   // backward: each block adds up the weight gradients of many rows
+   long long cap = BACKWARD ? static_cast<long long>(sm_count) * ROT_BACKWARD_BLOCKS_PER_SM / p.splits : 0x7fffffffLL;
+   cap = cap < 1 ? 1 : cap;
+   const dim3 grid(static_cast<unsigned>(blocks < cap ? blocks : cap), p.splits);
+   if (!vectors) launch_form<T, 1, ROT_SCALAR_UNITS, 5, BACKWARD>(p, grid, st);
+   else if (p.lanes_log2 == 2) launch_form<T, W, 1, 2, BACKWARD>(p, grid, st);
+   else if (p.lanes_log2 == 3) launch_form<T, W, 1, 3, BACKWARD>(p, grid, st);
+   else if (p.lanes_log2 == 4) launch_form<T, W, 1, 4, BACKWARD>(p, grid, st);
+   else launch_form<T, W, 1, -1, BACKWARD>(p, grid, st);
+   return static_cast<int>(grid.x * grid.y);
 }
 
 bool multiple(const void *p, long long a, long long b, int width, size_t elt)
@@ -353,6 +437,8 @@ int rotary_setup(RotaryParams &p, int32_t dtype, int64_t rows, int32_t hq, int32
    if (dtype != DT_F32 && dtype != DT_BF16 && dtype != DT_F16) return FUSEDMM_B200_ERR_ARG;
    if (rows < 0 || hq < 0 || hk < 0 || d < 1 || pairs < 0 || 2LL * pairs > d) return FUSEDMM_B200_ERR_ARG;
    if (d > FUSEDMM_B200_ATTN_MAX_WIDTH || hq > FUSEDMM_B200_ATTN_MAX_HEADS || hk > FUSEDMM_B200_ATTN_MAX_HEADS) return FUSEDMM_B200_ERR_LIMIT;
+   for (int64_t s : {ldq, hsq, ldk, hsk})  // the kernels form the addresses inside a tile with 32-bit strides
+      if (s < 0 || s * (dtype == DT_F32 ? 4 : 2) >= INT32_MAX) return FUSEDMM_B200_ERR_LIMIT;
    if (norm && !(eps >= 0.0)) return FUSEDMM_B200_ERR_ARG;
    if (!norm && (wq || wk)) return FUSEDMM_B200_ERR_ARG;
    if (w_dtype != DT_F32 && w_dtype != dtype) return FUSEDMM_B200_ERR_ARG;
@@ -430,8 +516,10 @@ int64_t fusedmm_b200_qk_norm_rotary_backward_workspace(int64_t rows, int32_t d)
    int sms = 0;
    if (rows < 0 || d < 1 || d > FUSEDMM_B200_ATTN_MAX_WIDTH) return FUSEDMM_B200_ERR_ARG;
    if (int s = sm_count(&sms)) return s;
-   const int64_t blocks = static_cast<int64_t>(sms) * ROT_BACKWARD_BLOCKS_PER_SM;
-   return (rows < blocks ? rows : blocks) * 2 * d * static_cast<int64_t>(sizeof(float));
+   // as many blocks as the backward launch may have: its cap, or one for each part of the heads (choose_splits: as many parts as
+   // wanted warps at most)
+   const int64_t blocks = static_cast<int64_t>(sms) * (ROT_WARPS > ROT_BACKWARD_BLOCKS_PER_SM ? ROT_WARPS : ROT_BACKWARD_BLOCKS_PER_SM);
+   return blocks * 2 * d * static_cast<int64_t>(sizeof(float));
 }
 
 int fusedmm_b200_qk_norm_rotary_backward(int32_t dtype, int64_t rows, int32_t hq, int32_t hk, int32_t d, const void *q,
@@ -446,6 +534,8 @@ int fusedmm_b200_qk_norm_rotary_backward(int32_t dtype, int64_t rows, int32_t hq
    if (int s = rotary_setup(p, dtype, rows, hq, hk, d, q, ldq, hsq, k, ldk, hsk, w_dtype, wq, wk, norm, eps, pos_type, pos,
                             ldp, asp, axes, freq, pairs, interleaved)) return s;
    if (!norm && (dwq || dwk)) return FUSEDMM_B200_ERR_ARG;
+   for (int64_t s : {lddq, hsdq, lddk, hsdk})
+      if (s < 0 || s * (dtype == DT_F32 ? 4 : 2) >= INT32_MAX) return FUSEDMM_B200_ERR_LIMIT;
    cudaStream_t st = static_cast<cudaStream_t>(stream);
    if (rows == 0 || hq + hk == 0) {  // sums over nothing
       if (!on_device({dwq, dwk})) return FUSEDMM_B200_ERR_ARG;
@@ -470,7 +560,7 @@ int fusedmm_b200_qk_norm_rotary_backward(int32_t dtype, int64_t rows, int32_t hq
    if (int s = sm_count(&sms)) return s;
    const int blocks = rotary_launch<true>(p, dtype, rotary_vectors(p, dtype, true), sms, st);
    if (p.dw_partial)
-      rotary_dw_kernel<<<(2 * d + 31) / 32, 256, 0, st>>>(p.dw_partial, blocks, d, dwq, dwk);
+      rotary_dw_kernel<<<(2 * d + 31) / 32, 1024, 0, st>>>(p.dw_partial, blocks, d, dwq, dwk);
    return finish_call(stream);
 }
 

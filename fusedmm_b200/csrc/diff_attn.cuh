@@ -31,7 +31,6 @@ namespace attn {
 constexpr int ROW_ITEMS = 8;        // what a row costs beside its edges, in edges
 constexpr int PIECE_WARPS = 4;      // warps of a block whose warps have pieces of their own
 constexpr int JOINT_WARPS = 8;      // warps of a block that share a row
-constexpr int JOIN_PIECES = 8;      // pieces a joining block looks after
 
 struct AttnParams {
    const void *rowptr, *colidx;  // row walks: the pattern; column walk: the transposed one (colidx: 32-bit row ids)
@@ -57,6 +56,7 @@ struct AttnParams {
    long long a_head, b_head;
    int a_width, b_width, subs, kv_log2;
    long long piece, row_limit, pieces;
+   int join_pieces;              // pieces a joining block looks after
    float *partial;
    long long *long_row;          // [pieces]: the long row that begins in a piece, or -1
 };
@@ -232,7 +232,7 @@ __device__ __forceinline__ void unpair(const F2 (&f)[N], float (&o)[2 * N])
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int G, int NV, int QB, int FORM>
 struct Forward {
-   static constexpr int W = Elt<T>::W, P = W / 2, U = 2, BLOCKS = QB * NV * W > 16 ? 2 : 4;
+   static constexpr int W = Elt<T>::W, P = W / 2, U = W == 4 && QB == 1 ? 4 : 2, BLOCKS = W == 4 ? (QB > 2 ? 2 : 3) : QB * NV * W > 16 ? 2 : 4;
    static constexpr int KSKIP = (G / 2) * W, VSKIP = G * W;
    static constexpr int LANE_FLOATS = QB * (2 * NV * W + 2);  // partial state of a lane
    struct State {
@@ -448,7 +448,7 @@ struct Forward {
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int G, int NV, int QB, int FORM>
 struct BackwardRows {
-   static constexpr int W = Elt<T>::W, P = W / 2, U = 2, BLOCKS = QB * NV * W > 16 ? 2 : 4;
+   static constexpr int W = Elt<T>::W, P = W / 2, U = W == 4 && QB == 1 ? 4 : 2, BLOCKS = W == 4 ? (QB > 2 ? 2 : 3) : QB * NV * W > 16 ? 2 : 4;
    static constexpr int KSKIP = (G / 2) * W, VSKIP = G * W;
    static constexpr int LANE_FLOATS = QB * (2 * NV * W + 2);
    struct State {
@@ -554,16 +554,19 @@ struct BackwardRows {
       const float *from = unit + at.in_slot * W;
 #pragma unroll
       for (int b = 0; b < QB; b++) {
+         F2 x[2][NV][P];  // all loads before the first sum
 #pragma unroll
          for (int t = 0; t < NV; t++) {
-            F2 x[P];
-            get_pairs<P>(from + (b * 2 * NV + t) * W * G, x);
-#pragma unroll
-            for (int j = 0; j < P; j++) s.a[b][t][j] = add2(s.a[b][t][j], x[j]);
-            get_pairs<P>(from + ((b * 2 + 1) * NV + t) * W * G, x);
-#pragma unroll
-            for (int j = 0; j < P; j++) s.b[b][t][j] = add2(s.b[b][t][j], x[j]);
+            get_pairs<P>(from + (b * 2 * NV + t) * W * G, x[0][t]);
+            get_pairs<P>(from + ((b * 2 + 1) * NV + t) * W * G, x[1][t]);
          }
+#pragma unroll
+         for (int t = 0; t < NV; t++)
+#pragma unroll
+            for (int j = 0; j < P; j++) {
+               s.a[b][t][j] = add2(s.a[b][t][j], x[0][t][j]);
+               s.b[b][t][j] = add2(s.b[b][t][j], x[1][t][j]);
+            }
          s.delta[b] += unit[QB * 2 * NV * W * G + (b * G + at.in_slot) * 2];
       }
    }
@@ -612,7 +615,7 @@ struct BackwardRows {
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int G, int NV, int QB, int FORM>
 struct BackwardColumns {
-   static constexpr int W = Elt<T>::W, P = W / 2, U = 2, BLOCKS = W == 4 ? 4 : 3;
+   static constexpr int W = Elt<T>::W, P = W / 2, U = W == 4 ? 4 : 2, BLOCKS = 3;
    static constexpr int KSKIP = (G / 2) * W, VSKIP = G * W;
    static constexpr int LANE_FLOATS = 2 * NV * W;
    struct State {
@@ -707,16 +710,19 @@ struct BackwardColumns {
    __device__ __forceinline__ void join_from(const float *unit, const Place &at)
    {
       const float *from = unit + at.in_slot * W;
+      F2 x[2][NV][P];  // all loads before the first sum
 #pragma unroll
       for (int t = 0; t < NV; t++) {
-         F2 x[P];
-         get_pairs<P>(from + t * W * G, x);
-#pragma unroll
-         for (int j = 0; j < P; j++) s.dk[t][j] = add2(s.dk[t][j], x[j]);
-         get_pairs<P>(from + (NV + t) * W * G, x);
-#pragma unroll
-         for (int j = 0; j < P; j++) s.dv[t][j] = add2(s.dv[t][j], x[j]);
+         get_pairs<P>(from + t * W * G, x[0][t]);
+         get_pairs<P>(from + (NV + t) * W * G, x[1][t]);
       }
+#pragma unroll
+      for (int t = 0; t < NV; t++)
+#pragma unroll
+         for (int j = 0; j < P; j++) {
+            s.dk[t][j] = add2(s.dk[t][j], x[0][t][j]);
+            s.dv[t][j] = add2(s.dv[t][j], x[1][t][j]);
+         }
    }
    __device__ __forceinline__ void put(float *unit, const Place &at) const
    {
@@ -835,7 +841,7 @@ __global__ void __launch_bounds__(JOINT_WARPS * 32) join_kernel(const AttnParams
    const Place at = Place::make<G>(p, static_cast<int>(blockIdx.x - group * p.unit_blocks));
    const Rows rows(p);
    Op op;
-   for (long long piece = group * JOIN_PIECES; piece < (group + 1) * JOIN_PIECES && piece < p.pieces; piece++) {
+   for (long long piece = group * p.join_pieces; piece < (group + 1) * p.join_pieces && piece < p.pieces; piece++) {
       const long long u = p.long_row[piece];
       if (u < 0) continue;
       const long long last = (rows.items(u + 1) - 1) / p.piece, parts = last - piece + 1;
@@ -872,7 +878,7 @@ int launch_op(const AttnParams &p, bool together, cudaStream_t st)
    } else {
       walk_kernel<Op, G, false><<<static_cast<unsigned>((jobs + PIECE_WARPS - 1) / PIECE_WARPS), PIECE_WARPS * 32, 0, st>>>(p);
    }
-   const long long groups = (p.pieces + JOIN_PIECES - 1) / JOIN_PIECES;
+   const long long groups = (p.pieces + p.join_pieces - 1) / p.join_pieces;
    join_kernel<Op, G><<<static_cast<unsigned>(groups * p.unit_blocks), JOINT_WARPS * 32, bytes, st>>>(p);
    return 0;
 }

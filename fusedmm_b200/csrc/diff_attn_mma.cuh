@@ -155,7 +155,7 @@ struct Ring {
    }
    __device__ __forceinline__ void setup(const AttnParams &p, const Lanes &l, int lane, const void *array_a, const void *array_b, int head)
    {
-      const int x = lane % CHUNKS, pair = lane / CHUNKS, s = PER >= 4 ? pair & (l.slots - 1) : 0;
+      const int x = lane % CHUNKS, pair = lane / CHUNKS, s = PER >= 2 ? pair & (l.slots - 1) : 0;
       const int map = x / (CHUNKS / 2), xa = (x % (CHUNKS / 2)) * 8, xb = x * 8;
       a = static_cast<const char *>(array_a) + (head + s) * p.a_head + static_cast<long long>(map * p.a_width + xa) * sizeof(T);
       b = static_cast<const char *>(array_b) + (head + s) * p.b_head + static_cast<long long>(xb) * sizeof(T);
@@ -209,6 +209,7 @@ struct Ring {
             la += (sub << p.kv_log2) * p.a_head;
             lb += (sub << p.kv_log2) * p.b_head;
          }
+         const long long odd_a = l.slots == 4 ? 2 * p.a_head : 0, odd_b = l.slots == 4 ? 2 * p.b_head : 0;
 #pragma unroll
          for (int i = 0; i < ROUNDS; i++) {
             const int pair = i * PER + pair0;
@@ -217,10 +218,14 @@ struct Ring {
             const unsigned row = live ? id : 0;
             const bool here = PER >= 4 ? live : live && (on >> i & 1);
             const char *ra = la + static_cast<unsigned long long>(row) * p.a_stride, *rb = lb + static_cast<unsigned long long>(row) * p.b_stride;
-            if constexpr (PER < 4) {
-               const int s = pair & (l.slots - 1);
-               ra += s * p.a_head;
-               rb += s * p.b_head;
+            if constexpr (PER == 2) {  // the lane's slot is its own in the even rounds, two further in the odd
+               if (i & 1) {
+                  ra += odd_a;
+                  rb += odd_b;
+               }
+            } else if constexpr (PER == 1) {  // the round's
+               ra += (i & (l.slots - 1)) * p.a_head;
+               rb += (i & (l.slots - 1)) * p.b_head;
             }
             // the pair's bits that change from round to round, as in offset()
             const unsigned at = to + ((place + i * PER * ROW) ^ (CHUNKS >= 8 ? ((i * PER) & 7) << 4 : 0));
@@ -364,7 +369,7 @@ enum { WALK_FORWARD, WALK_ROWS, WALK_COLUMNS };
 template <int DK, int WALK>
 struct Budget {
    static constexpr int STAGES = DK == 16 ? 4 : DK == 32 ? 3 : 2;
-   static constexpr int SOLO = DK == 128 ? 2 : 4, JOINT = DK == 128 ? 4 : 8;
+   static constexpr int SOLO = DK == 128 ? 2 : 4, JOINT = DK >= 64 ? 4 : 8;
    // The backward walks run faster with fewer warps and their registers: R-MAT training at d 32 columns 2.45 ms with four
    // blocks, 2.19 with three, rows 1.84 and 1.57 (forward 1.26 and 1.30); window training at d 64 columns 419 us with three blocks,
    // 375 with two, rows 102 and 98 (forward 82 and 89).
@@ -520,6 +525,9 @@ struct ForwardMma {
    {
       const float2 *from = reinterpret_cast<const float2 *>(unit) + at.lane;
       const float2 top = from[32 * TILES], sum = from[32 * (TILES + 1)];
+      float2 o[TILES];
+#pragma unroll
+      for (int t = 0; t < TILES; t++) o[t] = from[32 * t];
       float f[N], g[N];
 #pragma unroll
       for (int x = 0; x < N; x++) {
@@ -533,9 +541,8 @@ struct ForwardMma {
       const float fr = Cols::of_row(f, l.r), gr = Cols::of_row(g, l.r);
 #pragma unroll
       for (int t = 0; t < TILES; t++) {
-         const float2 o = from[32 * t];
-         s.acc[t][0] = s.acc[t][0] * fr + o.x * gr;
-         s.acc[t][1] = s.acc[t][1] * fr + o.y * gr;
+         s.acc[t][0] = s.acc[t][0] * fr + o[t].x * gr;
+         s.acc[t][1] = s.acc[t][1] * fr + o[t].y * gr;
       }
    }
    __device__ __forceinline__ void put(float *unit, const Place &at, int only) const
@@ -734,15 +741,19 @@ struct BackwardRowsMma {
    __device__ __forceinline__ void join_from(const float *unit, const Place &at)
    {
       const float2 *from = reinterpret_cast<const float2 *>(unit) + at.lane;
+      float2 o[2][TILES];  // all loads before the first sum
+#pragma unroll
+      for (int m = 0; m < 2; m++)
+#pragma unroll
+         for (int t = 0; t < TILES; t++) o[m][t] = from[32 * (m * TILES + t)];
+      const float2 d = from[64 * TILES];
 #pragma unroll
       for (int m = 0; m < 2; m++)
 #pragma unroll
          for (int t = 0; t < TILES; t++) {
-            const float2 o = from[32 * (m * TILES + t)];
-            s.acc[m][t][0] += o.x;
-            s.acc[m][t][1] += o.y;
+            s.acc[m][t][0] += o[m][t].x;
+            s.acc[m][t][1] += o[m][t].y;
          }
-      const float2 d = from[64 * TILES];
       s.delta[0] += d.x;
       if constexpr (!ONE) s.delta[N - 1] += d.y;
    }
@@ -939,11 +950,13 @@ struct BackwardColumnsMma {
    __device__ __forceinline__ void join_from(const float *unit, const Place &at)
    {
       const float4 *from = reinterpret_cast<const float4 *>(unit) + at.lane;
+      float4 o[2 * KT + VT];  // all loads before the first sum
+#pragma unroll
+      for (int i = 0; i < 2 * KT + VT; i++) o[i] = from[32 * i];
 #pragma unroll
       for (int i = 0; i < 2 * KT + VT; i++) {
-         const float4 o = from[32 * i];
          float (&f)[4] = i < KT ? s.dk[0][i] : i < 2 * KT ? s.dk[1][i - KT] : s.dv[i - 2 * KT];
-         f[0] += o.x; f[1] += o.y; f[2] += o.z; f[3] += o.w;
+         f[0] += o[i].x; f[1] += o[i].y; f[2] += o[i].z; f[3] += o[i].w;
       }
    }
    // a head's sums lie in the results' columns 2c, 2c + 1 (and 4 further): the lane's kv heads 2c % 4, 2c % 4 + 1
@@ -1137,7 +1150,7 @@ __global__ void __launch_bounds__(Op::Width::JOINT * 32) ring_join_kernel(const 
    Op op;
    typename Op::Gathered ring;
    op.setup(p, at, ring);
-   for (long long piece = group * JOIN_PIECES; piece < (group + 1) * JOIN_PIECES && piece < p.pieces; piece++) {
+   for (long long piece = group * p.join_pieces; piece < (group + 1) * p.join_pieces && piece < p.pieces; piece++) {
       const long long u = p.long_row[piece];
       if (u < 0) continue;
       const long long last = (rows.items(u + 1) - 1) / p.piece, parts = last - piece + 1;
@@ -1167,7 +1180,7 @@ int launch_ring(const AttnParams &p, bool together, cudaStream_t st)
       ring_walk_kernel<Op, false><<<static_cast<unsigned>((jobs + Op::Width::SOLO - 1) / Op::Width::SOLO), Op::Width::SOLO * 32, bytes, st>>>(p);
    }
    if (!allow_shared(reinterpret_cast<const void *>(ring_join_kernel<Op>), JOIN)) return -1;
-   const long long groups = (p.pieces + JOIN_PIECES - 1) / JOIN_PIECES;
+   const long long groups = (p.pieces + p.join_pieces - 1) / p.join_pieces;
    ring_join_kernel<Op><<<static_cast<unsigned>(groups * p.unit_blocks), Op::Width::JOINT * 32, JOIN, st>>>(p);
    return 0;
 }
