@@ -130,24 +130,27 @@ struct Lanes {
 template <typename T, int DK, int FORM, int STAGES_, bool RECORDS>
 struct Ring {
    static constexpr int STAGES = STAGES_, ROW = 4 * DK, CHUNKS = DK / 4, REGION = 16 * ROW;
-   static constexpr int BIAS = 2 * REGION, RECORD = BIAS + 128, USED = RECORD + (RECORDS ? 16 * 32 : 0);
+   static constexpr int BIAS = 2 * REGION, RECORD = BIAS + 64, USED = RECORD + (RECORDS ? 16 * 32 : 0);
    static constexpr int STAGE = (USED + ROW - 1) / ROW * ROW;  // rows are aligned to their size, so that chunks can be named by exclusive or
    // one round of copies: 32 lanes take PER pairs of CHUNKS chunks of 8 elements
    static constexpr int PER = 32 / CHUNKS, ROUNDS = CHUNKS / 2;
    const char *a, *b;       // the two arrays at the lane's chunk of the unit's head 0 (of the lane's slot, if that is the same in all rounds)
+   const char *a2, *b2;     // with two pairs a round: the slot of the odd rounds
    const char *records;     // [row][head][32 bytes], of the unit's first head
    EdgeStream edges;
    int batch_id;            // the present 32 edges
    float batch_bias;
-   unsigned ring, place;    // shared addresses: block 0; the lane's chunk in a block
+   unsigned ring, place;    // shared address of block 0; the lane's chunk in a block
    unsigned fill, slot;     // block to fill next, block in use
    long long first;         // the run of edges
    int length;
    int issued, current;     // blocks
    unsigned on;             // bit i: the lane's pair of round i is gathered (all, but where the kv heads are taken one by one)
 
-   // byte offset of a chunk of 8 elements of a pair.  The chunk is exchanged by bits of the pair, so that the 8 pairs that
+   // Byte offset of a chunk of 8 elements of a pair.  The chunk is exchanged by bits of the pair, so that the 8 pairs that
    // ldmatrix reads at one chunk lie in 8 different groups of banks; offset(pair, chunk ^ x) = offset(pair, chunk) ^ (x << 4).
+   // (Rows 16 bytes longer do that too and save the exclusive ors, but the copies then end inside 32-byte sectors: window
+   // training's columns 349 us against 338.)
    static __device__ __forceinline__ unsigned offset(int pair, int chunk)
    {
       const int key = CHUNKS >= 8 ? pair & 7 : (pair >> 1) & 3;
@@ -159,7 +162,11 @@ struct Ring {
       const int map = x / (CHUNKS / 2), xa = (x % (CHUNKS / 2)) * 8, xb = x * 8;
       a = static_cast<const char *>(array_a) + (head + s) * p.a_head + static_cast<long long>(map * p.a_width + xa) * sizeof(T);
       b = static_cast<const char *>(array_b) + (head + s) * p.b_head + static_cast<long long>(xb) * sizeof(T);
-      place = ring + offset(pair, x);
+      place = offset(pair, x);
+      if constexpr (PER == 2) {
+         a2 = a + (l.slots == 4 ? 2 * p.a_head : 0);
+         b2 = b + (l.slots == 4 ? 2 * p.b_head : 0);
+      }
    }
 
    __device__ __forceinline__ void chunk_in(unsigned to, const T *from, int left, int step) const
@@ -193,7 +200,6 @@ struct Ring {
             batch_bias = batch_id >= 0 ? edges.bias : -INFINITY;
             edges.fetch(p, first + e + 32, lane);
          }
-         const unsigned to = fill - ring;
          const float bias = __shfl_sync(FULL, batch_bias, off + (lane & ((1 << per_log2) - 1)));
          if ((lane >> per_log2) == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(fill + BIAS + 4 * lane), "f"(bias) : "memory");
          const int pair0 = lane / CHUNKS;
@@ -204,12 +210,7 @@ struct Ring {
             left_b = p.b_width - x * 8;
          }
          if (PER >= 4 && on == 0) left_a = left_b = 0;  // a lane whose pairs are all of one slot
-         const char *la = a, *lb = b;
-         if (sub > 0) {
-            la += (sub << p.kv_log2) * p.a_head;
-            lb += (sub << p.kv_log2) * p.b_head;
-         }
-         const long long odd_a = l.slots == 4 ? 2 * p.a_head : 0, odd_b = l.slots == 4 ? 2 * p.b_head : 0;
+         const long long sub_a = sub > 0 ? (sub << p.kv_log2) * p.a_head : 0, sub_b = sub > 0 ? (sub << p.kv_log2) * p.b_head : 0;
 #pragma unroll
          for (int i = 0; i < ROUNDS; i++) {
             const int pair = i * PER + pair0;
@@ -217,18 +218,18 @@ struct Ring {
             const bool live = id >= 0;
             const unsigned row = live ? id : 0;
             const bool here = PER >= 4 ? live : live && (on >> i & 1);
-            const char *ra = la + static_cast<unsigned long long>(row) * p.a_stride, *rb = lb + static_cast<unsigned long long>(row) * p.b_stride;
-            if constexpr (PER == 2) {  // the lane's slot is its own in the even rounds, two further in the odd
-               if (i & 1) {
-                  ra += odd_a;
-                  rb += odd_b;
-               }
-            } else if constexpr (PER == 1) {  // the round's
+            const char *ra = (PER == 2 && (i & 1) ? a2 : a) + static_cast<unsigned long long>(row) * p.a_stride;
+            const char *rb = (PER == 2 && (i & 1) ? b2 : b) + static_cast<unsigned long long>(row) * p.b_stride;
+            if (p.subs > 1) {
+               ra += sub_a;
+               rb += sub_b;
+            }
+            if constexpr (PER == 1) {  // the slot is the round's
                ra += (i & (l.slots - 1)) * p.a_head;
                rb += (i & (l.slots - 1)) * p.b_head;
             }
             // the pair's bits that change from round to round, as in offset()
-            const unsigned at = to + ((place + i * PER * ROW) ^ (CHUNKS >= 8 ? ((i * PER) & 7) << 4 : 0));
+            const unsigned at = fill + (place ^ (CHUNKS >= 8 ? ((i * PER) & 7) << 4 : 0)) + i * PER * ROW;
             chunk_in(at, reinterpret_cast<const T *>(ra), here ? left_a : 0, p.step);
             chunk_in(at + REGION, reinterpret_cast<const T *>(rb), here ? left_b : 0, p.step);
          }
@@ -437,7 +438,8 @@ struct ForwardMma {
       for (int i = 0; i < DK / 8; i++) q[i] = next[i];
       if (Width::AHEAD && follow >= 0) fetch(p, follow);
       const int per_log2 = 4 - l.slots_log2;
-      const unsigned mine = Gathered::offset(at.lane & 15, at.lane >> 4);  // the lane's row of ldmatrix; chunks by exclusive or
+      // the lane's row and chunk of ldmatrix: pairs 0..7 and 8..15 of one chunk, then of the next; chunks by exclusive or
+      const unsigned mine = Gathered::offset(at.lane & 15, at.lane >> 4);
       for (int e = e0; e < e1;) {
          const int block = e >> per_log2;
          if (block != ring.current) ring.advance(p, l, at.lane);
@@ -662,7 +664,8 @@ struct BackwardRowsMma {
       for (int i = 0; i < DV / 8; i++) dout[i] = next_out[i];
       if (Width::AHEAD && follow >= 0) fetch(p, follow);
       const int per_log2 = 4 - l.slots_log2;
-      const unsigned mine = Gathered::offset(at.lane & 15, at.lane >> 4);  // the lane's row of ldmatrix; chunks by exclusive or
+      // the lane's row and chunk of ldmatrix: pairs 0..7 and 8..15 of one chunk, then of the next; chunks by exclusive or
+      const unsigned mine = Gathered::offset(at.lane & 15, at.lane >> 4);
       for (int e = e0; e < e1;) {
          const int block = e >> per_log2;
          if (block != ring.current) ring.advance(p, l, at.lane);
@@ -867,7 +870,10 @@ struct BackwardColumnsMma {
       for (int i = 0; i < DV / 8; i++) v[i] = next_v[i];
       if (Width::AHEAD && follow >= 0) fetch(p, follow);
       const int per_log2 = 4 - l.slots_log2;
-      const unsigned mine = Gathered::offset(at.lane & 15, at.lane >> 4);  // the lane's row of ldmatrix; chunks by exclusive or
+      // the lane's row and chunk of ldmatrix: pairs 0..7 and 8..15 of one chunk, then of the next; chunks by exclusive or
+      const unsigned mine = Gathered::offset(at.lane & 15, at.lane >> 4);
+      // ... and as columns: pairs 0..7 of one chunk and the next, then pairs 8..15, the order of the A operand's registers
+      const unsigned mine_t = Gathered::offset((at.lane & 7) + (at.lane >> 4) * 8, at.lane >> 3 & 1);
       // of the columns 2c, 2c + 1 at most one is of the pairs' kv head
       const bool valid = (l.c & 1) == pair_kv >> 1;
       const int x = pair_kv & 1, map = l.c >> 1;
@@ -921,16 +927,16 @@ struct BackwardColumnsMma {
 #pragma unroll
             for (int t = 0; t < KT; t++) {
                unsigned q[4];
-               ldmatrix4_trans(q, (slot + mine) ^ ((2 * t) << 4));
-               mma16816<T>(s.dk[0][t], q[0], q[2], q[1], q[3], b0[0], b0[1]);
-               ldmatrix4_trans(q, (slot + mine) ^ ((DK / 8 + 2 * t) << 4));
-               mma16816<T>(s.dk[1][t], q[0], q[2], q[1], q[3], b1[0], b1[1]);
+               ldmatrix4_trans(q, (slot + mine_t) ^ ((2 * t) << 4));
+               mma16816<T>(s.dk[0][t], q[0], q[1], q[2], q[3], b0[0], b0[1]);
+               ldmatrix4_trans(q, (slot + mine_t) ^ ((DK / 8 + 2 * t) << 4));
+               mma16816<T>(s.dk[1][t], q[0], q[1], q[2], q[3], b1[0], b1[1]);
             }
 #pragma unroll
             for (int t = 0; t < VT; t++) {
                unsigned d[4];
-               ldmatrix4_trans(d, (slot + mine + Gathered::REGION) ^ ((2 * t) << 4));
-               mma16816<T>(s.dv[t], d[0], d[2], d[1], d[3], bw[0], bw[1]);
+               ldmatrix4_trans(d, (slot + mine_t + Gathered::REGION) ^ ((2 * t) << 4));
+               mma16816<T>(s.dv[t], d[0], d[1], d[2], d[3], bw[0], bw[1]);
             }
          }
          e = (edges << per_log2) + hi;
