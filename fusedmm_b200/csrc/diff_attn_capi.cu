@@ -241,6 +241,7 @@ int fusedmm_b200_diff_attention(int32_t dtype, int32_t ptr_bits, int32_t idx_bit
    if (!on_device({rowptr, q, lam, out, lse, workspace, nnz > 0 ? colidx : nullptr, nnz > 0 ? bias : nullptr,
                    gathers ? k : nullptr, gathers ? v : nullptr}))
       return FUSEDMM_B200_ERR_ARG;
+   if (n == 0) k = v = workspace;  // nothing is gathered, but copies of nothing want an address too
    Step step(dtype);
    step.with(q, ldq, hsq, d);
    step.with(k, ldk, hsk, d);
@@ -291,6 +292,8 @@ int fusedmm_b200_diff_attention_backward(int32_t dtype, int32_t ptr_bits, int32_
    float *row_dlam = reinterpret_cast<float *>(ws + round256(m * heads * 32));
    float *lam_part = reinterpret_cast<float *>(ws + round256(m * heads * 32) + round256(m * heads * 4));
    char *scratch = ws + backward_front(m, heads, nnz);
+   if (n == 0) k = v = workspace;  // nothing is gathered, but copies of nothing want an address too
+   if (m == 0) q = dout = workspace;
    Step step(dtype);
    step.with(q, ldq, hsq, d);
    step.with(k, ldk, hsk, d);

@@ -249,7 +249,7 @@ struct Ring {
    {
       drain();
       first = from;
-      length = static_cast<int>(to - from);
+      length = to > from ? static_cast<int>(to - from) : 0;
       on = ~0u;
       if (only_kv >= 0)
          for (int i = 0; i < 32; i++)  // (with PER >= 4 all rounds are alike)

@@ -491,9 +491,10 @@ int fusedmm_b200_release(void);
  * to enqueue on (cudaStreamLegacy, the value 1, for the legacy default stream); with NULL the call runs on the legacy
  * default stream and returns when it is done.  They may be captured into a CUDA graph.  Inputs must not overlap outputs.
  *
- * dtype: 0 float, 2 bfloat16, 3 half; sums, softmax statistics and norms are held in float.  Strides count elements;
- * the last axis of every array is dense.  Rows of any length, stride and alignment work; where address, strides and
- * widths are multiples of 16 bytes the loads are 16 bytes wide.  Results are the same bits on every run.
+ * dtype: 0 float, 2 bfloat16, 3 half; sums, softmax statistics and norms are held in float.  Strides count elements and
+ * are below 2^31 bytes (FUSEDMM_B200_ERR_LIMIT beyond); the last axis of every array is dense.  Rows of any length, stride and
+ * alignment work; where address, strides and widths are multiples of 16 bytes the loads are 16 bytes wide.  Results are
+ * the same bits on every run.
  * ---------------------------------------------------------------------------------------------- */
 #define FUSEDMM_B200_ATTN_MAX_WIDTH 256    /* d of qk_norm_rotary, 2 d and dv of diff_attention */
 #define FUSEDMM_B200_ATTN_MAX_HEADS 65536
@@ -551,7 +552,8 @@ int fusedmm_b200_qk_norm_rotary_backward(int32_t dtype, int64_t rows, int32_t hq
  * q is [m][heads][2][d] with the strides ldq, hsq; k is [n][kv_heads][2][d]; v is [n][kv_heads][dv]; lam is
  * [m][heads] with the row stride ldlam, or [heads] with ldlam 0.  out [m][heads][dv] and lse [m][heads][2] (natural
  * logarithms of the two maps' sums; may be NULL) are dense.  Long rows are cut, so that one row of many edges (a single
- * token's) fills the GPU.
+ * token's) fills the GPU.  n is below 2^31 - 1, m and nnz below 2^48.  (Row pointers that decrease or leave [0, nnz] give
+ * wrong rows, but no access outside the arrays; fusedmm_b200_check_csr finds them.)
  */
 int64_t fusedmm_b200_diff_attention_workspace(int32_t backward, int32_t dtype, int64_t m, int64_t n, int64_t nnz,
                                               int32_t heads, int32_t kv_heads, int32_t d, int32_t dv);

@@ -209,14 +209,15 @@ def test_heads_in_another_order_of_axes(cuda_device):
     compare(t, 0.125, randn(gen, BF16, 20, 4, 128).cuda())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("m,n,nnz", [(0, 5, 0), (5, 0, 0), (4, 3, 0), (3, 0, 6)])
-def test_nothing_to_attend_to(cuda_device, m, n, nnz):
+def test_nothing_to_attend_to(cuda_device, m, n, nnz, dtype):
     """No rows, no columns, no edges, or edges that all point outside: zeros, and no gradient."""
     rowptr = torch.zeros(m + 1, dtype=torch.int64)
     if nnz:
         rowptr[1:] = torch.arange(1, m + 1) * (nnz // m)
-    t = make(gen_of(1), F32, rowptr, torch.zeros(nnz, dtype=torch.int32), m, n, 2, 1, 8, 8)
-    got = run_all(t, 1.0, torch.ones(m, 2, 8).cuda())
+    t = make(gen_of(1), dtype, rowptr, torch.zeros(nnz, dtype=torch.int32), m, n, 2, 1, 8, 8)
+    got = run_all(t, 1.0, torch.ones(m, 2, 8, dtype=dtype).cuda())
     assert got["out"].shape == (m, 2, 8) and not got["out"].any()
     for name in ("dq", "dk", "dv", "dlam"):
         assert not got[name].any(), name
@@ -328,6 +329,40 @@ def test_transposed_pattern(cuda_device, m, n, mean, ptr, idx):
     assert t_rowptr.dtype == ptr and int(t_rowptr[-1]) == len(keep)
     assert torch.equal(t_rowptr.long(), torch.cat((torch.zeros(1, dtype=torch.long), torch.cumsum(torch.bincount(colidx[keep].long(), minlength=n), 0))))
     assert torch.equal(t_edge[:len(keep)].long(), order) and torch.equal(t_row[:len(keep)].long(), row[order])
+
+
+def test_transposed_pattern_of_many_edges(cuda_device):
+    """The sort's long tiles, three digits of columns."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    m, n, nnz = 40000, 100000, (4 << 20) + 77
+    rowptr = torch.zeros(m + 1, dtype=torch.int64, device="cuda")
+    rowptr[1:-1] = torch.sort(torch.randint(0, nnz, (m - 1,), generator=gen, device="cuda")).values
+    rowptr[-1] = nnz
+    colidx = torch.randint(0, n, (nnz,), generator=gen, device="cuda", dtype=torch.int32)
+    t_rowptr, t_row, t_edge = torch_op.csr_transpose(rowptr, colidx, n)
+    order = torch.sort(colidx, stable=True).indices
+    row = torch.repeat_interleave(torch.arange(m, device="cuda"), rowptr[1:] - rowptr[:-1])
+    assert torch.equal(t_edge.long(), order) and torch.equal(t_row.long(), row[order])
+    assert torch.equal(t_rowptr[1:], torch.cumsum(torch.bincount(colidx.long(), minlength=n), 0)) and int(t_rowptr[0]) == 0
+
+
+def test_patterns_that_break_their_contract_stay_in_bounds(cuda_device):
+    """Row pointers that decrease or leave the list, and wild column ids: wrong rows, no access outside, later calls are right."""
+    gen = gen_of(19)
+    rowptr, colidx = random_pattern(gen, 300, 200, 8, torch.int64, torch.int64, hub=700)
+    for dtype in (F32, BF16, F16):
+        t = make(gen, dtype, rowptr, colidx, 300, 200, 4, 2, 16, 32)
+        dout = randn(gen, dtype, 300, 4, 32).cuda()
+        bad = dict(t)
+        bad["rowptr"] = t["rowptr"][torch.randperm(301, generator=gen).cuda()].contiguous()
+        bad["rowptr"][::7] += 10 ** 12
+        bad["rowptr"][::11] -= 10 ** 12
+        bad["colidx"] = t["colidx"].clone()
+        bad["colidx"][::3] += 10 ** 15
+        bad["colidx"][::5] -= 2 ** 33
+        run_all(bad, 0.25, dout)
+        torch.cuda.synchronize()
+        compare(t, 0.25, dout)
 
 
 def test_row_pointers_that_start_behind_the_first_edge(cuda_device):
