@@ -460,10 +460,16 @@ def attention_args(rowptr, colidx, bias, q, k, v, lam, scale):
             k.data_ptr(), ldk, hsk, v.data_ptr(), ldv, hsv, lam.data_ptr(), ldlam, float(scale))
 
 
-def diff_attention_workspace(backward, args):
-    """Bytes of workspace (``fusedmm_b200_diff_attention_workspace``) of a call with these arguments."""
-    fn = _attn_fn("diff_attention_workspace", _l, _i, _i, _l, _l, _l, _i, _i, _i, _i)
-    return fn(int(backward), args[0], args[3], args[4], args[5], args[9], args[10], args[11], args[12])
+def diff_attention_workspace(backward, args, *more):
+    """Bytes of workspace (``fusedmm_b200_diff_attention_workspace``) of a call with these arguments; ``more``: addresses, and
+    strides in elements, of the arrays that come with them (``dout``'s; results of torch are aligned)."""
+    fn = _attn_fn("diff_attention_workspace", _l, _i, _i, _i, _l, _l, _l, _i, _i, _i, _i)
+    elt = 4 if args[0] == 0 else 2
+    # addresses and strides of q, k and v, all in bytes: one multiple of 16 where all are
+    bits = args[13] | args[16] | args[19] | (args[14] | args[15] | args[17] | args[18] | args[20] | args[21]) * elt
+    if more:
+        bits |= more[0] | (more[1] | more[2]) * elt
+    return fn(int(backward), int(bits & 15 == 0), args[0], args[3], args[4], args[5], args[9], args[10], args[11], args[12])
 
 
 def diff_attention(args, out, lse, workspace, stream=LEGACY_STREAM):

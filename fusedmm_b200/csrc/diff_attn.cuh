@@ -50,11 +50,14 @@ struct AttnParams {
    int units, unit_blocks, slot_heads;  // head units of QB heads; warps (blocks) that share them; slots of a warp across units
    // the walks on the matrix units: kv heads of a unit, query heads of each of them, units that share a kv head
    int unit_kv, unit_heads, head_blocks;
-   // ... and the two gathered arrays there: bytes from row to row and from head to head, elements of a row (of one map for
-   // the first); the groups of heads that a unit takes one after the other, and the heads of a group for one kv head (log2)
+   // the groups of heads that a unit takes one after the other, and the heads of a group for one kv head (log2)
+   int subs, kv_log2;
+   // the two gathered arrays (k and v, or q and do; packed copies of them where they are no vectors): bytes from row to row and
+   // from head to head, elements of a row (of one map for the first)
+   const char *a, *b;
    unsigned a_stride, b_stride;
    long long a_head, b_head;
-   int a_width, b_width, subs, kv_log2;
+   int a_width, b_width;
    long long piece, row_limit, pieces;
    int join_pieces;              // pieces a joining block looks after
    float *partial;
@@ -180,10 +183,10 @@ struct EdgeStream {
    }
 };
 
-// Rows of one gathered array as a slot's lanes hold them: vector t of a lane is `skip` elements behind vector t - 1.
-// EXACT: the lanes' vectors cover the row and nothing else; RAGGED: vectors, some lanes past the row's end; PIECES: rows
-// that are no vectors.  Edges that are none read zeros from `zero_row`, so that nothing of theirs is touched and no lane
-// needs a branch.
+// Rows of one gathered array as a slot's lanes hold them: vector t of a lane is SKIP elements behind vector t - 1.
+// EXACT: the lanes' vectors cover the row and nothing else; RAGGED: vectors, some lanes past the row's end; PIECES: the walk's
+// own rows and its results are no vectors (what is gathered has been packed then).  Edges that are none read zeros from
+// `zero_row`, so that nothing of theirs is touched and no lane needs a branch.
 enum Form { PIECES = 0, RAGGED = 1, EXACT = 2 };
 static __device__ __align__(16) uint4 zero_row[64];
 
@@ -192,29 +195,38 @@ struct Gather {
    const char *base;
    unsigned stride;  // bytes
    int left;         // elements from the lane's first vector to the row's end
-   __device__ __forceinline__ Gather(const void *array, long long ld, long long offset, int x, int width)
-      : base(static_cast<const char *>(array) + (offset + x) * static_cast<long long>(sizeof(T))),
-        stride(static_cast<unsigned>(ld * static_cast<long long>(sizeof(T)))), left(width - x) {}
    template <int SKIP>
-   __device__ __forceinline__ void load(int id, uint4 (&r)[NV], int step) const
+   __device__ __forceinline__ void load(int id, uint4 (&r)[NV]) const
    {
       const T *row = reinterpret_cast<const T *>(base + static_cast<unsigned long long>(static_cast<unsigned>(id)) * stride);
       if (FORM == EXACT && id < 0) row = reinterpret_cast<const T *>(zero_row);
 #pragma unroll
       for (int t = 0; t < NV; t++) {
          if constexpr (FORM == EXACT) r[t] = ldg16(row + t * SKIP);
-         else r[t] = ld_row<T, FORM != PIECES>(row + t * SKIP, id >= 0 ? left - t * SKIP : 0, step);
+         else r[t] = ld_row<T, true>(row + t * SKIP, id >= 0 ? left - t * SKIP : 0, Elt<T>::W);
       }
    }
-   // a row of the walk itself: it is there
-   template <int SKIP>
-   __device__ __forceinline__ void load_pairs(long long row, F2 (&f)[NV][Elt<T>::W / 2], int step) const
-   {
-      const T *src = reinterpret_cast<const T *>(base + row * static_cast<long long>(stride));
-#pragma unroll
-      for (int t = 0; t < NV; t++) unpack_pairs<T>(ld_row<T, FORM != PIECES>(src + t * SKIP, left - t * SKIP, step), f[t]);
-   }
 };
+// the part of a lane that begins at element x: of the first array at a head and map, of the second at a head
+template <typename T, int NV, int FORM>
+__device__ __forceinline__ Gather<T, NV, FORM> gather_a(const AttnParams &p, int head, int map, int x)
+{
+   return {p.a + head * p.a_head + static_cast<long long>(map * p.a_width + x) * static_cast<long long>(sizeof(T)), p.a_stride, p.a_width - x};
+}
+template <typename T, int NV, int FORM>
+__device__ __forceinline__ Gather<T, NV, FORM> gather_b(const AttnParams &p, int head, int x)
+{
+   return {p.b + head * p.b_head + static_cast<long long>(x) * static_cast<long long>(sizeof(T)), p.b_stride, p.b_width - x};
+}
+
+// a row of the walk itself, likewise
+template <typename T, int NV, int FORM, int SKIP>
+__device__ __forceinline__ void load_own(const AttnParams &p, const void *array, long long offset, int x, int width, F2 (&f)[NV][Elt<T>::W / 2])
+{
+   const T *src = static_cast<const T *>(array) + offset + x;
+#pragma unroll
+   for (int t = 0; t < NV; t++) unpack_pairs<T>(ld_row<T, FORM != PIECES>(src + t * SKIP, width - x - t * SKIP, p.step), f[t]);
+}
 
 template <int N>
 __device__ __forceinline__ void unpair(const F2 (&f)[N], float (&o)[2 * N])
@@ -263,11 +275,11 @@ struct Forward {
       if (e0 + 32 * warp >= e1) return;
       const int kv = at.unit / (p.group / QB), head0 = at.unit * QB;
       const int x = at.in_half * W, y = at.in_slot * W;
-      const Gather<T, NV, FORM> kg(p.k, p.ldk, kv * p.hsk + at.half * p.d, x, p.d), vg(p.v, p.ldv, kv * p.hsv, y, p.dv);
+      const Gather<T, NV, FORM> kg = gather_a<T, NV, FORM>(p, kv, at.half, x), vg = gather_b<T, NV, FORM>(p, kv, y);
       F2 q[QB][NV][P];
 #pragma unroll
       for (int b = 0; b < QB; b++)
-         Gather<T, NV, FORM>(p.q, p.ldq, (head0 + b) * p.hsq + at.half * p.d, x, p.d).template load_pairs<KSKIP>(row, q[b], p.step);
+         load_own<T, NV, FORM, KSKIP>(p, p.q, row * p.ldq + (head0 + b) * p.hsq + at.half * p.d, x, p.d, q[b]);
       for (long long base = e0 + 32 * warp; base < e1; base += 32 * warps) {
          const int my_id = edges.take(p, base, e1, at.lane);
          const float my_bias = edges.bias;
@@ -279,8 +291,8 @@ struct Forward {
 #pragma unroll
             for (int i = 0; i < U; i++) {
                id[i] = __shfl_sync(FULL, my_id, first + i * at.edge_slots + at.edge_slot);
-               kg.template load<KSKIP>(id[i], kr[i], p.step);
-               vg.template load<VSKIP>(id[i], vr[i], p.step);
+               kg.template load<KSKIP>(id[i], kr[i]);
+               vg.template load<VSKIP>(id[i], vr[i]);
             }
             float score[QB][U];
 #pragma unroll
@@ -476,14 +488,14 @@ struct BackwardRows {
       if (e0 + 32 * warp >= e1) return;
       const int kv = at.unit / (p.group / QB), head0 = at.unit * QB;
       const int x = at.in_half * W, y = at.in_slot * W;
-      const Gather<T, NV, FORM> kg(p.k, p.ldk, kv * p.hsk + at.half * p.d, x, p.d), vg(p.v, p.ldv, kv * p.hsv, y, p.dv);
+      const Gather<T, NV, FORM> kg = gather_a<T, NV, FORM>(p, kv, at.half, x), vg = gather_b<T, NV, FORM>(p, kv, y);
       F2 q[QB][NV][P], dout[QB][NV][P];
       float lse[QB];
 #pragma unroll
       for (int b = 0; b < QB; b++) {
          lse[b] = __ldg(p.lse + (row * p.heads + head0 + b) * 2 + at.half);
-         Gather<T, NV, FORM>(p.q, p.ldq, (head0 + b) * p.hsq + at.half * p.d, x, p.d).template load_pairs<KSKIP>(row, q[b], p.step);
-         Gather<T, NV, FORM>(p.dout, p.ldo, (head0 + b) * p.hso, y, p.dv).template load_pairs<VSKIP>(row, dout[b], p.step);
+         load_own<T, NV, FORM, KSKIP>(p, p.q, row * p.ldq + (head0 + b) * p.hsq + at.half * p.d, x, p.d, q[b]);
+         load_own<T, NV, FORM, VSKIP>(p, p.dout, row * p.ldo + (head0 + b) * p.hso, y, p.dv, dout[b]);
       }
       for (long long base = e0 + 32 * warp; base < e1; base += 32 * warps) {
          const int my_id = edges.take(p, base, e1, at.lane);
@@ -496,8 +508,8 @@ struct BackwardRows {
 #pragma unroll
             for (int i = 0; i < U; i++) {
                id[i] = __shfl_sync(FULL, my_id, first + i * at.edge_slots + at.edge_slot);
-               kg.template load<KSKIP>(id[i], kr[i], p.step);
-               vg.template load<VSKIP>(id[i], vr[i], p.step);
+               kg.template load<KSKIP>(id[i], kr[i]);
+               vg.template load<VSKIP>(id[i], vr[i]);
             }
 #pragma unroll
             for (int i = 0; i < U; i++) {
@@ -639,8 +651,8 @@ struct BackwardColumns {
       const int kv = at.unit;
       const int x = at.in_half * W, y = at.in_slot * W;
       F2 k[NV][P], v[NV][P];
-      Gather<T, NV, FORM>(p.k, p.ldk, kv * p.hsk + at.half * p.d, x, p.d).template load_pairs<KSKIP>(col, k, p.step);
-      Gather<T, NV, FORM>(p.v, p.ldv, kv * p.hsv, y, p.dv).template load_pairs<VSKIP>(col, v, p.step);
+      load_own<T, NV, FORM, KSKIP>(p, p.k, col * p.ldk + kv * p.hsk + at.half * p.d, x, p.d, k);
+      load_own<T, NV, FORM, VSKIP>(p, p.v, col * p.ldv + kv * p.hsv, y, p.dv, v);
       for (long long base = e0 + 32 * warp; base < e1; base += 32 * warps) {
          const int my_id = edges.take(p, base, e1, at.lane);
          const float my_bias = edges.bias;
@@ -656,15 +668,15 @@ struct BackwardColumns {
             }
             for (int g = 0; g < p.group; g++) {
                const int head = kv * p.group + g;
-               const Gather<T, NV, FORM> qg(p.q, p.ldq, head * p.hsq + at.half * p.d, x, p.d), dg(p.dout, p.ldo, head * p.hso, y, p.dv);
+               const Gather<T, NV, FORM> qg = gather_a<T, NV, FORM>(p, head, at.half, x), dg = gather_b<T, NV, FORM>(p, head, y);
                uint4 qr[U][NV], dr[U][NV];
                float4 stat[U];
 #pragma unroll
                for (int i = 0; i < U; i++) {
                   stat[i] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
                   if (id[i] >= 0) stat[i] = __ldg(p.stats + (static_cast<long long>(id[i]) * p.heads + head) * 2 + at.half);
-                  qg.template load<KSKIP>(id[i], qr[i], p.step);
-                  dg.template load<VSKIP>(id[i], dr[i], p.step);
+                  qg.template load<KSKIP>(id[i], qr[i]);
+                  dg.template load<VSKIP>(id[i], dr[i]);
                }
 #pragma unroll
                for (int i = 0; i < U; i++) {

@@ -49,6 +49,31 @@ __global__ void __launch_bounds__(256) lam_sum_kernel(const float *in, long long
    }
 }
 
+// Rows that are no vectors (their width, stride or address is no multiple of 16 bytes), packed: [rows][heads][maps][packed width],
+// zeros behind the width.  Gathered as they are, such rows cost a load for each element at every edge (a cache of 220699 slots
+// of 4 x (2 x 97 + 97) in bf16: 2149 us); packing costs two passes over them once.  With `ids` row e of the result is
+// the row that edge e names, and `ids_out` names it: for few edges of a large cache.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_rows_kernel(const T *src, long long ld, long long hs, int heads, int maps, int width, int step,
+                                                        long long rows, const void *ids, int idx64, long long n, T *dst, int *ids_out)
+{
+   constexpr int W = Elt<T>::W;
+   const int vectors = (width + W - 1) / W, per_row = heads * maps * vectors;
+   const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, row = i / per_row;
+   if (row >= rows) return;
+   const int rest = static_cast<int>(i - row * per_row), x = rest % vectors * W, map = rest / vectors % maps, head = rest / vectors / maps;
+   long long from = row;
+   bool live = true;
+   if (ids) {
+      from = load_index(ids, idx64, row);
+      live = from >= 0 && from < n;
+      if (ids_out && rest == 0) ids_out[row] = live ? static_cast<int>(row) : -1;
+   }
+   uint4 v = make_uint4(0u, 0u, 0u, 0u);
+   if (live) v = ld_pieces(src + from * ld + head * hs + map * width + x, width - x, step < W ? step : W / 2);
+   reinterpret_cast<uint4 *>(dst)[i] = v;
+}
+
 // the bias of the edges in the order of the transposed pattern
 __global__ void __launch_bounds__(256) permute_bias_kernel(const float *bias, const int *t_edge, long long nnz, const void *t_rowptr,
                                                            int ptr64, long long n, float *out)
@@ -60,6 +85,9 @@ __global__ void __launch_bounds__(256) permute_bias_kernel(const float *bias, co
 }
 
 namespace {
+
+long long round256(long long b) { return (b + 255) / 256 * 256; }
+long long max_ll(long long a, long long b) { return a > b ? a : b; }
 
 enum Walk { FORWARD, ROWS, COLUMNS };
 
@@ -135,18 +163,79 @@ void apply(AttnParams &p, const Shape &s, char *scratch)
    p.long_row = reinterpret_cast<long long *>(scratch + (s.pieces * 2 * s.units * s.part_bytes + 255) / 256 * 256);
 }
 
-int launch(Walk w, int dtype, const Shape &s, AttnParams &p, cudaStream_t st)
+// Two gathered arrays packed: bytes, and where they lie.
+struct Packed {
+   long long rows = 0;
+   int heads = 0, a_width = 0, b_width = 0;
+   size_t elt = 2;
+   Packed(int dtype, long long rows_, int heads_, int d, int dv) : rows(rows_), heads(heads_), elt(dtype == DT_F32 ? 4 : 2)
+   {
+      const int w = dtype == DT_F32 ? 4 : 8;
+      a_width = (d + w - 1) / w * w;
+      b_width = (dv + w - 1) / w * w;
+   }
+   long long a_bytes() const { return round256(rows * heads * 2 * a_width * static_cast<long long>(elt)); }
+   long long bytes() const { return a_bytes() + round256(rows * heads * b_width * static_cast<long long>(elt)); }
+};
+
+template <typename T>
+void pack_array(const void *src, long long ld, long long hs, int heads, int maps, int width, int step, long long rows, const void *ids, int idx64,
+                long long n, void *dst, int *ids_out, cudaStream_t st)
 {
-   const long long b = dtype == DT_F32 ? 4 : 2;
-   const bool columns = w == COLUMNS;
-   p.a_stride = static_cast<unsigned>((columns ? p.ldq : p.ldk) * b);
-   p.b_stride = static_cast<unsigned>((columns ? p.ldo : p.ldv) * b);
-   p.a_head = (columns ? p.hsq : p.hsk) * b;
-   p.b_head = (columns ? p.hso : p.hsv) * b;
+   const long long vectors = rows * heads * maps * ((width + Elt<T>::W - 1) / Elt<T>::W);
+   if (vectors == 0) return;
+   pack_rows_kernel<T><<<static_cast<unsigned>((vectors + 255) / 256), 256, 0, st>>>(static_cast<const T *>(src), ld, hs, heads, maps, width, step, rows,
+                                                                                   ids, idx64, n, static_cast<T *>(dst), ids_out);
+}
+
+// The arrays a walk gathers: as they are, or (pack) packed into `room`; with by_edge the rows in the order of the edges, then
+// p.colidx becomes `room`'s list behind them.
+void set_gathered(AttnParams &p, int dtype, bool columns, bool pack, bool by_edge, char *room, cudaStream_t st)
+{
+   const long long elt = dtype == DT_F32 ? 4 : 2;
+   const void *a = columns ? p.q : p.k, *b = columns ? p.dout : p.v;
+   const long long lda = columns ? p.ldq : p.ldk, ha = columns ? p.hsq : p.hsk, ldb = columns ? p.ldo : p.ldv, hb = columns ? p.hso : p.hsv;
+   const int heads = columns ? p.heads : p.kv_heads;
+   p.a = static_cast<const char *>(a);
+   p.b = static_cast<const char *>(b);
+   p.a_stride = static_cast<unsigned>(lda * elt);
+   p.b_stride = static_cast<unsigned>(ldb * elt);
+   p.a_head = ha * elt;
+   p.b_head = hb * elt;
    p.a_width = p.d;
    p.b_width = p.dv;
-   p.subs = columns ? p.group / s.unit_heads : 1;
-   p.kv_log2 = columns ? s.unit_heads >> 1 : 0;  // 1, 2, 4 -> 0, 1, 2
+   if (!pack) return;
+   const Packed k(dtype, by_edge ? p.nnz : p.n, heads, p.d, p.dv);
+   char *pa = room, *pb = room + k.a_bytes();
+   int *ids = by_edge ? reinterpret_cast<int *>(room + k.bytes()) : nullptr;
+   const void *from = by_edge ? p.colidx : nullptr;
+   auto both = [&](auto zero) {
+      using T = decltype(zero);
+      pack_array<T>(a, lda, ha, heads, 2, p.d, p.step, k.rows, from, p.idx64, p.n, pa, ids, st);
+      pack_array<T>(b, ldb, hb, heads, 1, p.dv, p.step, k.rows, from, p.idx64, p.n, pb, nullptr, st);
+   };
+   if (dtype == DT_F32) both(0.0f);
+   else if (dtype == DT_BF16) both(__nv_bfloat16());
+   else both(__half());
+   p.a = pa;
+   p.b = pb;
+   p.a_width = k.a_width;
+   p.b_width = k.b_width;
+   p.a_head = 2 * k.a_width * elt;
+   p.b_head = k.b_width * elt;
+   p.a_stride = static_cast<unsigned>(heads * p.a_head);
+   p.b_stride = static_cast<unsigned>(heads * p.b_head);
+   if (by_edge) {
+      p.colidx = ids;
+      p.idx64 = 0;
+      p.n = p.nnz;
+   }
+}
+
+int launch(Walk w, int dtype, const Shape &s, AttnParams &p, cudaStream_t st)
+{
+   p.subs = w == COLUMNS ? p.group / s.unit_heads : 1;
+   p.kv_log2 = w == COLUMNS ? s.unit_heads >> 1 : 0;  // 1, 2, 4 -> 0, 1, 2
    int r = -1;
    if (w == FORWARD) r = dtype == DT_F32 ? walk_forward_f32(s.walk, p, st) : dtype == DT_BF16 ? walk_forward_bf16(s.walk, p, st) : walk_forward_f16(s.walk, p, st);
    if (w == ROWS) r = dtype == DT_F32 ? walk_rows_f32(s.walk, p, st) : dtype == DT_BF16 ? walk_rows_bf16(s.walk, p, st) : walk_rows_f16(s.walk, p, st);
@@ -186,14 +275,22 @@ struct Step {
    bool vector() const { return step * elt == 16; }
 };
 
-long long round256(long long b) { return (b + 255) / 256 * 256; }
-long long max_ll(long long a, long long b) { return a > b ? a : b; }
-
-long long walk_scratch(Walk w, int dtype, long long rows, long long edges, int heads, int kv_heads, int d, int dv, int sms)
+long long walk_scratch(Walk w, int dtype, bool vector, long long rows, long long edges, int heads, int kv_heads, int d, int dv, int sms)
 {
-   if (rows == 0) return 0;
-   return max_ll(choose_shape(w, dtype, true, rows, edges, heads, kv_heads, d, dv, sms).scratch_bytes(),
-                 choose_shape(w, dtype, false, rows, edges, heads, kv_heads, d, dv, sms).scratch_bytes());
+   return rows == 0 ? 0 : choose_shape(w, dtype, vector, rows, edges, heads, kv_heads, d, dv, sms).scratch_bytes();
+}
+
+// forward: packed rows of the cache or, where they are fewer, of the edges
+bool pack_by_edge(long long n, long long nnz) { return nnz < n; }
+long long forward_pack(int dtype, long long n, long long nnz, int kv_heads, int d, int dv)
+{
+   const bool by_edge = pack_by_edge(n, nnz);
+   return Packed(dtype, by_edge ? nnz : n, kv_heads, d, dv).bytes() + (by_edge ? round256(nnz * 4) : 0);
+}
+// backward: first of k and v, then of q and do in the same place
+long long backward_pack(int dtype, long long m, long long n, int heads, int kv_heads, int d, int dv)
+{
+   return max_ll(Packed(dtype, n, kv_heads, d, dv).bytes(), Packed(dtype, m, heads, d, dv).bytes());
 }
 
 // scratch of the backward pass in front of the walks': stats, dlam of every row, the sums of runs of rows,
@@ -211,15 +308,18 @@ using namespace fmm::attn;
 
 extern "C" {
 
-int64_t fusedmm_b200_diff_attention_workspace(int32_t backward, int32_t dtype, int64_t m, int64_t n, int64_t nnz,
+int64_t fusedmm_b200_diff_attention_workspace(int32_t backward, int32_t aligned, int32_t dtype, int64_t m, int64_t n, int64_t nnz,
                                               int32_t heads, int32_t kv_heads, int32_t d, int32_t dv)
 {
    if (int s = check_sizes(dtype, m, n, nnz, heads, kv_heads, d, dv)) return s;
    int sms = 0;
    if (int s = sm_count(&sms)) return s;
-   if (!backward) return walk_scratch(FORWARD, dtype, m, nnz, heads, kv_heads, d, dv, sms);
-   return backward_front(m, heads, nnz) + max_ll(walk_scratch(ROWS, dtype, m, nnz, heads, kv_heads, d, dv, sms),
-                                            walk_scratch(COLUMNS, dtype, n, nnz, heads, kv_heads, d, dv, sms));
+   const int width = dtype == DT_F32 ? 4 : 8;
+   const bool vector = aligned && d % width == 0 && dv % width == 0;
+   if (!backward) return walk_scratch(FORWARD, dtype, vector, m, nnz, heads, kv_heads, d, dv, sms) + (vector ? 0 : forward_pack(dtype, n, nnz, kv_heads, d, dv));
+   return backward_front(m, heads, nnz) + max_ll(walk_scratch(ROWS, dtype, vector, m, nnz, heads, kv_heads, d, dv, sms),
+                                                 walk_scratch(COLUMNS, dtype, vector, n, nnz, heads, kv_heads, d, dv, sms)) +
+          (vector ? 0 : backward_pack(dtype, m, n, heads, kv_heads, d, dv));
 }
 
 int fusedmm_b200_diff_attention(int32_t dtype, int32_t ptr_bits, int32_t idx_bits, int64_t m, int64_t n, int64_t nnz,
@@ -236,17 +336,17 @@ int fusedmm_b200_diff_attention(int32_t dtype, int32_t ptr_bits, int32_t idx_bit
    if (!rowptr || !q || !lam || !out || (nnz > 0 && !colidx) || (gathers && (!k || !v))) return FUSEDMM_B200_ERR_ARG;
    int sms = 0;
    if (int s = sm_count(&sms)) return s;
-   const long long need = walk_scratch(FORWARD, dtype, m, nnz, heads, kv_heads, d, dv, sms);
-   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256) return FUSEDMM_B200_ERR_ARG;
-   if (!on_device({rowptr, q, lam, out, lse, workspace, nnz > 0 ? colidx : nullptr, nnz > 0 ? bias : nullptr,
-                   gathers ? k : nullptr, gathers ? v : nullptr}))
-      return FUSEDMM_B200_ERR_ARG;
    if (n == 0) k = v = workspace;  // nothing is gathered, but copies of nothing want an address too
    Step step(dtype);
    step.with(q, ldq, hsq, d);
    step.with(k, ldk, hsk, d);
    step.with(v, ldv, hsv, dv);
    step.with(out, 0, 0, dv);
+   const int64_t need = fusedmm_b200_diff_attention_workspace(0, step.vector(), dtype, m, n, nnz, heads, kv_heads, d, dv);
+   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256) return FUSEDMM_B200_ERR_ARG;
+   if (!on_device({rowptr, q, lam, out, lse, workspace, nnz > 0 ? colidx : nullptr, nnz > 0 ? bias : nullptr,
+                   gathers ? k : nullptr, gathers ? v : nullptr}))
+      return FUSEDMM_B200_ERR_ARG;
    AttnParams p = {};
    p.rowptr = rowptr; p.colidx = colidx; p.ptr64 = ptr_bits == 64; p.idx64 = idx_bits == 64;
    p.m = m; p.n = n; p.nnz = nnz; p.bias = bias;
@@ -257,6 +357,8 @@ int fusedmm_b200_diff_attention(int32_t dtype, int32_t ptr_bits, int32_t idx_bit
    p.scale = static_cast<float>(scale);
    const Shape s = choose_shape(FORWARD, dtype, step.vector(), m, nnz, heads, kv_heads, d, dv, sms);
    apply(p, s, static_cast<char *>(workspace));
+   set_gathered(p, dtype, false, !step.vector() && gathers, pack_by_edge(n, nnz), static_cast<char *>(workspace) + s.scratch_bytes(),
+                static_cast<cudaStream_t>(stream));
    if (int r = launch(FORWARD, dtype, s, p, static_cast<cudaStream_t>(stream))) return r;
    return finish_call(stream);
 }
@@ -277,7 +379,17 @@ int fusedmm_b200_diff_attention_backward(int32_t dtype, int32_t ptr_bits, int32_
    if (!dlam || (m > 0 && (!rowptr || !q || !lam || !lse || !dout || !dq)) || (n > 0 && (!k || !v || !dk || !dv_out || !t_rowptr)) ||
        (nnz > 0 && (!colidx || !t_row || (bias && !t_edge))))
       return FUSEDMM_B200_ERR_ARG;
-   const int64_t need = fusedmm_b200_diff_attention_workspace(1, dtype, m, n, nnz, heads, kv_heads, d, dv);
+   const void *k0 = n == 0 ? workspace : k, *v0 = n == 0 ? workspace : v;  // nothing is gathered, but copies of nothing want an address too
+   const void *q0 = m == 0 ? workspace : q, *dout0 = m == 0 ? workspace : dout;
+   Step step(dtype);
+   step.with(q0, ldq, hsq, d);
+   step.with(k0, ldk, hsk, d);
+   step.with(v0, ldv, hsv, dv);
+   step.with(dout0, lddo, hsdo, dv);
+   step.with(dq, 0, 0, d);
+   step.with(dk, 0, 0, d);
+   step.with(dv_out, 0, 0, dv);
+   const int64_t need = fusedmm_b200_diff_attention_workspace(1, step.vector(), dtype, m, n, nnz, heads, kv_heads, d, dv);
    if (need < 0) return static_cast<int>(need);
    if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256) return FUSEDMM_B200_ERR_ARG;
    if (!on_device({m > 0 ? rowptr : nullptr, m > 0 ? q : nullptr, m > 0 ? lam : nullptr, m > 0 ? lse : nullptr, m > 0 ? dout : nullptr,
@@ -292,19 +404,11 @@ int fusedmm_b200_diff_attention_backward(int32_t dtype, int32_t ptr_bits, int32_
    float *row_dlam = reinterpret_cast<float *>(ws + round256(m * heads * 32));
    float *lam_part = reinterpret_cast<float *>(ws + round256(m * heads * 32) + round256(m * heads * 4));
    char *scratch = ws + backward_front(m, heads, nnz);
-   if (n == 0) k = v = workspace;  // nothing is gathered, but copies of nothing want an address too
-   if (m == 0) q = dout = workspace;
-   Step step(dtype);
-   step.with(q, ldq, hsq, d);
-   step.with(k, ldk, hsk, d);
-   step.with(v, ldv, hsv, dv);
-   step.with(dout, lddo, hsdo, dv);
-   step.with(dq, 0, 0, d);
-   step.with(dk, 0, 0, d);
-   step.with(dv_out, 0, 0, dv);
+   const long long walks = max_ll(walk_scratch(ROWS, dtype, step.vector(), m, nnz, heads, kv_heads, d, dv, sms),
+                                  walk_scratch(COLUMNS, dtype, step.vector(), n, nnz, heads, kv_heads, d, dv, sms));
    AttnParams p = {};
    p.bias = bias;
-   p.q = q; p.k = k; p.v = v; p.lam = lam; p.dout = dout;
+   p.q = q0; p.k = k0; p.v = v0; p.lam = lam; p.dout = dout0;
    p.ldq = ldq; p.hsq = hsq; p.ldk = ldk; p.hsk = hsk; p.ldv = ldv; p.hsv = hsv; p.ldo = lddo; p.hso = hsdo; p.ldlam = ldlam;
    p.lse = const_cast<float *>(lse);
    p.stats = reinterpret_cast<float4 *>(ws);
@@ -317,6 +421,7 @@ int fusedmm_b200_diff_attention_backward(int32_t dtype, int32_t ptr_bits, int32_
       p.rowptr = rowptr; p.colidx = colidx; p.idx64 = idx_bits == 64; p.m = m; p.n = n; p.out = dq;
       const Shape s = choose_shape(ROWS, dtype, step.vector(), m, p.nnz, heads, kv_heads, d, dv, sms);
       apply(p, s, scratch);
+      set_gathered(p, dtype, false, !step.vector(), false, scratch + walks, st);
       if (int r = launch(ROWS, dtype, s, p, st)) return r;
    }
    if (!ldlam) {
@@ -337,6 +442,7 @@ int fusedmm_b200_diff_attention_backward(int32_t dtype, int32_t ptr_bits, int32_
       }
       const Shape s = choose_shape(COLUMNS, dtype, step.vector(), n, p.nnz, heads, kv_heads, d, dv, sms);
       apply(p, s, scratch);
+      set_gathered(p, dtype, true, !step.vector(), false, scratch + walks, st);
       if (int r = launch(COLUMNS, dtype, s, p, st)) return r;
    }
    return finish_call(stream);

@@ -67,12 +67,10 @@ __device__ __forceinline__ void ldmatrix4_trans(unsigned (&r)[4], unsigned at)
    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
-// `there` bytes from global memory, zeros behind them (0: nothing is read)
-template <int BYTES>
+// `there` (0 or 16) bytes from global memory, zeros in the place of the others (0: nothing is read)
 __device__ __forceinline__ void copy_async(unsigned to, const void *from, int there)
 {
-   if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there) : "memory");
-   else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(there) : "memory");
+   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there) : "memory");
 }
 // v as the sum of two numbers of T, for two neighbours
 template <typename T>
@@ -156,34 +154,16 @@ struct Ring {
       const int key = CHUNKS >= 8 ? pair & 7 : (pair >> 1) & 3;
       return pair * ROW + ((chunk ^ key) << 4);
    }
-   __device__ __forceinline__ void setup(const AttnParams &p, const Lanes &l, int lane, const void *array_a, const void *array_b, int head)
+   __device__ __forceinline__ void setup(const AttnParams &p, const Lanes &l, int lane, int head)
    {
       const int x = lane % CHUNKS, pair = lane / CHUNKS, s = PER >= 2 ? pair & (l.slots - 1) : 0;
       const int map = x / (CHUNKS / 2), xa = (x % (CHUNKS / 2)) * 8, xb = x * 8;
-      a = static_cast<const char *>(array_a) + (head + s) * p.a_head + static_cast<long long>(map * p.a_width + xa) * sizeof(T);
-      b = static_cast<const char *>(array_b) + (head + s) * p.b_head + static_cast<long long>(xb) * sizeof(T);
+      a = p.a + (head + s) * p.a_head + static_cast<long long>(map * p.a_width + xa) * sizeof(T);
+      b = p.b + (head + s) * p.b_head + static_cast<long long>(xb) * sizeof(T);
       place = offset(pair, x);
       if constexpr (PER == 2) {
          a2 = a + (l.slots == 4 ? 2 * p.a_head : 0);
          b2 = b + (l.slots == 4 ? 2 * p.b_head : 0);
-      }
-   }
-
-   __device__ __forceinline__ void chunk_in(unsigned to, const T *from, int left, int step) const
-   {
-      if constexpr (FORM != PIECES) {
-         copy_async<16>(to, from, left > 0 ? 16 : 0);
-      } else {
-         if (step >= 4) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) copy_async<8>(to + 8 * i, left > 4 * i ? from + 4 * i : from, left > 4 * i ? 8 : 0);
-         } else if (step >= 2) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) copy_async<4>(to + 4 * i, left > 2 * i ? from + 2 * i : from, left > 2 * i ? 4 : 0);
-         } else {
-            const uint4 v = ld_pieces(from, left, 1);
-            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-         }
       }
    }
 
@@ -230,14 +210,14 @@ struct Ring {
             }
             // the pair's bits that change from round to round, as in offset()
             const unsigned at = fill + (place ^ (CHUNKS >= 8 ? ((i * PER) & 7) << 4 : 0)) + i * PER * ROW;
-            chunk_in(at, reinterpret_cast<const T *>(ra), here ? left_a : 0, p.step);
-            chunk_in(at + REGION, reinterpret_cast<const T *>(rb), here ? left_b : 0, p.step);
+            copy_async(at, ra, here && left_a > 0 ? 16 : 0);
+            copy_async(at + REGION, rb, here && left_b > 0 ? 16 : 0);
          }
          if constexpr (RECORDS) {
             const int pair = lane >> 1, s = (pair & (l.slots - 1)) + (sub << p.kv_log2);
             const int id = __shfl_sync(FULL, batch_id, off + (pair >> l.slots_log2));
             const unsigned row = id >= 0 ? id : 0;
-            copy_async<16>(fill + RECORD + lane * 16, records + static_cast<unsigned long long>(row) * (p.heads * 32u) + (s * 32 + (lane & 1) * 16),
+            copy_async(fill + RECORD + lane * 16, records + static_cast<unsigned long long>(row) * (p.heads * 32u) + (s * 32 + (lane & 1) * 16),
                            id >= 0 ? 16 : 0);
          }
       }
@@ -404,7 +384,7 @@ struct ForwardMma {
       l.set(at, p.unit_kv);
       kv0 = (at.unit / p.head_blocks) * p.unit_kv;
       heads.set(p, at, l, kv0);
-      ring.setup(p, l, at.lane, p.k, p.v, kv0);
+      ring.setup(p, l, at.lane, kv0);
    }
    static __device__ __forceinline__ void clear(State &s)
    {
@@ -626,7 +606,7 @@ struct BackwardRowsMma {
       l.set(at, p.unit_kv);
       kv0 = (at.unit / p.head_blocks) * p.unit_kv;
       heads.set(p, at, l, kv0);
-      ring.setup(p, l, at.lane, p.k, p.v, kv0);
+      ring.setup(p, l, at.lane, kv0);
    }
    static __device__ __forceinline__ void clear(State &s)
    {
@@ -838,7 +818,7 @@ struct BackwardColumnsMma {
       per_kv = p.unit_heads;
       pair_kv = l.pair_slot / per_kv;
       const long long head = kv0 * p.group;
-      ring.setup(p, l, at.lane, p.q, p.dout, kv0 * p.group);
+      ring.setup(p, l, at.lane, kv0 * p.group);
       ring.records = reinterpret_cast<const char *>(p.stats + head * 2);
    }
    static __device__ __forceinline__ void clear(State &s)

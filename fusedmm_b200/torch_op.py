@@ -138,7 +138,7 @@ def _attention_backward_cuda(rowptr, colidx, bias, q, k, v, lam, scale, lse, dou
     with _On(q.device) as on:
         dq, dk, dv = on.empty(q.shape, q.dtype), on.empty(k.shape, k.dtype), on.empty(v.shape, v.dtype)
         dlam = on.empty(lam.shape, torch.float32)
-        ws = on.scratch(api.diff_attention_workspace(True, args), "diff_attention_backward")
+        ws = on.scratch(api.diff_attention_workspace(True, args, dout.data_ptr(), *api._rows(dout, "dout")), "diff_attention_backward")
         _check(api.diff_attention_backward(args, q, k, v, lse, dout, (t_rowptr, t_row, t_edge), dq, dk, dv, dlam, ws, on.stream),
                "diff_attention_backward")
     return dq, dk, dv, dlam

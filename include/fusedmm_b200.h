@@ -554,9 +554,12 @@ int fusedmm_b200_qk_norm_rotary_backward(int32_t dtype, int64_t rows, int32_t hq
  * logarithms of the two maps' sums; may be NULL) are dense.  Long rows are cut, so that one row of many edges (a single
  * token's) fills the GPU.  n is below 2^31 - 1, m and nnz below 2^48.  (Row pointers that decrease or leave [0, nnz] give
  * wrong rows, but no access outside the arrays; fusedmm_b200_check_csr finds them.)
+ *
+ * Workspace: `aligned` says that the addresses and strides of all arrays of the call are multiples of 16 bytes; where they or
+ * the widths are not, the gathered rows are packed first and the workspace holds the packed ones.
  */
-int64_t fusedmm_b200_diff_attention_workspace(int32_t backward, int32_t dtype, int64_t m, int64_t n, int64_t nnz,
-                                              int32_t heads, int32_t kv_heads, int32_t d, int32_t dv);
+int64_t fusedmm_b200_diff_attention_workspace(int32_t backward, int32_t aligned, int32_t dtype, int64_t m, int64_t n,
+                                              int64_t nnz, int32_t heads, int32_t kv_heads, int32_t d, int32_t dv);
 int fusedmm_b200_diff_attention(int32_t dtype, int32_t ptr_bits, int32_t idx_bits, int64_t m, int64_t n, int64_t nnz,
                                 const void *rowptr, const void *colidx, const float *bias, int32_t heads, int32_t kv_heads,
                                 int32_t d, int32_t dv, const void *q, int64_t ldq, int64_t hsq, const void *k, int64_t ldk,

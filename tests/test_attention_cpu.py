@@ -77,12 +77,12 @@ def test_c_entries_check_their_arguments_first():
     """Statuses of calls that are wrong whatever the machine: -3 invalid argument, -4 beyond a limit."""
     lib = api.lib()
     ws = lib.fusedmm_b200_diff_attention_workspace
-    ws.restype, ws.argtypes = L, [I, I, L, L, L, I, I, I, I]
-    assert ws(0, 1, 4, 4, 8, 2, 1, 8, 8) == -3           # double
-    assert ws(0, 0, -1, 4, 8, 2, 1, 8, 8) == -3
-    assert ws(0, 0, 4, 4, 8, 3, 2, 8, 8) == -3           # heads no multiple of kv heads
-    assert ws(0, 0, 4, 4, 8, 2, 1, 129, 8) == -4
-    assert ws(0, 0, 4, 4, 8, 2, 1, 8, 257) == -4
+    ws.restype, ws.argtypes = L, [I, I, I, L, L, L, I, I, I, I]
+    assert ws(0, 1, 1, 4, 4, 8, 2, 1, 8, 8) == -3           # double
+    assert ws(0, 1, 0, -1, 4, 8, 2, 1, 8, 8) == -3
+    assert ws(0, 1, 0, 4, 4, 8, 3, 2, 8, 8) == -3           # heads no multiple of kv heads
+    assert ws(0, 1, 0, 4, 4, 8, 2, 1, 129, 8) == -4
+    assert ws(0, 1, 0, 4, 4, 8, 2, 1, 8, 257) == -4
     fwd = lib.fusedmm_b200_diff_attention
     fwd.restype, fwd.argtypes = I, list(api._ATTN_IN) + [P, P, P, L, P]
     good = dict(dtype=0, pb=32, ib=32, m=4, n=4, nnz=8, rp=256, ci=256, bias=None, h=2, kvh=1, d=8, dv=8, q=256, ldq=32, hsq=16, k=256,
