@@ -63,22 +63,32 @@ __device__ __forceinline__ void angle_of(const RotaryParams &p, const double (&p
    sincospif(static_cast<float>(half_turns - 2.0 * rint(half_turns * 0.5)), &s, &c);
 }
 
-// One unit: 2W elements in two vectors.  Unit u < pairs/W of the halves form holds elements [uW, uW+W) and
-// [P+uW, P+uW+W); of the interleaved form [2uW, 2uW+2W); behind the pairs units are consecutive vectors.
+// One unit: 2W elements in two vectors, W pairs.  Of the halves form unit u < pairs / W holds elements [uW, uW+W) and
+// [P+uW, P+uW+W), and units behind the pairs consecutive vectors; of the interleaved form every unit is two consecutive vectors.
 template <int W>
 struct Unit {
    int at[2];    // element index of the two vectors, -1: none
    int pair;     // first pair, -1: nothing to turn
-   __device__ __forceinline__ void place(const RotaryParams &p, int u)
+   bool whole;   // both vectors turn (interleaved pairs may end after the first)
+   __device__ __forceinline__ void place(const RotaryParams &p, int u, bool inter)
    {
-      const int up = p.pairs / W;
       pair = -1;
+      whole = true;
       at[0] = at[1] = -1;
+      if (u >= p.units) return;
+      if (inter && W > 1) {
+         at[0] = 2 * u * W;
+         at[1] = at[0] + W < p.d ? at[0] + W : -1;
+         if (u * W < p.pairs) pair = u * W;
+         whole = u * W + W <= p.pairs;
+         return;
+      }
+      const int up = p.pairs / W;
       if (u < up) {
          pair = u * W;
-         at[0] = p.interleaved ? 2 * u * W : u * W;
+         at[0] = p.interleaved ? 2 * u * W : u * W;  // (W = 1: both forms)
          at[1] = p.interleaved ? at[0] + W : p.pairs + u * W;
-      } else if (u < p.units) {
+      } else {
          at[0] = 2 * p.pairs + 2 * (u - up) * W;
          at[1] = at[0] + W < p.d ? at[0] + W : -1;
       }
@@ -87,12 +97,13 @@ struct Unit {
 
 // Turns a unit, back with BACK.  c, s: cosines and sines of its pairs, two to a register pair.
 template <int W, bool INTER, bool BACK>
-__device__ __forceinline__ void turn(F2 (&lo)[(W + 1) / 2], F2 (&hi)[(W + 1) / 2], const F2 (&c)[(W + 1) / 2], const F2 (&s)[(W + 1) / 2])
+__device__ __forceinline__ void turn(F2 (&lo)[(W + 1) / 2], F2 (&hi)[(W + 1) / 2], const F2 (&c)[(W + 1) / 2], const F2 (&s)[(W + 1) / 2], bool whole)
 {
    if constexpr (INTER && W > 1) {
       // the two vectors are consecutive: pair j is elements 2j, 2j + 1 of their 2W, one register pair
 #pragma unroll
       for (int j = 0; j < W; j++) {
+         if (j >= W / 2 && !whole) break;
          F2 &x = j < W / 2 ? lo[j % (W / 2)] : hi[j % (W / 2)];
          const float2 v = f2_parts(x), cc = f2_parts(c[j / 2]), ss = f2_parts(s[j / 2]);
          const float cj = j & 1 ? cc.y : cc.x, sj = BACK ? -(j & 1 ? ss.y : ss.x) : (j & 1 ? ss.y : ss.x);
@@ -114,22 +125,35 @@ __device__ __forceinline__ void turn(F2 (&lo)[(W + 1) / 2], F2 (&hi)[(W + 1) / 2
 template <typename T, int W>
 struct Unpacked {
    static constexpr int P = (W + 1) / 2;
-   uint4 r[2];  // (W = 1: the number's bits)
+   uint4 r[2];  // (W = 1: the number's bits; 8-byte vectors: the first half)
    __device__ __forceinline__ void load(const T *base, const Unit<W> &u, bool live)
    {
 #pragma unroll
       for (int s = 0; s < 2; s++) {
          const bool there = live && u.at[s] >= 0;
-         if constexpr (W == 1) r[s].x = there ? __float_as_uint(Elt<T>::up(base[u.at[s]])) : 0u;
-         else r[s] = there ? ldg16(base + u.at[s]) : make_uint4(0u, 0u, 0u, 0u);
+         if constexpr (W == 1) {
+            r[s].x = there ? __float_as_uint(Elt<T>::up(base[u.at[s]])) : 0u;
+         } else if constexpr (W * sizeof(T) == 8) {
+            const uint2 v = there ? __ldg(reinterpret_cast<const uint2 *>(base + u.at[s])) : make_uint2(0u, 0u);
+            r[s] = make_uint4(v.x, v.y, 0u, 0u);
+         } else r[s] = there ? ldg16(base + u.at[s]) : make_uint4(0u, 0u, 0u, 0u);
       }
    }
    __device__ __forceinline__ void unpack(F2 (&f)[2][P]) const
    {
 #pragma unroll
       for (int s = 0; s < 2; s++) {
-         if constexpr (W == 1) f[s][0] = f2(__uint_as_float(r[s].x), 0.0f);
-         else unpack_pairs<T>(r[s], f[s]);
+         if constexpr (W == 1) {
+            f[s][0] = f2(__uint_as_float(r[s].x), 0.0f);
+         } else if constexpr (W * sizeof(T) == 8) {
+            float a, b;
+            Elt<T>::unpack2(r[s].x, a, b);
+            f[s][0] = f2(a, b);
+            Elt<T>::unpack2(r[s].y, a, b);
+            f[s][1] = f2(a, b);
+         } else {
+            unpack_pairs<T>(r[s], f[s]);
+         }
       }
    }
 };
@@ -147,7 +171,8 @@ __device__ __forceinline__ void store_part(T *base, int at, const F2 (&f)[(W + 1
          o[2 * i] = v.x;
          o[2 * i + 1] = v.y;
       }
-      *reinterpret_cast<uint4 *>(base + at) = Elt<T>::pack(o);
+      if constexpr (W * sizeof(T) == 8) *reinterpret_cast<uint2 *>(base + at) = make_uint2(Elt<T>::pack2(o[0], o[1]), Elt<T>::pack2(o[2], o[3]));
+      else *reinterpret_cast<uint4 *>(base + at) = Elt<T>::pack(o);
    }
 }
 
@@ -165,8 +190,10 @@ __device__ __forceinline__ float sum_over(float v, int lanes_log2)
 }
 
 // NU: units of a lane (1 with vectors).  INTER: pairs side by side.  AHEAD heads of a row are on their way from memory.
+// (Float forward: three blocks of a multiprocessor, 64 us for 100003 x 8 heads of 40 against 82 with two; the others want their
+// registers: 16384 rows of 20 heads backward 42 us, 52 with two blocks, 89 with three.)
 template <typename T, int W, int NU, int LOG2, bool INTER, bool BACKWARD>
-__global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotaryParams p)
+__global__ void __launch_bounds__(ROT_THREADS, sizeof(T) == 4 && !BACKWARD ? 3 : 1) rotary_kernel(const RotaryParams p)
 {
    constexpr int P = (W + 1) / 2, AHEAD = NU > 1 ? 1 : ROT_AHEAD;
    __shared__ float sums[BACKWARD ? ROT_THREADS * NU * 2 * W : 1];
@@ -174,7 +201,7 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotaryParams 
    const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x >> lanes_log2, slots = ROT_THREADS >> lanes_log2;
    Unit<W> unit[NU];
 #pragma unroll
-   for (int i = 0; i < NU; i++) unit[i].place(p, lane + i * 32);
+   for (int i = 0; i < NU; i++) unit[i].place(p, lane + i * 32, INTER);
    F2 dw[BACKWARD ? 2 : 1][NU][2][P] = {};
    const float inv_d = 1.0f / p.d;
    // the block's part of the heads
@@ -222,7 +249,7 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotaryParams 
                   float cc[2] = {1.0f, 1.0f}, ss[2] = {0.0f, 0.0f};
 #pragma unroll
                   for (int o = 0; o < (W == 1 ? 1 : 2); o++)
-                     if (unit[i].pair >= 0) angle_of(p, pos, unit[i].pair + 2 * j + o, cc[o], ss[o]);
+                     if (unit[i].pair >= 0 && unit[i].pair + 2 * j + o < p.pairs) angle_of(p, pos, unit[i].pair + 2 * j + o, cc[o], ss[o]);
                   c[i][j] = f2(cc[0], cc[1]);
                   s[i][j] = f2(ss[0], ss[1]);
                }
@@ -273,7 +300,7 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotaryParams 
 #pragma unroll
                            for (int j = 0; j < P; j++) v[i][o][j] = mul2(mul2(v[i][o][j], rr), w[i][o][j]);
                      }
-                     if (unit[i].pair >= 0) turn<W, INTER, false>(v[i][0], v[i][1], c[i], s[i]);
+                     if (unit[i].pair >= 0) turn<W, INTER, false>(v[i][0], v[i][1], c[i], s[i], unit[i].whole);
                      if (live) {
                         store_part<T, W>(y, unit[i].at[0], v[i][0]);
                         store_part<T, W>(y, unit[i].at[1], v[i][1]);
@@ -283,7 +310,7 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotaryParams 
                   F2 dots = 0;
 #pragma unroll
                   for (int i = 0; i < NU; i++) {
-                     if (unit[i].pair >= 0) turn<W, INTER, true>(g[i][0], g[i][1], c[i], s[i]);
+                     if (unit[i].pair >= 0) turn<W, INTER, true>(g[i][0], g[i][1], c[i], s[i], unit[i].whole);
                      if (p.norm) {
 #pragma unroll
                         for (int o = 0; o < 2; o++)
@@ -399,15 +426,14 @@ void launch_form(const RotaryParams &p, dim3 grid, cudaStream_t st)
    else rotary_kernel<T, W, NU, LOG2, false, BACKWARD><<<grid, ROT_THREADS, 0, st>>>(p);
 }
 
-// returns the number of blocks
+// returns the number of blocks; width: elements of a vector (16 or 8 bytes of them, or 1)
 template <typename T, bool BACKWARD>
-int launch(RotaryParams &p, bool vectors, int sm_count, cudaStream_t st)
+int launch(RotaryParams &p, int width, int sm_count, cudaStream_t st)
 {
-   constexpr int W = Elt<T>::W;
-   const int width = vectors ? W : 1;
+   constexpr int W = Elt<T>::W, HALF = sizeof(T) == 2 ? W / 2 : W;
    const int behind = (p.d - 2 * p.pairs) / width;
-   p.units = p.pairs / width + (behind + 1) / 2;
-   p.lanes_log2 = vectors ? ceil_log2(p.units) : 5;
+   p.units = p.interleaved && width > 1 ? (p.d / width + 1) / 2 : p.pairs / width + (behind + 1) / 2;
+   p.lanes_log2 = width > 1 ? ceil_log2(p.units) : 5;
    p.splits = choose_splits(p, sm_count);
    const int slots = ROT_THREADS >> p.lanes_log2;
    const long long blocks = (p.rows + slots - 1) / slots;
@@ -415,7 +441,8 @@ int launch(RotaryParams &p, bool vectors, int sm_count, cudaStream_t st)
    long long cap = BACKWARD ? static_cast<long long>(sm_count) * ROT_BACKWARD_BLOCKS_PER_SM / p.splits : 0x7fffffffLL;
    cap = cap < 1 ? 1 : cap;
    const dim3 grid(static_cast<unsigned>(blocks < cap ? blocks : cap), p.splits);
-   if (!vectors) launch_form<T, 1, ROT_SCALAR_UNITS, 5, BACKWARD>(p, grid, st);
+   if (width == 1) launch_form<T, 1, ROT_SCALAR_UNITS, 5, BACKWARD>(p, grid, st);
+   else if (width < W) launch_form<T, HALF, 1, -1, BACKWARD>(p, grid, st);
    else if (p.lanes_log2 == 2) launch_form<T, W, 1, 2, BACKWARD>(p, grid, st);
    else if (p.lanes_log2 == 3) launch_form<T, W, 1, 3, BACKWARD>(p, grid, st);
    else if (p.lanes_log2 == 4) launch_form<T, W, 1, 4, BACKWARD>(p, grid, st);
@@ -463,25 +490,30 @@ int rotary_setup(RotaryParams &p, int32_t dtype, int64_t rows, int32_t hq, int32
    return 0;
 }
 
-bool rotary_vectors(const RotaryParams &p, int32_t dtype, bool backward)
+// Elements of the vectors the rows can be taken in: 16 bytes, for 16-bit types also 8, else 1.
+int rotary_width(const RotaryParams &p, int32_t dtype, bool backward)
 {
-   const int width = dtype == DT_F32 ? 4 : 8;
    const size_t elt = dtype == DT_F32 ? 4 : 2;
-   if (p.d % width || p.pairs % width) return false;
-   for (int i = 0; i < 2; i++) {
-      if (!p.heads[i]) continue;
-      if (!multiple(p.x[i], p.ldx[i], p.hsx[i], width, elt) || !multiple(p.y[i], 0, 0, width, elt)) return false;
-      if (backward && !multiple(p.dy[i], p.ldd[i], p.hsd[i], width, elt)) return false;
+   for (int width = dtype == DT_F32 ? 4 : 8; width >= 4; width /= 2) {
+      // pairs: whole vectors of halves; interleaved whole vectors
+      bool fits = p.d % width == 0 && (p.interleaved ? 2 * p.pairs % width == 0 : p.pairs % width == 0);
+      for (int i = 0; i < 2 && fits; i++) {
+         if (!p.heads[i]) continue;
+         fits = multiple(p.x[i], p.ldx[i], p.hsx[i], width, elt) && multiple(p.y[i], 0, 0, width, elt) &&
+                (!backward || multiple(p.dy[i], p.ldd[i], p.hsd[i], width, elt));
+      }
+      // (a lane takes one unit of 2 width elements: 32 of them hold 256 elements in vectors of 4 and more)
+      if (fits) return width;
    }
-   return true;
+   return 1;
 }
 
 template <bool BACKWARD>
-int rotary_launch(RotaryParams &p, int32_t dtype, bool vectors, int sm_count, cudaStream_t st)
+int rotary_launch(RotaryParams &p, int32_t dtype, int width, int sm_count, cudaStream_t st)
 {
-   if (dtype == DT_F32) return launch<float, BACKWARD>(p, vectors, sm_count, st);
-   if (dtype == DT_BF16) return launch<__nv_bfloat16, BACKWARD>(p, vectors, sm_count, st);
-   return launch<__half, BACKWARD>(p, vectors, sm_count, st);
+   if (dtype == DT_F32) return launch<float, BACKWARD>(p, width, sm_count, st);
+   if (dtype == DT_BF16) return launch<__nv_bfloat16, BACKWARD>(p, width, sm_count, st);
+   return launch<__half, BACKWARD>(p, width, sm_count, st);
 }
 
 }  // namespace
@@ -507,7 +539,7 @@ int fusedmm_b200_qk_norm_rotary(int32_t dtype, int64_t rows, int32_t hq, int32_t
    p.y[0] = q_out; p.y[1] = k_out;
    int sms = 0;
    if (int s = sm_count(&sms)) return s;
-   rotary_launch<false>(p, dtype, rotary_vectors(p, dtype, false), sms, static_cast<cudaStream_t>(stream));
+   rotary_launch<false>(p, dtype, rotary_width(p, dtype, false), sms, static_cast<cudaStream_t>(stream));
    return finish_call(stream);
 }
 
@@ -558,7 +590,7 @@ int fusedmm_b200_qk_norm_rotary_backward(int32_t dtype, int64_t rows, int32_t hq
    p.ldd[0] = lddq; p.ldd[1] = lddk; p.hsd[0] = hsdq; p.hsd[1] = hsdk;
    int sms = 0;
    if (int s = sm_count(&sms)) return s;
-   const int blocks = rotary_launch<true>(p, dtype, rotary_vectors(p, dtype, true), sms, st);
+   const int blocks = rotary_launch<true>(p, dtype, rotary_width(p, dtype, true), sms, st);
    if (p.dw_partial)
       rotary_dw_kernel<<<(2 * d + 31) / 32, 1024, 0, st>>>(p.dw_partial, blocks, d, dwq, dwk);
    return finish_call(stream);

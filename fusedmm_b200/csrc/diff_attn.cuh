@@ -59,7 +59,7 @@ struct AttnParams {
    long long a_head, b_head;
    int a_width, b_width;
    long long piece, row_limit, pieces;
-   int join_pieces;              // pieces a joining block looks after
+   int join_rows, join_pieces;   // a joining block looks after one row, or after so many pieces
    float *partial;
    long long *long_row;          // [pieces]: the long row that begins in a piece, or -1
 };
@@ -777,18 +777,50 @@ __device__ __forceinline__ float *part_at(const AttnParams &p, const Place &at, 
    return p.partial + (part * p.units + at.unit) * part_floats<Op, G>;
 }
 
-// the warps of a block that shared a row: warp 0 takes the others' states in order
+// the warps of a block that shared a row join their states by halves, in a fixed order
 template <typename Op, int G>
 __device__ __forceinline__ void join_warps(Op &op, const Place &at, float *shared)
 {
    constexpr int STRIDE = Op::LANE_FLOATS * 32;  // slots side by side, as in scratch
    float *mine = shared + (at.lane / G) * part_floats<Op, G>;
-   __syncthreads();
-   if (at.warp > 0) op.put(mine + (at.warp - 1) * STRIDE, at);
-   __syncthreads();
-   if (at.warp == 0)
-      for (int w = 1; w < JOINT_WARPS; w++) op.join_from(mine + (w - 1) * STRIDE, at);
+   for (int half = JOINT_WARPS / 2; half > 0; half /= 2) {
+      __syncthreads();
+      if (at.warp >= half && at.warp < 2 * half) op.put(mine + (at.warp - half) * STRIDE, at);
+      __syncthreads();
+      if (at.warp < half) op.join_from(mine + at.warp * STRIDE, at);
+   }
 }
+
+// The long rows a joining block looks after: the block's row, where there are fewer rows than pieces, or the rows that begin in
+// its pieces.
+struct LongRows {
+   long long at, end;
+   __device__ __forceinline__ LongRows(const AttnParams &p, long long group)
+   {
+      at = p.join_rows ? group : group * p.join_pieces;
+      end = p.join_rows ? group + 1 : at + p.join_pieces < p.pieces ? at + p.join_pieces : p.pieces;
+   }
+   // the next: the row, the piece it begins in, its parts
+   __device__ __forceinline__ bool next(const AttnParams &p, const Rows &rows, long long &u, long long &piece, long long &parts)
+   {
+      for (; at < end; at++) {
+         if (p.join_rows) {
+            u = at;
+            const long long fb = rows.items(u);
+            if (rows.items(u + 1) - fb <= p.row_limit) continue;
+            piece = fb / p.piece;
+         } else {
+            piece = at;
+            u = p.long_row[piece];
+            if (u < 0) continue;
+         }
+         parts = (rows.items(u + 1) - 1) / p.piece - piece + 1;
+         at++;
+         return true;
+      }
+      return false;
+   }
+};
 
 // TOGETHER: the warps of a block share every row (few, long rows), else each warp has a piece of its own.
 template <typename Op, int G, bool TOGETHER>
@@ -843,20 +875,18 @@ __global__ void __launch_bounds__((TOGETHER ? JOINT_WARPS : PIECE_WARPS) * 32, T
    if (teller) p.long_row[piece] = begun;
 }
 
-// The parts of the long rows that begin in this block's pieces; a row's parts go to the warps in runs, joined in order.
+// The parts of the long rows; a row's parts go to the warps in runs, joined in order.
 template <typename Op, int G>
 __global__ void __launch_bounds__(JOINT_WARPS * 32) join_kernel(const AttnParams p)
 {
    extern __shared__ __align__(16) float shared[];
    const int warp = threadIdx.x >> 5;
-   const long long group = blockIdx.x / p.unit_blocks;
-   const Place at = Place::make<G>(p, static_cast<int>(blockIdx.x - group * p.unit_blocks));
+   const Place at = Place::make<G>(p, static_cast<int>(blockIdx.x % p.unit_blocks));
    const Rows rows(p);
    Op op;
-   for (long long piece = group * p.join_pieces; piece < (group + 1) * p.join_pieces && piece < p.pieces; piece++) {
-      const long long u = p.long_row[piece];
-      if (u < 0) continue;
-      const long long last = (rows.items(u + 1) - 1) / p.piece, parts = last - piece + 1;
+   LongRows todo(p, blockIdx.x / p.unit_blocks);
+   long long u, piece, parts;
+   while (todo.next(p, rows, u, piece, parts)) {
       const long long each = (parts + JOINT_WARPS - 1) / JOINT_WARPS;
       Op::clear(op.s);
       for (long long i = warp * each; i < (warp + 1) * each && i < parts; i++)
@@ -878,10 +908,15 @@ struct WalkShape {
 // Lets a kernel have this much shared memory on the current device (kept by the runtime per kernel and device: asked once)
 bool allow_shared(const void *kernel, int bytes);
 
+inline unsigned join_blocks(const AttnParams &p)
+{
+   return static_cast<unsigned>((p.join_rows ? p.m : (p.pieces + p.join_pieces - 1) / p.join_pieces) * p.unit_blocks);
+}
+
 template <typename Op, int G>
 int launch_op(const AttnParams &p, bool together, cudaStream_t st)
 {
-   const int bytes = (JOINT_WARPS - 1) * 32 * Op::LANE_FLOATS * static_cast<int>(sizeof(float));
+   const int bytes = JOINT_WARPS / 2 * 32 * Op::LANE_FLOATS * static_cast<int>(sizeof(float));
    if (!allow_shared(reinterpret_cast<const void *>(join_kernel<Op, G>), bytes)) return -1;
    const long long jobs = p.pieces * p.unit_blocks;
    if (together) {
@@ -890,8 +925,7 @@ int launch_op(const AttnParams &p, bool together, cudaStream_t st)
    } else {
       walk_kernel<Op, G, false><<<static_cast<unsigned>((jobs + PIECE_WARPS - 1) / PIECE_WARPS), PIECE_WARPS * 32, 0, st>>>(p);
    }
-   const long long groups = (p.pieces + p.join_pieces - 1) / p.join_pieces;
-   join_kernel<Op, G><<<static_cast<unsigned>(groups * p.unit_blocks), JOINT_WARPS * 32, bytes, st>>>(p);
+   join_kernel<Op, G><<<join_blocks(p), JOINT_WARPS * 32, bytes, st>>>(p);
    return 0;
 }
 

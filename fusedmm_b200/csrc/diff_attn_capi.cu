@@ -142,7 +142,7 @@ Shape choose_shape(Walk w, int dtype, bool vector, long long rows, long long edg
    const bool few = rows * s.unit_blocks < 8LL * sms;
    s.walk.together = mean >= 256 || (few && mean >= 64);
    const long long lo = s.walk.together ? 256 : 128, hi = s.walk.together ? 8192 : 1024;
-   const long long jobs = static_cast<long long>(sms) * (s.walk.together ? 12 : 128);
+   const long long jobs = static_cast<long long>(sms) * (!s.walk.together ? 128 : s.walk.width ? 6 : 12);
    s.piece = (items * s.unit_blocks + jobs - 1) / jobs;
    s.piece = s.piece < lo ? lo : s.piece > hi ? hi : s.piece;
    for (;; s.piece *= 2) {
@@ -158,6 +158,7 @@ void apply(AttnParams &p, const Shape &s, char *scratch)
    p.units = s.units; p.unit_blocks = s.unit_blocks; p.slot_heads = s.slot_heads;
    p.unit_kv = s.unit_kv; p.unit_heads = s.unit_heads; p.head_blocks = s.head_blocks;
    p.piece = s.piece; p.row_limit = s.row_limit; p.pieces = s.pieces;
+   p.join_rows = s.walk.together && p.m <= s.pieces;
    p.join_pieces = s.pieces * s.unit_blocks <= 8192 ? 1 : 8;  // few pieces: their long rows side by side
    p.partial = reinterpret_cast<float *>(scratch);
    p.long_row = reinterpret_cast<long long *>(scratch + (s.pieces * 2 * s.units * s.part_bytes + 255) / 256 * 256);

@@ -999,16 +999,17 @@ struct BackwardColumnsMma {
 // ---------------------------------------------------------------------------------------------------------------------
 // the walk
 // ---------------------------------------------------------------------------------------------------------------------
-// the warps of a block that shared a row: warp 0 takes the others' states in order; the rings serve as the place
+// the warps of a block that shared a row join their states by halves; the rings serve as the place
 template <typename Op>
-__device__ __forceinline__ void join_ring_warps(Op &op, const Place &at, float *shared)
+__device__ __forceinline__ void join_ring_warps(Op &op, const Place &at, float *shared, int warps)
 {
    constexpr int STRIDE = Op::LANE_FLOATS * 32;
-   __syncthreads();
-   if (at.warp > 0) op.put(shared + (at.warp - 1) * STRIDE, at, -1);
-   __syncthreads();
-   if (at.warp == 0)
-      for (int w = 1; w < Op::Width::JOINT; w++) op.join_from(shared + (w - 1) * STRIDE, at);
+   for (int half = warps / 2; half > 0; half /= 2) {
+      __syncthreads();
+      if (at.warp >= half && at.warp < 2 * half) op.put(shared + (at.warp - half) * STRIDE, at, -1);
+      __syncthreads();
+      if (at.warp < half) op.join_from(shared + at.warp * STRIDE, at);
+   }
 }
 
 // Where a sum came out infinite or as no number, a weight of 0 may have met an infinity or NaN of another row's edge in the same
@@ -1040,7 +1041,7 @@ __device__ __forceinline__ void ring_segment(Op &op, typename Op::Gathered &ring
       }
       if (TOGETHER) {
          ring.drain();
-         join_ring_warps(op, at, shared);
+         join_ring_warps(op, at, shared, Op::Width::JOINT);
       }
       if (!TOGETHER || at.warp == 0) {
          if (part < 0) op.finish(p, at, row, only);
@@ -1126,25 +1127,24 @@ ring_walk_kernel(const AttnParams p)
 
 // the parts of the long rows, as join_kernel
 template <typename Op>
-__global__ void __launch_bounds__(Op::Width::JOINT * 32) ring_join_kernel(const AttnParams p)
+__global__ void __launch_bounds__(512) ring_join_kernel(const AttnParams p)
 {
    extern __shared__ __align__(16) float shared[];
-   const int warp = threadIdx.x >> 5;
-   const long long group = blockIdx.x / p.unit_blocks;
-   const Place at = Place::make<32>(p, static_cast<int>(blockIdx.x - group * p.unit_blocks));
+   const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+   const Place at = Place::make<32>(p, static_cast<int>(blockIdx.x % p.unit_blocks));
    const Rows rows(p);
    Op op;
    typename Op::Gathered ring;
+   ring.ring = 0;
    op.setup(p, at, ring);
-   for (long long piece = group * p.join_pieces; piece < (group + 1) * p.join_pieces && piece < p.pieces; piece++) {
-      const long long u = p.long_row[piece];
-      if (u < 0) continue;
-      const long long last = (rows.items(u + 1) - 1) / p.piece, parts = last - piece + 1;
-      const long long each = (parts + Op::Width::JOINT - 1) / Op::Width::JOINT;
+   LongRows todo(p, blockIdx.x / p.unit_blocks);
+   long long u, piece, parts;
+   while (todo.next(p, rows, u, piece, parts)) {
+      const long long each = (parts + warps - 1) / warps;
       Op::clear(op.s);
       for (long long i = warp * each; i < (warp + 1) * each && i < parts; i++)
          op.join_from(part_at<Op, 32>(p, at, 2 * (piece + i) + (i == 0 ? 1 : 0)), at);
-      join_ring_warps(op, at, shared);
+      join_ring_warps(op, at, shared, warps);
       if (warp == 0) op.finish(p, at, u, -1);
    }
 }
@@ -1153,8 +1153,8 @@ template <typename Op>
 int launch_ring(const AttnParams &p, bool together, cudaStream_t st)
 {
    constexpr int RING = Op::Gathered::STAGES * Op::Gathered::STAGE;
-   constexpr int JOIN = (Op::Width::JOINT - 1) * 32 * Op::LANE_FLOATS * static_cast<int>(sizeof(float));
-   static_assert(JOIN <= Op::Width::JOINT * RING, "the rings serve as the place where warps meet");
+   constexpr int STATE = 32 * Op::LANE_FLOATS * static_cast<int>(sizeof(float));
+   static_assert(Op::Width::JOINT / 2 * STATE <= Op::Width::JOINT * RING, "the rings serve as the place where warps meet");
    const long long jobs = p.pieces * p.unit_blocks;
    if (together) {
       constexpr int bytes = Op::Width::JOINT * RING + RING_ALIGN;
@@ -1165,9 +1165,10 @@ int launch_ring(const AttnParams &p, bool together, cudaStream_t st)
       if (!allow_shared(reinterpret_cast<const void *>(ring_walk_kernel<Op, false>), bytes)) return -1;
       ring_walk_kernel<Op, false><<<static_cast<unsigned>((jobs + Op::Width::SOLO - 1) / Op::Width::SOLO), Op::Width::SOLO * 32, bytes, st>>>(p);
    }
-   if (!allow_shared(reinterpret_cast<const void *>(ring_join_kernel<Op>), JOIN)) return -1;
-   const long long groups = (p.pieces + p.join_pieces - 1) / p.join_pieces;
-   ring_join_kernel<Op><<<static_cast<unsigned>(groups * p.unit_blocks), Op::Width::JOINT * 32, JOIN, st>>>(p);
+   // one row of a long list has hundreds of parts: many warps for it; few where many rows have a few
+   const int join_warps = together ? 16 : 4;
+   if (!allow_shared(reinterpret_cast<const void *>(ring_join_kernel<Op>), 8 * STATE)) return -1;
+   ring_join_kernel<Op><<<join_blocks(p), join_warps * 32, join_warps / 2 * STATE, st>>>(p);
    return 0;
 }
 

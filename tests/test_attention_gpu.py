@@ -64,6 +64,15 @@ SHAPES = [
     (F16, 29, 60, 5, 555, 8, 8, 4, 4, False, False),
     (F16, 29, 60, 5, 0, 2, 1, 128, 1, True, False),
     (F16, 29, 60, 5, 0, 2, 1, 1, 200, True, False),
+    (BF16, 41, 60, 6, 600, 8, 1, 64, 64, True, False),     # more query heads of a kv head than a product holds
+    (BF16, 41, 60, 6, 600, 6, 2, 32, 64, True, True),      # three query heads: columns left over, three rounds of the columns
+    (BF16, 41, 60, 6, 0, 14, 2, 16, 32, False, False),
+    (BF16, 41, 60, 6, 600, 4, 2, 128, 256, True, False),
+    (BF16, 41, 60, 6, 600, 5, 5, 128, 100, False, False),
+    (BF16, 41, 60, 6, 600, 4, 4, 9, 18, True, False),      # packed rows, four kv heads at once
+    (F16, 41, 60, 6, 600, 8, 8, 12, 20, True, True),
+    (F32, 41, 60, 6, 600, 8, 2, 16, 32, True, False),
+    (F32, 41, 60, 6, 600, 2, 2, 4, 4, True, False),
 ]
 
 
@@ -89,6 +98,52 @@ def test_single_row(cuda_device, dtype, length):
     colidx = torch.randperm(n, generator=gen)[:length].to(torch.int32)
     t = make(gen, dtype, rowptr, colidx, 1, n, 8, 2, 64, 128)
     compare(t, 0.125, randn(gen, dtype, 1, 8, 128).cuda())
+
+
+@pytest.mark.parametrize("dtype,d,dv", [(BF16, 33, 47), (F16, 20, 36), (F32, 7, 9)])
+@pytest.mark.parametrize("n", [300, 40000])
+def test_rows_that_are_no_vectors_of_small_and_large_caches(cuda_device, dtype, d, dv, n):
+    """They are packed first: all rows of a small cache, the listed ones of a large one."""
+    gen = gen_of(n + d)
+    rowptr = torch.tensor([0, 700, 700, 1500], dtype=torch.int32)
+    colidx = torch.randint(-1, n + 1, (1500,), generator=gen).to(torch.int64)
+    t = make(gen, dtype, rowptr, colidx, 3, n, 4, 2, d, dv, bias=True)
+    want = attention_reference(t["rowptr"], t["colidx"], t["bias"], t["q"], t["k"], t["v"], t["lam"], 0.2)
+    out, lse = torch_op.diff_attention(t["rowptr"], t["colidx"], t["q"], t["k"], t["v"], t["lam"], bias=t["bias"], scale=0.2, return_lse=True)
+    check(out, want["out"], "out")
+    check(lse, want["lse"], "lse")
+
+
+@pytest.mark.parametrize("dtype,heads,kvh,d,dv", [(BF16, 8, 2, 64, 128), (BF16, 4, 4, 128, 256), (F32, 2, 1, 32, 64), (F16, 3, 3, 16, 32)])
+def test_one_long_row(cuda_device, dtype, heads, kvh, d, dv):
+    """Hundreds of parts joined; the gradients too."""
+    gen = gen_of(77)
+    n, length = 3000, 60000
+    rowptr = torch.tensor([0, 0, length, length + 2], dtype=torch.int64)
+    colidx = torch.randint(0, n, (length + 2,), generator=gen, dtype=torch.int32)
+    t = make(gen, dtype, rowptr, colidx, 3, n, heads, kvh, d, dv)
+    compare(t, d ** -0.5, randn(gen, dtype, 3, heads, dv).cuda())
+
+
+def test_two_streams_at_once(cuda_device):
+    """Calls that run side by side have scratch of their own."""
+    gen = gen_of(21)
+    rowptr, colidx = random_pattern(gen, 2000, 1500, 20, torch.int64, torch.int32, hub=30000)
+    t = make(gen, BF16, rowptr, colidx, 2000, 1500, 8, 2, 64, 128)
+    u = make(gen, BF16, rowptr, colidx, 2000, 1500, 8, 2, 64, 128)
+    dout = randn(gen, BF16, 2000, 8, 128).cuda()
+    want = [run_all(x, 0.125, dout) for x in (t, u)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        got = []
+        for s, x in zip(streams, (t, u)):
+            with torch.cuda.stream(s):
+                got.append(run_all(x, 0.125, dout))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            for name in b:
+                assert torch.equal(a[name], b[name]), name
 
 
 def test_rows_of_very_different_lengths(cuda_device):
@@ -390,6 +445,12 @@ ROTARY = [
     (F16, 64, 5, 3, 80, 40, 2, torch.int32, False, True, True, F16),
     (F16, 64, 5, 3, 90, 21, 2, torch.int32, True, True, True, F16),
     (F16, 2000, 2, 1, 96, 16, 1, torch.int64, True, True, True, F32),
+    (BF16, 90, 3, 2, 40, 20, 1, F32, True, True, True, F32),      # interleaved pairs that end inside a unit
+    (BF16, 90, 3, 2, 40, 20, 2, F32, False, True, True, F32),     # halves of whole 8-byte vectors
+    (F16, 90, 1, 2, 44, 8, 1, torch.int32, True, True, False, F32),
+    (F32, 90, 1, 2, 24, 6, 1, torch.int32, True, True, True, F32),
+    (F16, 50, 2, 0, 252, 126, 1, torch.int64, False, True, True, F16),
+    (F32, 50, 2, 0, 252, 126, 1, torch.int64, True, True, True, F32),
 ]
 
 
