@@ -125,8 +125,9 @@ struct Lanes {
 // The ring of a warp: STAGES blocks of 16 pairs, each of two gathered rows of 2 DK elements (k of both maps and v, or q and
 // do), 16 biases and, where the walk wants them, 16 records of 32 bytes.  What a block costs beside its products is mostly
 // the addresses of its copies: everything that a lane's copies share is worked out once (Lane pointers, places).
-template <typename T, int DK, int FORM, int STAGES_, bool RECORDS>
+template <typename T, int DK, int FORM, int STAGES_, bool RECORDS, bool SINGLE_>
 struct Ring {
+   static constexpr bool SINGLE = SINGLE_;  // one group of heads: every edge lies in one block
    static constexpr int STAGES = STAGES_, ROW = 4 * DK, CHUNKS = DK / 4, REGION = 16 * ROW;
    static constexpr int BIAS = 2 * REGION, RECORD = BIAS + 64, USED = RECORD + (RECORDS ? 16 * 32 : 0);
    static constexpr int STAGE = (USED + ROW - 1) / ROW * ROW;  // rows are aligned to their size, so that chunks can be named by exclusive or
@@ -171,7 +172,7 @@ struct Ring {
    __device__ __forceinline__ void issue(const AttnParams &p, const Lanes &l, int lane)
    {
       const int per_log2 = 4 - l.slots_log2;
-      const int edge_block = p.subs == 1 ? issued : issued / p.subs, sub = p.subs == 1 ? 0 : issued - edge_block * p.subs;
+      const int edge_block = SINGLE ? issued : issued / p.subs, sub = SINGLE ? 0 : issued - edge_block * p.subs;
       const int e = edge_block << per_log2;  // from the run's start
       if (e < length) {
          const int off = e & 31;
@@ -190,7 +191,13 @@ struct Ring {
             left_b = p.b_width - x * 8;
          }
          if (PER >= 4 && on == 0) left_a = left_b = 0;  // a lane whose pairs are all of one slot
-         const long long sub_a = sub > 0 ? (sub << p.kv_log2) * p.a_head : 0, sub_b = sub > 0 ? (sub << p.kv_log2) * p.b_head : 0;
+         const char *la = a, *lb = b, *la2 = a2, *lb2 = b2;
+         if (!SINGLE && sub > 0) {
+            la += (sub << p.kv_log2) * p.a_head;
+            lb += (sub << p.kv_log2) * p.b_head;
+            la2 += (sub << p.kv_log2) * p.a_head;
+            lb2 += (sub << p.kv_log2) * p.b_head;
+         }
 #pragma unroll
          for (int i = 0; i < ROUNDS; i++) {
             const int pair = i * PER + pair0;
@@ -198,12 +205,8 @@ struct Ring {
             const bool live = id >= 0;
             const unsigned row = live ? id : 0;
             const bool here = PER >= 4 ? live : live && (on >> i & 1);
-            const char *ra = (PER == 2 && (i & 1) ? a2 : a) + static_cast<unsigned long long>(row) * p.a_stride;
-            const char *rb = (PER == 2 && (i & 1) ? b2 : b) + static_cast<unsigned long long>(row) * p.b_stride;
-            if (p.subs > 1) {
-               ra += sub_a;
-               rb += sub_b;
-            }
+            const char *ra = (PER == 2 && (i & 1) ? la2 : la) + static_cast<unsigned long long>(row) * p.a_stride;
+            const char *rb = (PER == 2 && (i & 1) ? lb2 : lb) + static_cast<unsigned long long>(row) * p.b_stride;
             if constexpr (PER == 1) {  // the slot is the round's
                ra += (i & (l.slots - 1)) * p.a_head;
                rb += (i & (l.slots - 1)) * p.b_head;
@@ -366,7 +369,7 @@ struct ForwardMma {
    using Cols = Columns<ONE>;
    static constexpr int N = Cols::N;
    static constexpr int DV = 2 * DK, TILES = DV / 8, LANE_FLOATS = 2 * TILES + 4;
-   using Gathered = Ring<T, DK, FORM, Budget<DK, WALK_FORWARD>::STAGES, false>;
+   using Gathered = Ring<T, DK, FORM, Budget<DK, WALK_FORWARD>::STAGES, false, true>;
    using Width = Budget<DK, WALK_FORWARD>;
    struct State {
       float acc[TILES][2];   // rows n = r: sums of weights times v, columns 8t + 2c, + 1
@@ -587,7 +590,7 @@ struct BackwardRowsMma {
    using Cols = Columns<ONE>;
    static constexpr int N = Cols::N;
    static constexpr int DV = 2 * DK, TILES = DK / 8, LANE_FLOATS = 4 * TILES + 2;
-   using Gathered = Ring<T, DK, FORM, Budget<DK, WALK_ROWS>::STAGES, false>;
+   using Gathered = Ring<T, DK, FORM, Budget<DK, WALK_ROWS>::STAGES, false, true>;
    using Width = Budget<DK, WALK_ROWS>;
    struct State {
       float acc[2][TILES][2];
@@ -796,10 +799,10 @@ struct BackwardRowsMma {
 // the unit).  dk and dv are [16 elements x 8] products over the pairs: the columns 0..3 take the upper and 4..7 the lower part
 // of the split ds (or weight) of the unit's kv heads.
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int DK, int FORM, bool>
+template <typename T, int DK, int FORM, bool SINGLE>
 struct BackwardColumnsMma {
    static constexpr int DV = 2 * DK, KT = DK / 16, VT = DV / 16, LANE_FLOATS = 4 * (2 * KT + VT);
-   using Gathered = Ring<T, DK, FORM, Budget<DK, WALK_COLUMNS>::STAGES, true>;
+   using Gathered = Ring<T, DK, FORM, Budget<DK, WALK_COLUMNS>::STAGES, true, SINGLE>;
    using Width = Budget<DK, WALK_COLUMNS>;
    struct State {
       float dk[2][KT][4], dv[VT][4];
@@ -860,8 +863,8 @@ struct BackwardColumnsMma {
       for (int e = e0; e < e1;) {
          const int edges = e >> per_log2;
          const int lo = e - (edges << per_log2), left = e1 - (edges << per_log2), hi = left < (1 << per_log2) ? left : 1 << per_log2;
-         for (int sub = 0; sub < p.subs; sub++) {
-            const int block = edges * p.subs + sub;
+         for (int sub = 0; sub < (SINGLE ? 1 : p.subs); sub++) {
+            const int block = SINGLE ? edges : edges * p.subs + sub;
             if (block != ring.current) ring.advance(p, l, at.lane);
             const unsigned slot = ring.slot;
             float s0[4], s1[4], dp[4], dp2[4];
@@ -963,22 +966,23 @@ struct BackwardColumnsMma {
       }
    }
 
+   // Tile t of a head's sums lies in the lanes as rows r (elements 16t + r) and r + 8, upper parts of the kv heads 2c, 2c + 1 at
+   // c < 2, lower parts at c + 2.  Those two lanes trade so that one has the elements 16t + r whole and the other 16t + 8 + r;
+   // then neighbouring r trade so that one has two consecutive elements of the first head and the other of the second.
    template <int TILES>
    __device__ __forceinline__ void write(const float (&f)[TILES][4], T *row, long long head_step, int width, float factor, int only)
    {
+      const bool low = l.c >= 2, odd = l.r & 1;
+      const int kv = 2 * (l.c & 1) + odd, y = (low ? 8 : 0) + (l.r & ~1);
+      const bool mine = only < 0 ? kv * per_kv < l.slots : kv == only;
+      T *to = row + kv * head_step + y;
 #pragma unroll
-      for (int t = 0; t < TILES; t++)
-#pragma unroll
-         for (int x = 0; x < 2; x++) {
-            // elements 16t + r and 16t + 8 + r; neighbouring r trade one so that each has two consecutive elements
-            const float a = factor * (f[t][x] + __shfl_xor_sync(FULL, f[t][x], 2));
-            const float b = factor * (f[t][2 + x] + __shfl_xor_sync(FULL, f[t][2 + x], 2));
-            const bool odd = l.r & 1;
-            const float got = __shfl_xor_sync(FULL, odd ? a : b, 4);
-            const int kv = 2 * l.c + x, y = 16 * t + (odd ? 8 + l.r - 1 : l.r);
-            if (l.c < 2 && (only < 0 ? kv * per_kv < l.slots : kv == only))
-               store_two<T, FORM>(row + kv * head_step + y, odd ? got : a, odd ? b : got, width - y);
-         }
+      for (int t = 0; t < TILES; t++) {
+         const float g0 = __shfl_xor_sync(FULL, low ? f[t][0] : f[t][2], 2), g1 = __shfl_xor_sync(FULL, low ? f[t][1] : f[t][3], 2);
+         const float v0 = factor * ((low ? f[t][2] : f[t][0]) + g0), v1 = factor * ((low ? f[t][3] : f[t][1]) + g1);
+         const float got = __shfl_xor_sync(FULL, odd ? v0 : v1, 4);
+         if (mine) store_two<T, FORM>(to + 16 * t, odd ? got : v0, odd ? v1 : got, width - y - 16 * t);
+      }
    }
    __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long col, int only)
    {
@@ -1049,7 +1053,7 @@ __device__ __forceinline__ void ring_segment(Op &op, typename Op::Gathered &ring
       }
       if (TOGETHER) __syncthreads();
    }
-   if (lost && !TOGETHER && p.subs == 1) ring.begin(p, op.l, at.lane, e1, run_end, -1);
+   if (lost && !TOGETHER && Op::Gathered::SINGLE) ring.begin(p, op.l, at.lane, e1, run_end, -1);
 }
 
 constexpr int RING_ALIGN = 512;  // the longest row of a ring
@@ -1097,7 +1101,7 @@ ring_walk_kernel(const AttnParams p)
       part_of(u, rows.begin(u), rows.begin(u + 1), run_begin, x);
       part_of(last - 1, rows.begin(last - 1), rows.begin(last), x, run_end);
       // (where a row's edges are taken once for each of several groups of heads, every row is a run of its own)
-      if (!TOGETHER && p.subs == 1) ring.begin(p, op.l, at.lane, run_begin, run_end, -1);
+      if (!TOGETHER && Op::Gathered::SINGLE) ring.begin(p, op.l, at.lane, run_begin, run_end, -1);
       // rows 31 at a time, their pointers one to a lane; rows with edges are found by their bits
       for (long long from = u; from < last; from += 31) {
          const int here = static_cast<int>(last - from < 31 ? last - from : 31);
@@ -1115,7 +1119,7 @@ ring_walk_kernel(const AttnParams p)
             const int i = __ffs(todo) - 1;
             todo &= todo - 1;
             const long long e0 = __shfl_sync(FULL, m0, i), e1 = __shfl_sync(FULL, m1, i), pt = __shfl_sync(FULL, part, i);
-            if (!TOGETHER && p.subs != 1) ring.begin(p, op.l, at.lane, e0, e1, -1);
+            if (!TOGETHER && !Op::Gathered::SINGLE) ring.begin(p, op.l, at.lane, e0, e1, -1);
             if (!Op::Width::AHEAD) op.fetch(p, from + i);
             ring_segment<Op, TOGETHER>(op, ring, p, at, shared, from + i, e0, e1, pt, todo ? from + __ffs(todo) - 1 : -1, run_end);
          }
@@ -1180,15 +1184,15 @@ int launch_mma_form(const WalkShape &s, const AttnParams &p, cudaStream_t st)
    return launch_ring<Op<T, DK, PIECES, ONE>>(p, s.together, st);
 }
 
-// ONES: the walk has a form of its own for four kv heads to a unit
-template <typename T, bool ONES, template <typename, int, int, bool> class Op>
+// The last parameter of a walk: over the rows, four kv heads to a unit; over the columns, one group of heads.
+template <typename T, bool ROWS, template <typename, int, int, bool> class Op>
 int launch_mma(const WalkShape &s, const AttnParams &p, cudaStream_t st)
 {
-   if (ONES && p.unit_kv == 4) {
-      if (s.width == 16) return launch_mma_form<T, 16, ONES, Op>(s, p, st);
-      if (s.width == 32) return launch_mma_form<T, 32, ONES, Op>(s, p, st);
-      if (s.width == 64) return launch_mma_form<T, 64, ONES, Op>(s, p, st);
-      if (s.width == 128) return launch_mma_form<T, 128, ONES, Op>(s, p, st);
+   if (ROWS ? p.unit_kv == 4 : p.subs == 1) {
+      if (s.width == 16) return launch_mma_form<T, 16, true, Op>(s, p, st);
+      if (s.width == 32) return launch_mma_form<T, 32, true, Op>(s, p, st);
+      if (s.width == 64) return launch_mma_form<T, 64, true, Op>(s, p, st);
+      if (s.width == 128) return launch_mma_form<T, 128, true, Op>(s, p, st);
    }
    if (s.width == 16) return launch_mma_form<T, 16, false, Op>(s, p, st);
    if (s.width == 32) return launch_mma_form<T, 32, false, Op>(s, p, st);
