@@ -23,6 +23,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "attn_common.cuh"
 
 namespace fmm {
@@ -905,8 +907,15 @@ struct WalkShape {
    bool together = false;
 };
 
-// Lets a kernel have this much shared memory on the current device (kept by the runtime per kernel and device: asked once)
-bool allow_shared(const void *kernel, int bytes);
+// Lets a kernel have this much shared memory on the current device.  The runtime keeps that per kernel and device, so it is asked
+// once for each (the devices behind the 64th every time).
+bool set_shared(const void *kernel, int bytes, std::atomic<unsigned long long> &devices);
+template <auto KERNEL>
+bool allow_shared(int bytes)
+{
+   static std::atomic<unsigned long long> devices{0};
+   return bytes <= 48 << 10 || set_shared(reinterpret_cast<const void *>(KERNEL), bytes, devices);
+}
 
 inline unsigned join_blocks(const AttnParams &p)
 {
@@ -917,10 +926,10 @@ template <typename Op, int G>
 int launch_op(const AttnParams &p, bool together, cudaStream_t st)
 {
    const int bytes = JOINT_WARPS / 2 * 32 * Op::LANE_FLOATS * static_cast<int>(sizeof(float));
-   if (!allow_shared(reinterpret_cast<const void *>(join_kernel<Op, G>), bytes)) return -1;
+   if (!allow_shared<join_kernel<Op, G>>(bytes)) return -1;
    const long long jobs = p.pieces * p.unit_blocks;
    if (together) {
-      if (!allow_shared(reinterpret_cast<const void *>(walk_kernel<Op, G, true>), bytes)) return -1;
+      if (!allow_shared<walk_kernel<Op, G, true>>(bytes)) return -1;
       walk_kernel<Op, G, true><<<static_cast<unsigned>(jobs), JOINT_WARPS * 32, bytes, st>>>(p);
    } else {
       walk_kernel<Op, G, false><<<static_cast<unsigned>((jobs + PIECE_WARPS - 1) / PIECE_WARPS), PIECE_WARPS * 32, 0, st>>>(p);

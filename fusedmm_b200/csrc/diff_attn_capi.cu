@@ -4,26 +4,20 @@
 #include "diff_attn.cuh"
 
 #include <climits>
-#include <mutex>
-#include <set>
-#include <utility>
 
 namespace fmm {
 namespace attn {
 
 constexpr int LAM_BLOCKS = 256;
 
-bool allow_shared(const void *kernel, int bytes)
+bool set_shared(const void *kernel, int bytes, std::atomic<unsigned long long> &devices)
 {
-   if (bytes <= 48 << 10) return true;
-   static std::mutex mu;
-   static std::set<std::pair<const void *, int>> *done = new std::set<std::pair<const void *, int>>;
    int dev = 0;
    if (cudaGetDevice(&dev) != cudaSuccess) return false;
-   std::lock_guard<std::mutex> lock(mu);
-   if (done->count({kernel, dev})) return true;
+   const unsigned long long bit = dev < 64 ? 1ULL << dev : 0;
+   if (devices.load(std::memory_order_relaxed) & bit) return true;
    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
-   done->insert({kernel, dev});
+   devices.fetch_or(bit, std::memory_order_relaxed);
    return true;
 }
 
@@ -107,6 +101,9 @@ Shape choose_shape(Walk w, int dtype, bool vector, long long rows, long long edg
    const int nk = 2 * ((d + width - 1) / width), nvv = (dv + width - 1) / width, need = nk > nvv ? nk : nvv;
    const int group = heads / kv_heads;
    int lane_floats;
+   // 16-bit types go to the matrix units: a window of 128 over 4096 rows, 8 heads on 2, d 64: forward 76 us, 204 on the ordinary
+   // units; 2^23 R-MAT edges, 4 heads of d 32: forward 1.13 and 1.51 ms, rows 1.47 and 1.92, columns 1.57 and 2.19.  Not half's
+   // backward walks: their factors p dP and ds have no bound that half's 65504 covers, and they are operands there.
    if (dtype == DT_BF16 || (dtype == DT_F16 && w == FORWARD)) {
       s.walk.width = need <= 4 ? 16 : need <= 8 ? 32 : need <= 16 ? 64 : 128;
       s.walk.form = !vector ? PIECES : d == s.walk.width && dv == 2 * d ? EXACT : RAGGED;
@@ -139,6 +136,11 @@ Shape choose_shape(Walk w, int dtype, bool vector, long long rows, long long edg
    }
    s.unit_blocks = s.units / s.slot_heads;
    const long long items = edges + ROW_ITEMS * rows, mean = edges / rows;
+   // The warps of a block share every row where rows are long, or too few to give each warp one: a row then has 8 warps from its
+   // first edge on (48 tokens over 262144 slots, 4 kv heads of d 64: 94 us, a piece to a warp 144).  Blocks for an SM: the rings
+   // fill an SM with one or two, and each part costs the join (the same tokens: 94 us with 6, 102 with 9, 104 with 12); the
+   // ordinary units' blocks are smaller (37 tokens over 84276 slots in float: 275 us with 12, 362 with 6).  Otherwise pieces are
+   // short, so that hub rows spread, but no shorter than 128 items: the search for the first row costs as much as some edges.
    const bool few = rows * s.unit_blocks < 8LL * sms;
    s.walk.together = mean >= 256 || (few && mean >= 64);
    const long long lo = s.walk.together ? 256 : 128, hi = s.walk.together ? 8192 : 1024;

@@ -1162,16 +1162,16 @@ int launch_ring(const AttnParams &p, bool together, cudaStream_t st)
    const long long jobs = p.pieces * p.unit_blocks;
    if (together) {
       constexpr int bytes = Op::Width::JOINT * RING + RING_ALIGN;
-      if (!allow_shared(reinterpret_cast<const void *>(ring_walk_kernel<Op, true>), bytes)) return -1;
+      if (!allow_shared<ring_walk_kernel<Op, true>>(bytes)) return -1;
       ring_walk_kernel<Op, true><<<static_cast<unsigned>(jobs), Op::Width::JOINT * 32, bytes, st>>>(p);
    } else {
       constexpr int bytes = Op::Width::SOLO * RING + RING_ALIGN;
-      if (!allow_shared(reinterpret_cast<const void *>(ring_walk_kernel<Op, false>), bytes)) return -1;
+      if (!allow_shared<ring_walk_kernel<Op, false>>(bytes)) return -1;
       ring_walk_kernel<Op, false><<<static_cast<unsigned>((jobs + Op::Width::SOLO - 1) / Op::Width::SOLO), Op::Width::SOLO * 32, bytes, st>>>(p);
    }
    // one row of a long list has hundreds of parts: many warps for it; few where many rows have a few
    const int join_warps = together ? 16 : 4;
-   if (!allow_shared(reinterpret_cast<const void *>(ring_join_kernel<Op>), 8 * STATE)) return -1;
+   if (!allow_shared<ring_join_kernel<Op>>(8 * STATE)) return -1;
    ring_join_kernel<Op><<<join_blocks(p), join_warps * 32, join_warps / 2 * STATE, st>>>(p);
    return 0;
 }
