@@ -15,10 +15,8 @@ namespace fmm {
 namespace attn {
 
 constexpr int TR_THREADS = 256, TR_WARPS = TR_THREADS / 32;
-// Edges of a tile: TR_THREADS * ROUNDS.  Short tiles fill the GPU where there are few edges (524288: 57 us a transposition with
-// 16 rounds, 44 with 4), long ones keep the table of digit counts small where there are many.
-constexpr int TR_SHORT = 4, TR_LONG = 16;
-constexpr long long TR_MANY = 4LL << 20;
+// Edges of a tile: TR_THREADS * TR_ROUNDS (524288 edges: 57 us a transposition with 16 rounds, 44 with 4; 2^23 edges: 564 and 453).
+constexpr int TR_ROUNDS = 4;
 constexpr int TR_DIGITS = 256;
 
 __device__ __forceinline__ long long load_int(const void *p, int is64, long long i)
@@ -45,14 +43,14 @@ __device__ __forceinline__ unsigned first_key(const SortParams &p, long long e)
    return c >= 0 && c < p.n ? static_cast<unsigned>(c) : static_cast<unsigned>(p.n);
 }
 
-template <bool FIRST, int ROUNDS>
+template <bool FIRST>
 __global__ void __launch_bounds__(TR_THREADS) sort_count_kernel(const SortParams p)
 {
    __shared__ unsigned count[TR_DIGITS];
    count[threadIdx.x] = 0;
    __syncthreads();
-   const long long base = static_cast<long long>(blockIdx.x) * TR_THREADS * ROUNDS;
-   for (int r = 0; r < ROUNDS; r++) {
+   const long long base = static_cast<long long>(blockIdx.x) * TR_THREADS * TR_ROUNDS;
+   for (int r = 0; r < TR_ROUNDS; r++) {
       const long long e = base + r * TR_THREADS + threadIdx.x;
       if (e >= p.nnz) break;
       const unsigned key = FIRST ? first_key(p, e) : p.key_in[e];
@@ -92,7 +90,7 @@ __global__ void __launch_bounds__(TR_THREADS) sort_scan_kernel(const SortParams 
    if (threadIdx.x == 0) p.totals[blockIdx.x] = carry;
 }
 
-template <bool FIRST, int ROUNDS>
+template <bool FIRST>
 __global__ void __launch_bounds__(TR_THREADS) sort_move_kernel(const SortParams p)
 {
    __shared__ unsigned place[TR_WARPS][TR_DIGITS];  // first the warp's counts, then where its next edge of the digit goes
@@ -100,11 +98,11 @@ __global__ void __launch_bounds__(TR_THREADS) sort_move_kernel(const SortParams 
    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
    for (int i = 0; i < TR_WARPS; i++) place[i][threadIdx.x] = 0;
    __syncthreads();
-   const long long base = (static_cast<long long>(blockIdx.x) * TR_THREADS + w * 32) * ROUNDS;
-   unsigned key[ROUNDS], rank[ROUNDS];
+   const long long base = (static_cast<long long>(blockIdx.x) * TR_THREADS + w * 32) * TR_ROUNDS;
+   unsigned key[TR_ROUNDS], rank[TR_ROUNDS];
    const unsigned lower = (1u << lane) - 1;
 #pragma unroll
-   for (int r = 0; r < ROUNDS; r++) {
+   for (int r = 0; r < TR_ROUNDS; r++) {
       const long long e = base + r * 32 + lane;
       const bool live = e < p.nnz;
       key[r] = !live ? 0u : FIRST ? first_key(p, e) : p.key_in[e];
@@ -136,7 +134,7 @@ __global__ void __launch_bounds__(TR_THREADS) sort_move_kernel(const SortParams 
    }
    __syncthreads();
 #pragma unroll
-   for (int r = 0; r < ROUNDS; r++) {
+   for (int r = 0; r < TR_ROUNDS; r++) {
       const long long e = base + r * 32 + lane;
       if (e >= p.nnz) continue;
       const unsigned to = place[w][(key[r] >> p.shift) & (TR_DIGITS - 1)] + rank[r];
@@ -188,18 +186,16 @@ __global__ void __launch_bounds__(256) transpose_rows_kernel(const unsigned *edg
 namespace {
 
 long long round256(long long b) { return (b + 255) / 256 * 256; }
-int sort_rounds(long long nnz) { return nnz < TR_MANY ? TR_SHORT : TR_LONG; }
-long long sort_tiles(long long nnz) { return (nnz + TR_THREADS * sort_rounds(nnz) - 1) / (TR_THREADS * sort_rounds(nnz)); }
+long long sort_tiles(long long nnz) { return (nnz + TR_THREADS * TR_ROUNDS - 1) / (TR_THREADS * TR_ROUNDS); }
 
-template <int ROUNDS>
 void sort_pass(const SortParams &p, cudaStream_t st)
 {
    const unsigned grid = static_cast<unsigned>(p.tiles);
-   if (p.shift == 0) sort_count_kernel<true, ROUNDS><<<grid, TR_THREADS, 0, st>>>(p);
-   else sort_count_kernel<false, ROUNDS><<<grid, TR_THREADS, 0, st>>>(p);
+   if (p.shift == 0) sort_count_kernel<true><<<grid, TR_THREADS, 0, st>>>(p);
+   else sort_count_kernel<false><<<grid, TR_THREADS, 0, st>>>(p);
    sort_scan_kernel<<<TR_DIGITS, TR_THREADS, 0, st>>>(p);
-   if (p.shift == 0) sort_move_kernel<true, ROUNDS><<<grid, TR_THREADS, 0, st>>>(p);
-   else sort_move_kernel<false, ROUNDS><<<grid, TR_THREADS, 0, st>>>(p);
+   if (p.shift == 0) sort_move_kernel<true><<<grid, TR_THREADS, 0, st>>>(p);
+   else sort_move_kernel<false><<<grid, TR_THREADS, 0, st>>>(p);
 }
 
 }  // namespace
@@ -249,8 +245,7 @@ int fusedmm_b200_csr_transpose(int32_t ptr_bits, int32_t idx_bits, int64_t m, in
       p.shift = shift;
       p.key_in = key[now]; p.edge_in = edge[now];
       p.key_out = key[now ^ 1]; p.edge_out = edge[now ^ 1];
-      if (sort_rounds(nnz) == TR_SHORT) sort_pass<TR_SHORT>(p, st);
-      else sort_pass<TR_LONG>(p, st);
+      sort_pass(p, st);
       now ^= 1;
    }
    // edges outside every row keep row 0; they are behind t_rowptr[n] and no reader reaches them
