@@ -22,7 +22,8 @@ namespace attn {
 // 205), and four take the registers of a quarter of the warps from float (100003 x 8 heads of 40: 67, 65, 63, 77 us).
 constexpr int ROT_AHEAD = 3;
 constexpr int ROT_THREADS = 256;
-constexpr int ROT_SCALAR_UNITS = 4;  // units of a lane in the element-wise form: 32 lanes x 4 units x 2 elements = 256
+// Units of a lane where a row in single elements or in twos has more than 32: 32 lanes x 4 units of 2 elements, or x 2 of 4, are 256.
+constexpr int ROT_SCALAR_UNITS = 4, ROT_PAIR_UNITS = 2;
 
 struct RotaryParams {
    const void *x[2];     // queries, keys
@@ -133,6 +134,8 @@ struct Unpacked {
          const bool there = live && u.at[s] >= 0;
          if constexpr (W == 1) {
             r[s].x = there ? __float_as_uint(Elt<T>::up(base[u.at[s]])) : 0u;
+         } else if constexpr (W * sizeof(T) == 4) {
+            r[s].x = there ? __ldg(reinterpret_cast<const unsigned *>(base + u.at[s])) : 0u;
          } else if constexpr (W * sizeof(T) == 8) {
             const uint2 v = there ? __ldg(reinterpret_cast<const uint2 *>(base + u.at[s])) : make_uint2(0u, 0u);
             r[s] = make_uint4(v.x, v.y, 0u, 0u);
@@ -145,6 +148,12 @@ struct Unpacked {
       for (int s = 0; s < 2; s++) {
          if constexpr (W == 1) {
             f[s][0] = f2(__uint_as_float(r[s].x), 0.0f);
+         } else if constexpr (W == 2 && sizeof(T) == 4) {
+            f[s][0] = f2(__uint_as_float(r[s].x), __uint_as_float(r[s].y));
+         } else if constexpr (W == 2) {
+            float a, b;
+            Elt<T>::unpack2(r[s].x, a, b);
+            f[s][0] = f2(a, b);
          } else if constexpr (W * sizeof(T) == 8) {
             float a, b;
             Elt<T>::unpack2(r[s].x, a, b);
@@ -171,7 +180,9 @@ __device__ __forceinline__ void store_part(T *base, int at, const F2 (&f)[(W + 1
          o[2 * i] = v.x;
          o[2 * i + 1] = v.y;
       }
-      if constexpr (W * sizeof(T) == 8) *reinterpret_cast<uint2 *>(base + at) = make_uint2(Elt<T>::pack2(o[0], o[1]), Elt<T>::pack2(o[2], o[3]));
+      if constexpr (W == 2 && sizeof(T) == 4) *reinterpret_cast<float2 *>(base + at) = make_float2(o[0], o[1]);
+      else if constexpr (W == 2) *reinterpret_cast<unsigned *>(base + at) = Elt<T>::pack2(o[0], o[1]);
+      else if constexpr (W * sizeof(T) == 8) *reinterpret_cast<uint2 *>(base + at) = make_uint2(Elt<T>::pack2(o[0], o[1]), Elt<T>::pack2(o[2], o[3]));
       else *reinterpret_cast<uint4 *>(base + at) = Elt<T>::pack(o);
    }
 }
@@ -189,13 +200,13 @@ __device__ __forceinline__ float sum_over(float v, int lanes_log2)
    return v;
 }
 
-// NU: units of a lane (1 with vectors).  INTER: pairs side by side.  AHEAD heads of a row are on their way from memory.
+// NU: units of a lane (1 with vectors of 16 or 8 bytes).  INTER: pairs side by side.  AHEAD heads of a row are on their way from memory.
 // (Float forward: three blocks of a multiprocessor, 64 us for 100003 x 8 heads of 40 against 82 with two; the others want their
 // registers: 16384 rows of 20 heads backward 42 us, 52 with two blocks, 89 with three.)
 template <typename T, int W, int NU, int LOG2, bool INTER, bool BACKWARD>
-__global__ void __launch_bounds__(ROT_THREADS, sizeof(T) == 4 && !BACKWARD ? 3 : 1) rotary_kernel(const RotaryParams p)
+__global__ void __launch_bounds__(ROT_THREADS, sizeof(T) == 4 && NU == 1 && !BACKWARD ? 3 : 1) rotary_kernel(const RotaryParams p)
 {
-   constexpr int P = (W + 1) / 2, AHEAD = NU > 1 ? 1 : ROT_AHEAD;
+   constexpr int P = (W + 1) / 2, AHEAD = NU > 2 ? 1 : ROT_AHEAD;
    __shared__ float sums[BACKWARD ? ROT_THREADS * NU * 2 * W : 1];
    const int lanes_log2 = LOG2 >= 0 ? LOG2 : p.lanes_log2, lanes = 1 << lanes_log2;
    const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x >> lanes_log2, slots = ROT_THREADS >> lanes_log2;
@@ -426,14 +437,14 @@ void launch_form(const RotaryParams &p, dim3 grid, cudaStream_t st)
    else rotary_kernel<T, W, NU, LOG2, false, BACKWARD><<<grid, ROT_THREADS, 0, st>>>(p);
 }
 
-// returns the number of blocks; width: elements of a vector (16 or 8 bytes of them, or 1)
+// returns the number of blocks; width: elements of a vector (16 or 8 bytes of them, 2 or 1)
 template <typename T, bool BACKWARD>
 int launch(RotaryParams &p, int width, int sm_count, cudaStream_t st)
 {
    constexpr int W = Elt<T>::W, HALF = sizeof(T) == 2 ? W / 2 : W;
    const int behind = (p.d - 2 * p.pairs) / width;
    p.units = p.interleaved && width > 1 ? (p.d / width + 1) / 2 : p.pairs / width + (behind + 1) / 2;
-   p.lanes_log2 = width > 1 ? ceil_log2(p.units) : 5;
+   p.lanes_log2 = p.units <= 32 ? ceil_log2(p.units) : 5;
    p.splits = choose_splits(p, sm_count);
    const int slots = ROT_THREADS >> p.lanes_log2;
    const long long blocks = (p.rows + slots - 1) / slots;
@@ -441,7 +452,10 @@ int launch(RotaryParams &p, int width, int sm_count, cudaStream_t st)
    long long cap = BACKWARD ? static_cast<long long>(sm_count) * ROT_BACKWARD_BLOCKS_PER_SM / p.splits : 0x7fffffffLL;
    cap = cap < 1 ? 1 : cap;
    const dim3 grid(static_cast<unsigned>(blocks < cap ? blocks : cap), p.splits);
-   if (width == 1) launch_form<T, 1, ROT_SCALAR_UNITS, 5, BACKWARD>(p, grid, st);
+   if (width == 1 && p.units > 32) launch_form<T, 1, ROT_SCALAR_UNITS, 5, BACKWARD>(p, grid, st);
+   else if (width == 1) launch_form<T, 1, 1, -1, BACKWARD>(p, grid, st);
+   else if (width == 2 && p.units > 32) launch_form<T, 2, ROT_PAIR_UNITS, 5, BACKWARD>(p, grid, st);
+   else if (width == 2) launch_form<T, 2, 1, -1, BACKWARD>(p, grid, st);
    else if (width < W) launch_form<T, HALF, 1, -1, BACKWARD>(p, grid, st);
    else if (p.lanes_log2 == 2) launch_form<T, W, 1, 2, BACKWARD>(p, grid, st);
    else if (p.lanes_log2 == 3) launch_form<T, W, 1, 3, BACKWARD>(p, grid, st);
@@ -490,11 +504,11 @@ int rotary_setup(RotaryParams &p, int32_t dtype, int64_t rows, int32_t hq, int32
    return 0;
 }
 
-// Elements of the vectors the rows can be taken in: 16 bytes, for 16-bit types also 8, else 1.
+// Elements of the vectors the rows can be taken in: 16 bytes, for 16-bit types also 8, else two, else 1.
 int rotary_width(const RotaryParams &p, int32_t dtype, bool backward)
 {
    const size_t elt = dtype == DT_F32 ? 4 : 2;
-   for (int width = dtype == DT_F32 ? 4 : 8; width >= 4; width /= 2) {
+   for (int width = dtype == DT_F32 ? 4 : 8; width >= 2; width /= 2) {
       // pairs: whole vectors of halves; interleaved whole vectors
       bool fits = p.d % width == 0 && (p.interleaved ? 2 * p.pairs % width == 0 : p.pairs % width == 0);
       for (int i = 0; i < 2 && fits; i++) {
@@ -502,7 +516,7 @@ int rotary_width(const RotaryParams &p, int32_t dtype, bool backward)
          fits = multiple(p.x[i], p.ldx[i], p.hsx[i], width, elt) && multiple(p.y[i], 0, 0, width, elt) &&
                 (!backward || multiple(p.dy[i], p.ldd[i], p.hsd[i], width, elt));
       }
-      // (a lane takes one unit of 2 width elements: 32 of them hold 256 elements in vectors of 4 and more)
+      // (a lane takes one unit of 2 width elements: 32 of them hold 256 elements in vectors of 4 and more; two units in twos)
       if (fits) return width;
    }
    return 1;
