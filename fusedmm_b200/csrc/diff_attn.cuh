@@ -201,12 +201,10 @@ struct Gather {
    __device__ __forceinline__ void load(int id, uint4 (&r)[NV]) const
    {
       const T *row = reinterpret_cast<const T *>(base + static_cast<unsigned long long>(static_cast<unsigned>(id)) * stride);
-      if (FORM == EXACT && id < 0) row = reinterpret_cast<const T *>(zero_row);
+      const T *zero = reinterpret_cast<const T *>(zero_row);
+      if (FORM == EXACT && id < 0) row = zero;
 #pragma unroll
-      for (int t = 0; t < NV; t++) {
-         if constexpr (FORM == EXACT) r[t] = ldg16(row + t * SKIP);
-         else r[t] = ld_row<T, true>(row + t * SKIP, id >= 0 ? left - t * SKIP : 0, Elt<T>::W);
-      }
+      for (int t = 0; t < NV; t++) r[t] = ldg16(FORM == EXACT || (id >= 0 && left > t * SKIP) ? row + t * SKIP : zero);
    }
 };
 // the part of a lane that begins at element x: of the first array at a head and map, of the second at a head

@@ -135,15 +135,19 @@ Shape choose_shape(Walk w, int dtype, bool vector, long long rows, long long edg
       s.part_bytes = static_cast<long long>(lane_floats) * s.walk.g * 4;
    }
    s.unit_blocks = s.units / s.slot_heads;
+   // The warps of a block share every row where there are too few long rows to give each warp one: 48 tokens over 262144 slots, 4
+   // kv heads of d 64: 103 us against 132, and 256 tokens 116 against 139; but 4096 rows of 512 edges, of which each warp can have
+   // some, 1.71 ms shared and 1.61 not.  Blocks for an SM: the rings fill an SM with one or two, and each part costs the join (the
+   // 48 tokens: 94 us with 6, 102 with 9, 104 with 12); the ordinary units' blocks are smaller (37 tokens over 84276 slots in
+   // float: 275 us with 12, 362 with 6).
+   // Otherwise a warp takes pieces of at most 128 items, or so many more that the table of parts stays short, and fewer where that
+   // leaves warps without work (7600 edges over 400 rows, forward, rows and columns: 75 us with 128, 38 with 32).  Rows longer than a
+   // piece (and a quarter, of short pieces) are cut: a hub row in one warp's hands is the walk's end (425984 R-MAT edges in float,
+   // all walks: 457 us with rows of up to 512 items whole, 341 now).
    const long long items = edges + ROW_ITEMS * rows, mean = edges / rows;
-   // The warps of a block share every row where rows are long, or too few to give each warp one: a row then has 8 warps from its
-   // first edge on (48 tokens over 262144 slots, 4 kv heads of d 64: 94 us, a piece to a warp 144).  Blocks for an SM: the rings
-   // fill an SM with one or two, and each part costs the join (the same tokens: 94 us with 6, 102 with 9, 104 with 12); the
-   // ordinary units' blocks are smaller (37 tokens over 84276 slots in float: 275 us with 12, 362 with 6).  Otherwise pieces are
-   // short, so that hub rows spread, but no shorter than 128 items: the search for the first row costs as much as some edges.
-   const bool few = rows * s.unit_blocks < 8LL * sms;
-   s.walk.together = mean >= 256 || (few && mean >= 64);
-   const long long lo = s.walk.together ? 256 : 128, hi = s.walk.together ? 8192 : 1024;
+   s.walk.together = rows * s.unit_blocks < 8LL * sms && mean >= 64;
+   const long long share = items * s.unit_blocks / (16LL * sms);
+   const long long lo = s.walk.together ? 256 : share < 32 ? 32 : share > 128 ? 128 : share, hi = s.walk.together ? 8192 : 1024;
    const long long jobs = static_cast<long long>(sms) * (!s.walk.together ? 128 : s.walk.width ? 6 : 12);
    s.piece = (items * s.unit_blocks + jobs - 1) / jobs;
    s.piece = s.piece < lo ? lo : s.piece > hi ? hi : s.piece;
@@ -151,7 +155,7 @@ Shape choose_shape(Walk w, int dtype, bool vector, long long rows, long long edg
       s.pieces = (items + s.piece - 1) / s.piece;
       if (s.pieces * 2 * s.units * s.part_bytes <= SCRATCH_LIMIT && s.pieces * s.unit_blocks < INT_MAX / 2) break;
    }
-   s.row_limit = s.walk.together ? s.piece : s.piece > 512 ? s.piece : 512;
+   s.row_limit = s.walk.together || s.piece >= 256 ? s.piece : s.piece < 64 ? 80 : s.piece + s.piece / 4;
    return s;
 }
 
