@@ -242,6 +242,8 @@ __device__ __forceinline__ void unpair(const F2 (&f)[N], float (&o)[2 * N])
 // ---------------------------------------------------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------------------------------------------------
+// U: edges of a slot on their way at once; BLOCKS: of an SM.  Float with U = 4 and three blocks, all walks of 425984 R-MAT edges
+// with 4 heads of d 32: 511 us, with U = 2 and four 584; forward 104 us now, 8.4 TB/s of gathered rows, most from L2.
 template <typename T, int G, int NV, int QB, int FORM>
 struct Forward {
    static constexpr int W = Elt<T>::W, P = W / 2, U = W == 4 && QB == 1 ? 4 : 2, BLOCKS = W == 4 ? (QB > 2 ? 2 : 3) : QB * NV * W > 16 ? 2 : 4;

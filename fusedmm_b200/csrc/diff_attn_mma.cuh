@@ -148,8 +148,8 @@ struct Ring {
 
    // Byte offset of a chunk of 8 elements of a pair.  The chunk is exchanged by bits of the pair, so that the 8 pairs that
    // ldmatrix reads at one chunk lie in 8 different groups of banks; offset(pair, chunk ^ x) = offset(pair, chunk) ^ (x << 4).
-   // (Rows 16 bytes longer do that too and save the exclusive ors, but the copies then end inside 32-byte sectors: window
-   // training's columns 349 us against 338.)
+   // (Rows 16 bytes longer do that too and save the exclusive ors, but the copies then end inside 32-byte sectors: columns 3 %
+   // slower for a window of 128 over 4096 rows at d 64.)
    static __device__ __forceinline__ unsigned offset(int pair, int chunk)
    {
       const int key = CHUNKS >= 8 ? pair & 7 : (pair >> 1) & 3;
@@ -354,15 +354,16 @@ template <int DK, int WALK>
 struct Budget {
    static constexpr int STAGES = DK == 16 ? 4 : DK == 32 ? 3 : 2;
    static constexpr int SOLO = DK == 128 ? 2 : 4, JOINT = DK >= 64 ? 4 : 8;
-   // The backward walks run faster with fewer warps and their registers: R-MAT training at d 32 columns 2.45 ms with four
-   // blocks, 2.19 with three, rows 1.84 and 1.57 (forward 1.26 and 1.30); window training at d 64 columns 419 us with three blocks,
-   // 375 with two, rows 102 and 98 (forward 82 and 89).
+   // The backward walks run faster with fewer warps and their registers: 2^23 R-MAT edges at d 32 columns 1.77 ms with four
+   // blocks, 1.57 with three, rows 1.69 and 1.47; a window of 128 over 4096 rows at d 64 columns 347 us with three blocks, 267 with
+   // two, rows 95 and 88.  (Forward with one block less and a stage more: 1.21 ms for 1.13, 81 us for 76.)
    static constexpr int BLOCKS = DK == 16 ? 4 : DK == 32 ? (WALK == WALK_FORWARD ? 4 : 3) : DK == 64 ? (WALK == WALK_FORWARD ? 3 : 2) : 3;
    static constexpr bool AHEAD = DK <= 32;  // a row's own operands are fetched during the row before (wider: no registers left)
 };
 
 // ---------------------------------------------------------------------------------------------------------------------
-// forward
+// forward.  2^23 R-MAT edges, 4 heads of d 32, bf16: 1.13 ms, 7.6 TB/s of gathered rows (hubs from L2), 310 instructions a block
+// of 16 pairs, issue slots 0.56 busy; 48 tokens over 262144 slots of 4 kv heads of d 64: 94 us, 5.7 TB/s from HBM.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DK, int FORM, bool ONE>
 struct ForwardMma {
@@ -798,6 +799,8 @@ struct BackwardRowsMma {
 // backward over the columns: dk and dv.  A pair is an edge with a query head; the columns of the products are (map, kv head of
 // the unit).  dk and dv are [16 elements x 8] products over the pairs: the columns 0..3 take the upper and 4..7 the lower part
 // of the split ds (or weight) of the unit's kv heads.
+// 2^23 R-MAT edges, 4 heads of d 32, bf16: 1.57 ms, 5.5 TB/s gathered, 402 instructions a block, bound by their latency (without
+// SINGLE, which leaves out the division of blocks among groups of heads, and with a longer exchange in write(): 518, 2.14 ms).
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DK, int FORM, bool SINGLE>
 struct BackwardColumnsMma {

@@ -516,7 +516,7 @@ int fusedmm_b200_release(void);
  * turned.  A pair that belongs to one axis has freq 0 on the others.  q is [rows][hq][d] with the strides ldq (rows) and
  * hsq (heads), k likewise; either may have no heads.  wq, wk have d elements of w_dtype (0, or dtype).  pos is
  * [rows][axes] of pos_type with the strides ldp, asp; freq is [axes][pairs], dense.  Angles are formed in double.  With
- * pairs 0 nothing is turned and pos, freq are not read.  q_out and k_out are dense.
+ * pairs 0 nothing is turned and pos, freq are not read.  q_out and k_out are dense and overlap no input.
  */
 int fusedmm_b200_qk_norm_rotary(int32_t dtype, int64_t rows, int32_t hq, int32_t hk, int32_t d, const void *q, int64_t ldq,
                                 int64_t hsq, const void *k, int64_t ldk, int64_t hsk, int32_t w_dtype, const void *wq,

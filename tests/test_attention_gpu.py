@@ -157,6 +157,19 @@ def test_rows_of_very_different_lengths(cuda_device):
         compare(t, 0.2, randn(gen, BF16, 11, heads, dv).cuda())
 
 
+@pytest.mark.parametrize("dtype,heads,kvh,d,dv", [(BF16, 4, 4, 16, 32), (F32, 2, 2, 8, 16), (F16, 2, 1, 20, 36)])
+def test_many_long_rows(cuda_device, dtype, heads, kvh, d, dv):
+    """More long rows than there are warps: each warp has rows of its own, cut at its pieces."""
+    gen = gen_of(15)
+    m, n = 2600, 400
+    lengths = torch.randint(60, 700, (m,), generator=gen)
+    rowptr = torch.zeros(m + 1, dtype=torch.int64)
+    rowptr[1:] = torch.cumsum(lengths, 0)
+    colidx = torch.randint(0, n, (int(rowptr[-1]),), generator=gen, dtype=torch.int32)
+    t = make(gen, dtype, rowptr, colidx, m, n, heads, kvh, d, dv)
+    compare(t, 0.2, randn(gen, dtype, m, heads, dv).cuda())
+
+
 def test_many_short_rows_and_columns_nobody_asks_for(cuda_device):
     gen = gen_of(6)
     rowptr, colidx = random_pattern(gen, 20000, 100, 2, torch.int64, torch.int32)
@@ -451,6 +464,14 @@ ROTARY = [
     (F32, 90, 1, 2, 24, 6, 1, torch.int32, True, True, True, F32),
     (F16, 50, 2, 0, 252, 126, 1, torch.int64, False, True, True, F16),
     (F32, 50, 2, 0, 252, 126, 1, torch.int64, True, True, True, F32),
+    (F16, 90, 3, 2, 234, 36, 1, torch.int64, False, True, True, F16),     # rows in twos, more of them than two a lane
+    (BF16, 90, 3, 2, 254, 127, 2, torch.int32, True, True, True, F32),
+    (F32, 90, 3, 2, 254, 2, 1, torch.int64, False, True, True, F32),
+    (BF16, 90, 3, 2, 46, 16, 2, F32, False, True, True, F32),             # in twos, one unit a lane
+    (F32, 90, 3, 2, 10, 3, 1, torch.int32, True, True, True, F32),
+    (F16, 90, 1, 2, 2, 1, 1, torch.int32, True, True, True, F32),
+    (BF16, 90, 3, 2, 40, 15, 2, F32, False, True, True, F32),             # single elements, fewer than the lanes
+    (F32, 90, 3, 2, 255, 127, 1, torch.int64, True, True, True, F32),     # and more
 ]
 
 
