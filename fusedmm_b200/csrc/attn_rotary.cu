@@ -505,6 +505,8 @@ int rotary_setup(RotaryParams &p, int32_t dtype, int64_t rows, int32_t hq, int32
 }
 
 // Elements of the vectors the rows can be taken in: 16 bytes, for 16-bit types also 8, else two, else 1.
+// (15688 rows of 20 heads of 234 in half: 98 us in twos, 290 in single elements; the bytes need 45.  50000 rows of 12 heads of 40 in
+// bf16 with 15 pairs, single elements: 116 us with the 32 lanes its 20 units take, 341 with four units to a lane.)
 int rotary_width(const RotaryParams &p, int32_t dtype, bool backward)
 {
    const size_t elt = dtype == DT_F32 ? 4 : 2;
