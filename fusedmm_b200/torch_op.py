@@ -16,6 +16,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import api
 
@@ -164,6 +165,8 @@ def _plain(*tensors):
     """True if these are ordinary CUDA tensors and nothing watches torch's operators: the call may then go straight to the
     library, without a round through the dispatcher (some 30 us)."""
     if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack():
+        return False
+    if forward_ad._current_level >= 0:  # tensors may have a tangent, which the dispatcher refuses
         return False
     for t in tensors:
         if t is not None and ((type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter) or not t.is_cuda):

@@ -137,3 +137,48 @@ def test_shapes_for_a_compiler():
         assert out.shape == (6, 4, 12) and out.dtype == torch.bfloat16 and lse.shape == (6, 4, 2)
         a, b = torch_op.qk_norm_rotary(torch.empty(6, 4, 8, device=dev), torch.empty(6, 2, 8, device=dev), eps=1e-6)
         assert a.shape == (6, 4, 8) and b.shape == (6, 2, 8)
+
+
+@pytest.fixture
+def stand_in(monkeypatch):
+    """Host tensors in the place of CUDA ones: the library calls of the forward pass are stood in for and log their inputs."""
+    calls = []
+
+    def rotary(q, k, pos, freq, q_weight, k_weight, eps, interleaved):
+        calls.append((q, k, pos, freq, q_weight, k_weight))
+        return torch.zeros_like(q), torch.zeros_like(q if k is None else k)
+
+    def attention(rowptr, colidx, bias, q, k, v, lam, scale, *_):
+        calls.append((rowptr, colidx, bias, q, k, v, lam))
+        return q.new_zeros(q.shape[0], q.shape[1], v.shape[2]), torch.zeros(q.shape[:3])
+
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True), raising=False)
+    monkeypatch.setattr(torch_op, "_rotary_cuda", rotary)
+    monkeypatch.setattr(torch_op, "_attention_forward", attention)
+    kernels = torch.library.Library("fusedmm_b200", "IMPL")
+    kernels.impl("qk_norm_rotary", rotary, "CPU")
+    kernels.impl("diff_attention", attention, "CPU")
+    kernels.impl("qk_norm_rotary", lambda *args: torch_op._Rotary.apply(*args), "AutogradCPU")
+    kernels.impl("diff_attention", lambda *args: torch_op._Attention.apply(*args), "AutogradCPU")
+    yield calls
+    kernels._destroy()
+
+
+def attention_call(**change):
+    a = {**good_attention(), **change}
+    return torch_op.diff_attention(a["rowptr"], a["colidx"], a["q"], a["k"], a["v"], a["lam"], scale=a["scale"])
+
+
+def test_forward_mode_is_refused(stand_in):
+    """There is no forward-mode derivative: a tangent is refused and not dropped, also without a gradient mode."""
+    from torch.autograd import forward_ad
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            dual = lambda *shape: forward_ad.make_dual(torch.ones(shape), torch.ones(shape))
+            with pytest.raises(NotImplementedError, match="jvp"):
+                torch_op.qk_norm_rotary(dual(3, 2, 8), eps=1e-6)
+            with pytest.raises(NotImplementedError, match="jvp"):
+                torch_op.qk_norm_rotary(torch.ones(3, 2, 8), q_weight=dual(8), eps=1e-6)
+            with pytest.raises(NotImplementedError, match="jvp"):
+                attention_call(lam=dual(4))
+    assert not torch_op.qk_norm_rotary(torch.ones(3, 2, 8), eps=1e-6).requires_grad
