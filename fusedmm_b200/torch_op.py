@@ -166,7 +166,8 @@ def _plain(*tensors):
     library, without a round through the dispatcher (some 30 us)."""
     if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack():
         return False
-    if forward_ad._current_level >= 0:  # tensors may have a tangent, which the dispatcher refuses
+    # under an open level of forward mode tensors may have a tangent, which the dispatcher refuses; a trace records operators
+    if forward_ad._current_level >= 0 or torch.jit.is_tracing():
         return False
     for t in tensors:
         if t is not None and ((type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter) or not t.is_cuda):

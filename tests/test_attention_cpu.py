@@ -182,3 +182,14 @@ def test_forward_mode_is_refused(stand_in):
             with pytest.raises(NotImplementedError, match="jvp"):
                 attention_call(lam=dual(4))
     assert not torch_op.qk_norm_rotary(torch.ones(3, 2, 8), eps=1e-6).requires_grad
+
+
+@pytest.mark.parametrize("trains", [False, True])
+def test_a_trace_holds_the_operators(stand_in, trains):
+    """torch.jit.trace records the operators, not the allocation of their results alone."""
+    a = good_attention()
+    for call, name, x in ((lambda q: torch_op.qk_norm_rotary(q, eps=1e-6), "fusedmm_b200::qk_norm_rotary", torch.ones(3, 2, 8)),
+                          (lambda q: torch_op.diff_attention(a["rowptr"], a["colidx"], q, a["k"], a["v"], a["lam"], scale=1.0),
+                           "fusedmm_b200::diff_attention", torch.ones(4, 4, 2, 8))):
+        nodes = [n.kind() for n in torch.jit.trace(call, (x.requires_grad_(trains),), check_trace=False).graph.nodes()]
+        assert name in nodes and not any(n.startswith(("aten::", "^")) for n in nodes), nodes
