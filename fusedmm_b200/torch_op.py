@@ -162,15 +162,15 @@ def _dense_rows(t):
 
 
 def _plain(*tensors):
-    """True if these are ordinary CUDA tensors and nothing watches torch's operators: the call may then go straight to the
-    library, without a round through the dispatcher (some 30 us)."""
+    """True if these are ordinary CUDA tensors (none that stores its numbers negated) and nothing watches torch's operators:
+    the call may then go straight to the library, without a round through the dispatcher (some 30 us)."""
     if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack():
         return False
     # under an open level of forward mode tensors may have a tangent, which the dispatcher refuses; a trace records operators
     if forward_ad._current_level >= 0 or torch.jit.is_tracing():
         return False
     for t in tensors:
-        if t is not None and ((type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter) or not t.is_cuda):
+        if t is not None and ((type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter) or not t.is_cuda or t.is_neg()):
             return False
     return torch._C._functorch.peek_interpreter_stack() is None
 
@@ -187,7 +187,7 @@ class _Rotary(torch.autograd.Function):
         ctx.save_for_backward(q, k, pos, freq, q_weight, k_weight)
         ctx.args = eps, interleaved
         args = (q, k, pos, freq, q_weight, k_weight, eps, interleaved)
-        return _rotary_cuda(*args) if _plain(q) else _below(torch.ops.fusedmm_b200.qk_norm_rotary, *args)
+        return _rotary_cuda(*args) if _plain(*args[:6]) else _below(torch.ops.fusedmm_b200.qk_norm_rotary, *args)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -197,7 +197,8 @@ class _Rotary(torch.autograd.Function):
         if need[2] or need[3]:
             raise api.FusedMMError("qk_norm_rotary has no gradient for pos and freq")
         eps, interleaved = ctx.args
-        run = _rotary_backward_cuda if _plain(q, dq_out) else torch.ops.fusedmm_b200.qk_norm_rotary_backward
+        plain = _plain(q, k, pos, freq, q_weight, k_weight, dq_out, dk_out)
+        run = _rotary_backward_cuda if plain else torch.ops.fusedmm_b200.qk_norm_rotary_backward
         dq, dk, dwq, dwk = run(q, k, pos, freq, q_weight, k_weight, eps, interleaved, _dense_rows(dq_out),
                                None if k is None else _dense_rows(dk_out))
         return (dq if need[0] else None, dk if need[1] else None, None, None, dwq.to(q_weight.dtype) if need[4] else None,
@@ -207,7 +208,7 @@ class _Rotary(torch.autograd.Function):
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rowptr, colidx, bias, q, k, v, lam, scale, t_rowptr, t_row, t_edge):
-        if _plain(q):
+        if _plain(rowptr, colidx, bias, q, k, v, lam):
             out, lse = _attention_forward(rowptr, colidx, bias, q, k, v, lam, scale, True)
         else:
             out, lse = _below(torch.ops.fusedmm_b200.diff_attention, rowptr, colidx, bias, q, k, v, lam, scale, t_rowptr, t_row, t_edge)
@@ -223,7 +224,7 @@ class _Attention(torch.autograd.Function):
         need = ctx.needs_input_grad
         if need[2]:
             raise api.FusedMMError("diff_attention has no gradient for bias")
-        plain = _plain(q, dout)
+        plain = _plain(rowptr, colidx, bias, q, k, v, lam, lse, dout, t_rowptr, t_row, t_edge)
         if t_rowptr is None:
             t_rowptr, t_row, t_edge = (_transpose_cuda if plain else torch.ops.fusedmm_b200.csr_transpose)(rowptr, colidx, k.shape[0])
         run = _attention_backward_cuda if plain else torch.ops.fusedmm_b200.diff_attention_backward

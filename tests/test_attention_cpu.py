@@ -193,3 +193,17 @@ def test_a_trace_holds_the_operators(stand_in, trains):
                            "fusedmm_b200::diff_attention", torch.ones(4, 4, 2, 8))):
         nodes = [n.kind() for n in torch.jit.trace(call, (x.requires_grad_(trains),), check_trace=False).graph.nodes()]
         assert name in nodes and not any(n.startswith(("aten::", "^")) for n in nodes), nodes
+
+
+@pytest.mark.parametrize("trains", [False, True])
+def test_numbers_that_are_stored_negated(stand_in, trains):
+    """The imaginary part of a conjugate is a view that stores its numbers negated: the library gets the numbers themselves."""
+    z = torch.complex(torch.rand(3), 1 + torch.rand(3))
+    pos = z.conj().imag
+    assert pos.is_neg()
+    torch_op.qk_norm_rotary(torch.ones(3, 2, 8, requires_grad=trains), None, pos, torch.ones(1, 4, dtype=torch.float64))
+    got = stand_in[-1][2]
+    assert not got.is_neg() and torch.equal(got, -z.imag)
+    q = torch._neg_view(torch.ones(4, 4, 2, 8)).requires_grad_(trains)
+    attention_call(q=q)
+    assert not stand_in[-1][3].is_neg()
