@@ -151,9 +151,12 @@ Shape choose_shape(Walk w, int dtype, bool vector, long long rows, long long edg
    const long long jobs = static_cast<long long>(sms) * (!s.walk.together ? 128 : s.walk.width ? 6 : 12);
    s.piece = (items * s.unit_blocks + jobs - 1) / jobs;
    s.piece = s.piece < lo ? lo : s.piece > hi ? hi : s.piece;
+   // One piece is the least there is, whatever its scratch (4097 units of 16 KB are above the limit); a warp counts the edges of a
+   // piece in 32 bits.  (check_sizes keeps items * heads below 2^56, so that nothing here passes 63 bits.)
    for (;; s.piece *= 2) {
       s.pieces = (items + s.piece - 1) / s.piece;
-      if (s.pieces * 2 * s.units * s.part_bytes <= SCRATCH_LIMIT && s.pieces * s.unit_blocks < INT_MAX / 2) break;
+      const bool fits = s.pieces * 2 * s.units * s.part_bytes <= SCRATCH_LIMIT;
+      if ((fits || s.pieces == 1 || s.piece >= 1 << 30) && s.pieces * s.unit_blocks < INT_MAX / 2) break;
    }
    s.row_limit = s.walk.together || s.piece >= 256 ? s.piece : s.piece < 64 ? 80 : s.piece + s.piece / 4;
    return s;
@@ -259,6 +262,7 @@ int check_sizes(int32_t dtype, int64_t m, int64_t n, int64_t nnz, int32_t heads,
    if (d > FUSEDMM_B200_ATTN_MAX_WIDTH / 2 || dv > FUSEDMM_B200_ATTN_MAX_WIDTH || heads > FUSEDMM_B200_ATTN_MAX_HEADS)
       return FUSEDMM_B200_ERR_LIMIT;
    if (m > (1LL << 48) || nnz > (1LL << 48) || n >= INT_MAX) return FUSEDMM_B200_ERR_LIMIT;
+   if (nnz + ROW_ITEMS * (m > n ? m : n) > (1LL << 56) / heads) return FUSEDMM_B200_ERR_LIMIT;  // (far beyond any memory)
    return 0;
 }
 

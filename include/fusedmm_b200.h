@@ -552,8 +552,8 @@ int fusedmm_b200_qk_norm_rotary_backward(int32_t dtype, int64_t rows, int32_t hq
  * q is [m][heads][2][d] with the strides ldq, hsq; k is [n][kv_heads][2][d]; v is [n][kv_heads][dv]; lam is
  * [m][heads] with the row stride ldlam, or [heads] with ldlam 0.  out [m][heads][dv] and lse [m][heads][2] (natural
  * logarithms of the two maps' sums; may be NULL) are dense.  Long rows are cut, so that one row of many edges (a single
- * token's) fills the GPU.  n is below 2^31 - 1, m and nnz below 2^48.  (Row pointers that decrease or leave [0, nnz] give
- * wrong rows, but no access outside the arrays; fusedmm_b200_check_csr finds them.)
+ * token's) fills the GPU.  n is below 2^31 - 1, m and nnz below 2^48, (nnz + 8 max(m, n)) heads below 2^56.  (Row pointers
+ * that decrease or leave [0, nnz] give wrong rows, but no access outside the arrays; fusedmm_b200_check_csr finds them.)
  *
  * Workspace: `aligned` says that the addresses and strides of all arrays of the call are multiples of 16 bytes; where they or
  * the widths are not, the gathered rows are packed first and the workspace holds the packed ones.

@@ -207,3 +207,10 @@ def test_numbers_that_are_stored_negated(stand_in, trains):
     q = torch._neg_view(torch.ones(4, 4, 2, 8)).requires_grad_(trains)
     attention_call(q=q)
     assert not stand_in[-1][3].is_neg()
+
+
+def test_sizes_whose_products_leave_64_bits():
+    ws = api.lib().fusedmm_b200_diff_attention_workspace
+    ws.restype, ws.argtypes = L, [I, I, I, L, L, L, I, I, I, I]
+    assert ws(0, 1, 0, 1 << 48, 4, 8, 65536, 1, 8, 8) == -4
+    assert ws(1, 1, 2, 4, 4, 1 << 48, 4096, 1, 8, 8) == -4
