@@ -140,6 +140,14 @@ __device__ __forceinline__ float exp2_fast(float x)
    return r;
 }
 
+// the smaller of the two, NaN if one of them is
+__device__ __forceinline__ float min_or_nan(float a, float b)
+{
+   float r;
+   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+   return r;
+}
+
 __device__ __forceinline__ uint4 ldg16(const void *p) { return __ldg(static_cast<const uint4 *>(p)); }
 
 // `left` elements (any number, also <= 0) of the vector at p; what lies behind them reads as zero.  `step`: the elements

@@ -5,6 +5,8 @@
 //   o_u = sum_e (p^0_e - lam p^1_e) v_v
 //   backward, with dP_e = do_u . v_v, D^c_u = sum_e p^c_e dP_e:  ds^0 = p^0 (dP - D^0), ds^1 = -lam p^1 (dP - D^1),
 //   dq^c_u = scale sum_e ds^c k^c_v, dk^c_v = scale sum_e ds^c q^c_u, dv_v = sum_e (p^0 - lam p^1) do_u, dlam_u = -D^1_u.
+//   The backward walks form p as exp(s - lse) / Z, where Z is the sum of these exponentials over the row, 1 but for rounding:
+//   lse is one 32-bit number, and next to a score of a mask's size (-1e9) the logarithm of the sum vanishes in it.
 //
 // Three walks of the same shape: the forward and the dq pass go over the rows and gather k and v; the dk, dv pass goes over
 // the columns of the transposed pattern and gathers q and do.  No atomics: every sum is taken in a fixed order.
@@ -45,7 +47,7 @@ struct AttnParams {
    void *out;                    // forward [m,H,Dv]; dq [m,H,2,D]; dk [n,Hk,2,D]
    void *out2;                   // dv [n,Hk,Dv]
    float *lse;                   // [m,H,2]
-   float4 *stats;                // [m,H,2]: lse and D of a map, its factor in the weight (1 or -lam)
+   float4 *stats;                // [m,H,2]: lse and D of a map, its factor in the weight (1 / Z or -lam / Z)
    float *dlam;                  // [m,H]
    int heads, kv_heads, group, d, dv, step;
    float scale;
@@ -153,6 +155,10 @@ __device__ __forceinline__ void get_pairs(const float *p, F2 (&f)[N])
       f[i + 1] = a.y;
    }
 }
+// exp(score - lse).  No score is above lse but for rounding, which next to a mask's size may be a power of thousands.
+__device__ __forceinline__ float weight_of(float score, float lse) { return exp2_fast(min_or_nan(score - lse, 0.0f) * LOG2E); }
+// 1 / Z; a row of no weights has no gradient
+__device__ __forceinline__ float reciprocal_total(float total) { return total == 0.0f ? 0.0f : 1.0f / total; }
 __device__ __forceinline__ F2 shfl_xor_pair(F2 v, int x) { return __shfl_xor_sync(FULL, v, x); }
 
 // 32 edges, one to a lane, fetched ahead: the ids of a row's next 32 edges, or of the next row's first, are under way while
@@ -458,7 +464,8 @@ struct Forward {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // backward over the rows: dq, dlam and the numbers the columns need.  With D^c unknown until the row's end, the sums
-// A = sum p dP k, B = sum p k and D = sum p dP are taken together; dq = scale (A - D B).
+// A = sum p dP k, B = sum p k, D = sum p dP and Z = sum p are taken together, of p before the division by Z;
+// dq = scale (A - D B / Z) / Z.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int G, int NV, int QB, int FORM>
 struct BackwardRows {
@@ -467,7 +474,7 @@ struct BackwardRows {
    static constexpr int LANE_FLOATS = QB * (2 * NV * W + 2);
    struct State {
       F2 a[QB][NV][P], b[QB][NV][P];  // of this half's map
-      float delta[QB];
+      float delta[QB], total[QB];
    };
    State s;
 
@@ -475,7 +482,7 @@ struct BackwardRows {
    {
 #pragma unroll
       for (int b = 0; b < QB; b++) {
-         s.delta[b] = 0.0f;
+         s.delta[b] = s.total[b] = 0.0f;
 #pragma unroll
          for (int t = 0; t < NV; t++)
 #pragma unroll
@@ -534,10 +541,11 @@ struct BackwardRows {
                      }
                   const float dot = add_over<G / 2>(sum2(dots)), dp = add_over<G>(sum2(dps));
                   // an edge that is masked has p = 0, and so has a row without edges (its lse is -inf)
-                  const float pr = id[i] >= 0 && lse[b] != -INFINITY ? exp2_fast((fmaf(dot, p.scale, bias) - lse[b]) * LOG2E) : 0.0f;
+                  const float pr = id[i] >= 0 && lse[b] != -INFINITY ? weight_of(fmaf(dot, p.scale, bias), lse[b]) : 0.0f;
                   const float w = pr * dp;
                   const F2 ww = f2(w, w), pp = f2(pr, pr);
                   s.delta[b] += w;
+                  s.total[b] += pr;
 #pragma unroll
                   for (int t = 0; t < NV; t++)
 #pragma unroll
@@ -553,6 +561,7 @@ struct BackwardRows {
 #pragma unroll
          for (int b = 0; b < QB; b++) {
             s.delta[b] += __shfl_xor_sync(FULL, s.delta[b], x2);
+            s.total[b] += __shfl_xor_sync(FULL, s.total[b], x2);
 #pragma unroll
             for (int t = 0; t < NV; t++)
 #pragma unroll
@@ -581,7 +590,9 @@ struct BackwardRows {
                s.a[b][t][j] = add2(s.a[b][t][j], x[0][t][j]);
                s.b[b][t][j] = add2(s.b[b][t][j], x[1][t][j]);
             }
-         s.delta[b] += unit[QB * 2 * NV * W * G + (b * G + at.in_slot) * 2];
+         const float2 sums = *reinterpret_cast<const float2 *>(unit + QB * 2 * NV * W * G + (b * G + at.in_slot) * 2);
+         s.delta[b] += sums.x;
+         s.total[b] += sums.y;
       }
    }
    __device__ __forceinline__ void put(float *unit, const Place &at) const
@@ -594,7 +605,7 @@ struct BackwardRows {
             put_pairs<P>(to + (b * 2 * NV + t) * W * G, s.a[b][t]);
             put_pairs<P>(to + ((b * 2 + 1) * NV + t) * W * G, s.b[b][t]);
          }
-         unit[QB * 2 * NV * W * G + (b * G + at.in_slot) * 2] = s.delta[b];
+         *reinterpret_cast<float2 *>(unit + QB * 2 * NV * W * G + (b * G + at.in_slot) * 2) = make_float2(s.delta[b], s.total[b]);
       }
    }
 
@@ -605,7 +616,8 @@ struct BackwardRows {
       for (int b = 0; b < QB; b++) {
          const int head = at.unit * QB + b;
          const long long rh = row * p.heads + head;
-         const float sign = at.half ? -__ldg(p.lam + row * p.ldlam + head) : 1.0f, factor = sign * p.scale;
+         const float inverse = reciprocal_total(s.total[b]), delta = s.delta[b] * inverse;
+         const float sign = (at.half ? -__ldg(p.lam + row * p.ldlam + head) : 1.0f) * inverse, factor = sign * p.scale;
 #pragma unroll
          for (int t = 0; t < NV; t++) {
             const int x = (at.in_half + (G / 2) * t) * W;
@@ -613,12 +625,12 @@ struct BackwardRows {
             unpair(s.a[b][t], a);
             unpair(s.b[b][t], c);
 #pragma unroll
-            for (int j = 0; j < W; j++) a[j] = factor * fmaf(-s.delta[b], c[j], a[j]);
+            for (int j = 0; j < W; j++) a[j] = factor * fmaf(-delta, c[j], a[j]);
             st_row<T, FORM != PIECES>(static_cast<T *>(p.out) + (rh * 2 + at.half) * p.d + x, a, p.d - x);
          }
          if (at.in_half == 0) {
-            p.stats[rh * 2 + at.half] = make_float4(__ldg(p.lse + rh * 2 + at.half), s.delta[b], sign, 0.0f);
-            if (at.half == 1) p.dlam[rh] = -s.delta[b];
+            p.stats[rh * 2 + at.half] = make_float4(__ldg(p.lse + rh * 2 + at.half), delta, sign, 0.0f);
+            if (at.half == 1) p.dlam[rh] = -delta;
          }
       }
    }
@@ -695,7 +707,7 @@ struct BackwardColumns {
                   }
                   const float dot = add_over<G / 2>(sum2(dots)), dp = add_over<G>(sum2(dps));
                   const bool live = stat[i].x != -INFINITY;  // an edge, and of a row that has any
-                  const float pr = live ? exp2_fast((fmaf(dot, p.scale, bias[i]) - stat[i].x) * LOG2E) : 0.0f;
+                  const float pr = live ? weight_of(fmaf(dot, p.scale, bias[i]), stat[i].x) : 0.0f;
                   const float mine = live ? stat[i].z * pr : 0.0f;  // this map's part of the weight
                   const float w = mine + __shfl_xor_sync(FULL, mine, G / 2);
                   const float ds = live ? mine * (dp - stat[i].y) : 0.0f;

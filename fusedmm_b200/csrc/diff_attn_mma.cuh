@@ -583,19 +583,19 @@ struct ForwardMma {
 };
 
 // ---------------------------------------------------------------------------------------------------------------------
-// backward over the rows (the sums A = sum p dP k, B = sum p k, D = sum p dP of BackwardRows).  For map 0 the rows of A's
+// backward over the rows (the sums A = sum p dP k, B = sum p k, D = sum p dP, Z = sum p of BackwardRows).  For map 0 the rows of A's
 // operand are w = p dP of the columns 0..3 and p of the same, for map 1 the other way round.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DK, int FORM, bool ONE>
 struct BackwardRowsMma {
    using Cols = Columns<ONE>;
    static constexpr int N = Cols::N;
-   static constexpr int DV = 2 * DK, TILES = DK / 8, LANE_FLOATS = 4 * TILES + 2;
+   static constexpr int DV = 2 * DK, TILES = DK / 8, LANE_FLOATS = 4 * TILES + 4;
    using Gathered = Ring<T, DK, FORM, Budget<DK, WALK_ROWS>::STAGES, false, true>;
    using Width = Budget<DK, WALK_ROWS>;
    struct State {
       float acc[2][TILES][2];
-      float delta[N];  // of this lane's columns
+      float delta[N], total[N];  // of this lane's columns
    };
    State s;
    Lanes l;
@@ -619,7 +619,7 @@ struct BackwardRowsMma {
 #pragma unroll
          for (int t = 0; t < TILES; t++) s.acc[m][t][0] = s.acc[m][t][1] = 0.0f;
 #pragma unroll
-      for (int x = 0; x < N; x++) s.delta[x] = 0.0f;
+      for (int x = 0; x < N; x++) s.delta[x] = s.total[x] = 0.0f;
    }
    __device__ __forceinline__ void fetch(const AttnParams &p, long long row)
    {
@@ -637,7 +637,7 @@ struct BackwardRowsMma {
 #pragma unroll
          for (int t = 0; t < TILES; t++) acc[m][t][0] = acc[m][t][1] = acc[m][t][2] = acc[m][t][3] = 0.0f;
 #pragma unroll
-      for (int x = 0; x < N; x++) s.delta[x] = 0.0f;
+      for (int x = 0; x < N; x++) s.delta[x] = s.total[x] = 0.0f;
       unsigned q[DK / 8], dout[DV / 8];
       float lse[N];
 #pragma unroll
@@ -683,9 +683,10 @@ struct BackwardRowsMma {
             for (int x = 0; x < N; x++) {
                // an edge that is masked has p = 0, and so has a row without edges (its lse is -inf)
                const bool live = heads.valid[x] && there && lse[x] != -INFINITY;
-               pr[x] = live ? exp2_fast((fmaf(Cols::pick(s0, s1, h, x, l), p.scale, bias) - lse[x]) * LOG2E) : 0.0f;
+               pr[x] = live ? weight_of(fmaf(Cols::pick(s0, s1, h, x, l), p.scale, bias), lse[x]) : 0.0f;
                w[x] = live ? pr[x] * Cols::pick(dp, h, x, l) : 0.0f;
                s.delta[x] += w[x];
+               s.total[x] += pr[x];
             }
             unsigned wh, wl, ph, pl;
             Cols::template split<T>(w, l, wh, wl);
@@ -722,7 +723,10 @@ struct BackwardRowsMma {
          }
       lost = all != all;
 #pragma unroll
-      for (int x = 0; x < N; x++) s.delta[x] = Cols::sum(s.delta[x]);
+      for (int x = 0; x < N; x++) {
+         s.delta[x] = Cols::sum(s.delta[x]);
+         s.total[x] = Cols::sum(s.total[x]);
+      }
    }
 
    __device__ __forceinline__ void join_from(const float *unit, const Place &at)
@@ -733,7 +737,7 @@ struct BackwardRowsMma {
       for (int m = 0; m < 2; m++)
 #pragma unroll
          for (int t = 0; t < TILES; t++) o[m][t] = from[32 * (m * TILES + t)];
-      const float2 d = from[64 * TILES];
+      const float2 d = from[64 * TILES], z = from[64 * TILES + 32];
 #pragma unroll
       for (int m = 0; m < 2; m++)
 #pragma unroll
@@ -742,7 +746,11 @@ struct BackwardRowsMma {
             s.acc[m][t][1] += o[m][t].y;
          }
       s.delta[0] += d.x;
-      if constexpr (!ONE) s.delta[N - 1] += d.y;
+      s.total[0] += z.x;
+      if constexpr (!ONE) {
+         s.delta[N - 1] += d.y;
+         s.total[N - 1] += z.y;
+      }
    }
    __device__ __forceinline__ void put(float *unit, const Place &at, int only) const
    {
@@ -753,19 +761,22 @@ struct BackwardRowsMma {
 #pragma unroll
             for (int t = 0; t < TILES; t++) to[32 * (m * TILES + t)] = make_float2(s.acc[m][t][0], s.acc[m][t][1]);
       }
-      float *delta = reinterpret_cast<float *>(to + 64 * TILES);
+      float *delta = reinterpret_cast<float *>(to + 64 * TILES), *total = reinterpret_cast<float *>(to + 64 * TILES + 32);
 #pragma unroll
       for (int x = 0; x < N; x++)
-         if (only < 0 || heads.col_kv[x] == only) delta[x] = s.delta[x];
+         if (only < 0 || heads.col_kv[x] == only) {
+            delta[x] = s.delta[x];
+            total[x] = s.total[x];
+         }
    }
 
    __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long row, int only)
    {
-      const float delta = Cols::of_row(s.delta, l.r);
+      const float inverse = reciprocal_total(Cols::of_row(s.total, l.r)), delta = Cols::of_row(s.delta, l.r) * inverse;
       const bool mine = heads.live && (only < 0 || heads.kv == only);
       const int map = l.r >> 2;
       const long long rh = row * p.heads + heads.head;
-      const float sign = map ? -__ldg(p.lam + row * p.ldlam + heads.head) : 1.0f, factor = sign * p.scale;
+      const float sign = (map ? -__ldg(p.lam + row * p.ldlam + heads.head) : 1.0f) * inverse, factor = sign * p.scale;
       T *out = static_cast<T *>(p.out) + (rh * 2 + map) * p.d + 2 * l.c;
 #pragma unroll
       for (int t = 0; t < TILES; t++) {
@@ -898,7 +909,7 @@ struct BackwardColumnsMma {
                // an edge of this column, of a row that has any, and this lane's column is the pair's
                const bool live = valid && edge >= lo && edge < hi && bias != -INFINITY && lse != -INFINITY;
                const float dot = map ? (x ? s1[2 * h + 1] : s1[2 * h]) : (x ? s0[2 * h + 1] : s0[2 * h]);
-               const float pr = live ? exp2_fast((fmaf(dot, p.scale, bias) - lse) * LOG2E) : 0.0f;
+               const float pr = live ? weight_of(fmaf(dot, p.scale, bias), lse) : 0.0f;
                const float part = live ? sign * pr : 0.0f;  // this map's part of the weight
                const float w = part + __shfl_xor_sync(FULL, part, 2);
                const float ds = live ? part * ((x ? dp[2 * h + 1] : dp[2 * h]) - delta) : 0.0f;

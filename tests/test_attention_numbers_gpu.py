@@ -1,0 +1,68 @@
+"""Differential attention where 32 bits are few: scores of a mask's size, values with a mean, one edge far above the others.
+Against plain evaluations in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from attention_cases import HALF_STEP, attention_reference, check
+from fusedmm_b200 import torch_op
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def rows_of(lengths, n, gen):
+    rowptr = torch.zeros(len(lengths) + 1, dtype=torch.int64)
+    rowptr[1:] = torch.cumsum(torch.tensor(lengths), 0)
+    return rowptr, torch.randint(0, n, (int(rowptr[-1]),), generator=gen, dtype=torch.int32)
+
+
+def gradients(rowptr, colidx, bias, q, k, v, lam, scale, dout):
+    leaves = [x.cuda().requires_grad_() for x in (q, k, v, lam)]
+    out = torch_op.diff_attention(rowptr.cuda(), colidx.cuda(), *leaves, bias=None if bias is None else bias.cuda(), scale=scale)
+    return dict(zip(("out", "dq", "dk", "dv", "dlam"), (out, *torch.autograd.grad(out, leaves, dout.cuda()))))
+
+
+SHAPES = [(F32, 4, 2, 32, 64), (F32, 4, 1, 8, 16), (F32, 3, 3, 5, 7), (BF16, 8, 2, 64, 128), (BF16, 4, 4, 16, 32), (BF16, 3, 1, 33, 20),
+          (BF16, 2, 2, 128, 256), (F16, 6, 3, 20, 36), (F16, 2, 1, 64, 128)]
+LENGTHS = {"few long rows": [1, 3, 700, 0, 5000], "many short rows": [1, 2, 30, 0, 9, 17] * 400}
+
+
+@pytest.mark.parametrize("lengths", LENGTHS)
+@pytest.mark.parametrize("mask", [-1e9, torch.finfo(F32).min])
+@pytest.mark.parametrize("dtype,heads,kvh,d,dv", SHAPES)
+def test_rows_whose_edges_all_carry_a_finite_mask(cuda_device, dtype, heads, kvh, d, dv, mask, lengths):
+    """A finite mask on all of a row's edges leaves equal weights, in the gradients too: next to it the products (below 32) and
+    the logarithm of the sum vanish (32-bit numbers near 1e9 are 64 apart).  Zero queries, or zero keys, without a mask give the
+    same weights, so the gradients are the 64-bit evaluation's of those: dk's with zero keys, the others' with zero queries."""
+    gen = torch.Generator().manual_seed(d)
+    n = 90
+    rowptr, colidx = rows_of(LENGTHS[lengths], n, gen)
+    m = len(rowptr) - 1
+    q, k, v, dout = (torch.randn(s, generator=gen).to(dtype) for s in ((m, heads, 2, d), (n, kvh, 2, d), (n, kvh, dv), (m, heads, dv)))
+    lam, bias, scale = torch.rand(m, heads, generator=gen), torch.full((colidx.numel(),), mask), d ** -0.5
+    got = gradients(rowptr, colidx, bias, q, k, v, lam, scale, dout)
+    want = attention_reference(rowptr, colidx, None, torch.zeros_like(q), k, v, lam, scale, dout)
+    want["dk"] = attention_reference(rowptr, colidx, None, q, torch.zeros_like(k), v, lam, scale, dout)["dk"]
+    for name in got:
+        check(got[name], want[name], name)
+
+
+@pytest.mark.parametrize("mask", [-3e4, -1e6])
+@pytest.mark.parametrize("dtype,heads,kvh,d,dv", [(F32, 2, 1, 16, 32), (BF16, 2, 1, 16, 32), (F16, 2, 1, 16, 32)])
+def test_weights_of_masked_rows_add_up(cuda_device, dtype, heads, kvh, d, dv, mask):
+    """With scores of some thousands the log-sum keeps few digits; each map's weights still add up to 1: with dout and v of ones
+    dP is dv on every edge, so dlam is -dv, dq is 0 and the sum of dv over the columns (1 - lam) for every row."""
+    gen = torch.Generator().manual_seed(1)
+    m, n = 300, 50
+    rowptr, colidx = rows_of([7, 100, 33] * (m // 3), n, gen)
+    q, k = (torch.randn(s, generator=gen).to(dtype) for s in ((m, heads, 2, d), (n, kvh, 2, d)))
+    v, dout, lam = torch.ones(n, kvh, dv, dtype=dtype), torch.ones(m, heads, dv, dtype=dtype), torch.full((m, heads), 0.25)
+    got = gradients(rowptr, colidx, torch.full((colidx.numel(),), mask), q, k, v, lam, 0.25, dout)
+    # sums of up to 100 positive terms and a division by another: 2 (100 + 8) steps of 2^-23; dq: weights split to 16 bits
+    assert float((got["dlam"] + dv).abs().max()) <= dv * 216 * 2.0 ** -23
+    assert float(got["dq"].abs().max()) <= 0.25 * dv * 4 * (216 * 2.0 ** -23 + 2.0 ** -16)
+    # dv: a column's sum of p is rounded to the type
+    total = got["dv"].double().sum((0, 1))
+    assert float((total - m * heads * 0.75).abs().max()) <= m * heads * 0.75 * (2 * HALF_STEP[dtype] + 216 * 2.0 ** -23 + 2.0 ** -16)
