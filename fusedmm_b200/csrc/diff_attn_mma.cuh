@@ -12,9 +12,11 @@
 //           lane sums of a product on the ordinary units.
 //   output  [8 rows x dv] over the 16 pairs: A = weights, 0 where the heads differ or the edge is another row's,
 //           B = gathered v.
-// Weights are split into two 16-bit numbers whose sum has 16 bits (bf16) or 22 (half) of the 32-bit value; the second lies in
-// the rows 8..15 of A that the first leaves free, so the split costs no product.  They change from "pair by column" to "row
-// by pair" with movmatrix.
+// Weights are split into two 16-bit numbers, the second of which lies in the rows 8..15 of A that the first leaves free, so the
+// split costs no product.  Their sum has 16 bits of the 32-bit value in bf16.  Half's numbers are 2^-24 apart below 2^-14, so there
+// weights are carried 2^8 times larger (the row's sum with them) and the second parts another 2^11 times (taken out where the two
+// rows are added up): 22 bits of weights down to 2^-22 of the row's largest, and 2^-44 of that largest is what smaller ones lose at
+// most.  Weights change from "pair by column" to "row by pair" with movmatrix.
 // Why not tcgen05: a tile there has 64 or 128 rows that share one operand; here a gathered row meets at most 8 rows of q,
 // and consecutive rows of the pattern gather different rows.
 #pragma once
@@ -72,14 +74,19 @@ __device__ __forceinline__ void copy_async(unsigned to, const void *from, int th
 {
    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there) : "memory");
 }
-// v as the sum of two numbers of T, for two neighbours
+// powers of two that half's weights, and the second parts of its split numbers, are carried larger by
+template <typename T>
+constexpr float WEIGHT_LOG2 = std::is_same<T, __half>::value ? 8.0f : 0.0f;
+template <typename T>
+constexpr float LOWER_SCALE = std::is_same<T, __half>::value ? 2048.0f : 1.0f;
+// v as hi + lo / LOWER_SCALE, two numbers of T, for two neighbours
 template <typename T>
 __device__ __forceinline__ void split2(float a, float b, unsigned &hi, unsigned &lo)
 {
    hi = Elt<T>::pack2(a, b);
    float x, y;
    Elt<T>::unpack2(hi, x, y);
-   lo = Elt<T>::pack2(a - x, b - y);
+   lo = Elt<T>::pack2((a - x) * LOWER_SCALE<T>, (b - y) * LOWER_SCALE<T>);
 }
 
 // two elements of a row, those of them that are there
@@ -345,7 +352,7 @@ struct QueryHeads {
 };
 
 // the maximum may grow by this much (as a power of e) before sums are scaled anew: weights then stay below e^5 and a
-// row's scaling is done once as a rule.  32-bit sums and 16-bit weights (half: up to 65504) hold e^5 with room.
+// row's scaling is done once as a rule.  32-bit sums and 16-bit weights hold that (half: 2^8 e^5 = 37994 of 65504).
 constexpr float SLACK = 5.0f;
 
 // warps of a block and blocks of a multiprocessor: registers and rings decide (a warp's ring is STAGES x 128 DK bytes)
@@ -451,7 +458,7 @@ struct ForwardMma {
 #pragma unroll
          for (int x = 0; x < N; x++) {
             high[x] = fmaxf(score[0][x], score[1][x]);
-            grown |= high[x] > s.top[x] + SLACK;
+            grown |= high[x] - s.top[x] > SLACK;  // (the difference: next to large scores a sum with 5 may be rounded to 8 more)
          }
          if (__any_sync(FULL, grown)) {
             float f[N];
@@ -478,7 +485,7 @@ struct ForwardMma {
             for (int x = 0; x < N; x++) {
                // a row that has met no edge yet has the maximum -inf: its differences are taken from 0.
                // The difference is taken before the factor: scores near the type's largest numbers keep their order.
-               w[x] = exp2_fast((score[h][x] - (s.top[x] == -INFINITY ? 0.0f : s.top[x])) * LOG2E);
+               w[x] = exp2_fast(fmaf(score[h][x] - (s.top[x] == -INFINITY ? 0.0f : s.top[x]), LOG2E, WEIGHT_LOG2<T>));
                s.sum[x] += w[x];
             }
             unsigned up, low;
@@ -498,8 +505,8 @@ struct ForwardMma {
       float all = 0.0f;
 #pragma unroll
       for (int t = 0; t < TILES; t++) {
-         s.acc[t][0] = acc[t][0] + acc[t][2];
-         s.acc[t][1] = acc[t][1] + acc[t][3];
+         s.acc[t][0] = fmaf(acc[t][2], 1.0f / LOWER_SCALE<T>, acc[t][0]);
+         s.acc[t][1] = fmaf(acc[t][3], 1.0f / LOWER_SCALE<T>, acc[t][1]);
          all += s.acc[t][0] * 0.0f + s.acc[t][1] * 0.0f;  // 0, or NaN once anything is infinite or NaN
       }
       lost = all != all;
@@ -567,7 +574,7 @@ struct ForwardMma {
          }
          if (mine) store_two<T, FORM>(out + 8 * t, o[0], o[1], p.dv - 8 * (t + odd) - 2 * l.c);
       }
-      if (mine && l.c == 0 && p.lse) p.lse[rh * 2 + odd] = top + LN2 * log2f(sum);
+      if (mine && l.c == 0 && p.lse) p.lse[rh * 2 + odd] = top + LN2 * (log2f(sum) - WEIGHT_LOG2<T>);
    }
    __device__ __forceinline__ void finish_empty(const AttnParams &p, const Place &at, long long row)
    {
@@ -588,6 +595,7 @@ struct ForwardMma {
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DK, int FORM, bool ONE>
 struct BackwardRowsMma {
+   static_assert(LOWER_SCALE<T> == 1.0f, "the parts of split numbers are added up as they are");
    using Cols = Columns<ONE>;
    static constexpr int N = Cols::N;
    static constexpr int DV = 2 * DK, TILES = DK / 8, LANE_FLOATS = 4 * TILES + 4;
@@ -815,6 +823,7 @@ struct BackwardRowsMma {
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DK, int FORM, bool SINGLE>
 struct BackwardColumnsMma {
+   static_assert(LOWER_SCALE<T> == 1.0f, "the parts of split numbers are added up as they are");
    static constexpr int DV = 2 * DK, KT = DK / 16, VT = DV / 16, LANE_FLOATS = 4 * (2 * KT + VT);
    using Gathered = Ring<T, DK, FORM, Budget<DK, WALK_COLUMNS>::STAGES, true, SINGLE>;
    using Width = Budget<DK, WALK_COLUMNS>;

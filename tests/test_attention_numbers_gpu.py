@@ -66,3 +66,43 @@ def test_weights_of_masked_rows_add_up(cuda_device, dtype, heads, kvh, d, dv, ma
     # dv: a column's sum of p is rounded to the type
     total = got["dv"].double().sum((0, 1))
     assert float((total - m * heads * 0.75).abs().max()) <= m * heads * 0.75 * (2 * HALF_STEP[dtype] + 216 * 2.0 ** -23 + 2.0 ** -16)
+
+
+@pytest.mark.parametrize("lengths", ["one row", "rows", "long row"])
+@pytest.mark.parametrize("gap", [5, 10, 14, 17, 18, 24])
+@pytest.mark.parametrize("dtype,heads,kvh,d,dv", [(F16, 8, 2, 64, 128), (F16, 4, 4, 16, 32), (F16, 3, 1, 20, 36), (F16, 2, 1, 128, 256), (BF16, 8, 2, 64, 128),
+                                                  (F32, 4, 2, 32, 64)])
+def test_a_first_edge_far_above_the_others(cuda_device, dtype, heads, kvh, d, dv, gap, lengths):
+    """The edge with the largest score has a value of zero, so the result is what the small weights bring."""
+    gen = torch.Generator().manual_seed(gap)
+    n = 3000
+    rowptr, colidx = rows_of({"one row": [1000], "rows": [250] * 700, "long row": [100000]}[lengths], n, gen)
+    m = len(rowptr) - 1
+    colidx[colidx == 0] = 1
+    colidx[rowptr[:-1]] = 0
+    bias = torch.zeros(colidx.numel())
+    bias[rowptr[:-1]] = gap
+    q, k = ((0.3 * torch.randn(s, generator=gen)).to(dtype) for s in ((m, heads, 2, d), (n, kvh, 2, d)))
+    v = (1 + 0.1 * torch.randn(n, kvh, dv, generator=gen)).to(dtype)
+    v[0] = 0
+    lam = torch.full((heads,), 0.25)
+    out = torch_op.diff_attention(*(x.cuda() for x in (rowptr, colidx, q, k, v, lam)), bias=bias.cuda(), scale=0.1)
+    value, bound = attention_reference(rowptr, colidx, bias, q, k, v, lam, 0.1)["out"]
+    # beside the bound of large weights: half's weights lie on a grid of 2^-44 of the row's largest at worst
+    grid = 2.0 ** -45 * 1.25 * 1.5 * (rowptr[1:] - rowptr[:-1])[:, None, None] if dtype == F16 else 0
+    check(out, (value, bound + grid))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("base,gap", [(1e8, 8), (-1e8, 8), (3e7, 6), (3e7, 4), (1e6, 5.5), (0, 5)])
+def test_a_later_edge_a_little_above_the_others(cuda_device, dtype, base, gap):
+    """Scores whose 32-bit neighbours are 8, 2 and 1/16 apart: the edge above the others comes late in its row, after sums were
+    taken against a smaller maximum.  Zero queries: the scores are the biases, exactly."""
+    gen = torch.Generator().manual_seed(3)
+    rowptr, colidx = rows_of([200, 1, 777, 90], 60, gen)
+    q, k, v = torch.zeros(4, 4, 2, 16, dtype=dtype), torch.randn(60, 2, 2, 16, generator=gen).to(dtype), torch.randn(60, 2, 32, generator=gen).to(dtype)
+    bias, lam = torch.full((colidx.numel(),), float(base)), torch.full((4,), 0.25)
+    bias[rowptr[1:] - 1] += gap
+    assert bool((bias[rowptr[1:] - 1] - base == gap).all())
+    out = torch_op.diff_attention(*(x.cuda() for x in (rowptr, colidx, q, k, v, lam)), bias=bias.cuda())
+    check(out, attention_reference(rowptr, colidx, bias - base, q, k, v, lam, 0.25)["out"])
