@@ -157,6 +157,14 @@ __device__ __forceinline__ void get_pairs(const float *p, F2 (&f)[N])
 }
 // exp(score - lse).  No score is above lse but for rounding, which next to a mask's size may be a power of thousands.
 __device__ __forceinline__ float weight_of(float score, float lse) { return exp2_fast(min_or_nan(score - lse, 0.0f) * LOG2E); }
+// What sums with the reference `ref_o` lack (times the sums of their weights) against `ref`, which becomes theirs where there are no
+// weights yet (all sums are 0 then).
+__device__ __forceinline__ float reference_shift(float total, float &ref, float total_o, float ref_o)
+{
+   const float shift = total != 0.0f && total_o != 0.0f ? ref_o - ref : 0.0f;
+   if (total == 0.0f) ref = ref_o;
+   return shift;
+}
 // 1 / Z; a row of no weights has no gradient
 __device__ __forceinline__ float reciprocal_total(float total) { return total == 0.0f ? 0.0f : 1.0f / total; }
 __device__ __forceinline__ F2 shfl_xor_pair(F2 v, int x) { return __shfl_xor_sync(FULL, v, x); }
@@ -464,17 +472,18 @@ struct Forward {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // backward over the rows: dq, dlam and the numbers the columns need.  With D^c unknown until the row's end, the sums
-// A = sum p dP k, B = sum p k, D = sum p dP and Z = sum p are taken together, of p before the division by Z;
-// dq = scale (A - D B / Z) / Z.
+// A = sum p (dP - c) k, B = sum p k, D = sum p (dP - c) and Z = sum p are taken together, of p before the division by Z;
+// dq = scale (A - D B / Z) / Z.  The reference c is the dP of one of the first edges: with values that have a mean A and D B
+// without it would be large and nearly equal.  Sums with two references join by A += (c' - c) B, D += (c' - c) Z.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int G, int NV, int QB, int FORM>
 struct BackwardRows {
    static constexpr int W = Elt<T>::W, P = W / 2, U = W == 4 && QB == 1 ? 4 : 2, BLOCKS = W == 4 ? (QB > 2 ? 2 : 3) : QB * NV * W > 16 ? 2 : 4;
    static constexpr int KSKIP = (G / 2) * W, VSKIP = G * W;
-   static constexpr int LANE_FLOATS = QB * (2 * NV * W + 2);
+   static constexpr int LANE_FLOATS = QB * (2 * NV * W + 4);
    struct State {
       F2 a[QB][NV][P], b[QB][NV][P];  // of this half's map
-      float delta[QB], total[QB];
+      float delta[QB], total[QB], ref[QB];
    };
    State s;
 
@@ -482,7 +491,7 @@ struct BackwardRows {
    {
 #pragma unroll
       for (int b = 0; b < QB; b++) {
-         s.delta[b] = s.total[b] = 0.0f;
+         s.delta[b] = s.total[b] = s.ref[b] = 0.0f;
 #pragma unroll
          for (int t = 0; t < NV; t++)
 #pragma unroll
@@ -542,7 +551,8 @@ struct BackwardRows {
                   const float dot = add_over<G / 2>(sum2(dots)), dp = add_over<G>(sum2(dps));
                   // an edge that is masked has p = 0, and so has a row without edges (its lse is -inf)
                   const float pr = id[i] >= 0 && lse[b] != -INFINITY ? weight_of(fmaf(dot, p.scale, bias), lse[b]) : 0.0f;
-                  const float w = pr * dp;
+                  if (s.total[b] == 0.0f && fabsf(dp) < INFINITY) s.ref[b] = dp;  // no weight so far: all sums are 0
+                  const float w = pr * (dp - s.ref[b]);
                   const F2 ww = f2(w, w), pp = f2(pr, pr);
                   s.delta[b] += w;
                   s.total[b] += pr;
@@ -560,17 +570,34 @@ struct BackwardRows {
       for (int x2 = G * p.slot_heads; x2 < 32; x2 <<= 1) {
 #pragma unroll
          for (int b = 0; b < QB; b++) {
-            s.delta[b] += __shfl_xor_sync(FULL, s.delta[b], x2);
-            s.total[b] += __shfl_xor_sync(FULL, s.total[b], x2);
+            const float delta = __shfl_xor_sync(FULL, s.delta[b], x2), total = __shfl_xor_sync(FULL, s.total[b], x2);
+            F2 a[NV][P], c[NV][P];
+            const float ref = __shfl_xor_sync(FULL, s.ref[b], x2);
 #pragma unroll
             for (int t = 0; t < NV; t++)
 #pragma unroll
                for (int j = 0; j < P; j++) {
-                  s.a[b][t][j] = add2(s.a[b][t][j], shfl_xor_pair(s.a[b][t][j], x2));
-                  s.b[b][t][j] = add2(s.b[b][t][j], shfl_xor_pair(s.b[b][t][j], x2));
+                  a[t][j] = shfl_xor_pair(s.a[b][t][j], x2);
+                  c[t][j] = shfl_xor_pair(s.b[b][t][j], x2);
                }
+            add(s, b, a, c, delta, total, ref);
          }
       }
+   }
+   // adds the sums of other edges
+   static __device__ __forceinline__ void add(State &s, int b, const F2 (&a)[NV][P], const F2 (&c)[NV][P], float delta, float total, float ref)
+   {
+      const float shift = reference_shift(s.total[b], s.ref[b], total, ref);
+      const F2 ss = f2(shift, shift);
+#pragma unroll
+      for (int t = 0; t < NV; t++)
+#pragma unroll
+         for (int j = 0; j < P; j++) {
+            s.a[b][t][j] = add2(s.a[b][t][j], fma2(ss, c[t][j], a[t][j]));
+            s.b[b][t][j] = add2(s.b[b][t][j], c[t][j]);
+         }
+      s.delta[b] += fmaf(shift, total, delta);
+      s.total[b] += total;
    }
    __device__ __forceinline__ void join_from(const float *unit, const Place &at)
    {
@@ -583,16 +610,8 @@ struct BackwardRows {
             get_pairs<P>(from + (b * 2 * NV + t) * W * G, x[0][t]);
             get_pairs<P>(from + ((b * 2 + 1) * NV + t) * W * G, x[1][t]);
          }
-#pragma unroll
-         for (int t = 0; t < NV; t++)
-#pragma unroll
-            for (int j = 0; j < P; j++) {
-               s.a[b][t][j] = add2(s.a[b][t][j], x[0][t][j]);
-               s.b[b][t][j] = add2(s.b[b][t][j], x[1][t][j]);
-            }
-         const float2 sums = *reinterpret_cast<const float2 *>(unit + QB * 2 * NV * W * G + (b * G + at.in_slot) * 2);
-         s.delta[b] += sums.x;
-         s.total[b] += sums.y;
+         const float4 sums = *reinterpret_cast<const float4 *>(unit + QB * 2 * NV * W * G + (b * G + at.in_slot) * 4);
+         add(s, b, x[0], x[1], sums.x, sums.y, sums.z);
       }
    }
    __device__ __forceinline__ void put(float *unit, const Place &at) const
@@ -605,7 +624,7 @@ struct BackwardRows {
             put_pairs<P>(to + (b * 2 * NV + t) * W * G, s.a[b][t]);
             put_pairs<P>(to + ((b * 2 + 1) * NV + t) * W * G, s.b[b][t]);
          }
-         *reinterpret_cast<float2 *>(unit + QB * 2 * NV * W * G + (b * G + at.in_slot) * 2) = make_float2(s.delta[b], s.total[b]);
+         *reinterpret_cast<float4 *>(unit + QB * 2 * NV * W * G + (b * G + at.in_slot) * 4) = make_float4(s.delta[b], s.total[b], s.ref[b], 0.0f);
       }
    }
 
@@ -616,7 +635,7 @@ struct BackwardRows {
       for (int b = 0; b < QB; b++) {
          const int head = at.unit * QB + b;
          const long long rh = row * p.heads + head;
-         const float inverse = reciprocal_total(s.total[b]), delta = s.delta[b] * inverse;
+         const float inverse = reciprocal_total(s.total[b]), rest = s.delta[b] * inverse, delta = inverse == 0.0f ? 0.0f : s.ref[b] + rest;
          const float sign = (at.half ? -__ldg(p.lam + row * p.ldlam + head) : 1.0f) * inverse, factor = sign * p.scale;
 #pragma unroll
          for (int t = 0; t < NV; t++) {
@@ -625,7 +644,7 @@ struct BackwardRows {
             unpair(s.a[b][t], a);
             unpair(s.b[b][t], c);
 #pragma unroll
-            for (int j = 0; j < W; j++) a[j] = factor * fmaf(-delta, c[j], a[j]);
+            for (int j = 0; j < W; j++) a[j] = factor * fmaf(-rest, c[j], a[j]);
             st_row<T, FORM != PIECES>(static_cast<T *>(p.out) + (rh * 2 + at.half) * p.d + x, a, p.d - x);
          }
          if (at.in_half == 0) {

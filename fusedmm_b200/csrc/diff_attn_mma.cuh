@@ -590,20 +590,21 @@ struct ForwardMma {
 };
 
 // ---------------------------------------------------------------------------------------------------------------------
-// backward over the rows (the sums A = sum p dP k, B = sum p k, D = sum p dP, Z = sum p of BackwardRows).  For map 0 the rows of A's
-// operand are w = p dP of the columns 0..3 and p of the same, for map 1 the other way round.
+// backward over the rows (the sums A = sum p (dP - c) k, B = sum p k, D = sum p (dP - c), Z = sum p of BackwardRows; c is the
+// largest dP of a column's first block with edges).  For map 0 the rows of A's operand are w = p (dP - c) of the columns 0..3 and p
+// of the same, for map 1 the other way round.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DK, int FORM, bool ONE>
 struct BackwardRowsMma {
    static_assert(LOWER_SCALE<T> == 1.0f, "the parts of split numbers are added up as they are");
    using Cols = Columns<ONE>;
    static constexpr int N = Cols::N;
-   static constexpr int DV = 2 * DK, TILES = DK / 8, LANE_FLOATS = 4 * TILES + 4;
+   static constexpr int DV = 2 * DK, TILES = DK / 8, LANE_FLOATS = 4 * TILES + 6;
    using Gathered = Ring<T, DK, FORM, Budget<DK, WALK_ROWS>::STAGES, false, true>;
    using Width = Budget<DK, WALK_ROWS>;
    struct State {
       float acc[2][TILES][2];
-      float delta[N], total[N];  // of this lane's columns
+      float delta[N], total[N], ref[N];  // of this lane's columns
    };
    State s;
    Lanes l;
@@ -627,7 +628,7 @@ struct BackwardRowsMma {
 #pragma unroll
          for (int t = 0; t < TILES; t++) s.acc[m][t][0] = s.acc[m][t][1] = 0.0f;
 #pragma unroll
-      for (int x = 0; x < N; x++) s.delta[x] = s.total[x] = 0.0f;
+      for (int x = 0; x < N; x++) s.delta[x] = s.total[x] = s.ref[x] = 0.0f;
    }
    __device__ __forceinline__ void fetch(const AttnParams &p, long long row)
    {
@@ -645,7 +646,7 @@ struct BackwardRowsMma {
 #pragma unroll
          for (int t = 0; t < TILES; t++) acc[m][t][0] = acc[m][t][1] = acc[m][t][2] = acc[m][t][3] = 0.0f;
 #pragma unroll
-      for (int x = 0; x < N; x++) s.delta[x] = s.total[x] = 0.0f;
+      for (int x = 0; x < N; x++) s.delta[x] = s.total[x] = s.ref[x] = 0.0f;
       unsigned q[DK / 8], dout[DV / 8];
       float lse[N];
 #pragma unroll
@@ -658,6 +659,7 @@ struct BackwardRowsMma {
       const int per_log2 = 4 - l.slots_log2;
       // the lane's row and chunk of ldmatrix: pairs 0..7 and 8..15 of one chunk, then of the next; chunks by exclusive or
       const unsigned mine = Gathered::offset(at.lane & 15, at.lane >> 4);
+      bool fresh = true;  // no edge so far
       for (int e = e0; e < e1;) {
          const int block = e >> per_log2;
          if (block != ring.current) ring.advance(p, l, at.lane);
@@ -680,19 +682,34 @@ struct BackwardRowsMma {
          }
 #pragma unroll
          for (int i = 0; i < 4; i++) dp[i] += dp2[i];
-         unsigned a0[4], a1[4];
+         float bias[2];
+         bool there[2];
 #pragma unroll
          for (int h = 0; h < 2; h++) {
             const int edge = (l.r + 8 * h) >> l.slots_log2;
-            const float bias = shared_float(slot + Gathered::BIAS + 4 * edge);
-            const bool there = edge >= lo && edge < hi && bias != -INFINITY;
+            bias[h] = shared_float(slot + Gathered::BIAS + 4 * edge);
+            there[h] = edge >= lo && edge < hi && bias[h] != -INFINITY;
+         }
+         if (fresh) {
+            fresh = !__any_sync(FULL, there[0] || there[1]);
+#pragma unroll
+            for (int x = 0; x < N; x++) {
+               const float d0 = heads.valid[x] && there[0] ? Cols::pick(dp, 0, x, l) : -INFINITY;
+               const float d1 = heads.valid[x] && there[1] ? Cols::pick(dp, 1, x, l) : -INFINITY;
+               const float high = Cols::max(fmaxf(d0, d1));
+               s.ref[x] = fabsf(high) < INFINITY ? high : 0.0f;
+            }
+         }
+         unsigned a0[4], a1[4];
+#pragma unroll
+         for (int h = 0; h < 2; h++) {
             float pr[N], w[N];
 #pragma unroll
             for (int x = 0; x < N; x++) {
                // an edge that is masked has p = 0, and so has a row without edges (its lse is -inf)
-               const bool live = heads.valid[x] && there && lse[x] != -INFINITY;
-               pr[x] = live ? weight_of(fmaf(Cols::pick(s0, s1, h, x, l), p.scale, bias), lse[x]) : 0.0f;
-               w[x] = live ? pr[x] * Cols::pick(dp, h, x, l) : 0.0f;
+               const bool live = heads.valid[x] && there[h] && lse[x] != -INFINITY;
+               pr[x] = live ? weight_of(fmaf(Cols::pick(s0, s1, h, x, l), p.scale, bias[h]), lse[x]) : 0.0f;
+               w[x] = live ? pr[x] * (Cols::pick(dp, h, x, l) - s.ref[x]) : 0.0f;
                s.delta[x] += w[x];
                s.total[x] += pr[x];
             }
@@ -745,20 +762,29 @@ struct BackwardRowsMma {
       for (int m = 0; m < 2; m++)
 #pragma unroll
          for (int t = 0; t < TILES; t++) o[m][t] = from[32 * (m * TILES + t)];
-      const float2 d = from[64 * TILES], z = from[64 * TILES + 32];
+      // rows 0..3 hold A of map 0 and B of map 1, rows 4..7 B of map 0 and A of map 1: the B of this lane's A lies 16 lanes away
+      const int map = l.r >> 2;
+      const float2 *other = reinterpret_cast<const float2 *>(unit) + (at.lane ^ 16) + 32 * map * TILES;
+      float2 c[TILES];
+#pragma unroll
+      for (int t = 0; t < TILES; t++) c[t] = other[32 * t];
+      const float2 d = from[64 * TILES], z = from[64 * TILES + 32], ref = from[64 * TILES + 64];
+      float shift[N];
+#pragma unroll
+      for (int x = 0; x < N; x++) {
+         shift[x] = reference_shift(s.total[x], s.ref[x], x ? z.y : z.x, x ? ref.y : ref.x);
+         s.delta[x] += fmaf(shift[x], x ? z.y : z.x, x ? d.y : d.x);
+         s.total[x] += x ? z.y : z.x;
+      }
+      const float row_shift = Cols::of_row(shift, l.r);
 #pragma unroll
       for (int m = 0; m < 2; m++)
 #pragma unroll
          for (int t = 0; t < TILES; t++) {
-            s.acc[m][t][0] += o[m][t].x;
-            s.acc[m][t][1] += o[m][t].y;
+            const float f = m == map ? row_shift : 0.0f;
+            s.acc[m][t][0] += f == 0.0f ? o[m][t].x : fmaf(f, c[t].x, o[m][t].x);
+            s.acc[m][t][1] += f == 0.0f ? o[m][t].y : fmaf(f, c[t].y, o[m][t].y);
          }
-      s.delta[0] += d.x;
-      s.total[0] += z.x;
-      if constexpr (!ONE) {
-         s.delta[N - 1] += d.y;
-         s.total[N - 1] += z.y;
-      }
    }
    __device__ __forceinline__ void put(float *unit, const Place &at, int only) const
    {
@@ -769,18 +795,20 @@ struct BackwardRowsMma {
 #pragma unroll
             for (int t = 0; t < TILES; t++) to[32 * (m * TILES + t)] = make_float2(s.acc[m][t][0], s.acc[m][t][1]);
       }
-      float *delta = reinterpret_cast<float *>(to + 64 * TILES), *total = reinterpret_cast<float *>(to + 64 * TILES + 32);
+      float *delta = reinterpret_cast<float *>(to + 64 * TILES), *total = delta + 64, *ref = delta + 128;
 #pragma unroll
       for (int x = 0; x < N; x++)
          if (only < 0 || heads.col_kv[x] == only) {
             delta[x] = s.delta[x];
             total[x] = s.total[x];
+            ref[x] = s.ref[x];
          }
    }
 
    __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long row, int only)
    {
-      const float inverse = reciprocal_total(Cols::of_row(s.total, l.r)), delta = Cols::of_row(s.delta, l.r) * inverse;
+      const float inverse = reciprocal_total(Cols::of_row(s.total, l.r)), rest = Cols::of_row(s.delta, l.r) * inverse;
+      const float ref = Cols::of_row(s.ref, l.r), delta = inverse == 0.0f ? 0.0f : ref + rest;
       const bool mine = heads.live && (only < 0 || heads.kv == only);
       const int map = l.r >> 2;
       const long long rh = row * p.heads + heads.head;
@@ -793,7 +821,7 @@ struct BackwardRowsMma {
          for (int x = 0; x < 2; x++) {
             // rows 0..3 hold A of map 0 and B of map 1, rows 4..7 B of map 0 and A of map 1
             const float b = __shfl_xor_sync(FULL, map ? s.acc[0][t][x] : s.acc[1][t][x], 16);
-            o[x] = factor * fmaf(-delta, b, map ? s.acc[1][t][x] : s.acc[0][t][x]);
+            o[x] = factor * fmaf(-rest, b, map ? s.acc[1][t][x] : s.acc[0][t][x]);
          }
          if (mine) store_two<T, FORM>(out + 8 * t, o[0], o[1], p.d - 8 * t - 2 * l.c);
       }

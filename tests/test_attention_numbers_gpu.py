@@ -106,3 +106,29 @@ def test_a_later_edge_a_little_above_the_others(cuda_device, dtype, base, gap):
     assert bool((bias[rowptr[1:] - 1] - base == gap).all())
     out = torch_op.diff_attention(*(x.cuda() for x in (rowptr, colidx, q, k, v, lam)), bias=bias.cuda())
     check(out, attention_reference(rowptr, colidx, bias - base, q, k, v, lam, 0.25)["out"])
+
+
+@pytest.mark.parametrize("dtype,low,high,degree,heads,kvh,d,dv", [
+    (F32, 1e5, 1e5 + 1, 60, 4, 2, 32, 64), (F32, 1e5, 1e5 + 1, 2500, 2, 1, 8, 16), (F32, 1e5, 1e5 + 1, 13, 3, 3, 5, 7),
+    (BF16, 256, 258, 53, 8, 2, 64, 128), (BF16, 256, 258, 53, 4, 4, 16, 32), (BF16, 256, 258, 53, 4, 1, 128, 256), (BF16, 256, 258, 1700, 2, 1, 32, 64),
+    (F16, 2000, 2001, 60, 4, 2, 32, 64), (F16, 2000, 2001, 60, 3, 1, 33, 20),
+])
+def test_gradient_of_queries_where_values_have_a_mean(cuda_device, dtype, low, high, degree, heads, kvh, d, dv):
+    """dq is a sum of p (dP - D) k: what it loses must go by the differences of dP and not by dP.  All scores are equal (zero
+    queries), dout has a single one, so p and dP are known and the bound can be close."""
+    gen = torch.Generator().manual_seed(degree)
+    m, n = (40, 70) if degree < 1000 else (3, 500)
+    rowptr, colidx = rows_of([degree] * m, n, gen)
+    q, k = torch.zeros(m, heads, 2, d, dtype=dtype), (1 + torch.rand(n, kvh, 2, d, generator=gen)).to(dtype)
+    v = torch.where(torch.rand(n, kvh, dv, generator=gen) < 0.5, low, high).to(dtype)
+    dout = torch.zeros(m, heads, dv, dtype=dtype)
+    dout[..., dv // 2] = 1
+    lam, scale = torch.full((m, heads), 0.5), 0.5
+    got = gradients(rowptr, colidx, None, q, k, v, lam, scale, dout)["dq"]
+    want = attention_reference(rowptr, colidx, None, q, k, v, lam, scale, dout)["dq"][0]
+    half = HALF_STEP[dtype]
+    # p = 1/degree up to a factor that all edges share; p (dP - c), with c one of the dP, and p are split (bf16) and summed with
+    # k up to 2; then (D - c) times the sum of p k: four terms of at most (high - low) 2
+    step, split = (2.0 ** -23, 2.0 ** -16) if dtype == BF16 else (2.0 ** -24, 0)
+    slack = scale * 4 * (high - low) * 2 * (split + (degree + 16) * step)
+    check(got, (want, half * want.abs() + (1 + half) * slack))
