@@ -478,8 +478,8 @@ int rotary_setup(RotaryParams &p, int32_t dtype, int64_t rows, int32_t hq, int32
    if (dtype != DT_F32 && dtype != DT_BF16 && dtype != DT_F16) return FUSEDMM_B200_ERR_ARG;
    if (rows < 0 || hq < 0 || hk < 0 || d < 1 || pairs < 0 || 2LL * pairs > d) return FUSEDMM_B200_ERR_ARG;
    if (d > FUSEDMM_B200_ATTN_MAX_WIDTH || hq > FUSEDMM_B200_ATTN_MAX_HEADS || hk > FUSEDMM_B200_ATTN_MAX_HEADS) return FUSEDMM_B200_ERR_LIMIT;
-   for (int64_t s : {ldq, hsq, ldk, hsk})  // the kernels form the addresses inside a tile with 32-bit strides
-      if (s < 0 || s * (dtype == DT_F32 ? 4 : 2) >= INT32_MAX) return FUSEDMM_B200_ERR_LIMIT;
+   for (int64_t s : {ldq, hsq, ldk, hsk})
+      if (s < 0) return FUSEDMM_B200_ERR_LIMIT;
    if (norm && !(eps >= 0.0)) return FUSEDMM_B200_ERR_ARG;
    if (!norm && (wq || wk)) return FUSEDMM_B200_ERR_ARG;
    if (w_dtype != DT_F32 && w_dtype != dtype) return FUSEDMM_B200_ERR_ARG;
@@ -583,7 +583,7 @@ int fusedmm_b200_qk_norm_rotary_backward(int32_t dtype, int64_t rows, int32_t hq
                             ldp, asp, axes, freq, pairs, interleaved)) return s;
    if (!norm && (dwq || dwk)) return FUSEDMM_B200_ERR_ARG;
    for (int64_t s : {lddq, hsdq, lddk, hsdk})
-      if (s < 0 || s * (dtype == DT_F32 ? 4 : 2) >= INT32_MAX) return FUSEDMM_B200_ERR_LIMIT;
+      if (s < 0) return FUSEDMM_B200_ERR_LIMIT;
    cudaStream_t st = static_cast<cudaStream_t>(stream);
    if (rows == 0 || hq + hk == 0) {  // sums over nothing
       if (!on_device({dwq, dwk})) return FUSEDMM_B200_ERR_ARG;

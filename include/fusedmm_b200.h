@@ -492,9 +492,9 @@ int fusedmm_b200_release(void);
  * default stream and returns when it is done.  They may be captured into a CUDA graph.  Inputs must not overlap outputs.
  *
  * dtype: 0 float, 2 bfloat16, 3 half; sums, softmax statistics and norms are held in float.  Strides count elements and
- * are below 2^31 bytes (FUSEDMM_B200_ERR_LIMIT beyond); the last axis of every array is dense.  Rows of any length, stride and
- * alignment work; where address, strides and widths are multiples of 16 bytes the loads are 16 bytes wide.  Results are
- * the same bits on every run.
+ * are not negative; diff_attention's are below 2^31 bytes (FUSEDMM_B200_ERR_LIMIT beyond).  The last axis of every array is dense.
+ * Rows of any length, stride and alignment work; where address, strides and widths are multiples of 16 bytes the loads are 16
+ * bytes wide.  Results are the same bits on every run.
  * ---------------------------------------------------------------------------------------------- */
 #define FUSEDMM_B200_ATTN_MAX_WIDTH 256    /* d of qk_norm_rotary, 2 d and dv of diff_attention */
 #define FUSEDMM_B200_ATTN_MAX_HEADS 65536

@@ -214,3 +214,14 @@ def test_sizes_whose_products_leave_64_bits():
     ws.restype, ws.argtypes = L, [I, I, I, L, L, L, I, I, I, I]
     assert ws(0, 1, 0, 1 << 48, 4, 8, 65536, 1, 8, 8) == -4
     assert ws(1, 1, 2, 4, 4, 1 << 48, 4096, 1, 8, 8) == -4
+
+
+def test_strides_of_the_rotation_have_no_limit():
+    """-3: the made-up addresses are no device memory, which is looked at behind the limits (-4)."""
+    rot = api.lib().fusedmm_b200_qk_norm_rotary
+    rot.restype, rot.argtypes = I, list(api._ROTARY_IN) + [P, P, P]
+    good = dict(dtype=2, rows=4, hq=2, hk=1, d=8, q=256, ldq=16, hsq=8, k=256, ldk=8, hsk=8, wt=0, wq=None, wk=None, norm=1, eps=1e-6, pt=0,
+                pos=256, ldp=1, asp=1, axes=1, freq=256, pairs=4, il=0, qo=256, ko=256, stream=None)
+    for name in ("ldq", "hsq", "ldk", "hsk"):
+        assert rot(*{**good, name: 1 << 31}.values()) == -3, name
+        assert rot(*{**good, name: -1}.values()) == -4, name

@@ -34,3 +34,33 @@ def test_many_heads(cuda_device, dtype, heads, kvh, d, dv):
     want = attention_reference(rowptr, colidx, None, q, k, v, lam, d ** -0.5, dout)
     for name, got in zip(("out", "dq", "dk", "dv", "dlam"), (out, *grads)):
         check(got, want[name], name)
+
+
+def spread(gen, dtype, shape, strides, base):
+    """A tensor of ``shape`` on the GPU with these strides, over ``base``."""
+    x = torch.as_strided(base, shape, strides)
+    x.copy_(torch.randn(shape, generator=gen).to(dtype))
+    return x
+
+
+@pytest.mark.parametrize("rows,heads,far", [(2, 3, "rows"), (3, 2, "heads")])
+def test_rotation_of_rows_and_heads_far_apart(cuda_device, rows, heads, far):
+    """Strides of 2^31 bytes and more; the results are those of dense copies, bit for bit."""
+    gen = torch.Generator().manual_seed(1)
+    d, wide = 64, (1 << 30) + 8
+    strides = (wide, 2 * d, 1) if far == "rows" else (2 * d, wide, 1)
+    base = [torch.empty(2 * wide + 1024, dtype=BF16, device="cuda") for _ in range(2)]
+    q = spread(gen, BF16, (rows, heads, d), strides, base[0])
+    k = spread(gen, BF16, (rows, heads, d), strides, base[0][d:])
+    dy = spread(gen, BF16, (rows, heads, d), strides, base[1])
+    pos, freq = torch.arange(rows, device="cuda") * 1000, torch.rand(1, 32, generator=gen, dtype=torch.float64).cuda()
+    w = torch.rand(d, generator=gen).cuda()
+    results = []
+    for dense in (False, True):
+        leaves = [x.contiguous() if dense else x for x in (q, k)]
+        leaves = [x.detach().requires_grad_() for x in leaves] + [w.detach().requires_grad_()]
+        y = torch_op.qk_norm_rotary(leaves[0], leaves[1], pos, freq, q_weight=leaves[2], k_weight=leaves[2], eps=1e-6)
+        g = dy.contiguous() if dense else dy
+        results.append((*y, *torch.autograd.grad(y, leaves, (g, g))))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
