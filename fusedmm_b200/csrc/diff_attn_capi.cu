@@ -266,13 +266,14 @@ int check_sizes(int32_t dtype, int64_t m, int64_t n, int64_t nnz, int32_t heads,
    return 0;
 }
 
-// the kernels form the address of a row as base + id * stride with 32-bit factors
-bool strides_fit(int32_t dtype, std::initializer_list<int64_t> strides)
+bool below(int64_t limit, std::initializer_list<int64_t> strides)
 {
    for (int64_t s : strides)
-      if (s < 0 || s * (dtype == DT_F32 ? 4 : 2) >= INT_MAX) return false;
+      if (s < 0 || s >= limit) return false;
    return true;
 }
+// the walks form the address of a row that they gather as base + id * stride with 32-bit factors (packed rows are near)
+bool gathered_strides_fit(int32_t dtype, std::initializer_list<int64_t> strides) { return below(INT_MAX / (dtype == DT_F32 ? 4 : 2), strides); }
 
 // elements that one load of these rows may take at once; 16 bytes' worth: whole vectors
 struct Step {
@@ -341,18 +342,19 @@ int fusedmm_b200_diff_attention(int32_t dtype, int32_t ptr_bits, int32_t idx_bit
 {
    if ((ptr_bits != 32 && ptr_bits != 64) || (idx_bits != 32 && idx_bits != 64)) return FUSEDMM_B200_ERR_ARG;
    if (int s = check_sizes(dtype, m, n, nnz, heads, kv_heads, d, dv)) return s;
-   if (!strides_fit(dtype, {ldq, hsq, ldk, hsk, ldv, hsv, ldlam})) return FUSEDMM_B200_ERR_LIMIT;
+   if (!below(INT64_MAX, {ldq, hsq, ldk, hsk, ldv, hsv, ldlam})) return FUSEDMM_B200_ERR_LIMIT;
    if (m == 0) return 0;
    const bool gathers = nnz > 0 && n > 0;
    if (!rowptr || !q || !lam || !out || (nnz > 0 && !colidx) || (gathers && (!k || !v))) return FUSEDMM_B200_ERR_ARG;
-   int sms = 0;
-   if (int s = sm_count(&sms)) return s;
    if (n == 0) k = v = workspace;  // nothing is gathered, but copies of nothing want an address too
    Step step(dtype);
    step.with(q, ldq, hsq, d);
    step.with(k, ldk, hsk, d);
    step.with(v, ldv, hsv, dv);
    step.with(out, 0, 0, dv);
+   if (step.vector() && !gathered_strides_fit(dtype, {ldk, ldv})) return FUSEDMM_B200_ERR_LIMIT;
+   int sms = 0;
+   if (int s = sm_count(&sms)) return s;
    const int64_t need = fusedmm_b200_diff_attention_workspace(0, step.vector(), dtype, m, n, nnz, heads, kv_heads, d, dv);
    if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256) return FUSEDMM_B200_ERR_ARG;
    if (!on_device({rowptr, q, lam, out, lse, workspace, nnz > 0 ? colidx : nullptr, nnz > 0 ? bias : nullptr,
@@ -386,7 +388,7 @@ int fusedmm_b200_diff_attention_backward(int32_t dtype, int32_t ptr_bits, int32_
    if ((ptr_bits != 32 && ptr_bits != 64) || (idx_bits != 32 && idx_bits != 64)) return FUSEDMM_B200_ERR_ARG;
    if (int s = check_sizes(dtype, m, n, nnz, heads, kv_heads, d, dv)) return s;
    if (m >= INT_MAX || nnz >= INT_MAX) return FUSEDMM_B200_ERR_LIMIT;
-   if (!strides_fit(dtype, {ldq, hsq, ldk, hsk, ldv, hsv, lddo, hsdo, ldlam})) return FUSEDMM_B200_ERR_LIMIT;
+   if (!below(INT64_MAX, {ldq, hsq, ldk, hsk, ldv, hsv, lddo, hsdo, ldlam})) return FUSEDMM_B200_ERR_LIMIT;
    if (!dlam || (m > 0 && (!rowptr || !q || !lam || !lse || !dout || !dq)) || (n > 0 && (!k || !v || !dk || !dv_out || !t_rowptr)) ||
        (nnz > 0 && (!colidx || !t_row || (bias && !t_edge))))
       return FUSEDMM_B200_ERR_ARG;
@@ -400,6 +402,7 @@ int fusedmm_b200_diff_attention_backward(int32_t dtype, int32_t ptr_bits, int32_
    step.with(dq, 0, 0, d);
    step.with(dk, 0, 0, d);
    step.with(dv_out, 0, 0, dv);
+   if (step.vector() && !gathered_strides_fit(dtype, {ldk, ldv, ldq, lddo})) return FUSEDMM_B200_ERR_LIMIT;
    const int64_t need = fusedmm_b200_diff_attention_workspace(1, step.vector(), dtype, m, n, nnz, heads, kv_heads, d, dv);
    if (need < 0) return static_cast<int>(need);
    if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256) return FUSEDMM_B200_ERR_ARG;

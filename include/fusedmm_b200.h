@@ -492,7 +492,7 @@ int fusedmm_b200_release(void);
  * default stream and returns when it is done.  They may be captured into a CUDA graph.  Inputs must not overlap outputs.
  *
  * dtype: 0 float, 2 bfloat16, 3 half; sums, softmax statistics and norms are held in float.  Strides count elements and
- * are not negative; diff_attention's are below 2^31 bytes (FUSEDMM_B200_ERR_LIMIT beyond).  The last axis of every array is dense.
+ * are not negative.  The last axis of every array is dense.
  * Rows of any length, stride and alignment work; where address, strides and widths are multiples of 16 bytes the loads are 16
  * bytes wide.  Results are the same bits on every run.
  * ---------------------------------------------------------------------------------------------- */
@@ -551,9 +551,11 @@ int fusedmm_b200_qk_norm_rotary_backward(int32_t dtype, int64_t rows, int32_t hq
  * no edge: its k and v are not read.  A row without edges gives out = 0 and lse = -inf.  bias (nnz floats) may be NULL.
  * q is [m][heads][2][d] with the strides ldq, hsq; k is [n][kv_heads][2][d]; v is [n][kv_heads][dv]; lam is
  * [m][heads] with the row stride ldlam, or [heads] with ldlam 0.  out [m][heads][dv] and lse [m][heads][2] (natural
- * logarithms of the two maps' sums; may be NULL) are dense.  Long rows are cut, so that one row of many edges (a single
- * token's) fills the GPU.  n is below 2^31 - 1, m and nnz below 2^48, (nnz + 8 max(m, n)) heads below 2^56.  (Row pointers
- * that decrease or leave [0, nnz] give wrong rows, but no access outside the arrays; fusedmm_b200_check_csr finds them.)
+ * logarithms of the two maps' sums; may be NULL) are dense.  Where the vectors are whole (`aligned` below), the row strides of
+ * k and v, and in the backward call of q and dout, are below 2^31 - 1 bytes (FUSEDMM_B200_ERR_LIMIT beyond).  Long rows are cut, so
+ * that one row of many edges (a single token's) fills the GPU.  n is below 2^31 - 1, m and nnz below 2^48,
+ * (nnz + 8 max(m, n)) heads below 2^56.  (Row pointers that decrease or leave [0, nnz] give wrong rows, but no access outside the
+ * arrays; fusedmm_b200_check_csr finds them.)
  *
  * Workspace: `aligned` says that the addresses and strides of all arrays of the call are multiples of 16 bytes; where they or
  * the widths are not, the gathered rows are packed first and the workspace holds the packed ones.

@@ -225,3 +225,22 @@ def test_strides_of_the_rotation_have_no_limit():
     for name in ("ldq", "hsq", "ldk", "hsk"):
         assert rot(*{**good, name: 1 << 31}.values()) == -3, name
         assert rot(*{**good, name: -1}.values()) == -4, name
+
+
+def test_strides_of_the_attention():
+    """-4 for row strides of gathered rows alone; what else is far apart gets on to the looks at the device."""
+    fwd, back = api.lib().fusedmm_b200_diff_attention, api.lib().fusedmm_b200_diff_attention_backward
+    fwd.restype, fwd.argtypes = I, list(api._ATTN_IN) + [P, P, P, L, P]
+    back.restype, back.argtypes = I, list(api._ATTN_IN) + [P, P, L, L, P, P, P, P, P, P, P, P, L, P]
+    good = dict(dtype=0, pb=32, ib=32, m=4, n=4, nnz=8, rp=256, ci=256, bias=None, h=2, kvh=1, d=8, dv=8, q=256, ldq=32, hsq=16, k=256,
+                ldk=16, hsk=16, v=256, ldv=8, hsv=8, lam=256, ldlam=0, scale=1.0, out=256, lse=None, ws=256, wb=1 << 40, stream=None)
+    more = dict(list(good.items())[:25], lse=256, do=256, ldo=16, hso=8, tp=256, tr=256, te=None, dq=256, dk=256, dvo=256, dlam=256, ws=256,
+                wb=1 << 40, stream=None)
+    for name in ("ldq", "hsq", "ldk", "hsk", "ldv", "hsv", "ldlam", "ldo", "hso"):
+        far = {name: 1 << 30}
+        if name in good:
+            assert (fwd(*{**good, **far}.values()) == -4) == (name in ("ldk", "ldv")), name
+            assert fwd(*{**good, name: -4}.values()) == -4, name
+        assert (back(*{**more, **far}.values()) == -4) == (name in ("ldk", "ldv", "ldq", "ldo")), name
+        assert back(*{**more, name: -4}.values()) == -4, name
+        assert back(*{**more, **far, "d": 7}.values()) != -4, name  # packed first

@@ -64,3 +64,46 @@ def test_rotation_of_rows_and_heads_far_apart(cuda_device, rows, heads, far):
         results.append((*y, *torch.autograd.grad(y, leaves, (g, g))))
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32, F16])
+def test_heads_of_a_cache_far_apart(cuda_device, dtype):
+    """A [kv heads, slots, ...] cache seen through a transposed view, its heads 2^31 bytes apart; queries, weights and the result's
+    gradient likewise.  The results are those of dense copies, bit for bit."""
+    gen = torch.Generator().manual_seed(2)
+    m, n, heads, kvh, d, dv = 4, 30, 4, 2, 16, 32
+    wide = (1 << 31) // dtype.itemsize + 64
+    base = torch.empty(3 * wide + 65536, dtype=dtype, device="cuda")
+    rowptr, colidx = torch.tensor([0, 20, 20, 25, 700]).cuda(), torch.randint(0, n, (700,), generator=gen, dtype=torch.int32).cuda()
+    q = spread(gen, dtype, (m, heads, 2, d), (2 * d, wide, d, 1), base)
+    k = spread(gen, dtype, (n, kvh, 2, d), (2 * d, wide, d, 1), base[8192:])
+    v = spread(gen, dtype, (n, kvh, dv), (dv, wide, 1), base[16384:])
+    dout = spread(gen, dtype, (m, heads, dv), (dv, wide, 1), base[32768:])
+    lam = spread(gen, F32, (m, heads), (heads, 1), torch.empty(64, device="cuda"))
+    assert k.stride(1) * dtype.itemsize > 1 << 31
+    results = []
+    for dense in (False, True):
+        leaves = [(x.contiguous() if dense else x).detach().requires_grad_() for x in (q, k, v, lam)]
+        out = torch_op.diff_attention(rowptr, colidx, *leaves)
+        results.append((out, *torch.autograd.grad(out, leaves, dout.contiguous() if dense else dout)))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+def test_rows_far_apart(cuda_device):
+    """Rows of queries and weights may be 2^31 bytes apart in the forward pass, and so may gathered rows that are packed first."""
+    gen = torch.Generator().manual_seed(3)
+    heads, kvh, d, dv = 4, 2, 16, 32
+    wide = (1 << 31) // 2 + 64
+    base = torch.empty(2 * wide + 65536, dtype=BF16, device="cuda")
+    rowptr, colidx = torch.tensor([0, 5, 9]).cuda(), torch.randint(0, 3, (9,), generator=gen, dtype=torch.int32).cuda()
+    q = spread(gen, BF16, (2, heads, 2, d), (wide, 2 * d, d, 1), base)
+    k = spread(gen, BF16, (3, kvh, 2, d), (2 * d * kvh, 2 * d, d, 1), base[8192:])
+    v = spread(gen, BF16, (3, kvh, dv), (kvh * dv, dv, 1), base[16384:])
+    lam = spread(gen, F32, (2, heads), (wide, 1), torch.empty(wide + 64, device="cuda"))
+    assert torch.equal(torch_op.diff_attention(rowptr, colidx, q, k, v, lam), torch_op.diff_attention(rowptr, colidx, q.contiguous(), k, v, lam.contiguous()))
+    far = spread(gen, BF16, (3, kvh, 2, d), (wide, 2 * d, d, 1), base[32768:])
+    with pytest.raises(api.FusedMMError, match="limit|-4"):
+        torch_op.diff_attention(rowptr, colidx, q, far, v, lam)
+    odd, q = spread(gen, BF16, (3, kvh, 2, 7), (wide, 14, 7, 1), base[32768:]), spread(gen, BF16, (2, heads, 2, 7), (wide, 14, 7, 1), base)
+    assert torch.equal(torch_op.diff_attention(rowptr, colidx, q, odd, v, lam), torch_op.diff_attention(rowptr, colidx, q.contiguous(), odd.contiguous(), v, lam))
