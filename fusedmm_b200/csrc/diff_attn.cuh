@@ -472,9 +472,10 @@ struct Forward {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // backward over the rows: dq, dlam and the numbers the columns need.  With D^c unknown until the row's end, the sums
-// A = sum p (dP - c) k, B = sum p k, D = sum p (dP - c) and Z = sum p are taken together, of p before the division by Z;
-// dq = scale (A - D B / Z) / Z.  The reference c is the dP of one of the first edges: with values that have a mean A and D B
-// without it would be large and nearly equal.  Sums with two references join by A += (c' - c) B, D += (c' - c) Z.
+// A = sum p (dP - c) k, B = sum p k, D' = sum p (dP - c), D = sum p dP and Z = sum p are taken together, of p before the division by
+// Z; dq = scale (A - D' B / Z) / Z.  The reference c is the dP of one of the first edges: with values that have a mean A and D' B
+// without it would be large and nearly equal, and D = c + D' loses digits where they have none.  Sums with two references join by
+// A += (c' - c) B, D' += (c' - c) Z.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int G, int NV, int QB, int FORM>
 struct BackwardRows {
@@ -483,7 +484,7 @@ struct BackwardRows {
    static constexpr int LANE_FLOATS = QB * (2 * NV * W + 4);
    struct State {
       F2 a[QB][NV][P], b[QB][NV][P];  // of this half's map
-      float delta[QB], total[QB], ref[QB];
+      float delta[QB], total[QB], rest[QB], ref[QB];  // D, Z, D', c
    };
    State s;
 
@@ -491,7 +492,7 @@ struct BackwardRows {
    {
 #pragma unroll
       for (int b = 0; b < QB; b++) {
-         s.delta[b] = s.total[b] = s.ref[b] = 0.0f;
+         s.delta[b] = s.total[b] = s.rest[b] = s.ref[b] = 0.0f;
 #pragma unroll
          for (int t = 0; t < NV; t++)
 #pragma unroll
@@ -554,7 +555,8 @@ struct BackwardRows {
                   if (s.total[b] == 0.0f && fabsf(dp) < INFINITY) s.ref[b] = dp;  // no weight so far: all sums are 0
                   const float w = pr * (dp - s.ref[b]);
                   const F2 ww = f2(w, w), pp = f2(pr, pr);
-                  s.delta[b] += w;
+                  s.rest[b] += w;
+                  s.delta[b] = fmaf(pr, dp, s.delta[b]);
                   s.total[b] += pr;
 #pragma unroll
                   for (int t = 0; t < NV; t++)
@@ -572,7 +574,7 @@ struct BackwardRows {
          for (int b = 0; b < QB; b++) {
             const float delta = __shfl_xor_sync(FULL, s.delta[b], x2), total = __shfl_xor_sync(FULL, s.total[b], x2);
             F2 a[NV][P], c[NV][P];
-            const float ref = __shfl_xor_sync(FULL, s.ref[b], x2);
+            const float rest = __shfl_xor_sync(FULL, s.rest[b], x2), ref = __shfl_xor_sync(FULL, s.ref[b], x2);
 #pragma unroll
             for (int t = 0; t < NV; t++)
 #pragma unroll
@@ -580,14 +582,14 @@ struct BackwardRows {
                   a[t][j] = shfl_xor_pair(s.a[b][t][j], x2);
                   c[t][j] = shfl_xor_pair(s.b[b][t][j], x2);
                }
-            add(s, b, a, c, delta, total, ref);
+            add(s, b, a, c, make_float4(delta, total, rest, ref));
          }
       }
    }
    // adds the sums of other edges
-   static __device__ __forceinline__ void add(State &s, int b, const F2 (&a)[NV][P], const F2 (&c)[NV][P], float delta, float total, float ref)
+   static __device__ __forceinline__ void add(State &s, int b, const F2 (&a)[NV][P], const F2 (&c)[NV][P], float4 o)
    {
-      const float shift = reference_shift(s.total[b], s.ref[b], total, ref);
+      const float shift = reference_shift(s.total[b], s.ref[b], o.y, o.w);
       const F2 ss = f2(shift, shift);
 #pragma unroll
       for (int t = 0; t < NV; t++)
@@ -596,8 +598,9 @@ struct BackwardRows {
             s.a[b][t][j] = add2(s.a[b][t][j], fma2(ss, c[t][j], a[t][j]));
             s.b[b][t][j] = add2(s.b[b][t][j], c[t][j]);
          }
-      s.delta[b] += fmaf(shift, total, delta);
-      s.total[b] += total;
+      s.delta[b] += o.x;
+      s.total[b] += o.y;
+      s.rest[b] += fmaf(shift, o.y, o.z);
    }
    __device__ __forceinline__ void join_from(const float *unit, const Place &at)
    {
@@ -610,8 +613,7 @@ struct BackwardRows {
             get_pairs<P>(from + (b * 2 * NV + t) * W * G, x[0][t]);
             get_pairs<P>(from + ((b * 2 + 1) * NV + t) * W * G, x[1][t]);
          }
-         const float4 sums = *reinterpret_cast<const float4 *>(unit + QB * 2 * NV * W * G + (b * G + at.in_slot) * 4);
-         add(s, b, x[0], x[1], sums.x, sums.y, sums.z);
+         add(s, b, x[0], x[1], *reinterpret_cast<const float4 *>(unit + QB * 2 * NV * W * G + (b * G + at.in_slot) * 4));
       }
    }
    __device__ __forceinline__ void put(float *unit, const Place &at) const
@@ -624,7 +626,7 @@ struct BackwardRows {
             put_pairs<P>(to + (b * 2 * NV + t) * W * G, s.a[b][t]);
             put_pairs<P>(to + ((b * 2 + 1) * NV + t) * W * G, s.b[b][t]);
          }
-         *reinterpret_cast<float4 *>(unit + QB * 2 * NV * W * G + (b * G + at.in_slot) * 4) = make_float4(s.delta[b], s.total[b], s.ref[b], 0.0f);
+         *reinterpret_cast<float4 *>(unit + QB * 2 * NV * W * G + (b * G + at.in_slot) * 4) = make_float4(s.delta[b], s.total[b], s.rest[b], s.ref[b]);
       }
    }
 
@@ -635,7 +637,7 @@ struct BackwardRows {
       for (int b = 0; b < QB; b++) {
          const int head = at.unit * QB + b;
          const long long rh = row * p.heads + head;
-         const float inverse = reciprocal_total(s.total[b]), rest = s.delta[b] * inverse, delta = inverse == 0.0f ? 0.0f : s.ref[b] + rest;
+         const float inverse = reciprocal_total(s.total[b]), delta = s.delta[b] * inverse, rest = s.rest[b] * inverse;
          const float sign = (at.half ? -__ldg(p.lam + row * p.ldlam + head) : 1.0f) * inverse, factor = sign * p.scale;
 #pragma unroll
          for (int t = 0; t < NV; t++) {

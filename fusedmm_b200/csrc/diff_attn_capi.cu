@@ -119,7 +119,7 @@ Shape choose_shape(Walk w, int dtype, bool vector, long long rows, long long edg
          while (s.unit_kv * 2 * s.unit_heads <= 4 && kv_heads % (s.unit_kv * 2) == 0) s.unit_kv *= 2;
       s.units = kv_heads / s.unit_kv * s.head_blocks;
       s.slot_heads = 1;
-      lane_floats = w == FORWARD ? s.walk.width / 2 + 4 : w == ROWS ? s.walk.width / 2 + 6 : s.walk.width;
+      lane_floats = w == FORWARD ? s.walk.width / 2 + 4 : w == ROWS ? s.walk.width / 2 + 8 : s.walk.width;
       s.part_bytes = static_cast<long long>(lane_floats) * 32 * 4;
    } else {
       s.walk.g = need <= 8 ? 4 : need <= 16 ? 8 : need <= 32 ? 16 : 32;

@@ -590,21 +590,21 @@ struct ForwardMma {
 };
 
 // ---------------------------------------------------------------------------------------------------------------------
-// backward over the rows (the sums A = sum p (dP - c) k, B = sum p k, D = sum p (dP - c), Z = sum p of BackwardRows; c is the
-// largest dP of a column's first block with edges).  For map 0 the rows of A's operand are w = p (dP - c) of the columns 0..3 and p
-// of the same, for map 1 the other way round.
+// backward over the rows (the sums A = sum p (dP - c) k, B = sum p k, D' = sum p (dP - c), D = sum p dP, Z = sum p of BackwardRows;
+// c is the mean dP of a column's first block with edges).  For map 0 the rows of A's operand are w = p (dP - c) of the columns 0..3
+// and p of the same, for map 1 the other way round.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DK, int FORM, bool ONE>
 struct BackwardRowsMma {
    static_assert(LOWER_SCALE<T> == 1.0f, "the parts of split numbers are added up as they are");
    using Cols = Columns<ONE>;
    static constexpr int N = Cols::N;
-   static constexpr int DV = 2 * DK, TILES = DK / 8, LANE_FLOATS = 4 * TILES + 6;
+   static constexpr int DV = 2 * DK, TILES = DK / 8, LANE_FLOATS = 4 * TILES + 8;
    using Gathered = Ring<T, DK, FORM, Budget<DK, WALK_ROWS>::STAGES, false, true>;
    using Width = Budget<DK, WALK_ROWS>;
    struct State {
       float acc[2][TILES][2];
-      float delta[N], total[N], ref[N];  // of this lane's columns
+      float delta[N], total[N], rest[N], ref[N];  // D, Z, D' and c of this lane's columns
    };
    State s;
    Lanes l;
@@ -628,7 +628,7 @@ struct BackwardRowsMma {
 #pragma unroll
          for (int t = 0; t < TILES; t++) s.acc[m][t][0] = s.acc[m][t][1] = 0.0f;
 #pragma unroll
-      for (int x = 0; x < N; x++) s.delta[x] = s.total[x] = s.ref[x] = 0.0f;
+      for (int x = 0; x < N; x++) s.delta[x] = s.total[x] = s.rest[x] = s.ref[x] = 0.0f;
    }
    __device__ __forceinline__ void fetch(const AttnParams &p, long long row)
    {
@@ -646,7 +646,7 @@ struct BackwardRowsMma {
 #pragma unroll
          for (int t = 0; t < TILES; t++) acc[m][t][0] = acc[m][t][1] = acc[m][t][2] = acc[m][t][3] = 0.0f;
 #pragma unroll
-      for (int x = 0; x < N; x++) s.delta[x] = s.total[x] = s.ref[x] = 0.0f;
+      for (int x = 0; x < N; x++) s.delta[x] = s.total[x] = s.rest[x] = s.ref[x] = 0.0f;
       unsigned q[DK / 8], dout[DV / 8];
       float lse[N];
 #pragma unroll
@@ -691,13 +691,15 @@ struct BackwardRowsMma {
             there[h] = edge >= lo && edge < hi && bias[h] != -INFINITY;
          }
          if (fresh) {
-            fresh = !__any_sync(FULL, there[0] || there[1]);
+            // a pair is seen by four lanes
+            const int live = (__popc(__ballot_sync(FULL, there[0])) + __popc(__ballot_sync(FULL, there[1]))) >> (2 + l.slots_log2);
+            fresh = live == 0;
 #pragma unroll
             for (int x = 0; x < N; x++) {
-               const float d0 = heads.valid[x] && there[0] ? Cols::pick(dp, 0, x, l) : -INFINITY;
-               const float d1 = heads.valid[x] && there[1] ? Cols::pick(dp, 1, x, l) : -INFINITY;
-               const float high = Cols::max(fmaxf(d0, d1));
-               s.ref[x] = fabsf(high) < INFINITY ? high : 0.0f;
+               const float d0 = heads.valid[x] && there[0] ? Cols::pick(dp, 0, x, l) : 0.0f;
+               const float d1 = heads.valid[x] && there[1] ? Cols::pick(dp, 1, x, l) : 0.0f;
+               const float mean = __fdividef(Cols::sum(d0 + d1), static_cast<float>(live));
+               s.ref[x] = fabsf(mean) < INFINITY ? mean : 0.0f;
             }
          }
          unsigned a0[4], a1[4];
@@ -709,8 +711,10 @@ struct BackwardRowsMma {
                // an edge that is masked has p = 0, and so has a row without edges (its lse is -inf)
                const bool live = heads.valid[x] && there[h] && lse[x] != -INFINITY;
                pr[x] = live ? weight_of(fmaf(Cols::pick(s0, s1, h, x, l), p.scale, bias[h]), lse[x]) : 0.0f;
-               w[x] = live ? pr[x] * (Cols::pick(dp, h, x, l) - s.ref[x]) : 0.0f;
-               s.delta[x] += w[x];
+               const float d = live ? Cols::pick(dp, h, x, l) : s.ref[x];
+               w[x] = pr[x] * (d - s.ref[x]);
+               s.rest[x] += w[x];
+               s.delta[x] = fmaf(pr[x], d, s.delta[x]);
                s.total[x] += pr[x];
             }
             unsigned wh, wl, ph, pl;
@@ -751,6 +755,7 @@ struct BackwardRowsMma {
       for (int x = 0; x < N; x++) {
          s.delta[x] = Cols::sum(s.delta[x]);
          s.total[x] = Cols::sum(s.total[x]);
+         s.rest[x] = Cols::sum(s.rest[x]);
       }
    }
 
@@ -768,12 +773,13 @@ struct BackwardRowsMma {
       float2 c[TILES];
 #pragma unroll
       for (int t = 0; t < TILES; t++) c[t] = other[32 * t];
-      const float2 d = from[64 * TILES], z = from[64 * TILES + 32], ref = from[64 * TILES + 64];
+      const float2 d = from[64 * TILES], z = from[64 * TILES + 32], rest = from[64 * TILES + 64], ref = from[64 * TILES + 96];
       float shift[N];
 #pragma unroll
       for (int x = 0; x < N; x++) {
          shift[x] = reference_shift(s.total[x], s.ref[x], x ? z.y : z.x, x ? ref.y : ref.x);
-         s.delta[x] += fmaf(shift[x], x ? z.y : z.x, x ? d.y : d.x);
+         s.delta[x] += x ? d.y : d.x;
+         s.rest[x] += fmaf(shift[x], x ? z.y : z.x, x ? rest.y : rest.x);
          s.total[x] += x ? z.y : z.x;
       }
       const float row_shift = Cols::of_row(shift, l.r);
@@ -795,20 +801,21 @@ struct BackwardRowsMma {
 #pragma unroll
             for (int t = 0; t < TILES; t++) to[32 * (m * TILES + t)] = make_float2(s.acc[m][t][0], s.acc[m][t][1]);
       }
-      float *delta = reinterpret_cast<float *>(to + 64 * TILES), *total = delta + 64, *ref = delta + 128;
+      float *delta = reinterpret_cast<float *>(to + 64 * TILES), *total = delta + 64, *rest = delta + 128, *ref = delta + 192;
 #pragma unroll
       for (int x = 0; x < N; x++)
          if (only < 0 || heads.col_kv[x] == only) {
             delta[x] = s.delta[x];
             total[x] = s.total[x];
+            rest[x] = s.rest[x];
             ref[x] = s.ref[x];
          }
    }
 
    __device__ __forceinline__ void finish(const AttnParams &p, const Place &at, long long row, int only)
    {
-      const float inverse = reciprocal_total(Cols::of_row(s.total, l.r)), rest = Cols::of_row(s.delta, l.r) * inverse;
-      const float ref = Cols::of_row(s.ref, l.r), delta = inverse == 0.0f ? 0.0f : ref + rest;
+      const float inverse = reciprocal_total(Cols::of_row(s.total, l.r));
+      const float delta = Cols::of_row(s.delta, l.r) * inverse, rest = Cols::of_row(s.rest, l.r) * inverse;
       const bool mine = heads.live && (only < 0 || heads.kv == only);
       const int map = l.r >> 2;
       const long long rh = row * p.heads + heads.head;
