@@ -152,11 +152,11 @@ Shape choose_shape(Walk w, int dtype, bool vector, long long rows, long long edg
    s.piece = (items * s.unit_blocks + jobs - 1) / jobs;
    s.piece = s.piece < lo ? lo : s.piece > hi ? hi : s.piece;
    // One piece is the least there is, whatever its scratch (4097 units of 16 KB are above the limit); a warp counts the edges of a
-   // piece in 32 bits.  (check_sizes keeps items * heads below 2^56, so that nothing here passes 63 bits.)
+   // piece and the row behind it in 32 bits.  (check_sizes keeps items * heads below 2^56, so that nothing here passes 63 bits.)
    for (;; s.piece *= 2) {
       s.pieces = (items + s.piece - 1) / s.piece;
       const bool fits = s.pieces * 2 * s.units * s.part_bytes <= SCRATCH_LIMIT;
-      if ((fits || s.pieces == 1 || s.piece >= 1 << 30) && s.pieces * s.unit_blocks < INT_MAX / 2) break;
+      if ((fits || s.pieces == 1 || s.piece >= 1 << 29) && s.pieces * s.unit_blocks < INT_MAX / 2) break;
    }
    s.row_limit = s.walk.together || s.piece >= 256 ? s.piece : s.piece < 64 ? 80 : s.piece + s.piece / 4;
    return s;

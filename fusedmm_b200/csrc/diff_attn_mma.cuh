@@ -20,6 +20,8 @@
 // Why not tcgen05: a tile there has 64 or 128 rows that share one operand; here a gathered row meets at most 8 rows of q,
 // and consecutive rows of the pattern gather different rows.
 #pragma once
+#include <climits>
+
 #include "diff_attn.cuh"
 
 namespace fmm {
@@ -1090,9 +1092,6 @@ __device__ __forceinline__ void ring_segment(Op &op, typename Op::Gathered &ring
       w1 = w1 < e1 ? w1 : e1;
       ring.begin(p, op.l, at.lane, w0, w1, -1);
    }
-   // (row pointers that decrease must not lead out of the ring)
-   w0 = w0 < ring.first ? ring.first : w0;
-   w1 = w1 < w0 ? w0 : w1;
    op.run(p, at, ring, static_cast<int>(w0 - ring.first), static_cast<int>(w1 - ring.first), follow);
    const bool lost = TOGETHER ? p.unit_kv > 1 && __syncthreads_or(op.lost) : __any_sync(FULL, op.lost);
    for (int only = lost ? 0 : -1; only < (lost ? p.unit_kv : 0); only++) {
@@ -1158,6 +1157,7 @@ ring_walk_kernel(const AttnParams p)
       long long run_begin, run_end, x;
       part_of(u, rows.begin(u), rows.begin(u + 1), run_begin, x);
       part_of(last - 1, rows.begin(last - 1), rows.begin(last), x, run_end);
+      if (run_end - run_begin > INT_MAX - 64) run_end = run_begin + (INT_MAX - 64);  // (row pointers that decrease: the ring counts in 32 bits)
       // (where a row's edges are taken once for each of several groups of heads, every row is a run of its own)
       if (!TOGETHER && Op::Gathered::SINGLE) ring.begin(p, op.l, at.lane, run_begin, run_end, -1);
       // rows 31 at a time, their pointers one to a lane; rows with edges are found by their bits
@@ -1167,6 +1167,11 @@ ring_walk_kernel(const AttnParams p)
          const long long behind = __shfl_down_sync(FULL, mine, 1);
          long long m0 = 0, m1 = 0, part = -1;
          if (at.lane < here) part = part_of(from + at.lane, mine, behind, m0, m1);
+         if (!TOGETHER && Op::Gathered::SINGLE) {  // likewise: no row leads out of the ring's run
+            const long long end = ring.first + ring.length;
+            m0 = m0 < ring.first ? ring.first : m0 > end ? end : m0;
+            m1 = m1 < m0 ? m0 : m1 > end ? end : m1;
+         }
          const unsigned busy = __ballot_sync(FULL, at.lane < here && (m1 > m0 || part >= 0));
          const unsigned starts = __ballot_sync(FULL, part >= 0 && (part & 1));
          if (starts) begun = from + __ffs(starts) - 1;

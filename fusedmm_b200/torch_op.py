@@ -295,7 +295,7 @@ def diff_attention(rowptr, colidx, q, k, v, lam, *, bias=None, scale=None, trans
     first, and the rows of ``v`` are summed with the differences: [m, heads, dv].  ``colidx`` lists rows of k and v (nodes,
     or the slots of a cache); an id outside [0, n) or a ``bias`` of -inf drops the edge; rows without edges give zeros.
     ``scale`` is 1/sqrt(d) if left out.  ``transposed``: what :func:`csr_transpose` made of this pattern; without it a
-    backward pass makes it again.  With ``return_lse`` also the logarithms of the maps' sums, [m, heads, 2]."""
+    backward pass makes it again.  With ``return_lse`` also the logarithms of the maps' sums, [m, heads, 2] (no gradient)."""
     t = (None, None, None) if transposed is None else transposed
     scale = q.shape[-1] ** -0.5 if scale is None else scale
     if not _plain(rowptr, colidx, bias, q, k, v, lam, *t):
