@@ -157,13 +157,14 @@ __device__ __forceinline__ void get_pairs(const float *p, F2 (&f)[N])
 }
 // exp(score - lse).  No score is above lse but for rounding, which next to a mask's size may be a power of thousands.
 __device__ __forceinline__ float weight_of(float score, float lse) { return exp2_fast(min_or_nan(score - lse, 0.0f) * LOG2E); }
-// What sums with the reference `ref_o` lack (times the sums of their weights) against `ref`, which becomes theirs where there are no
-// weights yet (all sums are 0 then).
-__device__ __forceinline__ float reference_shift(float total, float &ref, float total_o, float ref_o)
+constexpr float REFERENCE_GROWTH = 4.0f;
+// Where sums with two references join: what each side's sums lack, in units of the sums of its weights.  `ref` becomes the heavier's.
+__device__ __forceinline__ void join_references(float total, float &ref, float total_o, float ref_o, float &shift, float &shift_o)
 {
-   const float shift = total != 0.0f && total_o != 0.0f ? ref_o - ref : 0.0f;
-   if (total == 0.0f) ref = ref_o;
-   return shift;
+   const bool other = total_o > total;
+   shift = other ? ref - ref_o : 0.0f;
+   shift_o = other ? 0.0f : ref_o - ref;
+   ref = other ? ref_o : ref;
 }
 // 1 / Z; a row of no weights has no gradient
 __device__ __forceinline__ float reciprocal_total(float total) { return total == 0.0f ? 0.0f : 1.0f / total; }
@@ -473,9 +474,10 @@ struct Forward {
 // ---------------------------------------------------------------------------------------------------------------------
 // backward over the rows: dq, dlam and the numbers the columns need.  With D^c unknown until the row's end, the sums
 // A = sum p (dP - c) k, B = sum p k, D' = sum p (dP - c), D = sum p dP and Z = sum p are taken together, of p before the division by
-// Z; dq = scale (A - D' B / Z) / Z.  The reference c is the dP of one of the first edges: with values that have a mean A and D' B
-// without it would be large and nearly equal, and D = c + D' loses digits where they have none.  Sums with two references join by
-// A += (c' - c) B, D' += (c' - c) Z.
+// Z; dq = scale (A - D' B / Z) / Z.  With c = 0 A and D' B would be large and nearly equal where values have a mean, or where one edge
+// has nearly all the weight.  So the reference c is the dP of the first edge, and of every later one with REFERENCE_GROWTH times the
+// weight that had come in when c was last set; D is kept too, as c + D' loses digits where dP has no mean.  Another reference:
+// A += (c - c') B, D' += (c - c') Z; where sums join, the heavier side's stays.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int G, int NV, int QB, int FORM>
 struct BackwardRows {
@@ -509,9 +511,10 @@ struct BackwardRows {
       const int x = at.in_half * W, y = at.in_slot * W;
       const Gather<T, NV, FORM> kg = gather_a<T, NV, FORM>(p, kv, at.half, x), vg = gather_b<T, NV, FORM>(p, kv, y);
       F2 q[QB][NV][P], dout[QB][NV][P];
-      float lse[QB];
+      float lse[QB], mark[QB];
 #pragma unroll
       for (int b = 0; b < QB; b++) {
+         mark[b] = 0.0f;
          lse[b] = __ldg(p.lse + (row * p.heads + head0 + b) * 2 + at.half);
          load_own<T, NV, FORM, KSKIP>(p, p.q, row * p.ldq + (head0 + b) * p.hsq + at.half * p.d, x, p.d, q[b]);
          load_own<T, NV, FORM, VSKIP>(p, p.dout, row * p.ldo + (head0 + b) * p.hso, y, p.dv, dout[b]);
@@ -552,7 +555,17 @@ struct BackwardRows {
                   const float dot = add_over<G / 2>(sum2(dots)), dp = add_over<G>(sum2(dps));
                   // an edge that is masked has p = 0, and so has a row without edges (its lse is -inf)
                   const float pr = id[i] >= 0 && lse[b] != -INFINITY ? weight_of(fmaf(dot, p.scale, bias), lse[b]) : 0.0f;
-                  if (s.total[b] == 0.0f && fabsf(dp) < INFINITY) s.ref[b] = dp;  // no weight so far: all sums are 0
+                  if (pr > mark[b] && fabsf(dp) < INFINITY) {
+                     const float shift = s.ref[b] - dp;
+                     const F2 ss = f2(shift, shift);
+#pragma unroll
+                     for (int t = 0; t < NV; t++)
+#pragma unroll
+                        for (int j = 0; j < P; j++) s.a[b][t][j] = fma2(ss, s.b[b][t][j], s.a[b][t][j]);
+                     s.rest[b] = fmaf(shift, s.total[b], s.rest[b]);
+                     s.ref[b] = dp;
+                     mark[b] = REFERENCE_GROWTH * (s.total[b] + pr);
+                  }
                   const float w = pr * (dp - s.ref[b]);
                   const F2 ww = f2(w, w), pp = f2(pr, pr);
                   s.rest[b] += w;
@@ -589,18 +602,19 @@ struct BackwardRows {
    // adds the sums of other edges
    static __device__ __forceinline__ void add(State &s, int b, const F2 (&a)[NV][P], const F2 (&c)[NV][P], float4 o)
    {
-      const float shift = reference_shift(s.total[b], s.ref[b], o.y, o.w);
-      const F2 ss = f2(shift, shift);
+      float shift, shift_o;
+      join_references(s.total[b], s.ref[b], o.y, o.w, shift, shift_o);
+      const F2 ss = f2(shift, shift), so = f2(shift_o, shift_o);
 #pragma unroll
       for (int t = 0; t < NV; t++)
 #pragma unroll
          for (int j = 0; j < P; j++) {
-            s.a[b][t][j] = add2(s.a[b][t][j], fma2(ss, c[t][j], a[t][j]));
+            s.a[b][t][j] = add2(fma2(ss, s.b[b][t][j], s.a[b][t][j]), fma2(so, c[t][j], a[t][j]));
             s.b[b][t][j] = add2(s.b[b][t][j], c[t][j]);
          }
       s.delta[b] += o.x;
+      s.rest[b] = fmaf(shift, s.total[b], s.rest[b]) + fmaf(shift_o, o.y, o.z);
       s.total[b] += o.y;
-      s.rest[b] += fmaf(shift, o.y, o.z);
    }
    __device__ __forceinline__ void join_from(const float *unit, const Place &at)
    {

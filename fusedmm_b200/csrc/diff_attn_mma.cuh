@@ -593,8 +593,8 @@ struct ForwardMma {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // backward over the rows (the sums A = sum p (dP - c) k, B = sum p k, D' = sum p (dP - c), D = sum p dP, Z = sum p of BackwardRows;
-// c is the mean dP of a column's first block with edges).  For map 0 the rows of A's operand are w = p (dP - c) of the columns 0..3
-// and p of the same, for map 1 the other way round.
+// c is the D / Z of the edges so far, after the first block and after each with an edge of REFERENCE_GROWTH times the weight then).
+// For map 0 the rows of A's operand are w = p (dP - c) of the columns 0..3 and p of the same, for map 1 the other way round.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DK, int FORM, bool ONE>
 struct BackwardRowsMma {
@@ -640,6 +640,41 @@ struct BackwardRowsMma {
       for (int x = 0; x < N; x++) next_lse[x] = __ldg(p.lse + (row * p.heads + heads.col_head[x]) * 2 + (l.c >> 1));
    }
 
+   // A new reference for the columns, the mean of dP so far; `pr`, `dp`: weights and dP of the present block, which are in no sum yet.
+   // `sums`: there are any.
+   __device__ __forceinline__ void rebase(float (&acc)[2][TILES][4], float (&mark)[N], const float (&pr)[2][N], const float (&dp)[4], int map, bool sums)
+   {
+      float shift[N];
+#pragma unroll
+      for (int x = 0; x < N; x++) {
+         float delta = s.delta[x], total = s.total[x];
+#pragma unroll
+         for (int h = 0; h < 2; h++)
+            if (pr[h][x] != 0.0f) {
+               delta = fmaf(pr[h][x], Cols::pick(dp, h, x, l), delta);
+               total += pr[h][x];
+            }
+         total = Cols::sum(total);
+         const float mean = __fdividef(Cols::sum(delta), total), ref = fabsf(mean) < INFINITY ? mean : s.ref[x];
+         shift[x] = s.ref[x] - ref;
+         s.rest[x] = fmaf(shift[x], s.total[x], s.rest[x]);
+         s.ref[x] = ref;
+         mark[x] = REFERENCE_GROWTH * total;
+      }
+      if (!sums) return;
+      const float row_shift = Cols::of_row(shift, l.r);
+#pragma unroll
+      for (int t = 0; t < TILES; t++)
+#pragma unroll
+         for (int i = 0; i < 2; i++) {
+            // the B of this lane's A lies 16 lanes away, in the sums of the same map
+            const float give = map ? acc[0][t][i] + acc[0][t][i + 2] : acc[1][t][i] + acc[1][t][i + 2];
+            const float b = __shfl_xor_sync(FULL, give, 16);
+            if (map) acc[1][t][i] = fmaf(row_shift, b, acc[1][t][i]);
+            else acc[0][t][i] = fmaf(row_shift, b, acc[0][t][i]);
+         }
+   }
+
    __device__ __forceinline__ void run(const AttnParams &p, const Place &at, Gathered &ring, int e0, int e1, long long follow)
    {
       float acc[2][TILES][4];
@@ -661,7 +696,10 @@ struct BackwardRowsMma {
       const int per_log2 = 4 - l.slots_log2;
       // the lane's row and chunk of ldmatrix: pairs 0..7 and 8..15 of one chunk, then of the next; chunks by exclusive or
       const unsigned mine = Gathered::offset(at.lane & 15, at.lane >> 4);
-      bool fresh = true;  // no edge so far
+      const int map = l.r >> 2;
+      float mark[N];
+#pragma unroll
+      for (int x = 0; x < N; x++) mark[x] = 0.0f;
       for (int e = e0; e < e1;) {
          const int block = e >> per_log2;
          if (block != ring.current) ring.advance(p, l, at.lane);
@@ -684,44 +722,37 @@ struct BackwardRowsMma {
          }
 #pragma unroll
          for (int i = 0; i < 4; i++) dp[i] += dp2[i];
-         float bias[2];
-         bool there[2];
+         float pr[2][N];
+         bool grown = false;
 #pragma unroll
          for (int h = 0; h < 2; h++) {
             const int edge = (l.r + 8 * h) >> l.slots_log2;
-            bias[h] = shared_float(slot + Gathered::BIAS + 4 * edge);
-            there[h] = edge >= lo && edge < hi && bias[h] != -INFINITY;
-         }
-         if (fresh) {
-            // a pair is seen by four lanes
-            const int live = (__popc(__ballot_sync(FULL, there[0])) + __popc(__ballot_sync(FULL, there[1]))) >> (2 + l.slots_log2);
-            fresh = live == 0;
+            const float bias = shared_float(slot + Gathered::BIAS + 4 * edge);
+            const bool there = edge >= lo && edge < hi && bias != -INFINITY;
 #pragma unroll
             for (int x = 0; x < N; x++) {
-               const float d0 = heads.valid[x] && there[0] ? Cols::pick(dp, 0, x, l) : 0.0f;
-               const float d1 = heads.valid[x] && there[1] ? Cols::pick(dp, 1, x, l) : 0.0f;
-               const float mean = __fdividef(Cols::sum(d0 + d1), static_cast<float>(live));
-               s.ref[x] = fabsf(mean) < INFINITY ? mean : 0.0f;
+               // an edge that is masked has p = -0, and so has a row without edges (its lse is -inf)
+               const bool live = heads.valid[x] && there && lse[x] != -INFINITY;
+               pr[h][x] = live ? weight_of(fmaf(Cols::pick(s0, s1, h, x, l), p.scale, bias), lse[x]) : -0.0f;
+               grown |= pr[h][x] > mark[x];
             }
          }
+         if (__any_sync(FULL, grown)) rebase(acc, mark, pr, dp, map, e != e0);
          unsigned a0[4], a1[4];
 #pragma unroll
          for (int h = 0; h < 2; h++) {
-            float pr[N], w[N];
+            float w[N];
 #pragma unroll
             for (int x = 0; x < N; x++) {
-               // an edge that is masked has p = 0, and so has a row without edges (its lse is -inf)
-               const bool live = heads.valid[x] && there[h] && lse[x] != -INFINITY;
-               pr[x] = live ? weight_of(fmaf(Cols::pick(s0, s1, h, x, l), p.scale, bias[h]), lse[x]) : 0.0f;
-               const float d = live ? Cols::pick(dp, h, x, l) : s.ref[x];
-               w[x] = pr[x] * (d - s.ref[x]);
+               const float d = signbit(pr[h][x]) ? s.ref[x] : Cols::pick(dp, h, x, l);
+               w[x] = pr[h][x] * (d - s.ref[x]);
                s.rest[x] += w[x];
-               s.delta[x] = fmaf(pr[x], d, s.delta[x]);
-               s.total[x] += pr[x];
+               s.delta[x] = fmaf(pr[h][x], d, s.delta[x]);
+               s.total[x] += pr[h][x];
             }
             unsigned wh, wl, ph, pl;
             Cols::template split<T>(w, l, wh, wl);
-            Cols::template split<T>(pr, l, ph, pl);
+            Cols::template split<T>(pr[h], l, ph, pl);
             wh = transpose8x8(wh);
             wl = transpose8x8(wl);
             ph = __shfl_xor_sync(FULL, transpose8x8(ph), 16);
@@ -776,22 +807,35 @@ struct BackwardRowsMma {
 #pragma unroll
       for (int t = 0; t < TILES; t++) c[t] = other[32 * t];
       const float2 d = from[64 * TILES], z = from[64 * TILES + 32], rest = from[64 * TILES + 64], ref = from[64 * TILES + 96];
-      float shift[N];
+      float shift[N], shift_o[N];
+      bool moved = false;
 #pragma unroll
       for (int x = 0; x < N; x++) {
-         shift[x] = reference_shift(s.total[x], s.ref[x], x ? z.y : z.x, x ? ref.y : ref.x);
+         const float total = x ? z.y : z.x;
+         join_references(s.total[x], s.ref[x], total, x ? ref.y : ref.x, shift[x], shift_o[x]);
+         moved |= shift[x] != 0.0f;
          s.delta[x] += x ? d.y : d.x;
-         s.rest[x] += fmaf(shift[x], x ? z.y : z.x, x ? rest.y : rest.x);
-         s.total[x] += x ? z.y : z.x;
+         s.rest[x] = fmaf(shift[x], s.total[x], s.rest[x]) + fmaf(shift_o[x], total, x ? rest.y : rest.x);
+         s.total[x] += total;
       }
-      const float row_shift = Cols::of_row(shift, l.r);
+      if (__any_sync(FULL, moved)) {
+         const float f = Cols::of_row(shift, l.r);
+#pragma unroll
+         for (int t = 0; t < TILES; t++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+               const float b = __shfl_xor_sync(FULL, map ? s.acc[0][t][i] : s.acc[1][t][i], 16);
+               if (map) s.acc[1][t][i] = fmaf(f, b, s.acc[1][t][i]);
+               else s.acc[0][t][i] = fmaf(f, b, s.acc[0][t][i]);
+            }
+      }
+      const float f = Cols::of_row(shift_o, l.r);
 #pragma unroll
       for (int m = 0; m < 2; m++)
 #pragma unroll
          for (int t = 0; t < TILES; t++) {
-            const float f = m == map ? row_shift : 0.0f;
-            s.acc[m][t][0] += f == 0.0f ? o[m][t].x : fmaf(f, c[t].x, o[m][t].x);
-            s.acc[m][t][1] += f == 0.0f ? o[m][t].y : fmaf(f, c[t].y, o[m][t].y);
+            s.acc[m][t][0] += m == map ? fmaf(f, c[t].x, o[m][t].x) : o[m][t].x;
+            s.acc[m][t][1] += m == map ? fmaf(f, c[t].y, o[m][t].y) : o[m][t].y;
          }
    }
    __device__ __forceinline__ void put(float *unit, const Place &at, int only) const

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from attention_cases import HALF_STEP, attention_reference, check
+from attention_cases import HALF_STEP, HALF_SUBNORMAL, attention_reference, check
 from fusedmm_b200 import torch_op
 
 pytestmark = pytest.mark.gpu
@@ -132,3 +132,47 @@ def test_gradient_of_queries_where_values_have_a_mean(cuda_device, dtype, low, h
     step, split = (2.0 ** -23, 2.0 ** -16) if dtype == BF16 else (2.0 ** -24, 0)
     slack = scale * 4 * (high - low) * 2 * (split + (degree + 16) * step)
     check(got, (want, half * want.abs() + (1 + half) * slack))
+
+
+@pytest.mark.parametrize("lengths", ["one row", "rows", "long row"])
+@pytest.mark.parametrize("gap", [6, 10, 14])
+@pytest.mark.parametrize("dtype,heads,kvh,d,dv", [(F32, 4, 2, 32, 64), (F32, 3, 3, 5, 7), (BF16, 8, 2, 64, 128), (BF16, 4, 4, 16, 32), (BF16, 2, 1, 32, 64),
+                                                  (BF16, 2, 2, 128, 256), (F16, 4, 2, 32, 64)])
+def test_gradient_of_queries_where_one_edge_has_nearly_all_the_weight(cuda_device, dtype, heads, kvh, d, dv, gap, lengths):
+    """dq = sum of p (dP - D) k is small there, since D is nearly the dP of the heavy edge, and must keep its digits.
+
+    dq is the covariance of dP and k under p.  To first order an error e_p of p (relative) brings p e_p (dP - D) (k - K), K the sum
+    of p k, and one of dP brings p e_dP (k - K).  The sums of p (dP - c) k and p k are rounded (split in bf16) relative to their
+    terms; c is some dP (R from D at most) until the heavy edge comes, and then within 2 W of D, W = sum p |dP - D|."""
+    gen = torch.Generator().manual_seed(gap + d)
+    n = 400
+    rowptr, colidx = rows_of({"one row": [1000], "rows": [250] * 300, "long row": [20000]}[lengths], n, gen)
+    m = len(rowptr) - 1
+    at = rowptr[:-1] + (torch.rand(m, generator=gen) * (rowptr[1:] - rowptr[:-1])).long()
+    bias = torch.zeros(colidx.numel())
+    bias[at] = gap + math.log(int(rowptr[1]) / 250)
+    q, k = ((0.3 * torch.randn(s, generator=gen)).to(dtype) for s in ((m, heads, 2, d), (n, kvh, 2, d)))
+    v = torch.randn(n, kvh, dv, generator=gen).to(dtype)
+    dout = (torch.randn(m, heads, dv, generator=gen) * (64 if dtype == F16 else 1)).to(dtype)
+    lam, scale = torch.full((m, heads), 0.5), d ** -0.5
+    got = gradients(rowptr, colidx, bias, q, k, v, lam, scale, dout)["dq"].detach().cpu().double()
+    step, split, half = (2.0 ** -24, 0, HALF_STEP[dtype]) if dtype != BF16 else (2.0 ** -23, 2.0 ** -16, HALF_STEP[dtype])
+    tiny = HALF_SUBNORMAL[dtype] + 1e-30
+    kv = torch.arange(heads) // (heads // kvh)
+    for u in range(0, m, max(1, m // 7)):
+        e = torch.arange(int(rowptr[u]), int(rowptr[u + 1]))
+        ke, ve, qu, du = k.double()[colidx[e].long()][:, kv], v.double()[colidx[e].long()][:, kv], q[u].double(), dout[u].double()
+        score = scale * (ke * qu).sum(-1) + bias[e].double()[:, None, None]
+        p = torch.softmax(score, 0)
+        dp, dpabs = (ve * du).sum(-1)[..., None], (ve.abs() * du.abs()).sum(-1)[..., None]
+        off = dp - (p * dp).sum(0)
+        factor = scale * torch.tensor([1.0, -0.5], dtype=torch.float64)[:, None]
+        want = factor * (p[..., None] * off[..., None] * ke).sum(0)
+        away, wide = (ke - (p[..., None] * ke).sum(0)).abs(), off.abs().amax(0)
+        mean_off = (p * off.abs()).sum(0)
+        of_p = 2 * step * (16 + (d + 2) * scale * (ke.abs() * qu.abs()).sum(-1) + 2 * score.abs())
+        heavy = (e == at[u])[:, None, None]
+        sums = (p[..., None] * torch.where(heavy, 2 * mean_off, 2 * wide)[..., None] * ke.abs()).sum(0) + 2 * mean_off[..., None] * (p[..., None] * ke.abs()).sum(0)
+        slack = factor.abs() * ((p * of_p)[..., None] * off.abs()[..., None] * away + (p * step * (dv + 2) * dpabs)[..., None] * away).sum(0)
+        slack = slack + factor.abs() * (2 * split + step * (len(e) + 32)) * sums
+        check(got[u], (want, half * want.abs() + (1 + half) * slack + tiny), "dq")
