@@ -157,7 +157,10 @@ __device__ __forceinline__ void get_pairs(const float *p, F2 (&f)[N])
 }
 // exp(score - lse).  No score is above lse but for rounding, which next to a mask's size may be a power of thousands.
 __device__ __forceinline__ float weight_of(float score, float lse) { return exp2_fast(min_or_nan(score - lse, 0.0f) * LOG2E); }
-constexpr float REFERENCE_GROWTH = 4.0f;
+// The weight from which on an edge is the next reference: so many times what had come in when the last was set, and a part of the row's
+// whole (1 but for rounding) that leaves little to the others.
+constexpr float REFERENCE_GROWTH = 4.0f, REFERENCE_LEAST = 0.25f;
+__device__ __forceinline__ float reference_mark(float total) { return fmaxf(REFERENCE_GROWTH * total, REFERENCE_LEAST); }
 // Where sums with two references join: what each side's sums lack, in units of the sums of its weights.  `ref` becomes the heavier's.
 __device__ __forceinline__ void join_references(float total, float &ref, float total_o, float ref_o, float &shift, float &shift_o)
 {
@@ -475,9 +478,9 @@ struct Forward {
 // backward over the rows: dq, dlam and the numbers the columns need.  With D^c unknown until the row's end, the sums
 // A = sum p (dP - c) k, B = sum p k, D' = sum p (dP - c), D = sum p dP and Z = sum p are taken together, of p before the division by
 // Z; dq = scale (A - D' B / Z) / Z.  With c = 0 A and D' B would be large and nearly equal where values have a mean, or where one edge
-// has nearly all the weight.  So the reference c is the dP of the first edge, and of every later one with REFERENCE_GROWTH times the
-// weight that had come in when c was last set; D is kept too, as c + D' loses digits where dP has no mean.  Another reference:
-// A += (c - c') B, D' += (c - c') Z; where sums join, the heavier side's stays.
+// has nearly all the weight.  So the reference c is the dP of one of the first edges, and of every later one that is heavy against all
+// before it (reference_mark); D is kept too, as c + D' loses digits where dP has no mean.  Another reference: A += (c - c') B,
+// D' += (c - c') Z; where sums join, the heavier side's stays.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int G, int NV, int QB, int FORM>
 struct BackwardRows {
@@ -499,6 +502,31 @@ struct BackwardRows {
          for (int t = 0; t < NV; t++)
 #pragma unroll
             for (int j = 0; j < P; j++) s.a[b][t][j] = s.b[b][t][j] = 0;
+      }
+   }
+
+   // the heaviest of some edges, which are in no sum yet, becomes the reference where it is heavy enough
+   __device__ __forceinline__ void rebase(float (&mark)[QB], const float (&pr)[U][QB], const float (&dp)[U][QB])
+   {
+#pragma unroll
+      for (int b = 0; b < QB; b++) {
+         float most = mark[b], ref = s.ref[b], total = s.total[b];
+#pragma unroll
+         for (int i = 0; i < U; i++) {
+            const bool heavy = pr[i][b] > most && fabsf(dp[i][b]) < INFINITY;
+            ref = heavy ? dp[i][b] : ref;
+            most = heavy ? pr[i][b] : most;
+            total += pr[i][b];
+         }
+         if (most > mark[b]) mark[b] = reference_mark(total);
+         const float shift = s.ref[b] - ref;
+         const F2 ss = f2(shift, shift);
+#pragma unroll
+         for (int t = 0; t < NV; t++)
+#pragma unroll
+            for (int j = 0; j < P; j++) s.a[b][t][j] = fma2(ss, s.b[b][t][j], s.a[b][t][j]);
+         s.rest[b] = fmaf(shift, s.total[b], s.rest[b]);
+         s.ref[b] = ref;
       }
    }
 
@@ -533,6 +561,8 @@ struct BackwardRows {
                kg.template load<KSKIP>(id[i], kr[i]);
                vg.template load<VSKIP>(id[i], vr[i]);
             }
+            float pr[U][QB], dp[U][QB];
+            bool grown = false;
 #pragma unroll
             for (int i = 0; i < U; i++) {
                F2 k[NV][P], v[NV][P];
@@ -552,25 +582,26 @@ struct BackwardRows {
                         dots = fma2(q[b][t][j], k[t][j], dots);
                         dps = fma2(dout[b][t][j], v[t][j], dps);
                      }
-                  const float dot = add_over<G / 2>(sum2(dots)), dp = add_over<G>(sum2(dps));
+                  const float dot = add_over<G / 2>(sum2(dots));
+                  dp[i][b] = add_over<G>(sum2(dps));
                   // an edge that is masked has p = 0, and so has a row without edges (its lse is -inf)
-                  const float pr = id[i] >= 0 && lse[b] != -INFINITY ? weight_of(fmaf(dot, p.scale, bias), lse[b]) : 0.0f;
-                  if (pr > mark[b] && fabsf(dp) < INFINITY) {
-                     const float shift = s.ref[b] - dp;
-                     const F2 ss = f2(shift, shift);
+                  pr[i][b] = id[i] >= 0 && lse[b] != -INFINITY ? weight_of(fmaf(dot, p.scale, bias), lse[b]) : 0.0f;
+                  grown |= pr[i][b] > mark[b];
+               }
+            }
+            if (grown) rebase(mark, pr, dp);
 #pragma unroll
-                     for (int t = 0; t < NV; t++)
+            for (int i = 0; i < U; i++) {
+               F2 k[NV][P];
 #pragma unroll
-                        for (int j = 0; j < P; j++) s.a[b][t][j] = fma2(ss, s.b[b][t][j], s.a[b][t][j]);
-                     s.rest[b] = fmaf(shift, s.total[b], s.rest[b]);
-                     s.ref[b] = dp;
-                     mark[b] = REFERENCE_GROWTH * (s.total[b] + pr);
-                  }
-                  const float w = pr * (dp - s.ref[b]);
-                  const F2 ww = f2(w, w), pp = f2(pr, pr);
+               for (int t = 0; t < NV; t++) unpack_pairs<T>(kr[i][t], k[t]);
+#pragma unroll
+               for (int b = 0; b < QB; b++) {
+                  const float w = pr[i][b] * (dp[i][b] - s.ref[b]);
+                  const F2 ww = f2(w, w), pp = f2(pr[i][b], pr[i][b]);
                   s.rest[b] += w;
-                  s.delta[b] = fmaf(pr, dp, s.delta[b]);
-                  s.total[b] += pr;
+                  s.delta[b] = fmaf(pr[i][b], dp[i][b], s.delta[b]);
+                  s.total[b] += pr[i][b];
 #pragma unroll
                   for (int t = 0; t < NV; t++)
 #pragma unroll

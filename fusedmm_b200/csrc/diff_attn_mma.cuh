@@ -593,8 +593,8 @@ struct ForwardMma {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // backward over the rows (the sums A = sum p (dP - c) k, B = sum p k, D' = sum p (dP - c), D = sum p dP, Z = sum p of BackwardRows;
-// c is the D / Z of the edges so far, after the first block and after each with an edge of REFERENCE_GROWTH times the weight then).
-// For map 0 the rows of A's operand are w = p (dP - c) of the columns 0..3 and p of the same, for map 1 the other way round.
+// c is the D / Z of the edges so far, after the first block and after each with an edge that is heavy against all before it).  For
+// map 0 the rows of A's operand are w = p (dP - c) of the columns 0..3 and p of the same, for map 1 the other way round.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DK, int FORM, bool ONE>
 struct BackwardRowsMma {
@@ -659,7 +659,7 @@ struct BackwardRowsMma {
          shift[x] = s.ref[x] - ref;
          s.rest[x] = fmaf(shift[x], s.total[x], s.rest[x]);
          s.ref[x] = ref;
-         mark[x] = REFERENCE_GROWTH * total;
+         mark[x] = reference_mark(total);
       }
       if (!sums) return;
       const float row_shift = Cols::of_row(shift, l.r);
