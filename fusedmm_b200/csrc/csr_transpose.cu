@@ -6,7 +6,8 @@
 // outside [0, n) get the key n and stay behind the last column.  A pass is three launches: the digit counts of every tile
 // of edges, their running sums (one block per digit), and the move.  Inside a tile a warp owns a run of consecutive edges
 // and ranks them 32 at a time: lanes with the same digit find each other with match.any, the earlier lanes and the warp's
-// count so far give the place.  Bound: bytes, about 36 an edge and pass.
+// count so far give the place.  Bytes of an edge: 16 in the first pass (32-bit ids), 20 in each other, 24 for rows and positions at
+// the end: 2^23 edges of 2^19 columns take 451 us, and these bytes need 103.
 #include "../../include/fusedmm_b200.h"
 #include "attn_common.cuh"
 #include "attn_host.h"

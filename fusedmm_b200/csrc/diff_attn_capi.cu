@@ -101,8 +101,8 @@ Shape choose_shape(Walk w, int dtype, bool vector, long long rows, long long edg
    const int nk = 2 * ((d + width - 1) / width), nvv = (dv + width - 1) / width, need = nk > nvv ? nk : nvv;
    const int group = heads / kv_heads;
    int lane_floats;
-   // 16-bit types go to the matrix units: a window of 128 over 4096 rows, 8 heads on 2, d 64: forward 76 us, 204 on the ordinary
-   // units; 2^23 R-MAT edges, 4 heads of d 32: forward 1.13 and 1.51 ms, rows 1.47 and 1.92, columns 1.57 and 2.19.  Not half's
+   // 16-bit types go to the matrix units: a window of 128 over 4096 rows, 8 heads on 2, d 64: forward 78 us, 235 on the ordinary
+   // units; 2^23 R-MAT edges, 4 heads of d 32: forward 1.13 and 1.49 ms, rows 1.58 and 2.02, columns 1.57 and 1.94.  Not half's
    // backward walks: their factors p dP and ds have no bound that half's 65504 covers, and they are operands there.
    if (dtype == DT_BF16 || (dtype == DT_F16 && w == FORWARD)) {
       s.walk.width = need <= 4 ? 16 : need <= 8 ? 32 : need <= 16 ? 64 : 128;
@@ -143,7 +143,7 @@ Shape choose_shape(Walk w, int dtype, bool vector, long long rows, long long edg
    // Otherwise a warp takes pieces of at most 128 items, or so many more that the table of parts stays short, and fewer where that
    // leaves warps without work (7600 edges over 400 rows, forward, rows and columns: 75 us with 128, 38 with 32).  Rows longer than a
    // piece (and a quarter, of short pieces) are cut: a hub row in one warp's hands is the walk's end (425984 R-MAT edges in float,
-   // all walks: 457 us with rows of up to 512 items whole, 341 now).
+   // all walks: 457 us with rows of up to 512 items whole, 345 now).
    const long long items = edges + ROW_ITEMS * rows, mean = edges / rows;
    s.walk.together = rows * s.unit_blocks < 8LL * sms && mean >= 64;
    const long long share = items * s.unit_blocks / (16LL * sms);

@@ -17,8 +17,9 @@
 // weights are carried 2^8 times larger (the row's sum with them) and the second parts another 2^11 times (taken out where the two
 // rows are added up): 22 bits of weights down to 2^-22 of the row's largest, and 2^-44 of that largest is what smaller ones lose at
 // most.  Weights change from "pair by column" to "row by pair" with movmatrix.
-// Why not tcgen05: a tile there has 64 or 128 rows that share one operand; here a gathered row meets at most 8 rows of q,
-// and consecutive rows of the pattern gather different rows.
+// Why not tcgen05: a tile there has 64 or 128 rows that share one operand; here a gathered row meets at most 8 rows of q, and
+// consecutive rows of a graph gather different rows.  (Those of a window share nearly all: 64 rows of a window of 128 have 191 between
+// them and gather 8192.  A form for runs of ids is not built.)
 #pragma once
 #include <climits>
 
@@ -363,16 +364,16 @@ template <int DK, int WALK>
 struct Budget {
    static constexpr int STAGES = DK == 16 ? 4 : DK == 32 ? 3 : 2;
    static constexpr int SOLO = DK == 128 ? 2 : 4, JOINT = DK >= 64 ? 4 : 8;
-   // The backward walks run faster with fewer warps and their registers: 2^23 R-MAT edges at d 32 columns 1.77 ms with four
-   // blocks, 1.57 with three, rows 1.69 and 1.47; a window of 128 over 4096 rows at d 64 columns 347 us with three blocks, 267 with
-   // two, rows 95 and 88.  (Forward with one block less and a stage more: 1.21 ms for 1.13, 81 us for 76.)
+   // The backward walks run faster with fewer warps and their registers: 2^23 R-MAT edges at d 32 columns 1.75 ms with four
+   // blocks, 1.57 with three, rows 1.75 and 1.58; a window of 128 over 4096 rows at d 64 columns 349 us with three blocks, 273 with
+   // two, rows 102 and 96.  (Forward with one block less and a stage more: 1.21 ms for 1.13, 81 us for 76.)
    static constexpr int BLOCKS = DK == 16 ? 4 : DK == 32 ? (WALK == WALK_FORWARD ? 4 : 3) : DK == 64 ? (WALK == WALK_FORWARD ? 3 : 2) : 3;
    static constexpr bool AHEAD = DK <= 32;  // a row's own operands are fetched during the row before (wider: no registers left)
 };
 
 // ---------------------------------------------------------------------------------------------------------------------
-// forward.  2^23 R-MAT edges, 4 heads of d 32, bf16: 1.13 ms, 7.6 TB/s of gathered rows (hubs from L2), 310 instructions a block
-// of 16 pairs, issue slots 0.56 busy; 48 tokens over 262144 slots of 4 kv heads of d 64: 94 us, 5.7 TB/s from HBM.
+// forward.  2^23 R-MAT edges, 4 heads of d 32, bf16: 1.13 ms, 7.6 TB/s of gathered rows (hubs from L2); 2^21 edges: 339 instructions
+// a block of 16 pairs, issue slots 0.54 busy; 48 tokens over 262144 slots of 4 kv heads of d 64: 94 us, 5.7 TB/s from HBM.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DK, int FORM, bool ONE>
 struct ForwardMma {
@@ -595,6 +596,8 @@ struct ForwardMma {
 // backward over the rows (the sums A = sum p (dP - c) k, B = sum p k, D' = sum p (dP - c), D = sum p dP, Z = sum p of BackwardRows;
 // c is the D / Z of the edges so far, after the first block and after each with an edge that is heavy against all before it).  For
 // map 0 the rows of A's operand are w = p (dP - c) of the columns 0..3 and p of the same, for map 1 the other way round.
+// 2^23 R-MAT edges, 4 heads of d 32, bf16: 1.58 ms, 5.4 TB/s gathered (1.48 with c = 0 and without Z); 2^21 edges: 411 instructions a
+// block.  Spilled: up to 76 bytes of a lane at d 64, 104 to 292 at d 128.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DK, int FORM, bool ONE>
 struct BackwardRowsMma {
@@ -899,8 +902,9 @@ struct BackwardRowsMma {
 // backward over the columns: dk and dv.  A pair is an edge with a query head; the columns of the products are (map, kv head of
 // the unit).  dk and dv are [16 elements x 8] products over the pairs: the columns 0..3 take the upper and 4..7 the lower part
 // of the split ds (or weight) of the unit's kv heads.
-// 2^23 R-MAT edges, 4 heads of d 32, bf16: 1.57 ms, 5.5 TB/s gathered, 402 instructions a block, bound by their latency (without
-// SINGLE, which leaves out the division of blocks among groups of heads, and with a longer exchange in write(): 518, 2.14 ms).
+// 2^23 R-MAT edges, 4 heads of d 32, bf16: 1.57 ms, 5.5 TB/s gathered, bound by the instructions' latency (2.14 ms without SINGLE,
+// which leaves out the division of blocks among groups of heads, and with a longer exchange in write()); 2^21 edges: 423
+// instructions a block.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int DK, int FORM, bool SINGLE>
 struct BackwardColumnsMma {

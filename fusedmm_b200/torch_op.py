@@ -161,18 +161,24 @@ def _dense_rows(t):
     return t if stride[-1] == 1 and stride[0] != 0 and stride[1] != 0 else t.contiguous()
 
 
+# (names of this module: looking them up in torch's takes as long as the calls)
+_is_compiling, _is_tracing = torch.compiler.is_compiling, torch._C._is_tracing
+_dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+_transforms, _Tensor, _Parameter = torch._C._functorch.peek_interpreter_stack, torch.Tensor, torch.nn.Parameter
+
+
 def _plain(*tensors):
     """True if these are ordinary CUDA tensors (none that stores its numbers negated) and nothing watches torch's operators:
     the call may then go straight to the library, without a round through the dispatcher (some 30 us)."""
-    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack():
+    if _is_compiling() or _dispatch_modes() or _function_modes():
         return False
     # under an open level of forward mode tensors may have a tangent, which the dispatcher refuses; a trace records operators
-    if forward_ad._current_level >= 0 or torch.jit.is_tracing():
+    if forward_ad._current_level >= 0 or _is_tracing() or _transforms() is not None:
         return False
     for t in tensors:
-        if t is not None and ((type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter) or not t.is_cuda or t.is_neg()):
+        if t is not None and ((type(t) is not _Tensor and type(t) is not _Parameter) or not t.is_cuda or t.is_neg()):
             return False
-    return torch._C._functorch.peek_interpreter_stack() is None
+    return True
 
 
 def _below(op, *args):
