@@ -107,3 +107,50 @@ def test_rows_far_apart(cuda_device):
         torch_op.diff_attention(rowptr, colidx, q, far, v, lam)
     odd, q = spread(gen, BF16, (3, kvh, 2, 7), (wide, 14, 7, 1), base[32768:]), spread(gen, BF16, (2, heads, 2, 7), (wide, 14, 7, 1), base)
     assert torch.equal(torch_op.diff_attention(rowptr, colidx, q, odd, v, lam), torch_op.diff_attention(rowptr, colidx, q.contiguous(), odd.contiguous(), v, lam))
+
+
+@pytest.mark.parametrize("dtype,kvh,d,dv,n", [(BF16, 2, 64, 128, 9_000_000), (F32, 1, 32, 64, 18_000_000), (BF16, 1, 60, 120, 19_000_000)])
+def test_offsets_beyond_32_bits_in_a_long_cache(cuda_device, dtype, kvh, d, dv, n):
+    """Slots behind 2^32 bytes (and elements' counts behind 2^31) of a cache give what dense copies of them give."""
+    gen = torch.Generator().manual_seed(5)
+    heads, length = 2 * kvh, 600
+    ids = torch.cat((torch.tensor([0, n - 1]), torch.randint(n // 2, n, (length,), generator=gen))).unique().int()[torch.randperm(400, generator=gen)]
+    rowptr = torch.tensor([0, 150, 400]).cuda()
+    small = [torch.randn(400, kvh, 2, d, generator=gen).to(dtype).cuda(), torch.randn(400, kvh, dv, generator=gen).to(dtype).cuda()]
+    large = [torch.empty(n, *x.shape[1:], dtype=dtype, device="cuda") for x in small]
+    assert large[0].nbytes > 1 << 32 and large[1].nbytes > 1 << 32
+    for x, y in zip(large, small):
+        x[ids.long().cuda()] = y
+    q, dout, lam = torch.randn(2, heads, 2, d, generator=gen).to(dtype).cuda(), torch.randn(2, heads, dv, generator=gen).to(dtype).cuda(), torch.rand(heads, generator=gen).cuda()
+    results = []
+    for kv, colidx in ((small, torch.arange(400, dtype=torch.int32)), (large, ids)):
+        leaves = [x.detach().requires_grad_() for x in (q, *kv, lam)]
+        out = torch_op.diff_attention(rowptr, colidx.cuda(), *leaves)
+        dq, dk, dvv, dlam = torch.autograd.grad(out, leaves, dout)
+        at = colidx.long().cuda()
+        assert bool(dk[at].any()) and int(torch.count_nonzero(dk[-1])) == int(torch.count_nonzero(dk[at[colidx == len(dk) - 1]]))
+        results.append((out, dq, dk[at], dvv[at], dlam))
+        del leaves, dk, dvv
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype,rows,heads,d", [(BF16, 2_200_000, 8, 128), (F32, 1_100_000, 9, 130)])
+def test_rotation_beyond_32_bits(cuda_device, dtype, rows, heads, d):
+    """The last rows of more than 2^31 elements and 2^32 bytes."""
+    gen = torch.Generator().manual_seed(6)
+    x = torch.empty(rows, heads, d, dtype=dtype, device="cuda")
+    assert x.numel() * dtype.itemsize > 1 << 32
+    x.zero_()
+    last = torch.randn(3, heads, d, generator=gen).to(dtype).cuda()
+    x[-3:] = last
+    pos, freq, w = torch.arange(rows, device="cuda"), torch.rand(1, 32, generator=gen, dtype=torch.float64).cuda(), torch.rand(d, generator=gen).cuda()
+    results = []
+    for a, p in ((x, pos), (last, pos[-3:])):
+        a, ww = a.detach().requires_grad_(), w.detach().requires_grad_()
+        y = torch_op.qk_norm_rotary(a, None, p, freq, q_weight=ww, eps=1e-6)
+        (dx,) = torch.autograd.grad(y, a, torch.ones_like(y))
+        results.append((y[-3:].clone(), dx[-3:].clone()))
+        del y, dx
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
