@@ -14,10 +14,10 @@
 //           B = gathered v.
 // Weights are split into two 16-bit numbers, the second of which lies in the rows 8..15 of A that the first leaves free, so the
 // split costs no product.  Their sum has 16 bits of the 32-bit value in bf16 (a result that is small against its values, where lam
-// is near 1 and the maps nearly equal, is off by some 2^-17 of the values; more bits would take a second product).  Half's numbers are 2^-24 apart below 2^-14, so there
-// weights are carried 2^8 times larger (the row's sum with them) and the second parts another 2^11 times (taken out where the two
-// rows are added up): 22 bits of weights down to 2^-22 of the row's largest, and 2^-44 of that largest is what smaller ones lose at
-// most.  Weights change from "pair by column" to "row by pair" with movmatrix.
+// is near 1 and the maps nearly equal, is off by some 2^-17 of the values; more bits would take a second product).  Half's numbers
+// are 2^-24 apart below 2^-14, so there weights are carried 2^8 times larger (the row's sum with them) and the second parts another
+// 2^11 times (taken out where the two rows are added up): 22 bits of weights down to 2^-22 of the row's largest, and 2^-44 of that
+// largest is what smaller ones lose at most.  Weights change from "pair by column" to "row by pair" with movmatrix.
 // Why not tcgen05: a tile there has 64 or 128 rows that share one operand; here a gathered row meets at most 8 rows of q, and
 // consecutive rows of a graph gather different rows.  (Those of a window share nearly all: 64 rows of a window of 128 have 191 between
 // them and gather 8192.  A form for runs of ids is not built.)
